@@ -1,0 +1,63 @@
+// Arguments of the windowed attention kernels and the checks their entry points share.
+#pragma once
+
+#include "attn_tile.h"
+
+namespace ghip {
+namespace win {
+
+struct Mat3 {
+  const void* p;
+  int64_t sb, sh, ss;  // element strides of batch, head, sequence (head dim contiguous)
+};
+
+struct Params {
+  Mat3 q, k, v, o, dout, dq, dk, dv;
+  float* lse;        // [B, H, Sq]; forward: written (may be null), gradient: read
+  float* ndelta;     // gradient: minus the row sums of do * o, [B, H, Sq]
+  const int32_t* lens;
+  int B, H, Hkv, Sq, Sk, D;
+  int q_start, window, sinks;
+  float scale;
+};
+
+// The tokens of sequence b that exist: lens[b] clamped to [0, Sk].
+__device__ __forceinline__ int length_of(const Params& p, int b) {
+  return p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+}
+
+template <typename T>
+__device__ __forceinline__ T* at(const Mat3& m, int b, int h) {
+  return static_cast<T*>(const_cast<void*>(m.p)) + b * m.sb + h * m.sh;
+}
+template <typename T>
+__device__ __forceinline__ tile::Rows rows_of(const Mat3& m, int b, int h, int rows, int D) {
+  const int64_t es = static_cast<int64_t>(sizeof(T));
+  return tile::Rows{reinterpret_cast<const char*>(at<T>(m, b, h)), m.ss * es,
+                    rows > 0 ? ((rows - 1) * m.ss + D) * es : 0};
+}
+
+// The key tiles of queries at positions [p0, p1]: those of the sinks, then those of the
+// windows; tile(i) for i < n.
+template <int kKT>
+struct Tiles {
+  int n, ns, first;
+  __device__ __forceinline__ Tiles(const Params& p, int p0, int end) {
+    const int lo = max(0, p0 - p.window + 1) / kKT;
+    const int hi = (end + kKT - 1) / kKT;  // end: one past the last key that any query sees
+    ns = min((min(p.sinks, end) + kKT - 1) / kKT, lo);
+    first = lo;
+    n = end > 0 ? ns + max(0, hi - lo) : 0;
+  }
+  __device__ __forceinline__ int operator()(int i) const { return i < ns ? i : first + i - ns; }
+};
+
+// The problem's sizes and types; fills p.  Returns GHIP_OK or the error.
+int check_problem(const char* what, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
+                  int64_t q_start, int64_t window, int64_t sinks, float scale, Params* p, GHipError* err);
+// One operand: its strides and alignment (out: 8-byte rows of 16-bit values suffice).
+int check_operand(const char* what, const char* name, int dtype, const void* ptr, const int64_t* strides, bool out,
+                  Mat3* m, GHipError* err);
+
+}  // namespace win
+}  // namespace ghip

@@ -73,12 +73,22 @@ SIGNATURES = {
                           ctypes.POINTER(_i64), _vp, _errp],
     "ghip_softmax_cols": [_int, _vp, _vp, _i64, _i64, _i64, _int, _vp, _errp],
     "ghip_layernorm_cols": [_int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _vp, _errp],
+    "ghip_sdpa_window_fwd": [_int] + [_vp] * 5 + [_i64] * 6 + [ctypes.POINTER(_i64)] * 4 + [_i64] * 3
+                            + [_vp, _f32, _vp, _errp],
+    "ghip_sdpa_window_bwd": [_int] + [_vp] * 9 + [_i64] * 6 + [ctypes.POINTER(_i64)] * 8 + [_i64] * 3
+                            + [_vp, _f32, _vp, _i64, _vp, _errp],
+    "ghip_kv_append": [_int] + [_vp] * 4 + [_i64] * 7 + [_vp, _i64, _vp, _vp] + [ctypes.POINTER(_i64)] * 4
+                      + [_vp, _errp],
+    "ghip_sdpa_paged": [_int] + [_vp] * 4 + [_i64] * 7 + [_vp, _i64, _vp] + [ctypes.POINTER(_i64)] * 4
+                       + [_i64, _i64, _f32, _vp, _i64, _vp, _errp],
 }
 
 # name -> argtypes of the entry points that return int64_t.
 SIGNATURES_I64 = {
     "ghip_sdpa_workspace_bytes": [_int, _i64, _i64, _i64, _i64, _i64, _i64, _int],
     "ghip_gemm_workspace_bytes": [_int, _int, _i64, _i64, _i64, _i64],
+    "ghip_sdpa_window_bwd_workspace_bytes": [_int] + [_i64] * 9,
+    "ghip_sdpa_paged_workspace_bytes": [_int] + [_i64] * 6,
 }
 
 _lib = None

@@ -5,6 +5,8 @@ current HIP stream; every computation runs in libgomlx_hip.so.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -255,6 +257,194 @@ def scale_mask_softmax_ex(x: torch.Tensor, scale: float, causal: bool, mask=None
     call("ghip_scale_mask_softmax_rows_ex", dtype_code(x.dtype), x.data_ptr(), y.data_ptr(), B, H, Sq, Sk,
          float(scale), int(causal), _ptr(mask), mdt, ms, _stream(stream))
     return y
+
+
+def _launch(dev: torch.device, name: str, stream, *args):
+    """Calls entry point `name` with `dev` current, on `stream` (None: dev's current one)."""
+    if dev.index is not None and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            call(name, *args, _stream(stream))
+    else:
+        call(name, *args, _stream(stream))
+
+
+def _one_device(*ts) -> torch.device:
+    """The device that every tensor lies on."""
+    _check_dev(*ts)
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"gomlx_hip: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _like(what: str, t: torch.Tensor, shape, dtype):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {tuple(shape)} is needed")
+
+
+def _ints(what: str, t, n: int):
+    """A dense int32 [n] operand (None stays None)."""
+    if t is not None:
+        _like(what, t, (n,), torch.int32)
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{what}: must be contiguous")
+
+
+_I3 = ctypes.c_int64 * 3
+
+
+def _rows3(what: str, t: torch.Tensor):
+    """The strides of a tensor's first three axes; the last one must be contiguous."""
+    st = t.stride()
+    if st[3] != 1 and t.shape[3] != 1:
+        raise ValueError(f"{what}: the head dim must be contiguous")
+    return _I3(st[0], st[1], st[2])
+
+
+def _window_shapes(q, k, v, q_start, lens):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("sdpa_window: q [B, H, Sq, D] and k / v [B, Hkv, Sk, D] are needed")
+    B, H, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    _like("sdpa_window: k", k, (B, Hkv, Sk, D), q.dtype)
+    _like("sdpa_window: v", v, (B, Hkv, Sk, D), q.dtype)
+    _ints("sdpa_window: lens", lens, B)
+    return (B, H, Hkv, Sq, Sk, D), Sk - Sq if q_start is None else int(q_start)
+
+
+def sdpa_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
+                q_start=None, lens=None, with_lse: bool = False, out=None, lse=None, stream=None):
+    """Causal attention over the last `window` keys (0: all) and the first `sinks` ones:
+    q [B, H, Sq, D] at positions q_start.. (None: the last Sq of the Sk keys), k / v
+    [B, Hkv, Sk, D], any strides with a contiguous head dim; lens: int32 [B], the
+    sequences' lengths (queries past them: zeros).  Returns o [B, H, Sq, D], with_lse: (o,
+    lse [B, H, Sq] float32), what sdpa_window_grad takes.  Wraps ghip_sdpa_window_fwd."""
+    dev = _one_device(q, k, v, lens, out, lse)
+    dims, start = _window_shapes(q, k, v, q_start, lens)
+    B, H, _, Sq, _, D = dims
+    if out is None:
+        out = torch.empty((B, H, Sq, D), dtype=q.dtype, device=dev)
+    else:
+        _like("sdpa_window: out", out, (B, H, Sq, D), q.dtype)
+    if lse is not None:
+        _like("sdpa_window: lse", lse, (B, H, Sq), torch.float32)
+        if not lse.is_contiguous():
+            raise ValueError("sdpa_window: lse must be contiguous")
+    elif with_lse:
+        lse = torch.empty((B, H, Sq), dtype=torch.float32, device=dev)
+    _launch(dev, "ghip_sdpa_window_fwd", stream, dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            out.data_ptr(), _ptr(lse), *dims, _rows3("q", q), _rows3("k", k), _rows3("v", v), _rows3("out", out), start,
+            int(window), int(sinks), _ptr(lens), float(scale))
+    return (out, lse) if with_lse else out
+
+
+def sdpa_window_grad_workspace(q: torch.Tensor, k: torch.Tensor, window: int = 0, sinks: int = 0, q_start=None):
+    """Workspace for sdpa_window_grad at these sizes."""
+    B, H, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    n = _lib.load().ghip_sdpa_window_bwd_workspace_bytes(dtype_code(q.dtype), B, H, Hkv, Sq, Sk, D,
+                                                         Sk - Sq if q_start is None else int(q_start), int(window),
+                                                         int(sinks))
+    return torch.empty((n,), dtype=torch.uint8, device=q.device)
+
+
+def sdpa_window_grad(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                     lse: torch.Tensor, scale: float, window: int = 0, sinks: int = 0, q_start=None, lens=None,
+                     outs=None, workspace=None, stream=None):
+    """(dq, dk, dv) of sdpa_window from its inputs, its o and lse, and d_out, the gradient
+    of o.  outs: the three tensors to write.  Wraps ghip_sdpa_window_bwd."""
+    dev = _one_device(d_out, q, k, v, o, lse, lens, workspace, *(outs or ()))
+    dims, start = _window_shapes(q, k, v, q_start, lens)
+    B, H, Hkv, Sq, Sk, D = dims
+    _like("sdpa_window_grad: o", o, q.shape, q.dtype)
+    _like("sdpa_window_grad: d_out", d_out, q.shape, q.dtype)
+    _like("sdpa_window_grad: lse", lse, (B, H, Sq), torch.float32)
+    if not lse.is_contiguous():
+        raise ValueError("sdpa_window_grad: lse must be contiguous")
+    if outs is None:
+        dq = torch.empty((B, H, Sq, D), dtype=q.dtype, device=dev)
+        dk = torch.empty((B, Hkv, Sk, D), dtype=q.dtype, device=dev)
+        dv = torch.empty((B, Hkv, Sk, D), dtype=q.dtype, device=dev)
+    else:
+        dq, dk, dv = outs
+        _like("sdpa_window_grad: dq", dq, q.shape, q.dtype)
+        _like("sdpa_window_grad: dk", dk, k.shape, q.dtype)
+        _like("sdpa_window_grad: dv", dv, k.shape, q.dtype)
+    ws = sdpa_window_grad_workspace(q, k, window, sinks, q_start) if workspace is None else workspace
+    _launch(dev, "ghip_sdpa_window_bwd", stream, dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            o.data_ptr(), d_out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims,
+            _rows3("q", q), _rows3("k", k), _rows3("v", v), _rows3("o", o), _rows3("d_out", d_out), _rows3("dq", dq),
+            _rows3("dk", dk), _rows3("dv", dv), start, int(window), int(sinks), _ptr(lens), float(scale), ws.data_ptr(),
+            ws.numel() * ws.element_size())
+    return dq, dk, dv
+
+
+def _paged_cache(what, k_cache, v_cache, block_table, B):
+    """(num_pages, page_size, max_pages, table stride) of caches viewed as [page, Hkv, token, D]."""
+    if k_cache.dim() != 4:
+        raise ValueError(f"{what}: the caches are [pages, Hkv, page_size, D]")
+    _like(f"{what}: v_cache", v_cache, k_cache.shape, k_cache.dtype)
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B:
+        raise ValueError(f"{what}: block_table is int32 [{B}, pages of a sequence]")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError(f"{what}: a sequence's table entries must be contiguous")
+    return k_cache.shape[0], k_cache.shape[2], block_table.shape[1], block_table.stride(0)
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              block_table: torch.Tensor, starts: torch.Tensor, counts=None, stream=None):
+    """Writes k / v [B, Hkv, S, D] into the pages of k_cache / v_cache (viewed as [pages,
+    Hkv, page_size, D], any strides with a contiguous head dim) as tokens starts[b] + i, i <
+    counts[b] (None: S), of the sequences whose pages block_table [B, pages] names.  Wraps
+    ghip_kv_append."""
+    dev = _one_device(k, v, k_cache, v_cache, block_table, starts, counts)
+    B, Hkv, S, D = k.shape
+    _like("kv_append: v", v, k.shape, k.dtype)
+    pages, size, per, ts = _paged_cache("kv_append", k_cache, v_cache, block_table, B)
+    _like("kv_append: k_cache", k_cache, (pages, Hkv, size, D), k.dtype)
+    _ints("kv_append: starts", starts, B)
+    _ints("kv_append: counts", counts, B)
+    _launch(dev, "ghip_kv_append", stream, k.element_size(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), B, S, Hkv, D, pages, size, per, block_table.data_ptr(), ts, starts.data_ptr(),
+            _ptr(counts), _rows3("k", k), _rows3("v", v), _rows3("k_cache", k_cache), _rows3("v_cache", v_cache))
+
+
+def sdpa_paged_workspace(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor):
+    """Workspace for sdpa_paged at these sizes (None when the sequences never split)."""
+    B, H, D = q.shape
+    n = _lib.load().ghip_sdpa_paged_workspace_bytes(dtype_code(q.dtype), B, H, k_cache.shape[1], D, k_cache.shape[2],
+                                                    block_table.shape[1])
+    return torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
+
+
+def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+               lens: torch.Tensor, scale: float, window: int = 0, sinks: int = 0, out=None, stream=None,
+               split: bool = True, workspace=None):
+    """Attention of one new token a sequence, q [B, H, D] at position lens[b] - 1, over its
+    pages (as kv_append wrote them), under sdpa_window's window and sinks.  split: with a
+    workspace (`workspace`, or one allocated here), so the sequences' tokens are dealt out
+    over the card.  Wraps ghip_sdpa_paged."""
+    dev = _one_device(q, k_cache, v_cache, block_table, lens, out, workspace)
+    B, H, D = q.shape
+    pages, size, per, ts = _paged_cache("sdpa_paged", k_cache, v_cache, block_table, B)
+    Hkv = k_cache.shape[1]
+    _like("sdpa_paged: k_cache", k_cache, (pages, Hkv, size, D), q.dtype)
+    _ints("sdpa_paged: lens", lens, B)
+    if out is None:
+        out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+    else:
+        _like("sdpa_paged: out", out, (B, H, D), q.dtype)
+    for what, t in (("q", q), ("out", out)):
+        if t.stride(2) != 1 and D != 1:
+            raise ValueError(f"sdpa_paged: {what}'s head dim must be contiguous")
+    ws = (sdpa_paged_workspace(q, k_cache, block_table) if workspace is None else workspace) if split else None
+    _launch(dev, "ghip_sdpa_paged", stream, dtype_code(q.dtype), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), B, H, Hkv, D, pages, size, per, block_table.data_ptr(), ts, lens.data_ptr(),
+            _I3(q.stride(0), q.stride(1)), _rows3("k_cache", k_cache), _rows3("v_cache", v_cache),
+            _I3(out.stride(0), out.stride(1)), int(window), int(sinks), float(scale), _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size())
+    return out
 
 
 def gather_rows(table: torch.Tensor, ids: torch.Tensor, out=None, stream=None):

@@ -255,6 +255,95 @@ int ghip_sdpa_fwd_masked_ws(int dtype, const void* q, const void* k, const void*
                             int mask_dtype, const int64_t* mask_strides, float scale, int causal,
                             void* workspace, int64_t workspace_bytes, void* stream, GHipError* err);
 
+/* Causal attention over a sliding window with sinks (training's forward pass and
+ * prompts).  The queries are positions q_start .. q_start + Sq - 1 of Sk tokens; the one
+ * at position p of sequence b sees key j iff
+ *   j <= p,  j < lens[b],  and  (j > p - window  or  j < sinks),
+ * so `window` keys up to its own and the first `sinks` ones; window 0: no bound.
+ *   lse[b, h, i] = log sum_j exp(scale * q[b,h,i,:].k[b,hk,j,:])        (over those j)
+ *   o[b, h, i, :] = sum_j exp(scale * q.k_j - lse) v[b, hk, j, :],  hk = h / (H / Hkv)
+ * lens: int32 [B] on the device (clamped to [0, Sk]); NULL: Sk.  A query at or past its
+ * sequence's length is padding: o is 0 and lse -inf, and nothing that q, k or v hold at
+ * padding reaches another row.  A NaN or an infinity in a token inside the length may
+ * reach any row of its sequence.
+ * Operands by ELEMENT strides (batch, head, sequence) as in ghip_sdpa_fwd, any of them
+ * 0 or shared; BFLOAT16 or FLOAT16 with D a multiple of 8 up to 256, or FLOAT32 with a
+ * multiple of 4 up to 128; strides multiples of 16 bytes (o: 4 elements), rows at
+ * strides below 32 MiB, slices of any size.  lse [B, H, Sq] float32, dense, may be NULL.
+ * q_start + Sq <= Sk.  Sums and statistics are fp32; the weights are rounded to the
+ * operands' type for the product with v only.  No reference op: it stands beside
+ * FusedScaledDotProductAttention (function.go:2669-2907), whose mask operand reads
+ * Sq x Sk values and computes every key tile. */
+int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
+                         int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* o_strides, int64_t q_start, int64_t window, int64_t sinks,
+                         const int32_t* lens, float scale, void* stream, GHipError* err);
+
+/* Gradient of ghip_sdpa_window_fwd with respect to q, k and v, from its inputs, its o and
+ * lse, and the gradient d_out of o:
+ *   P = exp(scale q.k - lse),  dS = P (d_out.v - sum_d d_out o)
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T d_out
+ * dk and dv are summed over the H / Hkv query heads of a kv head.  Sizes, types, strides,
+ * lens and the mask as there; padding gets zero gradients (dk, dv for every key, dq for
+ * every query) and what d_out and o hold there is not used.  workspace: device memory of
+ * ghip_sdpa_window_bwd_workspace_bytes() bytes, 16-byte aligned, written on `stream`
+ * (calls that share one must be ordered).  Sums are fp32 and in a fixed order: the same
+ * bits every run.  No reference op (GoMLX differentiates the composite). */
+int64_t ghip_sdpa_window_bwd_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq,
+                                             int64_t Sk, int64_t D, int64_t q_start, int64_t window,
+                                             int64_t sinks);
+int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
+                         const void* d_out, const float* lse, void* dq, void* dk, void* dv,
+                         int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* o_strides, const int64_t* d_out_strides,
+                         const int64_t* dq_strides, const int64_t* dk_strides,
+                         const int64_t* dv_strides, int64_t q_start, int64_t window, int64_t sinks,
+                         const int32_t* lens, float scale, void* workspace, int64_t workspace_bytes,
+                         void* stream, GHipError* err);
+
+/* Key-value cache in pages.  k_cache / v_cache hold num_pages pages of page_size tokens,
+ * addressed by ELEMENT strides (page, kv head, token) with the head dim contiguous, so
+ * both [page, token, head, D] and [page, head, token, D] storage work.  Token j of sequence
+ * b lies in row j % page_size of page block_table[b * table_stride + j / page_size]
+ * (int32, max_pages entries a sequence; entries past a sequence's tokens are not used).
+ *
+ * ghip_kv_append writes new tokens: k / v [B, Hkv, S, D] (strides batch, head, token) become
+ * tokens starts[b] + i, i < min(S, counts[b]) (counts NULL: S), copied bit for bit; other
+ * rows of the cache stay as they are.  Tokens at a negative position, past max_pages or on
+ * a page outside [0, num_pages) are skipped.  Two tokens that land in one row race.
+ * Elements of 1, 2, 4 or 8 bytes, any alignment of whole elements. */
+int ghip_kv_append(int elem_bytes, const void* k, const void* v, void* k_cache, void* v_cache,
+                   int64_t B, int64_t S, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                   int64_t max_pages, const int32_t* block_table, int64_t table_stride,
+                   const int32_t* starts, const int32_t* counts, const int64_t* k_strides,
+                   const int64_t* v_strides, const int64_t* k_cache_strides,
+                   const int64_t* v_cache_strides, void* stream, GHipError* err);
+
+/* Decoding attention over the paged cache: the newest token of each sequence, at position
+ * lens[b] - 1 (its key and value already appended), under the window and sinks of
+ * ghip_sdpa_window_fwd: it sees token j iff j >= lens[b] - window or j < sinks.  q and o
+ * [B, H, D] (strides batch, head).  lens is clamped to [0, max_pages * page_size]; a sequence
+ * of length 0 gets zeros, and tokens on a page outside [0, num_pages) are not seen.  Rows
+ * of the cache that are not seen are never used, whatever they hold.  Types and head dims as
+ * ghip_sdpa_window_fwd; q and the caches 16-byte aligned with strides of whole 16
+ * bytes, o of whole 4 elements.
+ * With a workspace of ghip_sdpa_paged_workspace_bytes() bytes (16-byte aligned; its size
+ * does not depend on the lengths) the tiles of all sequences are dealt out evenly over the
+ * card and joined by log-sum-exp in a second kernel, in a fixed order; without one each
+ * (sequence, kv head) is one workgroup's.  0 bytes: the cache's sequences are too short to
+ * split.  Calls that share a workspace must be ordered (one stream).  No reference op: the
+ * reference's decoding reads dense caches. */
+int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                        int64_t page_size, int64_t max_pages);
+int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,
+                    int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                    int64_t max_pages, const int32_t* block_table, int64_t table_stride,
+                    const int32_t* lens, const int64_t* q_strides, const int64_t* k_strides,
+                    const int64_t* v_strides, const int64_t* o_strides, int64_t window, int64_t sinks,
+                    float scale, void* workspace, int64_t workspace_bytes, void* stream, GHipError* err);
+
 /* Embedding lookup: out[i, :] = table[clamp(ids[i], 0, V-1), :] (row_bytes per
  * row, copied bit-exactly).  Replaces the gather fast path
  * (gather.go:61-203 -> mpsgraph_gather_along_axis, bridge.m:764-782). */
