@@ -31,17 +31,17 @@ struct Params {
   int B, H, Hkv, D, num_pages, page_size, max_pages;
   int window, sinks;
   float scale;
-  float* part_o;    // [2 workers][heads of a unit][D]: shares of units that several workers hold
-  float* part_lse;  // [2 workers][heads of a unit]
+  int unit_heads;   // min(16, heads of a kv head)
+  float* part_o;    // [2 workers][unit_heads][D]: shares of units that several workers hold
+  float* part_lse;  // [2 workers][unit_heads]
 };
 
 // Heads of one kv head's group that a unit of work holds: the columns of a 16-wide MFMA.
 constexpr int kHeads = 16;
-constexpr int kWaves = 4;
-// One workgroup a CU with 128 KiB of LDS tiles, most of it in flight: the workers that
-// share the tiles of all sequences.
-constexpr int kWorkers = 256;
-constexpr int kMinTiles = 2 * kWaves;  // tiles of a worker at least
+// The workers that share the tiles of all sequences: one wave each, four a CU with 32 KiB
+// of LDS tiles, most of it in flight.
+constexpr int kWorkers = 1024;
+constexpr int kMinTiles = 2;  // tiles of a worker at least
 
 // 16 zero bytes: what lanes without a token load.
 __device__ const uint4 kZero[1] = {};
@@ -79,18 +79,22 @@ struct Seen {
 };
 
 // Where the tiles of the sequences lie in the common order (sequence, unit of heads,
-// tile): total, and for a place in it the sequence and the place where that begins.
+// tile).  A lane counts one sequence; scans over the wave give the places.
 template <int KT>
 struct Order {
   int64_t total = 0;
   int lane, units;
+  int64_t n0, up0;  // the first 64 sequences' tiles, and their running sums
   __device__ __forceinline__ Order(const Params& p, int units_) : lane(threadIdx.x & 63), units(units_) {
-    for (int b0 = 0; b0 < p.B; b0 += 64) total += sum(count(p, b0 + lane));
+    n0 = count(p, lane);
+    up0 = scan(n0);
+    total = __shfl(up0, 63, 64);
+    for (int b0 = 64; b0 < p.B; b0 += 64) total += __shfl(scan(count(p, b0 + lane)), 63, 64);
   }
   __device__ __forceinline__ int64_t count(const Params& p, int b) const {
     return b < p.B ? static_cast<int64_t>(Seen(p, p.lens[b]).tiles(KT)) * units : 0;
   }
-  __device__ __forceinline__ static int64_t scan(int64_t x, int lane) {
+  __device__ __forceinline__ int64_t scan(int64_t x) const {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int64_t y = __shfl_up(x, d, 64);
@@ -98,12 +102,11 @@ struct Order {
     }
     return x;
   }
-  __device__ __forceinline__ int64_t sum(int64_t x) const { return __shfl(scan(x, lane), 63, 64); }
   // The sequence that place `at` < total lies in; *begin: where it begins.
   __device__ __forceinline__ int find(const Params& p, int64_t at, int64_t* begin) const {
     int64_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      const int64_t n = count(p, b0 + lane), up = scan(n, lane) + before;
+    for (int b0 = 0;; b0 += 64) {
+      const int64_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? scan(n) + before : up0;
       const uint64_t over = __builtin_amdgcn_ballot_w64(up > at);
       if (over) {
         const int l = __builtin_ctzll(over);
@@ -112,20 +115,27 @@ struct Order {
       }
       before = __shfl(up, 63, 64);
     }
-    *begin = before;
-    return p.B;
   }
   // Where sequence b begins.
   __device__ __forceinline__ int64_t begin(const Params& p, int b) const {
     int64_t before = 0;
-    for (int b0 = 0; b0 < b; b0 += 64) before += sum(b0 + lane < b ? count(p, b0 + lane) : 0);
-    return before;
+    for (int b0 = 0;; b0 += 64) {
+      const int64_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? scan(n) + before : up0;
+      if (b < b0 + 64) return __shfl(up - n, b - b0, 64);
+      before = __shfl(up, 63, 64);
+    }
   }
   __device__ __forceinline__ int64_t share() const {
     const int64_t per = (total + kWorkers - 1) / kWorkers;
     return per < kMinTiles ? kMinTiles : per;
   }
 };
+
+// a / b of non-negative values, in 32 bits where they fit.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
 
 template <typename T> struct Op;
 template <> struct Op<float> {
@@ -169,14 +179,14 @@ template <> struct Op<f16_t> {
   }
 };
 
-// Every wave works alone on tiles of KT tokens: K and V rows come by per-lane DMA into
-// its own two LDS stages, page numbers one tile further ahead by the same path, so one
+// A wave works alone on tiles of KT tokens: K and V rows come by per-lane DMA into
+// two LDS stages, page numbers one tile further ahead by the same path, so one
 // in-order counter (vmcnt) tells what has landed.  S^T = K Q^T with 16 tokens x 16
 // heads a product and the softmaxed columns as the operand of O^T += V^T P^T, as in the
 // prompt kernels.  SPLIT: the tiles of all sequences are dealt out evenly, whatever the
 // lengths; a unit that several workers hold is joined by the second kernel.
 template <typename T, int DP, bool SPLIT>
-__global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
+__global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
   constexpr int kEs = static_cast<int>(sizeof(T));
   constexpr int kRow = DP * kEs, kCh = kRow / 16;
   constexpr int KT = 8192 / kRow;              // 64, 32 or 16 tokens: 8 KiB of K and of V
@@ -184,14 +194,12 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
   constexpr int kTile = 8192;
   using O = Op<T>;
   using F = typename tile::Frag<T>::type;
-  __shared__ __attribute__((aligned(1024))) char smem[kWaves][2][2][kTile];
-  __shared__ __attribute__((aligned(16))) int32_t page_lds[kWaves][2][64];
-  __shared__ float stat[kWaves][2][kHeads];
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
+  __shared__ __attribute__((aligned(16))) int32_t page_lds[2][64];
 
-  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x, g = lane >> 4, col = lane & 15;
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
-  const uint32_t la0 = tile::lds_addr(smem[wave]), pa0 = tile::lds_addr(page_lds[wave]);
+  const uint32_t la0 = tile::lds_addr(smem), pa0 = tile::lds_addr(page_lds);
   const float c = p.scale * 1.4426950408889634f;
 
   int b;
@@ -215,8 +223,8 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
     const int nt = seen.tiles(KT), nst = seen.sink_tiles(KT);
     int unit, ta, te;
     if constexpr (SPLIT) {
-      unit = static_cast<int>((at - begin) / nt);
-      ta = static_cast<int>((at - begin) % nt);
+      unit = static_cast<int>(quotient(at - begin, nt));
+      ta = static_cast<int>(at - begin - static_cast<int64_t>(unit) * nt);
       te = static_cast<int>(min(static_cast<int64_t>(nt), ta + (end - at)));
     } else {
       unit = blockIdx.x % units;
@@ -258,7 +266,7 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
     // The DMA of tile t, its page numbers landed; returns its rows that hold a token.
     auto issue = [&](int t, int slot) -> uint64_t {
       const int tok = token0(t) + (lane & (KT - 1));
-      const int page = page_lds[wave][slot][lane];
+      const int page = page_lds[slot][lane];
       const int off = tok % p.page_size;
       const bool ok = (t < nst ? tok < seen.ns : tok >= seen.lo && tok < seen.len) && page >= 0 && page < p.num_pages;
       const uint64_t rows = __builtin_amdgcn_ballot_w64(ok);
@@ -281,9 +289,9 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
     for (int db = 0; db < DP / 16; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    // This wave's tiles: ta + wave, + 4, ...; the order of its DMA is pages(j + 1), K and V(j).
-    const int n = max(0, (te - ta - wave + kWaves - 1) / kWaves);
-    auto tile_of = [&](int j) { return ta + wave + j * kWaves; };
+    // The order of the DMA is pages(j + 1), K and V(j).
+    const int n = te - ta;
+    auto tile_of = [&](int j) { return ta + j; };
     uint64_t rows0 = 0, rows1 = 0;  // of tiles j and j + 1
     if (n > 0) {
       issue_pages(tile_of(0), 0);
@@ -301,8 +309,8 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
       if (j + 2 < n) wait_vm<2 * kN + 1>();
       else if (j + 1 < n) wait_vm<2 * kN>();
       else wait_vm<0>();
-      const char* sk = smem[wave][j & 1][0];
-      const char* sv = smem[wave][j & 1][1];
+      const char* sk = smem[j & 1][0];
+      const char* sv = smem[j & 1][1];
       f32x4 x[KT / 16];
 #pragma unroll
       for (int i = 0; i < KT / 16; ++i) {
@@ -380,44 +388,25 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
       }
     }
 
-    // The waves' shares, joined through LDS (their stages are free now).
+    // o[db][v] is d = 16 db + 4 g + v of head col.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    float* mine = reinterpret_cast<float*>(smem[wave]);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no token seen: zeros
+    if (col < heads) {
+      if (ta == 0 && te == nt) {
+        T* out = static_cast<T*>(p.o) + b * p.o_sb + (h0 + col) * p.o_sh + 4 * g;
 #pragma unroll
-    for (int db = 0; db < DP / 16; ++db)
-      *reinterpret_cast<f32x4*>(mine + col * DP + 16 * db + 4 * g) = o[db];
-    if (g == 0) {
-      stat[wave][0][col] = m * c;
-      stat[wave][1][col] = l;
-    }
-    __syncthreads();
-    const bool whole = ta == 0 && te == nt;
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at == first ? 0 : 1);
-    for (int e = threadIdx.x; e < heads * (DP / 4); e += 256) {
-      const int hd = e / (DP / 4), d = e % (DP / 4) * 4;
-      float mm = -INFINITY;
+        for (int db = 0; db < DP / 16; ++db)
+          if (16 * db + 4 * g < p.D)
+            tile::store4(out + 16 * db, o[db][0] * inv, o[db][1] * inv, o[db][2] * inv, o[db][3] * inv);
+      } else {
+        const int64_t r = (2 * static_cast<int64_t>(blockIdx.x) + (at == first ? 0 : 1)) * p.unit_heads + col;
+        float* out = p.part_o + r * p.D + 4 * g;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, stat[w][0][hd]);
-      float a[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[w][0][hd] - mm);
-        sum += f * stat[w][1][hd];
-        const f32x4 ow = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + hd * DP + d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] += f * ow[i];
-      }
-      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-      if (d < p.D) {
-        if (whole) {
-          T* out = static_cast<T*>(p.o) + b * p.o_sb + (h0 + hd) * p.o_sh + d;
-          tile::store4(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-        } else {
-          const int64_t r = slot * kHeads + hd;
-          tile::store4(p.part_o + r * p.D + d, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-          if (d == 0) p.part_lse[r] = sum > 0.f || sum != sum ? mm + __builtin_amdgcn_logf(sum) : -INFINITY;
-        }
+        for (int db = 0; db < DP / 16; ++db)
+          if (16 * db + 4 * g < p.D)
+            tile::store4(out + 16 * db, o[db][0] * inv, o[db][1] * inv, o[db][2] * inv, o[db][3] * inv);
+        if (g == 0) p.part_lse[r] = l > 0.f || l != l ? m * c + __builtin_amdgcn_logf(l) : -INFINITY;
       }
     }
     if constexpr (!SPLIT) {
@@ -426,63 +415,96 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Params p) {
       at += te - ta;
       if (at >= end) return;
       if (at - begin >= static_cast<int64_t>(nt) * units) b = order.find(p, at, &begin);
-      __syncthreads();
     }
   }
 }
 
-// Joins the shares of units that several workers hold, in the workers' order: a wave a
-// (sequence, head).  Sequences without a visible token, which no worker holds, get zeros.
+// Joins the shares of units that several workers hold: a workgroup a (sequence, head),
+// the shares dealt out over groups of lanes that each hold a row of the output, their
+// sums added in the groups' order.  Sequences without a visible token, which no worker
+// holds, get zeros.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int KT = 8192 / (DP * static_cast<int>(sizeof(T)));
+  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes;
+  __shared__ float weight[kWorkers];
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) float sums[kGroups][DP];
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= p.B * p.H) return;
-  const int b = row / p.H, h = row % p.H, hk = h / G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x, b = row / p.H, h = row % p.H, hk = h / G;
   const int unit = hk * blocks + (h - hk * G) / kHeads, hd = (h - hk * G) % kHeads;
+  const int d = threadIdx.x % kLanes * 4, grp = threadIdx.x / kLanes;
+  T* out = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + d;
   const Order<KT> order(p, units);
   const int nt = Seen(p, p.lens[b]).tiles(KT);
-  const int64_t per = order.share(), u0 = order.begin(p, b) + static_cast<int64_t>(unit) * nt;
-  const int d = lane * 4;
-  T* out = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + d;
   if (nt == 0) {
-    if (d < p.D) tile::store4(out, 0.f, 0.f, 0.f, 0.f);
+    if (grp == 0 && d < p.D) tile::store4(out, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  const int64_t w0 = u0 / per, w1 = (u0 + nt - 1) / per;
-  if (w0 == w1) return;
-  auto slot = [&](int64_t w) { return (2 * w + (w == w0 && u0 != w0 * per ? 1 : 0)) * kHeads + hd; };
+  const int64_t per = order.share(), u0 = order.begin(p, b) + static_cast<int64_t>(unit) * nt;
+  const int w0 = static_cast<int>(quotient(u0, per)), n = static_cast<int>(quotient(u0 + nt - 1, per)) - w0 + 1;
+  if (n == 1) return;
+  // The unit's share in worker w0 + i: its first piece, but for a worker that began before.
+  auto slot = [&](int i) {
+    return (2 * static_cast<int64_t>(w0 + i) + (i == 0 && u0 != w0 * per ? 1 : 0)) * p.unit_heads + hd;
+  };
   float mx = -INFINITY;
-  for (int64_t w = w0; w <= w1; ++w) mx = fmaxf(mx, p.part_lse[slot(w)]);
-  float a[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int64_t w = w0; w <= w1; ++w) {
-    const float ls = p.part_lse[slot(w)];
-    const float f = ls == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls - mx);
-    sum += f;
-    if (d < p.D) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(w) * p.D + d);
+  for (int i = threadIdx.x; i < n; i += 256) {
+    weight[i] = p.part_lse[slot(i)];
+    mx = fmaxf(mx, weight[i]);
+  }
+  mx = wave_max(mx);
+  if (lane == 0) red[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float ls = weight[i];
+    weight[i] = ls == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls - mx);  // (NaN stays NaN)
+    sum += weight[i];
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  sum = (red[0] + red[1]) + (red[2] + red[3]);
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (d < p.D) {
+#pragma unroll 4
+    for (int i = grp; i < n; i += kGroups) {
+      const float f = weight[i];
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(i) * p.D + d);
       a[0] += f * v.x;
       a[1] += f * v.y;
       a[2] += f * v.z;
       a[3] += f * v.w;
     }
+    *reinterpret_cast<float4*>(&sums[grp][d]) = make_float4(a[0], a[1], a[2], a[3]);
   }
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  if (d < p.D) tile::store4(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+  __syncthreads();
+  if (grp == 0 && d < p.D) {
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(&sums[i][d]);
+      a[0] += v.x;
+      a[1] += v.y;
+      a[2] += v.z;
+      a[3] += v.w;
+    }
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    tile::store4(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+  }
 }
 
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
   const int G = p.H / p.Hkv, units = p.Hkv * ((G + kHeads - 1) / kHeads);
   if (p.part_o) {
-    hipLaunchKernelGGL((attend_kernel<T, DP, true>), dim3(kWorkers), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((join_kernel<T, DP>), dim3(static_cast<unsigned>((static_cast<int64_t>(p.B) * p.H + 3) / 4)),
-                       dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attend_kernel<T, DP, true>), dim3(kWorkers), dim3(64), 0, s, p);
+    hipLaunchKernelGGL((join_kernel<T, DP>), dim3(static_cast<unsigned>(p.B * p.H)), dim3(256), 0, s, p);
   } else {
-    hipLaunchKernelGGL((attend_kernel<T, DP, false>), dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * units)),
-                       dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attend_kernel<T, DP, false>), dim3(static_cast<unsigned>(p.B * units)), dim3(64), 0, s, p);
   }
 }
 template <typename T>
@@ -537,8 +559,8 @@ using namespace ghip;
 
 extern "C" int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                    int64_t page_size, int64_t max_pages) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || max_pages <= 0) return 0;
-  return 2 * static_cast<int64_t>(paged::kWorkers) * paged::kHeads * (D + 1) * 4;
+  if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || page_size <= 0 || max_pages <= 0) return 0;
+  return 2 * static_cast<int64_t>(paged::kWorkers) * std::min<int64_t>(paged::kHeads, H / Hkv) * (D + 1) * 4;
 }
 
 extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o, int64_t B,
@@ -596,6 +618,7 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
   p.window = static_cast<int>(window == 0 || window > kMost ? kMost : window);
   p.sinks = static_cast<int>(sinks > kMost ? kMost : sinks);
   p.scale = scale;
+  p.unit_heads = static_cast<int>(std::min<int64_t>(paged::kHeads, H / Hkv));
   if (workspace) {
     const int64_t need = ghip_sdpa_paged_workspace_bytes(dtype, B, H, Hkv, D, page_size, max_pages);
     if (workspace_bytes < need)
@@ -603,7 +626,7 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
                        static_cast<long long>(workspace_bytes), static_cast<long long>(need));
     if (!al(workspace, 16)) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", kWhat);
     p.part_o = static_cast<float*>(workspace);
-    p.part_lse = p.part_o + 2 * static_cast<int64_t>(paged::kWorkers) * paged::kHeads * D;
+    p.part_lse = p.part_o + 2 * static_cast<int64_t>(paged::kWorkers) * p.unit_heads * D;
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (f32) paged::launch<float>(p, s);

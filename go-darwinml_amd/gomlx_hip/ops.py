@@ -261,25 +261,27 @@ def scale_mask_softmax_ex(x: torch.Tensor, scale: float, causal: bool, mask=None
 
 def _launch(dev: torch.device, name: str, stream, *args):
     """Calls entry point `name` with `dev` current, on `stream` (None: dev's current one)."""
-    if dev.index is not None and dev.index != torch.cuda.current_device():
+    if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             call(name, *args, _stream(stream))
     else:
-        call(name, *args, _stream(stream))
+        # The current stream's handle alone: a torch.cuda.Stream object costs 3 us.
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else int(stream))
 
 
-def _one_device(*ts) -> torch.device:
+def _one_device(first: torch.Tensor, *ts) -> torch.device:
     """The device that every tensor lies on."""
-    _check_dev(*ts)
-    dev = ts[0].device
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("gomlx_hip ops take device tensors")
     for t in ts:
         if t is not None and t.device != dev:
-            raise ValueError(f"gomlx_hip: tensors on {dev} and {t.device}")
+            raise ValueError(f"gomlx_hip: tensors on device {dev} and {t.device}")
     return dev
 
 
 def _like(what: str, t: torch.Tensor, shape, dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {tuple(shape)} is needed")
 
 
