@@ -94,28 +94,28 @@ struct Tile {
   static constexpr int kCh = kRow / 16;      // 16-byte chunks of a row
   using F = typename Frag<T>::type;
 
-  // Values 16 s + 8 h .. + 8 of row r (A operand whose rows are the tile's rows).
-  __device__ __forceinline__ static F frag_row(const char* lds, int r, int s, int h) {
+  // Values 16 s + 8 h .. + 8 of row lane % 32 of the 32 rows at `lds` (A operand whose
+  // rows are the tile's rows); `lds` at a multiple of 16 rows.
+  __device__ __forceinline__ static F frag_row(const char* lds, int s, int lane) {
+    const int r = lane & 31, h = lane >> 5, f = swz<kCh>(r);
     if constexpr (kEs == 2) {
-      return *reinterpret_cast<const F*>(lds + r * kRow + (((2 * s + h) ^ swz<kCh>(r)) << 4));
+      return *reinterpret_cast<const F*>(lds + (r * kRow + (((2 * s + h) ^ f) << 4)));
     } else {
-      const int f = swz<kCh>(r);
-      const float4 lo = *reinterpret_cast<const float4*>(lds + r * kRow + (((4 * s + 2 * h) ^ f) << 4));
-      const float4 hi = *reinterpret_cast<const float4*>(lds + r * kRow + (((4 * s + 2 * h + 1) ^ f) << 4));
+      const float4 lo = *reinterpret_cast<const float4*>(lds + (r * kRow + (((4 * s + 2 * h) ^ f) << 4)));
+      const float4 hi = *reinterpret_cast<const float4*>(lds + (r * kRow + (((4 * s + 2 * h + 1) ^ f) << 4)));
       return F{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     }
   }
-  // Column 32 db + lane % 32 of rows r0 + 16 s + 4 h + {0..3} and r0 + 16 s + 8 + 4 h +
-  // {0..3} (A operand of the transposed tile; r0 a multiple of 16).  16-bit:
-  // ds_read_b64_tr_b16 hands lane j of each 16-lane group element j of the four
-  // 4-element rows that the group points at.
-  __device__ __forceinline__ static F frag_tr(const char* lds, int db, int r0, int s, int lane) {
+  // Column 32 db + lane % 32 of rows 4 h + {0..3} and 8 + 4 h + {0..3} of the 16 rows at
+  // `lds` (A operand of the transposed tile).  16-bit: ds_read_b64_tr_b16 hands lane j of
+  // each 16-lane group element j of the four 4-element rows that the group points at.
+  __device__ __forceinline__ static F frag_tr(const char* lds, int db, int lane) {
     const int h = lane >> 5;
     if constexpr (kEs == 2) {
-      const int r = r0 + 16 * s + 4 * h + ((lane & 15) >> 2);
+      const int r = 4 * h + ((lane & 15) >> 2);
       const int col = db * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const char* p0 = lds + r * kRow + (((col >> 3) ^ swz<kCh>(r)) << 4) + (col & 7) * 2;
-      const char* p1 = lds + (r + 8) * kRow + (((col >> 3) ^ swz<kCh>(r + 8)) << 4) + (col & 7) * 2;
+      const char* p0 = lds + (r * kRow + (((col >> 3) ^ swz<kCh>(r)) << 4) + (col & 7) * 2);
+      const char* p1 = lds + (r * kRow + (((col >> 3) ^ swz<kCh>(r + 8)) << 4) + (col & 7) * 2) + 8 * kRow;
       const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((GHIP_LDS bf16x4*)(p0));
       const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((GHIP_LDS bf16x4*)(p1));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -124,8 +124,8 @@ struct Tile {
       const int col = db * 32 + (lane & 31);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int row = r0 + 16 * s + 8 * (e >> 2) + 4 * h + (e & 3);
-        r[e] = *reinterpret_cast<const float*>(lds + row * kRow + (((col >> 2) ^ swz<kCh>(row)) << 4) + (col & 3) * 4);
+        const int row = 8 * (e >> 2) + 4 * h + (e & 3);
+        r[e] = *reinterpret_cast<const float*>(lds + (row * kRow + (((col >> 2) ^ swz<kCh>(row)) << 4) + (col & 3) * 4));
       }
       return r;
     }

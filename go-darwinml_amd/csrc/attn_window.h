@@ -15,6 +15,10 @@ struct Params {
   Mat3 q, k, v, o, dout, dq, dk, dv;
   float* lse;        // [B, H, Sq]; forward: written (may be null), gradient: read
   float* ndelta;     // gradient: minus the row sums of do * o, [B, H, Sq]
+  float* far;        // gradient: shares of the sinks' sums, [B, Hkv, far_blocks][far_shares][dk, dv][32][D]
+  int64_t far_stride;                   // floats of one block's shares
+  int far_blocks, far_chunks, far_per;  // blocks of 32 sinks (0: no shares), chunks a block, tiles a chunk
+  int far_shares;
   const int32_t* lens;
   int B, H, Hkv, Sq, Sk, D;
   int q_start, window, sinks;
@@ -51,6 +55,19 @@ struct Tiles {
   }
   __device__ __forceinline__ int operator()(int i) const { return i < ns ? i : first + i - ns; }
 };
+
+// Bits [0, n) of a word, n clamped to 0 .. 32.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+// Which of keys key0 + kv, kv < 32, the query at position pos sees, as bits (none unless live).
+__device__ __forceinline__ uint32_t seen_keys(const Params& p, int pos, bool live, int len, int key0) {
+  if (!live) return 0u;
+  return low_bits(min(len, pos + 1) - key0) & (~low_bits(pos - p.window + 1 - key0) | low_bits(p.sinks - key0));
+}
+// x where bit `bit` of word is set, otherwise `other` (two instructions an element).
+__device__ __forceinline__ float select_bit(uint32_t word, int bit, float x, float other) {
+  const uint32_t t = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(word), bit, 1));
+  return __uint_as_float((t & __float_as_uint(x)) | (~t & __float_as_uint(other)));
+}
 
 // The problem's sizes and types; fills p.  Returns GHIP_OK or the error.
 int check_problem(const char* what, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,

@@ -5,6 +5,8 @@
 // scores never reach memory.  No reference op: this stands beside the causal attention
 // of FusedScaledDotProductAttention (mpsgraph/gomlx/function.go:2669-2907), whose mask
 // operand would cost Sq x Sk values and every key tile.
+#include <type_traits>
+
 #include "attn_window.h"
 
 namespace ghip {
@@ -63,30 +65,31 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * 1.4426950408889634f;
 
-  if (tl.n > 0) issue(0);
-  for (int i = 0; i < tl.n; ++i) {
+  // Tile i from stage ST (known when compiled: LDS addresses are a lane's constants plus
+  // immediate offsets).
+  auto step = [&](auto st, int i) {
+    constexpr int ST = decltype(st)::value;
     tile::landed_barrier();  // tile i is there, and nobody reads the other stage any more
     if (i + 1 < tl.n) issue(i + 1);
     const int key0 = tl(i) * kKT;
     // The wave's queries pw .. pw + 31 see nothing of this tile.
-    if (key0 > pw + kQW - 1 || (key0 + kKT - 1 <= pw - p.window && key0 >= p.sinks)) continue;
-    const char* sk = smem[i & 1][0];
-    const char* sv = smem[i & 1][1];
+    if (key0 > pw + kQW - 1 || (key0 + kKT - 1 <= pw - p.window && key0 >= p.sinks)) return;
+    const char* sk = smem[ST][0];
+    const char* sv = smem[ST][1];
     f32x16 s0 = tile::splat(0.f), s1 = s0;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
-      s0 = tile::mma<T>(Tl::frag_row(sk, lane & 31, s, h2), qf[s], s0);
-      s1 = tile::mma<T>(Tl::frag_row(sk, 32 + (lane & 31), s, h2), qf[s], s1);
+      s0 = tile::mma<T>(Tl::frag_row(sk, s, lane), qf[s], s0);
+      s1 = tile::mma<T>(Tl::frag_row(sk + 32 * Tl::kRow, s, lane), qf[s], s1);
     }
     // s{kb}[v] is key key0 + 32 kb + 4 h2 + kv, kv = 8 (v / 4) + v % 4.
     if (key0 + kKT - 1 > pw || key0 + kKT > len || key0 <= pw + kQW - 1 - p.window) {
-      const int base = key0 + 4 * h2;
-      const int hi = (live ? min(len, pos + 1) : 0) - base, lo = pos - p.window + 1 - base, sn = p.sinks - base;
+      const uint32_t w0 = seen_keys(p, pos, live, len, key0 + 4 * h2), w1 = seen_keys(p, pos, live, len, key0 + 32 + 4 * h2);
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int kv = (v >> 2) * 8 + (v & 3);
-        s0[v] = kv < hi && (kv >= lo || kv < sn) ? s0[v] : -INFINITY;
-        s1[v] = kv + 32 < hi && (kv + 32 >= lo || kv + 32 < sn) ? s1[v] : -INFINITY;
+        s0[v] = select_bit(w0, kv, s0[v], -INFINITY);
+        s1[v] = select_bit(w1, kv, s1[v], -INFINITY);
       }
     }
     // The first maximum is the compiler's, which waits for the products' last results;
@@ -120,8 +123,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
     for (int s = 0; s < 4; ++s) {
       const F pf = s < 2 ? tile::pack<T>(s0, s) : tile::pack<T>(s1, s - 2);
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) o[db] = tile::mma<T>(Tl::frag_tr(sv, db, 0, s, lane), pf, o[db]);
+      for (int db = 0; db < DP / 32; ++db)
+        o[db] = tile::mma<T>(Tl::frag_tr(sv + 16 * s * Tl::kRow, db, lane), pf, o[db]);
     }
+  };
+  if (tl.n > 0) issue(0);
+  for (int i = 0; i < tl.n; i += 2) {
+    step(std::integral_constant<int, 0>{}, i);
+    if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 

@@ -6,6 +6,9 @@
 // evaluate P and dS again, so nothing of size Sq x Sk is stored and no sum depends on
 // the order of atomics: the first owns queries (dQ, and delta for the second), the
 // second keys.
+#include <algorithm>
+#include <type_traits>
+
 #include "attn_window.h"
 
 namespace ghip {
@@ -13,7 +16,7 @@ namespace win {
 
 using tile::f32x16;
 
-constexpr int kWaves = 4, kRW = 32, kBR = kWaves * kRW, kKT = 64, kQT = 64;
+constexpr int kCols = 128;  // queries (dq_kernel) or keys (dkv_kernel) of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 
 // dQ: the transposed arrangement of the forward kernel.  A lane owns one query; S^T = K
@@ -22,22 +25,22 @@ constexpr float kLog2e = 1.4426950408889634f;
 // exponent (P scale = 2^(s c - lse2 + log2 scale)), so an element costs one FMA, one
 // exponential and one multiplication.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void dq_kernel(Params p) {
+__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel(Params p) {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
-  constexpr int kTile = kKT * Tl::kRow;
+  constexpr int kT = 64, kTile = kT * Tl::kRow, kQW = 32;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
   const uint32_t lds0 = tile::lds_addr(smem);
 
   const int lane = threadIdx.x & 63, h2 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nqb = (p.Sq + kBR - 1) / kBR;
+  const int nqb = (p.Sq + kCols - 1) / kCols;
   const int nbh = p.B * p.H;
   const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
   const int bh = blockIdx.x % nbh;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
   const int len = length_of(p, b);
-  const int q0 = qb * kBR, qw = q0 + wave * kRW, qi = qw + (lane & 31);
+  const int q0 = qb * kCols, qw = q0 + wave * kQW, qi = qw + (lane & 31);
   const int pos = p.q_start + qi, pw = p.q_start + qw;
   const bool live = qi < p.Sq && pos < len;
 
@@ -63,14 +66,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void dq_kernel(P
   const float nl = live ? __builtin_amdgcn_logf(p.scale) - p.lse[row] * kLog2e : 0.f;
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, len, p.D), V = rows_of<T>(p.v, b, hk, len, p.D);
-  tile::Loader<T, DP, kKT, kWaves> lk, lv;
+  tile::Loader<T, DP, kT, 4> lk, lv;
   lk.init(K.step, p.D, wave, lane);
   lv.init(V.step, p.D, wave, lane);
   const int p0 = p.q_start + q0;
-  const Tiles<kKT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kBR, p.Sq)) : 0);
+  const Tiles<kT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kCols, p.Sq)) : 0);
   auto issue = [&](int i) {
     const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    const int64_t r = static_cast<int64_t>(tl(i)) * kKT;
+    const int64_t r = static_cast<int64_t>(tl(i)) * kT;
     lk.issue(K, r, la, wave);
     lv.issue(V, r, la + kTile, wave);
   };
@@ -79,41 +82,43 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void dq_kernel(P
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) dq[db] = tile::splat(0.f);
 
-  if (tl.n > 0) issue(0);
-  for (int i = 0; i < tl.n; ++i) {
+  // Tile i from stage ST, known when compiled.
+  auto step = [&](auto st, int i) {
+    constexpr int ST = decltype(st)::value;
     tile::landed_barrier();
     if (i + 1 < tl.n) issue(i + 1);
-    const int key0 = tl(i) * kKT;
-    if (key0 > pw + kRW - 1 || (key0 + kKT - 1 <= pw - p.window && key0 >= p.sinks)) continue;
-    const char* sk = smem[i & 1][0];
-    const char* sv = smem[i & 1][1];
-    const bool masked = key0 + kKT - 1 > pw || key0 + kKT > len || key0 <= pw + kRW - 1 - p.window;
 #pragma unroll
-    for (int kb = 0; kb < kKT / 32; ++kb) {
+    for (int kb = 0; kb < kT / 32; ++kb) {
+      const int key0 = tl(i) * kT + 32 * kb;
+      if (key0 > pw + kQW - 1 || key0 >= len || (key0 + 31 <= pw - p.window && key0 >= p.sinks)) continue;
+      const char* sk = smem[ST][0] + 32 * kb * Tl::kRow;
+      const char* sv = smem[ST][1] + 32 * kb * Tl::kRow;
       f32x16 x = tile::splat(0.f), g = tile::splat(nd);
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
-        x = tile::mma<T>(Tl::frag_row(sk, 32 * kb + (lane & 31), s, h2), qf[s], x);
-        g = tile::mma<T>(Tl::frag_row(sv, 32 * kb + (lane & 31), s, h2), gf[s], g);
+        x = tile::mma<T>(Tl::frag_row(sk, s, lane), qf[s], x);
+        g = tile::mma<T>(Tl::frag_row(sv, s, lane), gf[s], g);
       }
 #pragma unroll
       for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nl)) * g[v];
-      if (masked) {
-        const int base = key0 + 32 * kb + 4 * h2;
-        const int hi = (live ? min(len, pos + 1) : 0) - base, lo = pos - p.window + 1 - base, sn = p.sinks - base;
+      if (key0 + 31 > pw || key0 + 32 > len || key0 <= pw + kQW - 1 - p.window) {
+        const uint32_t w = seen_keys(p, pos, live, len, key0 + 4 * h2);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int kv = (v >> 2) * 8 + (v & 3);
-          x[v] = kv < hi && (kv >= lo || kv < sn) ? x[v] : 0.f;
-        }
+        for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], 0.f);
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const F df = tile::pack<T>(x, s);
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) dq[db] = tile::mma<T>(Tl::frag_tr(sk, db, 32 * kb, s, lane), df, dq[db]);
+        for (int db = 0; db < DP / 32; ++db)
+          dq[db] = tile::mma<T>(Tl::frag_tr(sk + 16 * s * Tl::kRow, db, lane), df, dq[db]);
       }
     }
+  };
+  if (tl.n > 0) issue(0);
+  for (int i = 0; i < tl.n; i += 2) {
+    step(std::integral_constant<int, 0>{}, i);
+    if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
   }
   if (qi >= p.Sq) return;
   T* out = at<T>(p.dq, b, h) + static_cast<int64_t>(qi) * p.dq.ss;
@@ -130,151 +135,303 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void dq_kernel(P
     }
 }
 
-// dK, dV: a lane owns one key; S = Q K^T and dP = dO V^T come out with the lane's key
-// as their column, so P and dS enter dV^T += dO^T P and dK^T += Q^T dS from the
-// registers.  K and V stay in registers; Q and dO stream through two LDS stages, head
-// after head of the group, with each query's log-sum-exp and delta beside them.
+// dK, dV: a lane owns one key; S = Q K^T and dP = dO V^T come out with the lane's key as
+// their column, so P and dS enter dV^T += dO^T P and dK^T += Q^T dS from the registers.
+// Two waves share 32 keys, half of the registers each (K, V and both sums in one wave
+// left one wave a SIMD, which stood waiting 55% of its time): the first holds K and
+// the sum dV, and hands P over through LDS in fp32; the second holds V and the sum dK.
+// Q and dO stream through two LDS stages, head after head of the group, with each query's
+// log-sum-exp and delta beside them.
+//
+// Every query sees the sinks, so their keys' sums run over the whole sequence, not over a
+// window.  Where that matters (plan_far) the queries behind the window of the sinks' block
+// are left to workgroups of their own, which deal them out in chunks and hold 32 sinks
+// each, every pair of waves another 32 rows of a tile; their fp32 sums and the block's
+// own are added by join_kernel in a fixed order.
+//
 // f16 only: P is at most 1 and of order 1 / window, so it is rounded 2^8 times larger
 // (small weights would be subnormal), and dS is rounded with the scale applied.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(Params p) {
+struct Keys {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
-  constexpr bool kF16 = __is_same(T, f16_t);
-  constexpr int kTile = kQT * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][kQT];  // -lse in base 2, -delta
-  const uint32_t lds0 = tile::lds_addr(smem);
-
-  const int lane = threadIdx.x & 63, h2 = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nbh = p.B * p.Hkv;
-  const int kb = blockIdx.x / nbh;  // the sinks' block, which every query sees, first
-  const int b = blockIdx.x % nbh / p.Hkv, hk = blockIdx.x % p.Hkv;
-  const int G = p.H / p.Hkv;
-  const int len = length_of(p, b);
-  const int k0 = kb * kBR, kw = k0 + wave * kRW, key = kw + (lane & 31);
-  const bool live = key < len;
-
-  F kf[DP / 16], vf[DP / 16];
-  {
-    const T* K = at<T>(p.k, b, hk) + static_cast<int64_t>(key) * p.k.ss;
-    const T* V = at<T>(p.v, b, hk) + static_cast<int64_t>(key) * p.v.ss;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      kf[s] = Tl::frag_global(K, s, h2, p.D, live);
-      vf[s] = Tl::frag_global(V, s, h2, p.D, live);
-    }
-  }
-  // Queries qa .. qe - 1 see a key of the block.
-  const int nq = max(0, min(p.Sq, len - p.q_start));  // queries that exist
-  const int reach = k0 < p.sinks || k0 + kBR - 1 + p.window > p.q_start + p.Sq ? nq
-                    : min(nq, max(0, k0 + kBR - 1 + p.window - p.q_start));
-  const int ta = max(0, k0 - p.q_start) / kQT;
-  const int nt = max(0, (k0 < len ? (reach + kQT - 1) / kQT : 0) - ta);
-  const int n = nt * G;
-
-  tile::Loader<T, DP, kQT, kWaves> lq, lg;
-  lq.init(p.q.ss * Tl::kEs, p.D, wave, lane);
-  lg.init(p.dout.ss * Tl::kEs, p.D, wave, lane);
-  const float c = p.scale * kLog2e;
-  float st = 0.f;  // this thread's entry of the next tile's statistics
-  auto issue = [&](int i) {
-    const int h = hk * G + i / nt, t = ta + i % nt;
-    const int r = t * kQT + (threadIdx.x & (kQT - 1));
-    st = 0.f;
-    if (threadIdx.x < 2 * kQT && r < nq) {
-      const int64_t at_row = (static_cast<int64_t>(b) * p.H + h) * p.Sq + r;
-      st = threadIdx.x < kQT ? (kF16 ? 8.f : 0.f) - p.lse[at_row] * kLog2e : p.ndelta[at_row];
-    }
-    const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    lq.issue(rows_of<T>(p.q, b, h, nq, p.D), static_cast<int64_t>(t) * kQT, la, wave);
-    lg.issue(rows_of<T>(p.dout, b, h, nq, p.D), static_cast<int64_t>(t) * kQT, la + kTile, wave);
+  static constexpr bool kF16 = __is_same(T, f16_t);
+  static constexpr int kPairs = kCols / 32, kNW = 2 * kPairs;
+  static constexpr int kT = Tl::kRow > 256 ? 32 : 64;  // rows of a tile
+  static constexpr int kTile = kT * Tl::kRow;
+  struct Lds {
+    __attribute__((aligned(1024))) char tiles[2][2][kTile];      // [stage][Q, dO]
+    __attribute__((aligned(16))) float p[kPairs][kT / 32][4][64][4];  // P of a pair's keys, in accumulator order
+    __attribute__((aligned(16))) float stat[2][2][kT];           // [stage][-log-sum-exp in base 2, -delta]
   };
-  auto put = [&](int i) {
-    if (threadIdx.x < 2 * kQT) stat[i & 1][threadIdx.x / kQT][threadIdx.x % kQT] = st;
+  // What a workgroup works on: tiles tbase .. tbase + tcount - 1 of each head of the group
+  // as one list, its entries i0 .. i1 - 1; keys from kfirst on.
+  struct Work {
+    int b, hk, kfirst, tbase, tcount, i0, i1, nq;
+    float* part;
   };
 
-  f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = tile::splat(0.f);
+  // ROLE 0: P and dV; 1: dS and dK.
+  template <int ROLE, bool FAR>
+  __device__ __forceinline__ static void run(const Params& p, Lds& lds, const Work& w) {
+    const uint32_t lds0 = tile::lds_addr(lds.tiles);
+    const int lane = threadIdx.x & 63, h2 = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % kPairs;
+    const int len = length_of(p, w.b);
+    const int kw = FAR ? w.kfirst : w.kfirst + pair * 32, key = kw + (lane & 31);
+    const int G = p.H / p.Hkv;
+    const float c = p.scale * kLog2e;
 
-  if (n > 0) {
-    issue(0);
-    put(0);
-  }
-  for (int i = 0; i < n; ++i) {
-    tile::landed_barrier();
-    if (i + 1 < n) issue(i + 1);
-    const char* sq = smem[i & 1][0];
-    const char* sg = smem[i & 1][1];
+    F kf[DP / 16];  // K (ROLE 0) or V
+    {
+      const Mat3& m = ROLE == 0 ? p.k : p.v;
+      const T* K = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
 #pragma unroll
-    for (int rb = 0; rb < kQT / 32; ++rb) {
-      const int p0 = p.q_start + (ta + i % nt) * kQT + 32 * rb;  // the first row's position
-      if (p0 + 31 < kw || (p0 >= kw + 31 + p.window && kw >= p.sinks) || p0 - p.q_start >= nq) continue;
-      f32x16 x = tile::splat(0.f), g;
-      const float* nl = &stat[i & 1][0][32 * rb + 4 * h2];
-      const float* nd = &stat[i & 1][1][32 * rb + 4 * h2];
-#pragma unroll
-      for (int v = 0; v < 16; ++v) g[v] = nd[(v >> 2) * 8 + (v & 3)];
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        x = tile::mma<T>(Tl::frag_row(sq, 32 * rb + (lane & 31), s, h2), kf[s], x);
-        g = tile::mma<T>(Tl::frag_row(sg, 32 * rb + (lane & 31), s, h2), vf[s], g);
+      for (int s = 0; s < DP / 16; ++s) kf[s] = Tl::frag_global(K, s, h2, p.D, key < len);
+    }
+    tile::Loader<T, DP, kT, kNW> lq, lg;
+    lq.init(p.q.ss * Tl::kEs, p.D, wave, lane);
+    lg.init(p.dout.ss * Tl::kEs, p.D, wave, lane);
+    float st = 0.f;  // this thread's entry of the next tile's statistics
+    int hn = w.hk * G + w.i0 / max(w.tcount, 1), tn = w.tbase + w.i0 % max(w.tcount, 1);  // what issue() loads next
+    int tc = tn;                                                                          // the tile worked on
+    auto issue = [&](int stage) {
+      const int r = tn * kT + static_cast<int>(threadIdx.x % kT);
+      st = 0.f;
+      if (threadIdx.x < 2 * kT && r < w.nq) {
+        const int64_t row = (static_cast<int64_t>(w.b) * p.H + hn) * p.Sq + r;
+        st = threadIdx.x < kT ? (kF16 ? 8.f : 0.f) - p.lse[row] * kLog2e : p.ndelta[row];
       }
+      const uint32_t la = lds0 + stage * (2 * kTile);
+      lq.issue(rows_of<T>(p.q, w.b, hn, w.nq, p.D), static_cast<int64_t>(tn) * kT, la, wave);
+      lg.issue(rows_of<T>(p.dout, w.b, hn, w.nq, p.D), static_cast<int64_t>(tn) * kT, la + kTile, wave);
+      if (++tn == w.tbase + w.tcount) {
+        tn = w.tbase;
+        ++hn;
+      }
+    };
+    auto put = [&](int stage) {
+      if (threadIdx.x < 2 * kT) lds.stat[stage][threadIdx.x / kT][threadIdx.x % kT] = st;
+    };
+
+    f32x16 sum[DP / 32];  // dV (ROLE 0) or dK
 #pragma unroll
-      for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nl[(v >> 2) * 8 + (v & 3)]));
-      if (p0 < kw + 31 || p0 + 31 - p.q_start >= nq || (p0 + 31 >= kw + p.window && kw + 31 >= p.sinks)) {
-        const int end = p.q_start + nq;
-        const int lo = key - p0 - 4 * h2;
-        const int hi = (key < p.sinks ? end : min(end, key + p.window)) - p0 - 4 * h2;
+    for (int db = 0; db < DP / 32; ++db) sum[db] = tile::splat(0.f);
+
+    // Entry i from stage ST, known when compiled.
+    auto step = [&](auto stage, int i) {
+      constexpr int ST = decltype(stage)::value;
+      tile::landed_barrier();  // the tile is there; nobody reads the other stage or P any more
+      if (i + 1 < w.i1) issue(1 - ST);
+      const int t0 = p.q_start + tc * kT;  // the tile's first position
+      if (++tc == w.tbase + w.tcount) tc = w.tbase;
+      f32x16 x[kT / 32];
+      F pf[kT / 32][2];
+      bool on[kT / 32];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int rv = (v >> 2) * 8 + (v & 3);
-          x[v] = rv >= lo && rv < hi ? x[v] : 0.f;
+      for (int rb = 0; rb < kT / 32; ++rb) {
+        const int p0 = t0 + 32 * rb;
+        on[rb] = !(p0 + 31 < kw || (p0 >= kw + 31 + p.window && kw >= p.sinks) || p0 - p.q_start >= w.nq) &&
+                 (!FAR || rb == pair);
+        if (!on[rb]) continue;
+        const char* tl = lds.tiles[ST][ROLE] + 32 * rb * Tl::kRow;
+        const float* ps = &lds.stat[ST][ROLE][32 * rb + 4 * h2];
+        f32x16 stat;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) stat[v] = ps[(v >> 2) * 8 + (v & 3)];
+        x[rb] = ROLE == 0 ? tile::splat(0.f) : stat;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) x[rb] = tile::mma<T>(Tl::frag_row(tl, s, lane), kf[s], x[rb]);
+        if constexpr (ROLE == 0) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[rb][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[rb][v], c, stat[v]));
+          if (p0 < kw + 31 || p0 + 31 - p.q_start >= w.nq || (p0 + 31 >= kw + p.window && kw + 31 >= p.sinks)) {
+            // Rows key - p0 .. min(end, key + window) - p0 - 1 see the key.
+            const int end = p.q_start + w.nq;
+            const int first = key - p0 - 4 * h2, last = (key < p.sinks ? end : min(end, key + p.window)) - p0 - 4 * h2;
+            const uint32_t bits = low_bits(last) & ~low_bits(first);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[rb][v] = select_bit(bits, (v >> 2) * 8 + (v & 3), x[rb][v], 0.f);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(lds.p[pair][rb][j][lane]) =
+                make_float4(x[rb][4 * j], x[rb][4 * j + 1], x[rb][4 * j + 2], x[rb][4 * j + 3]);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) pf[rb][s] = tile::pack<T>(x[rb], s);
         }
       }
+      // P is there (the next tile's DMA stays in flight).
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-      for (int v = 0; v < 16; ++v) g[v] *= kF16 ? x[v] * (p.scale * 0x1p-8f) : x[v];
+      for (int rb = 0; rb < kT / 32; ++rb) {
+        if (!on[rb]) continue;
+        if constexpr (ROLE == 1) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const F pf = tile::pack<T>(x, s), df = tile::pack<T>(g, s);
+          for (int j = 0; j < 4; ++j) {
+            const float4 pv = *reinterpret_cast<const float4*>(lds.p[pair][rb][j][lane]);
+            const float f = kF16 ? p.scale * 0x1p-8f : 1.f;
+            x[rb][4 * j] *= kF16 ? pv.x * f : pv.x;
+            x[rb][4 * j + 1] *= kF16 ? pv.y * f : pv.y;
+            x[rb][4 * j + 2] *= kF16 ? pv.z * f : pv.z;
+            x[rb][4 * j + 3] *= kF16 ? pv.w * f : pv.w;
+          }
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-          dv[db] = tile::mma<T>(Tl::frag_tr(sg, db, 32 * rb, s, lane), pf, dv[db]);
-          dk[db] = tile::mma<T>(Tl::frag_tr(sq, db, 32 * rb, s, lane), df, dk[db]);
+          for (int s = 0; s < 2; ++s) pf[rb][s] = tile::pack<T>(x[rb], s);
         }
+        const char* tl = lds.tiles[ST][1 - ROLE] + 32 * rb * Tl::kRow;  // dO for dV, Q for dK
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db)
+            sum[db] = tile::mma<T>(Tl::frag_tr(tl + 16 * s * Tl::kRow, db, lane), pf[rb][s], sum[db]);
       }
+      if (i + 1 < w.i1) put(1 - ST);
+    };
+    if (w.i0 < w.i1) {
+      issue(0);
+      put(0);
     }
-    if (i + 1 < n) put(i + 1);
+    for (int i = w.i0; i < w.i1; i += 2) {
+      step(std::integral_constant<int, 0>{}, i);
+      if (i + 1 < w.i1) step(std::integral_constant<int, 1>{}, i + 1);
+    }
+
+    if (FAR ? pair < kT / 32 : w.part && kw < p.sinks) {  // shares of sinks' sums: [dk, dv][32 keys][D]
+      const int64_t block = FAR ? 0 : kw / 32 * p.far_stride;
+      float* to = w.part + block + (static_cast<int64_t>(FAR ? pair : 0) * 64 + (ROLE == 0 ? 32 : 0) + (lane & 31)) * p.D;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = db * 32 + g * 8 + 4 * h2;
+          if (d < p.D) tile::store4(to + d, sum[db][4 * g], sum[db][4 * g + 1], sum[db][4 * g + 2], sum[db][4 * g + 3]);
+        }
+    }
+    if (FAR || (w.part && key < p.sinks) || key >= p.Sk) return;
+    const Mat3& m = ROLE == 0 ? p.dv : p.dk;
+    T* out = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
+    const float f = ROLE == 0 ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + g * 8 + 4 * h2;
+        if (d >= p.D) continue;
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = key < len ? sum[db][4 * g + e] * f : 0.f;
+        tile::store4(out + d, r[0], r[1], r[2], r[3]);
+      }
   }
-  if (key >= p.Sk) return;
-  T* ok = at<T>(p.dk, b, hk) + static_cast<int64_t>(key) * p.dk.ss;
-  T* ov = at<T>(p.dv, b, hk) + static_cast<int64_t>(key) * p.dv.ss;
-  const float ck = kF16 ? 1.f : p.scale, cv = kF16 ? 0x1p-8f : 1.f;
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + g * 8 + 4 * h2;
-      if (d >= p.D) continue;
-      float rk[4], rv[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        rk[e] = live ? dk[db][4 * g + e] * ck : 0.f;
-        rv[e] = live ? dv[db][4 * g + e] * cv : 0.f;
-      }
-      tile::store4(ok + d, rk[0], rk[1], rk[2], rk[3]);
-      tile::store4(ov + d, rv[0], rv[1], rv[2], rv[3]);
-    }
+};
+
+// One past the last tile (of kT rows) of queries that see, through their windows, a key of
+// the block at k0.
+__device__ __host__ __forceinline__ int near_end(const Params& p, int k0, int kT) {
+  const int64_t last = static_cast<int64_t>(k0) + kCols - 1 + p.window - p.q_start;  // one past the last such query
+  const int64_t tiles = (p.Sq + kT - 1) / kT;
+  return static_cast<int>(last <= 0 ? 0 : (last + kT - 1) / kT < tiles ? (last + kT - 1) / kT : tiles);
 }
 
 template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
+  using K = Keys<T, DP>;
+  constexpr int kT = K::kT;
+  __shared__ typename K::Lds lds;
+  const int nbh = p.B * p.Hkv, G = p.H / p.Hkv;
+  const int bh = blockIdx.x % nbh, at_ = blockIdx.x / nbh;
+  typename K::Work w;
+  w.b = bh / p.Hkv;
+  w.hk = bh % p.Hkv;
+  const int len = length_of(p, w.b);
+  w.nq = max(0, min(p.Sq, len - p.q_start));  // queries that exist
+  const int tiles = (w.nq + kT - 1) / kT;
+  w.part = p.far_blocks ? p.far + static_cast<int64_t>(bh) * p.far_blocks * p.far_stride : nullptr;
+  const bool second = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= K::kPairs;
+  if (at_ < p.far_blocks * p.far_chunks) {
+    // Chunk ck of the queries that see the 32 sinks from 32 sb through no window.
+    const int sb = at_ / p.far_chunks, ck = at_ % p.far_chunks;
+    w.kfirst = 32 * sb;
+    w.tbase = near_end(p, w.kfirst / kCols * kCols, kT);
+    w.tcount = max(0, tiles - w.tbase);
+    w.i0 = min(w.tcount * G, ck * p.far_per);
+    w.i1 = min(w.tcount * G, w.i0 + p.far_per);
+    w.part += sb * p.far_stride + (1 + kT / 32 * ck) * (64 * static_cast<int64_t>(p.D));
+    if (second) K::template run<1, true>(p, lds, w);
+    else K::template run<0, true>(p, lds, w);
+  } else {
+    w.kfirst = (at_ - p.far_blocks * p.far_chunks) * kCols;
+    w.tbase = max(0, w.kfirst - p.q_start) / kT;
+    const int te = w.kfirst >= len ? 0 : w.kfirst < p.sinks && !w.part ? tiles : min(tiles, near_end(p, w.kfirst, kT));
+    w.tcount = max(0, te - w.tbase);
+    w.i0 = 0;
+    w.i1 = w.tcount * G;
+    if (second) K::template run<1, false>(p, lds, w);
+    else K::template run<0, false>(p, lds, w);
+  }
+}
+
+// dk, dv of the sinks: the shares of their block and of the chunks, added in that order.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(Params p) {
+  constexpr bool kF16 = __is_same(T, f16_t);
+  const int vecs = p.D / 4, wgs = (p.far_blocks * 64 * vecs + 255) / 256;  // workgroups of a (batch, kv head)
+  const int bh = blockIdx.x / wgs, b = bh / p.Hkv, hk = bh % p.Hkv;
+  const int e = blockIdx.x % wgs * 256 + threadIdx.x;
+  const int row = e / vecs, d = e % vecs * 4;  // row: block, then [dk, dv], then key
+  const int sb = row / 64, which = row / 32 % 2, key = sb * 32 + row % 32;
+  if (key >= p.sinks || sb >= p.far_blocks) return;
+  const float* part = p.far + (static_cast<int64_t>(bh) * p.far_blocks + sb) * p.far_stride +
+                      (which * 32 + row % 32) * static_cast<int64_t>(p.D) + d;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = 0; i < p.far_shares; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(part + i * (2 * 32 * static_cast<int64_t>(p.D)));
+    a[0] += v.x;
+    a[1] += v.y;
+    a[2] += v.z;
+    a[3] += v.w;
+  }
+  const float f = which ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
+  const Mat3& m = which ? p.dv : p.dk;
+  const bool live = key < length_of(p, b);
+  tile::store4(at<T>(m, b, hk) + key * m.ss + d, live ? a[0] * f : 0.f, live ? a[1] * f : 0.f, live ? a[2] * f : 0.f,
+               live ? a[3] * f : 0.f);
+}
+
+// The workgroups for the queries that see sinks through no window: none unless they are
+// as many as a block's own tiles, else in chunks of a block's tiles (each of half its
+// work or less).  Fills p's far fields; returns the floats of the shares.
+static int64_t plan_far(Params* p, int row_bytes) {
+  const int kT = row_bytes > 256 ? 32 : 64;
+  const int G = p->H / p->Hkv;
+  const int beyond = (p->Sq + kT - 1) / kT - near_end(*p, 0, kT);
+  const int own = (std::min(p->window, p->Sq) + kCols) / kT + 1;
+  if (p->sinks == 0 || beyond < own) return 0;
+  p->far_blocks = (p->sinks + 31) / 32;
+  p->far_per = std::max(8, own * G);
+  p->far_chunks = (beyond * G + p->far_per - 1) / p->far_per;
+  p->far_shares = 1 + kT / 32 * p->far_chunks;
+  p->far_stride = static_cast<int64_t>(p->far_shares) * 64 * p->D;
+  return static_cast<int64_t>(p->B) * p->Hkv * p->far_blocks * p->far_stride;
+}
+static int64_t plan_far(Params* p, bool f32) {
+  return plan_far(p, (p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256) * (f32 ? 4 : 2));
+}
+
+// Floats of delta, a whole number of 16 bytes.
+static int64_t delta_floats(const Params& p) { return (static_cast<int64_t>(p.B) * p.H * p.Sq + 3) / 4 * 4; }
+
+template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
-  const dim3 gq(static_cast<unsigned>((p.Sq + kBR - 1) / kBR * p.B * p.H));
-  const dim3 gk(static_cast<unsigned>((p.Sk + kBR - 1) / kBR * p.B * p.Hkv));
+  const dim3 gq(static_cast<unsigned>((p.Sq + kCols - 1) / kCols * p.B * p.H));
+  const dim3 gk(static_cast<unsigned>(((p.Sk + kCols - 1) / kCols + p.far_blocks * p.far_chunks) * p.B * p.Hkv));
   if (p.Sq > 0) hipLaunchKernelGGL((dq_kernel<T, DP>), gq, dim3(256), 0, s, p);
-  hipLaunchKernelGGL((dkv_kernel<T, DP>), gk, dim3(256), 0, s, p);
+  hipLaunchKernelGGL((dkv_kernel<T, DP>), gk, dim3(512), 0, s, p);
+  if (p.far_blocks)
+    hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>((p.far_blocks * 64 * (p.D / 4) + 255) / 256) * p.B * p.Hkv),
+                       dim3(256), 0, s, p);
 }
 template <typename T>
 static void launch(const Params& p, hipStream_t s) {
@@ -293,7 +450,7 @@ extern "C" int64_t ghip_sdpa_window_bwd_workspace_bytes(int dtype, int64_t B, in
                                                         int64_t sinks) {
   win::Params p{};
   if (win::check_problem("", dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, 1.f, &p, nullptr)) return 0;
-  return B * H * Sq * 4;
+  return (win::delta_floats(p) + win::plan_far(&p, dtype == GHIP_DTYPE_FLOAT32)) * 4;
 }
 
 extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
@@ -331,6 +488,8 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", kWhat);
   p.lse = const_cast<float*>(lse);
   p.ndelta = static_cast<float*>(workspace);
+  p.far = p.ndelta + win::delta_floats(p);
+  win::plan_far(&p, dtype == GHIP_DTYPE_FLOAT32);
   p.lens = lens;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GHIP_DTYPE_FLOAT32) win::launch<float>(p, s);
