@@ -148,6 +148,34 @@ struct Tile {
   }
 };
 
+// use(j, read(j)) for j < N with several reads in flight: left alone, the compiler reads an
+// operand from LDS right before the instruction that takes it and waits for each (1200
+// cycles for 8 matrix instructions that take 256).
+// Rows of 512 bytes leave registers for fewer.
+template <int ROW, typename F, int N, typename Read, typename Use>
+__device__ __forceinline__ void pipelined(const Read& read, const Use& use) {
+  constexpr int kAhead = ROW > 256 ? 2 : 6, A = N < kAhead ? N : kAhead;
+  F a[A];
+#pragma unroll
+  for (int j = 0; j < A; ++j) a[j] = read(j);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    use(j, a[j % A]);
+    if (j + A < N) a[j % A] = read(j + A);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The fragments are there: the compiler's wait for their loads falls here.  Left to their
+// first use, inside the loop over the tiles, that wait would also be one for each next
+// tile's DMA (both count in vmcnt).
+template <typename F, int N>
+__device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
+}
+
 // Four consecutive values of an accumulator column, rounded once.
 __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
   *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
@@ -172,11 +200,11 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t la, uint32_t voff) {
 
 constexpr uint32_t kPastEnd = 0x80000000u;  // past every descriptor's records: loads zeros
 
-// A matrix in global memory whose rows are loaded as tiles; rows past `rows` read zeros.
+// A matrix in global memory whose rows are loaded as tiles; rows from `rows` on read zeros.
 struct Rows {
   const char* base;
-  int64_t step;    // bytes from row to row (the host checks 64 of them against 2 GiB)
-  int64_t extent;  // bytes from base to the end of the last row that may be read
+  uint32_t step;  // bytes from row to row (the host checks 64 of them against 2 GiB)
+  int rows;
 };
 
 // The wave's share of the DMA of ROWS-row tiles (NW waves): per-lane offsets, computed once.
@@ -186,25 +214,26 @@ struct Loader {
   static constexpr int kPer = 1024 / (DP * static_cast<int>(sizeof(T)));  // rows of one DMA instruction
   static_assert(kN >= 1, "a wave loads at least 1 KiB of a tile");
   uint32_t off[kN];
-  __device__ __forceinline__ void init(int64_t step, int D, int wave, int lane) {
+  uint32_t row_bytes;
+  __device__ __forceinline__ void init(uint32_t step, int D, int wave, int lane) {
     constexpr int NCH = DP * static_cast<int>(sizeof(T)) / 16;
+    row_bytes = D * static_cast<int>(sizeof(T));
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int r = (wave * kN + i) * kPer + lane / NCH;
       const int c = (lane % NCH) ^ swz<NCH>(r);
-      off[i] = c * 16 < D * static_cast<int>(sizeof(T)) ? static_cast<uint32_t>(r * step + c * 16) : kPastEnd;
+      off[i] = c * 16u < row_bytes ? r * step + c * 16 : kPastEnd;
     }
   }
-  // Rows row0 .. row0 + ROWS of m to the tile at LDS address la.
-  __device__ __forceinline__ void issue(const Rows& m, int64_t row0, uint32_t la, int wave) const {
-    const int64_t d = row0 * m.step;
-    const int64_t left = m.extent - d;
-    const uint32_t rec = left <= 0 ? 0u : left >= static_cast<int64_t>(kPastEnd) ? kPastEnd : static_cast<uint32_t>(left);
-    const uint64_t b = reinterpret_cast<uint64_t>(m.base + d);
+  // Rows row0 .. row0 + ROWS of m to the tile at LDS address la.  The descriptor begins at
+  // row0 and holds the rows of the tile that exist, so its sizes stay within 32 bits.
+  __device__ __forceinline__ void issue(const Rows& m, int row0, uint32_t la, int wave) const {
+    const int left = min(m.rows - row0, ROWS);
+    const uint64_t b = reinterpret_cast<uint64_t>(m.base) + static_cast<uint64_t>(static_cast<uint32_t>(row0)) * m.step;
     i32x4 rs;
     rs.x = __builtin_amdgcn_readfirstlane(static_cast<int>(b));
     rs.y = __builtin_amdgcn_readfirstlane(static_cast<int>((b >> 32) & 0xffff));
-    rs.z = __builtin_amdgcn_readfirstlane(static_cast<int>(rec));
+    rs.z = __builtin_amdgcn_readfirstlane(left <= 0 ? 0 : static_cast<int>((left - 1) * m.step + row_bytes));
     rs.w = 0x00020000;
 #pragma unroll
     for (int i = 0; i < kN; ++i) dma16(rs, la + (wave * kN + i) * 1024, off[i]);

@@ -35,10 +35,8 @@ __device__ __forceinline__ T* at(const Mat3& m, int b, int h) {
   return static_cast<T*>(const_cast<void*>(m.p)) + b * m.sb + h * m.sh;
 }
 template <typename T>
-__device__ __forceinline__ tile::Rows rows_of(const Mat3& m, int b, int h, int rows, int D) {
-  const int64_t es = static_cast<int64_t>(sizeof(T));
-  return tile::Rows{reinterpret_cast<const char*>(at<T>(m, b, h)), m.ss * es,
-                    rows > 0 ? ((rows - 1) * m.ss + D) * es : 0};
+__device__ __forceinline__ tile::Rows rows_of(const Mat3& m, int b, int h, int rows) {
+  return tile::Rows{reinterpret_cast<const char*>(at<T>(m, b, h)), static_cast<uint32_t>(m.ss * sizeof(T)), rows};
 }
 
 // The key tiles of queries at positions [p0, p1]: those of the sinks, then those of the

@@ -46,7 +46,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) qf[s] = Tl::frag_global(Q, s, h2, p.D, live);
 
-  const tile::Rows K = rows_of<T>(p.k, b, hk, len, p.D), V = rows_of<T>(p.v, b, hk, len, p.D);
+  tile::settle(qf);
+
+  const tile::Rows K = rows_of<T>(p.k, b, hk, len), V = rows_of<T>(p.v, b, hk, len);
   tile::Loader<T, DP, kKT, kWaves> lk, lv;
   lk.init(K.step, p.D, wave, lane);
   lv.init(V.step, p.D, wave, lane);
@@ -54,7 +56,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
   const Tiles<kKT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kBQ, p.Sq)) : 0);
   auto issue = [&](int i) {
     const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    const int64_t row = static_cast<int64_t>(tl(i)) * kKT;
+    const int row = tl(i) * kKT;
     lk.issue(K, row, la, wave);
     lv.issue(V, row, la + kTile, wave);
   };
@@ -77,13 +79,14 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
     const char* sk = smem[ST][0];
     const char* sv = smem[ST][1];
     f32x16 s0 = tile::splat(0.f), s1 = s0;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      s0 = tile::mma<T>(Tl::frag_row(sk, s, lane), qf[s], s0);
-      s1 = tile::mma<T>(Tl::frag_row(sk + 32 * Tl::kRow, s, lane), qf[s], s1);
-    }
+    tile::pipelined<Tl::kRow, F, DP / 8>([&](int j) { return Tl::frag_row(sk + (j & 1) * 32 * Tl::kRow, j >> 1, lane); },
+                               [&](int j, const F& a) {
+                                 f32x16& x = j & 1 ? s1 : s0;
+                                 x = tile::mma<T>(a, qf[j >> 1], x);
+                               });
     // s{kb}[v] is key key0 + 32 kb + 4 h2 + kv, kv = 8 (v / 4) + v % 4.
     if (key0 + kKT - 1 > pw || key0 + kKT > len || key0 <= pw + kQW - 1 - p.window) {
+      asm volatile("");  // a branch: most tiles need no mask
       const uint32_t w0 = seen_keys(p, pos, live, len, key0 + 4 * h2), w1 = seen_keys(p, pos, live, len, key0 + 32 + 4 * h2);
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
@@ -119,13 +122,12 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
       l1 += s1[v];
     }
     l += l0 + l1;
+    F pf[4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const F pf = s < 2 ? tile::pack<T>(s0, s) : tile::pack<T>(s1, s - 2);
-#pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
-        o[db] = tile::mma<T>(Tl::frag_tr(sv + 16 * s * Tl::kRow, db, lane), pf, o[db]);
-    }
+    for (int s = 0; s < 4; ++s) pf[s] = s < 2 ? tile::pack<T>(s0, s) : tile::pack<T>(s1, s - 2);
+    constexpr int ND = DP / 32;
+    tile::pipelined<Tl::kRow, F, 4 * ND>([&](int j) { return Tl::frag_tr(sv + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+                               [&](int j, const F& a) { o[j % ND] = tile::mma<T>(a, pf[j / ND], o[j % ND]); });
   };
   if (tl.n > 0) issue(0);
   for (int i = 0; i < tl.n; i += 2) {

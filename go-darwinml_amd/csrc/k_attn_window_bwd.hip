@@ -63,9 +63,12 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
   const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Sq + qi;
   if (h2 == 0 && qi < p.Sq) p.ndelta[row] = nd;
   const float c = p.scale * kLog2e;
-  const float nl = live ? __builtin_amdgcn_logf(p.scale) - p.lse[row] * kLog2e : 0.f;
+  float nl = live ? __builtin_amdgcn_logf(p.scale) - p.lse[row] * kLog2e : 0.f;
+  tile::settle(qf);
+  tile::settle(gf);
+  asm volatile("" : "+v"(nl));
 
-  const tile::Rows K = rows_of<T>(p.k, b, hk, len, p.D), V = rows_of<T>(p.v, b, hk, len, p.D);
+  const tile::Rows K = rows_of<T>(p.k, b, hk, len), V = rows_of<T>(p.v, b, hk, len);
   tile::Loader<T, DP, kT, 4> lk, lv;
   lk.init(K.step, p.D, wave, lane);
   lv.init(V.step, p.D, wave, lane);
@@ -73,7 +76,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
   const Tiles<kT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kCols, p.Sq)) : 0);
   auto issue = [&](int i) {
     const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    const int64_t r = static_cast<int64_t>(tl(i)) * kT;
+    const int r = tl(i) * kT;
     lk.issue(K, r, la, wave);
     lv.issue(V, r, la + kTile, wave);
   };
@@ -94,25 +97,23 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
       const char* sk = smem[ST][0] + 32 * kb * Tl::kRow;
       const char* sv = smem[ST][1] + 32 * kb * Tl::kRow;
       f32x16 x = tile::splat(0.f), g = tile::splat(nd);
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        x = tile::mma<T>(Tl::frag_row(sk, s, lane), qf[s], x);
-        g = tile::mma<T>(Tl::frag_row(sv, s, lane), gf[s], g);
-      }
+      tile::pipelined<Tl::kRow, F, DP / 8>([&](int j) { return Tl::frag_row(j & 1 ? sv : sk, j >> 1, lane); },
+                                 [&](int j, const F& a) {
+                                   f32x16& to = j & 1 ? g : x;
+                                   to = tile::mma<T>(a, j & 1 ? gf[j >> 1] : qf[j >> 1], to);
+                                 });
 #pragma unroll
       for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nl)) * g[v];
       if (key0 + 31 > pw || key0 + 32 > len || key0 <= pw + kQW - 1 - p.window) {
+        asm volatile("");  // a branch: most tiles need no mask
         const uint32_t w = seen_keys(p, pos, live, len, key0 + 4 * h2);
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], 0.f);
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const F df = tile::pack<T>(x, s);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-          dq[db] = tile::mma<T>(Tl::frag_tr(sk + 16 * s * Tl::kRow, db, lane), df, dq[db]);
-      }
+      const F df[2] = {tile::pack<T>(x, 0), tile::pack<T>(x, 1)};
+      constexpr int ND = DP / 32;
+      tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(sk + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+                                 [&](int j, const F& a) { dq[j % ND] = tile::mma<T>(a, df[j / ND], dq[j % ND]); });
     }
   };
   if (tl.n > 0) issue(0);
@@ -168,17 +169,18 @@ struct Keys {
   // as one list, its entries i0 .. i1 - 1; keys from kfirst on.
   struct Work {
     int b, hk, kfirst, tbase, tcount, i0, i1, nq;
+    bool far;  // the 32 keys from kfirst on, a pair of waves each 32 rows of the tiles
     float* part;
   };
 
   // ROLE 0: P and dV; 1: dS and dK.
-  template <int ROLE, bool FAR>
+  template <int ROLE>
   __device__ __forceinline__ static void run(const Params& p, Lds& lds, const Work& w) {
     const uint32_t lds0 = tile::lds_addr(lds.tiles);
     const int lane = threadIdx.x & 63, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % kPairs;
     const int len = length_of(p, w.b);
-    const int kw = FAR ? w.kfirst : w.kfirst + pair * 32, key = kw + (lane & 31);
+    const int kw = w.far ? w.kfirst : w.kfirst + pair * 32, key = kw + (lane & 31);
     const int G = p.H / p.Hkv;
     const float c = p.scale * kLog2e;
 
@@ -189,29 +191,33 @@ struct Keys {
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) kf[s] = Tl::frag_global(K, s, h2, p.D, key < len);
     }
+    tile::settle(kf);
     tile::Loader<T, DP, kT, kNW> lq, lg;
-    lq.init(p.q.ss * Tl::kEs, p.D, wave, lane);
-    lg.init(p.dout.ss * Tl::kEs, p.D, wave, lane);
+    lq.init(static_cast<uint32_t>(p.q.ss * Tl::kEs), p.D, wave, lane);
+    lg.init(static_cast<uint32_t>(p.dout.ss * Tl::kEs), p.D, wave, lane);
     float st = 0.f;  // this thread's entry of the next tile's statistics
-    int hn = w.hk * G + w.i0 / max(w.tcount, 1), tn = w.tbase + w.i0 % max(w.tcount, 1);  // what issue() loads next
-    int tc = tn;                                                                          // the tile worked on
+    int tn = w.tbase + w.i0 % max(w.tcount, 1), tc = tn;  // the tile that issue() loads next, the tile worked on
+    const int h0 = w.hk * G + w.i0 / max(w.tcount, 1);
+    // Its head's rows; the heads of a group follow one another by a head stride.
+    tile::Rows Q = rows_of<T>(p.q, w.b, h0, w.nq), dO = rows_of<T>(p.dout, w.b, h0, w.nq);
+    const float* stats = (threadIdx.x < kT ? p.lse : p.ndelta) + (static_cast<int64_t>(w.b) * p.H + h0) * p.Sq;
+    const float sf = threadIdx.x < kT ? -kLog2e : 1.f, sa = kF16 && threadIdx.x < kT ? 8.f : 0.f;
     auto issue = [&](int stage) {
-      const int r = tn * kT + static_cast<int>(threadIdx.x % kT);
-      st = 0.f;
-      if (threadIdx.x < 2 * kT && r < w.nq) {
-        const int64_t row = (static_cast<int64_t>(w.b) * p.H + hn) * p.Sq + r;
-        st = threadIdx.x < kT ? (kF16 ? 8.f : 0.f) - p.lse[row] * kLog2e : p.ndelta[row];
-      }
+      // (Rows past the queries, which nothing sees, take the last one's: a load under a
+      // condition would be waited for at once.)
+      st = stats[min(tn * kT + static_cast<int>(threadIdx.x % kT), w.nq - 1)];
       const uint32_t la = lds0 + stage * (2 * kTile);
-      lq.issue(rows_of<T>(p.q, w.b, hn, w.nq, p.D), static_cast<int64_t>(tn) * kT, la, wave);
-      lg.issue(rows_of<T>(p.dout, w.b, hn, w.nq, p.D), static_cast<int64_t>(tn) * kT, la + kTile, wave);
+      lq.issue(Q, tn * kT, la, wave);
+      lg.issue(dO, tn * kT, la + kTile, wave);
       if (++tn == w.tbase + w.tcount) {
         tn = w.tbase;
-        ++hn;
+        Q.base += p.q.sh * Tl::kEs;
+        dO.base += p.dout.sh * Tl::kEs;
+        stats += p.Sq;
       }
     };
     auto put = [&](int stage) {
-      if (threadIdx.x < 2 * kT) lds.stat[stage][threadIdx.x / kT][threadIdx.x % kT] = st;
+      if (threadIdx.x < 2 * kT) lds.stat[stage][threadIdx.x / kT][threadIdx.x % kT] = __builtin_fmaf(st, sf, sa);
     };
 
     f32x16 sum[DP / 32];  // dV (ROLE 0) or dK
@@ -232,7 +238,7 @@ struct Keys {
       for (int rb = 0; rb < kT / 32; ++rb) {
         const int p0 = t0 + 32 * rb;
         on[rb] = !(p0 + 31 < kw || (p0 >= kw + 31 + p.window && kw >= p.sinks) || p0 - p.q_start >= w.nq) &&
-                 (!FAR || rb == pair);
+                 (!w.far || rb == pair);
         if (!on[rb]) continue;
         const char* tl = lds.tiles[ST][ROLE] + 32 * rb * Tl::kRow;
         const float* ps = &lds.stat[ST][ROLE][32 * rb + 4 * h2];
@@ -240,12 +246,13 @@ struct Keys {
 #pragma unroll
         for (int v = 0; v < 16; ++v) stat[v] = ps[(v >> 2) * 8 + (v & 3)];
         x[rb] = ROLE == 0 ? tile::splat(0.f) : stat;
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) x[rb] = tile::mma<T>(Tl::frag_row(tl, s, lane), kf[s], x[rb]);
+        tile::pipelined<Tl::kRow, F, DP / 16>([&](int s) { return Tl::frag_row(tl, s, lane); },
+                                    [&](int s, const F& a) { x[rb] = tile::mma<T>(a, kf[s], x[rb]); });
         if constexpr (ROLE == 0) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) x[rb][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[rb][v], c, stat[v]));
           if (p0 < kw + 31 || p0 + 31 - p.q_start >= w.nq || (p0 + 31 >= kw + p.window && kw + 31 >= p.sinks)) {
+            asm volatile("");  // a branch: most tiles need no mask
             // Rows key - p0 .. min(end, key + window) - p0 - 1 see the key.
             const int end = p.q_start + w.nq;
             const int first = key - p0 - 4 * h2, last = (key < p.sinks ? end : min(end, key + p.window)) - p0 - 4 * h2;
@@ -280,11 +287,10 @@ struct Keys {
           for (int s = 0; s < 2; ++s) pf[rb][s] = tile::pack<T>(x[rb], s);
         }
         const char* tl = lds.tiles[ST][1 - ROLE] + 32 * rb * Tl::kRow;  // dO for dV, Q for dK
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int db = 0; db < DP / 32; ++db)
-            sum[db] = tile::mma<T>(Tl::frag_tr(tl + 16 * s * Tl::kRow, db, lane), pf[rb][s], sum[db]);
+        constexpr int ND = DP / 32;
+        tile::pipelined<Tl::kRow, F, 2 * ND>(
+            [&](int j) { return Tl::frag_tr(tl + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+            [&](int j, const F& a) { sum[j % ND] = tile::mma<T>(a, pf[rb][j / ND], sum[j % ND]); });
       }
       if (i + 1 < w.i1) put(1 - ST);
     };
@@ -297,9 +303,9 @@ struct Keys {
       if (i + 1 < w.i1) step(std::integral_constant<int, 1>{}, i + 1);
     }
 
-    if (FAR ? pair < kT / 32 : w.part && kw < p.sinks) {  // shares of sinks' sums: [dk, dv][32 keys][D]
-      const int64_t block = FAR ? 0 : kw / 32 * p.far_stride;
-      float* to = w.part + block + (static_cast<int64_t>(FAR ? pair : 0) * 64 + (ROLE == 0 ? 32 : 0) + (lane & 31)) * p.D;
+    if (w.far ? pair < kT / 32 : w.part && kw < p.sinks) {  // shares of sinks' sums: [dk, dv][32 keys][D]
+      const int64_t block = w.far ? 0 : kw / 32 * p.far_stride;
+      float* to = w.part + block + (static_cast<int64_t>(w.far ? pair : 0) * 64 + (ROLE == 0 ? 32 : 0) + (lane & 31)) * p.D;
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -308,7 +314,7 @@ struct Keys {
           if (d < p.D) tile::store4(to + d, sum[db][4 * g], sum[db][4 * g + 1], sum[db][4 * g + 2], sum[db][4 * g + 3]);
         }
     }
-    if (FAR || (w.part && key < p.sinks) || key >= p.Sk) return;
+    if (w.far || (w.part && key < p.sinks) || key >= p.Sk) return;
     const Mat3& m = ROLE == 0 ? p.dv : p.dk;
     T* out = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
     const float f = ROLE == 0 ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
@@ -348,8 +354,8 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
   w.nq = max(0, min(p.Sq, len - p.q_start));  // queries that exist
   const int tiles = (w.nq + kT - 1) / kT;
   w.part = p.far_blocks ? p.far + static_cast<int64_t>(bh) * p.far_blocks * p.far_stride : nullptr;
-  const bool second = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= K::kPairs;
-  if (at_ < p.far_blocks * p.far_chunks) {
+  w.far = at_ < p.far_blocks * p.far_chunks;
+  if (w.far) {
     // Chunk ck of the queries that see the 32 sinks from 32 sb through no window.
     const int sb = at_ / p.far_chunks, ck = at_ % p.far_chunks;
     w.kfirst = 32 * sb;
@@ -358,8 +364,6 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
     w.i0 = min(w.tcount * G, ck * p.far_per);
     w.i1 = min(w.tcount * G, w.i0 + p.far_per);
     w.part += sb * p.far_stride + (1 + kT / 32 * ck) * (64 * static_cast<int64_t>(p.D));
-    if (second) K::template run<1, true>(p, lds, w);
-    else K::template run<0, true>(p, lds, w);
   } else {
     w.kfirst = (at_ - p.far_blocks * p.far_chunks) * kCols;
     w.tbase = max(0, w.kfirst - p.q_start) / kT;
@@ -367,9 +371,9 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
     w.tcount = max(0, te - w.tbase);
     w.i0 = 0;
     w.i1 = w.tcount * G;
-    if (second) K::template run<1, false>(p, lds, w);
-    else K::template run<0, false>(p, lds, w);
   }
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= K::kPairs) K::template run<1>(p, lds, w);
+  else K::template run<0>(p, lds, w);
 }
 
 // dk, dv of the sinks: the shares of their block and of the chunks, added in that order.
