@@ -14,92 +14,71 @@ namespace win {
 
 using tile::f32x16;
 
-constexpr int kWaves = 4, kQW = 32, kBQ = kWaves * kQW, kKT = 64;
 constexpr float kLazyLog2 = 8.f;  // the reference maximum may trail the true one by 2^8
 
-// S^T = K Q^T and O^T = V^T P^T: a lane owns one query (column), so the softmax's
-// maximum, sum and rescale stay in the lane but for one exchange between the halves of
-// the wave.  K and V stream through two LDS stages, the next tile's DMA in flight
-// during a tile.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(Params p) {
+// A wave's 32 queries, one a lane (in both halves): S^T = K Q^T and O^T = V^T P^T, so the
+// softmax's running maximum, sum and rescale stay in the lane but for one exchange between
+// the halves a tile of KT keys.
+template <typename T, int DP, int KT>
+struct Queries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
-  constexpr int kTile = kKT * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
-  const uint32_t lds0 = tile::lds_addr(smem);
-
-  const int lane = threadIdx.x & 63, h2 = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nqb = (p.Sq + kBQ - 1) / kBQ;
-  const int nbh = p.B * p.H;
-  const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
-  const int bh = blockIdx.x % nbh;
-  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
-  const int len = length_of(p, b);
-  const int q0 = qb * kBQ, qw = q0 + wave * kQW, qi = qw + (lane & 31);
-  const int pos = p.q_start + qi, pw = p.q_start + qw;
-  const bool live = qi < p.Sq && pos < len;
-
-  const T* Q = at<T>(p.q, b, h) + static_cast<int64_t>(qi) * p.q.ss;
+  static constexpr int NK = KT / 32, ND = DP / 32;
   F qf[DP / 16];
+  f32x16 o[ND];
+  float m, l, c;
+  int pw, pos;  // positions: the wave's first, the lane's own
+  int len;
+  bool live;    // the lane's query exists
+
+  __device__ __forceinline__ void init(const Params& p, int b, int h, int qw, int lane) {
+    const int qi = qw + (lane & 31);
+    len = length_of(p, b);
+    pw = p.q_start + qw;
+    pos = p.q_start + qi;
+    live = qi < p.Sq && pos < len;
+    const T* Q = at<T>(p.q, b, h) + static_cast<int64_t>(qi) * p.q.ss;
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) qf[s] = Tl::frag_global(Q, s, h2, p.D, live);
-
-  tile::settle(qf);
-
-  const tile::Rows K = rows_of<T>(p.k, b, hk, len), V = rows_of<T>(p.v, b, hk, len);
-  tile::Loader<T, DP, kKT, kWaves> lk, lv;
-  lk.init(K.step, p.D, wave, lane);
-  lv.init(V.step, p.D, wave, lane);
-  const int p0 = p.q_start + q0;
-  const Tiles<kKT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kBQ, p.Sq)) : 0);
-  auto issue = [&](int i) {
-    const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    const int row = tl(i) * kKT;
-    lk.issue(K, row, la, wave);
-    lv.issue(V, row, la + kTile, wave);
-  };
-
-  f32x16 o[DP / 32];
+    for (int s = 0; s < DP / 16; ++s) qf[s] = Tl::frag_global(Q, s, lane >> 5, p.D, live);
+    tile::settle(qf);
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db) o[db] = tile::splat(0.f);
-  float m = -INFINITY, l = 0.f;
-  const float c = p.scale * 1.4426950408889634f;
+    for (int db = 0; db < ND; ++db) o[db] = tile::splat(0.f);
+    m = -INFINITY;
+    l = 0.f;
+    c = p.scale * 1.4426950408889634f;
+  }
 
-  // Tile i from stage ST (known when compiled: LDS addresses are a lane's constants plus
-  // immediate offsets).
-  auto step = [&](auto st, int i) {
-    constexpr int ST = decltype(st)::value;
-    tile::landed_barrier();  // tile i is there, and nobody reads the other stage any more
-    if (i + 1 < tl.n) issue(i + 1);
-    const int key0 = tl(i) * kKT;
+  // Keys key0 .. key0 + KT - 1 from the tiles at sk, sv.
+  __device__ __forceinline__ void step(const Params& p, const char* sk, const char* sv, int key0, int lane) {
     // The wave's queries pw .. pw + 31 see nothing of this tile.
-    if (key0 > pw + kQW - 1 || (key0 + kKT - 1 <= pw - p.window && key0 >= p.sinks)) return;
-    const char* sk = smem[ST][0];
-    const char* sv = smem[ST][1];
-    f32x16 s0 = tile::splat(0.f), s1 = s0;
-    tile::pipelined<Tl::kRow, F, DP / 8>([&](int j) { return Tl::frag_row(sk + (j & 1) * 32 * Tl::kRow, j >> 1, lane); },
-                               [&](int j, const F& a) {
-                                 f32x16& x = j & 1 ? s1 : s0;
-                                 x = tile::mma<T>(a, qf[j >> 1], x);
-                               });
-    // s{kb}[v] is key key0 + 32 kb + 4 h2 + kv, kv = 8 (v / 4) + v % 4.
-    if (key0 + kKT - 1 > pw || key0 + kKT > len || key0 <= pw + kQW - 1 - p.window) {
-      asm volatile("");  // a branch: most tiles need no mask
-      const uint32_t w0 = seen_keys(p, pos, live, len, key0 + 4 * h2), w1 = seen_keys(p, pos, live, len, key0 + 32 + 4 * h2);
+    if (key0 > pw + 31 || (key0 + KT - 1 <= pw - p.window && key0 >= p.sinks)) return;
+    const int h2 = lane >> 5;
+    f32x16 x[NK];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int kv = (v >> 2) * 8 + (v & 3);
-        s0[v] = select_bit(w0, kv, s0[v], -INFINITY);
-        s1[v] = select_bit(w1, kv, s1[v], -INFINITY);
+    for (int k = 0; k < NK; ++k) x[k] = tile::splat(0.f);
+    tile::pipelined<Tl::kRow, F, NK * DP / 16>(
+        [&](int j) { return Tl::frag_row(sk + (j % NK) * 32 * Tl::kRow, j / NK, lane); },
+        [&](int j, const F& a) {
+          // fp32 products are 16 times as long: those of the padding are left out.
+          if (sizeof(T) == 4 && 16 * (j / NK) >= p.D) return;
+          x[j % NK] = tile::mma<T>(a, qf[j / NK], x[j % NK]);
+        });
+    // x[k][v] is key key0 + 32 k + 4 h2 + kv, kv = 8 (v / 4) + v % 4.
+    if (key0 + KT - 1 > pw || key0 + KT > len || key0 <= pw + 31 - p.window) {
+      asm volatile("");  // a branch: most tiles need no mask
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        const uint32_t w = seen_keys(p, pos, live, len, key0 + 32 * k + 4 * h2);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[k][v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[k][v], -INFINITY);
       }
     }
     // The first maximum is the compiler's, which waits for the products' last results;
     // v_max3_f32 directly for the others (fmaxf would quiet every one of them first).
-    float mx = fmaxf(s0[0], s1[0]);
+    float mx = fmaxf(x[0][0], x[NK - 1][15]);
 #pragma unroll
-    for (int v = 1; v < 16; ++v) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mx) : "v"(s0[v]), "v"(s1[v]));
+    for (int i = 1; i < 16 * NK - 1; i += 2)
+      asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mx) : "v"(x[i / 16][i % 16]), "v"(x[(i + 1) / 16][(i + 1) % 16]));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     // The reference maximum moves only when a tile's exceeds it by more than 2^8.
     if (__builtin_amdgcn_ballot_w64((mx - m) * c > kLazyLog2)) {
@@ -108,53 +87,175 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
       m = mnew;
       l *= alpha;
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
+      for (int db = 0; db < ND; ++db)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
     }
     const float nb = m == -INFINITY ? 0.f : -m * c;
-    float l0 = 0.f, l1 = 0.f;
+    F pf[2 * NK];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      s0[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s0[v], c, nb));
-      s1[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s1[v], c, nb));
-      l0 += s0[v];  // the sum takes the weights before they are rounded for P V
-      l1 += s1[v];
+    for (int k = 0; k < NK; ++k) {
+      float ls = 0.f;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        x[k][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][v], c, nb));
+        ls += x[k][v];  // the sum takes the weights before they are rounded for P V
+      }
+      l += ls;
+      pf[2 * k] = tile::pack<T>(x[k], 0);
+      pf[2 * k + 1] = tile::pack<T>(x[k], 1);
     }
-    l += l0 + l1;
-    F pf[4];
+    tile::pipelined<Tl::kRow, F, 2 * NK * ND>(
+        [&](int j) { return Tl::frag_tr(sv + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+        [&](int j, const F& a) {
+          if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
+          o[j % ND] = tile::mma<T>(a, pf[j / ND], o[j % ND]);
+        });
+  }
+
+  // o[db][v] is d = 32 db + 8 (v / 4) + 4 h2 + v % 4 of the lane's query.
+  __device__ __forceinline__ void finish(const Params& p, int b, int h, int qw, int lane) {
+    const int qi = qw + (lane & 31), h2 = lane >> 5;
+    const float lt = l + __shfl_xor(l, 32, 64);
+    if (qi >= p.Sq) return;
+    const float inv = live ? 1.f / lt : 0.f;
+    T* O = at<T>(p.o, b, h) + static_cast<int64_t>(qi) * p.o.ss;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) pf[s] = s < 2 ? tile::pack<T>(s0, s) : tile::pack<T>(s1, s - 2);
-    constexpr int ND = DP / 32;
-    tile::pipelined<Tl::kRow, F, 4 * ND>([&](int j) { return Tl::frag_tr(sv + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
-                               [&](int j, const F& a) { o[j % ND] = tile::mma<T>(a, pf[j / ND], o[j % ND]); });
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + g * 8 + 4 * h2;
+        if (d >= p.D) continue;
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = live ? o[db][4 * g + e] * inv : 0.f;
+        tile::store4(O + d, r[0], r[1], r[2], r[3]);
+      }
+    if (p.lse && h2 == 0)
+      p.lse[(static_cast<int64_t>(b) * p.H + h) * p.Sq + qi] =
+          live ? (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f : -INFINITY;
+  }
+};
+
+// Four waves of 32 queries each; K and V stream through two LDS stages, the next tile's DMA
+// in flight during a tile.
+constexpr int kBQ = 128;
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(Params p) {
+  using Tl = tile::Tile<T, DP>;
+  constexpr int KT = 64, kTile = KT * Tl::kRow;
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
+  const uint32_t lds0 = tile::lds_addr(smem);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nqb = (p.Sq + kBQ - 1) / kBQ;
+  const int nbh = p.B * p.H;
+  const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
+  const int bh = blockIdx.x % nbh;
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
+  const int q0 = qb * kBQ, qw = q0 + wave * 32, p0 = p.q_start + q0;
+  Queries<T, DP, KT> q;
+  q.init(p, b, h, qw, lane);
+
+  const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
+  tile::Loader<T, DP, KT, 4> lk, lv;
+  lk.init(K.step, p.D, wave, lane);
+  lv.init(V.step, p.D, wave, lane);
+  const Tiles<KT> tl(p, p0, p0 < q.len ? min(q.len, p.q_start + min(q0 + kBQ, p.Sq)) : 0);
+  auto issue = [&](int i) {
+    const uint32_t la = lds0 + (i & 1) * (2 * kTile);
+    lk.issue(K, tl(i) * KT, la, wave);
+    lv.issue(V, tl(i) * KT, la + kTile, wave);
+  };
+  // Tile i from stage ST (known when compiled: LDS addresses are a lane's constants plus
+  // immediate offsets).
+  auto step = [&](auto st, int i) {
+    constexpr int ST = decltype(st)::value;
+    tile::landed_barrier();  // tile i is there, and nobody reads the other stage any more
+    if (i + 1 < tl.n) issue(i + 1);
+    q.step(p, smem[ST][0], smem[ST][1], tl(i) * KT, lane);
   };
   if (tl.n > 0) issue(0);
   for (int i = 0; i < tl.n; i += 2) {
     step(std::integral_constant<int, 0>{}, i);
     if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  q.finish(p, b, h, qw, lane);
+}
 
-  // o[db][v] is d = 32 db + 8 (v / 4) + 4 h2 + v % 4 of query qi.
-  const float lt = l + __shfl_xor(l, 32, 64);
-  if (qi >= p.Sq) return;
-  const float inv = live ? 1.f / lt : 0.f;
-  T* O = at<T>(p.o, b, h) + static_cast<int64_t>(qi) * p.o.ss;
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + g * 8 + 4 * h2;
-      if (d >= p.D) continue;
-      float r[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = live ? o[db][4 * g + e] * inv : 0.f;
-      tile::store4(O + d, r[0], r[1], r[2], r[3]);
+// Grids of few workgroups (chunks of a prompt, single tokens): a workgroup has 32 queries,
+// and its four waves take the key tiles in turn, each with LDS stages of its own and no
+// barrier; their shares are joined through LDS at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
+  using Tl = tile::Tile<T, DP>;
+  constexpr int KT = 32, kTile = KT * Tl::kRow, ND = DP / 32;
+  constexpr int kStages = Tl::kRow > 256 ? 1 : 2;
+  constexpr int kDma = 2 * kTile / 1024;  // DMA instructions of a tile
+  __shared__ __attribute__((aligned(1024))) char smem[4][kStages][2][kTile];
+  __shared__ float stat[4][2][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds0 = tile::lds_addr(smem[wave]);
+  const int nbh = p.B * p.H;
+  const int bh = blockIdx.x % nbh, qw = blockIdx.x / nbh * 32;
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
+  Queries<T, DP, KT> q;
+  q.init(p, b, h, qw, lane);
+
+  const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
+  tile::Loader<T, DP, KT, 1> lk, lv;
+  lk.init(K.step, p.D, 0, lane);
+  lv.init(V.step, p.D, 0, lane);
+  const Tiles<KT> tl(p, q.pw, q.pw < q.len ? min(q.len, p.q_start + min(qw + 32, p.Sq)) : 0);
+  auto issue = [&](int i, int stage) {
+    const uint32_t la = lds0 + stage * (2 * kTile);
+    lk.issue(K, tl(i) * KT, la, 0);
+    lv.issue(V, tl(i) * KT, la + kTile, 0);
+  };
+  int stage = 0;
+  if (wave < tl.n) issue(wave, 0);
+  for (int i = wave; i < tl.n; i += 4) {
+    if (kStages > 1 && i + 4 < tl.n) {
+      issue(i + 4, stage ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma < 64 ? kDma : 0) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-  if (p.lse && h2 == 0)
-    p.lse[(static_cast<int64_t>(b) * p.H + h) * p.Sq + qi] =
-        live ? (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f : -INFINITY;
+    q.step(p, smem[wave][stage][0], smem[wave][stage][1], tl(i) * KT, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
+    if (kStages > 1) stage ^= 1;
+    else if (i + 4 < tl.n) issue(i + 4, 0);
+  }
+
+  // Every wave's sums against the largest maximum, added in the waves' order by the first.
+  float* mine = reinterpret_cast<float*>(smem[wave]);
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mine[(db * 16 + v) * 64 + lane] = q.o[db][v];
+  stat[wave][0][lane] = q.m;
+  stat[wave][1][lane] = q.l;
+  __syncthreads();
+  if (wave != 0) return;
+  float m = q.m;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) m = fmaxf(m, stat[w][0][lane]);
+  float f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) f[w] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((stat[w][0][lane] - m) * q.c);
+  q.l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) q.l += f[w] * stat[w][1][lane];
+  q.m = m;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) a += f[w] * reinterpret_cast<const float*>(smem[w])[(db * 16 + v) * 64 + lane];
+      q.o[db][v] = a;
+    }
+  q.finish(p, b, h, qw, lane);
 }
 
 int check_problem(const char* what, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
@@ -207,12 +308,27 @@ int check_operand(const char* what, const char* name, int dtype, const void* ptr
   return GHIP_OK;
 }
 
+// Which kernel: fwd_few_kernel while its workgroups, four times as many, run at once (one
+// a CU, rows of 128 bytes two), us a call: bf16 D 128, 64 queries of 32 heads over a window
+// of 1024 (64 workgroups) 18.0 against 25.5, 512 queries of 16 heads, window 128 (256) 9.6
+// against 11.5, of 32 heads without one (512) 20.5 against 14.9; f16 D 64 the same (512)
+// 9.4 against 11.5.  In fp32, where a tile's products take 16 times as long, up to fewer
+// than 1024: 64 queries, window 1024 52 against 165, 512 of 32 heads (512) 42 against 78, 1024
+// of 32 heads, window 2048 (1024) 349 against 320.
+template <typename T, int DP>
+static void launch_d(const Params& p, hipStream_t s) {
+  const int64_t bh = static_cast<int64_t>(p.B) * p.H, few = (p.Sq + 31) / 32 * bh, many = (p.Sq + kBQ - 1) / kBQ * bh;
+  constexpr int64_t kMost = sizeof(T) == 4 ? 1023 : DP * sizeof(T) > 128 ? 256 : 512;
+  if (few <= kMost)
+    hipLaunchKernelGGL((fwd_few_kernel<T, DP>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((fwd_kernel<T, DP>), dim3(static_cast<unsigned>(many)), dim3(256), 0, s, p);
+}
 template <typename T>
 static void launch_fwd(const Params& p, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.Sq + kBQ - 1) / kBQ * p.B * p.H));
-  if (p.D <= 64) hipLaunchKernelGGL((fwd_kernel<T, 64>), grid, dim3(256), 0, s, p);
-  else if (p.D <= 128) hipLaunchKernelGGL((fwd_kernel<T, 128>), grid, dim3(256), 0, s, p);
-  else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((fwd_kernel<T, 256>), grid, dim3(256), 0, s, p);
+  if (p.D <= 64) launch_d<T, 64>(p, s);
+  else if (p.D <= 128) launch_d<T, 128>(p, s);
+  else if constexpr (sizeof(T) == 2) launch_d<T, 256>(p, s);
 }
 
 }  // namespace win

@@ -16,7 +16,13 @@ namespace win {
 
 using tile::f32x16;
 
-constexpr int kCols = 128;  // queries (dq_kernel) or keys (dkv_kernel) of a workgroup
+constexpr int kCols = 128;  // queries of a workgroup of dq_kernel
+#ifndef KPAIRS
+#define KPAIRS 2
+#define KTILE 32
+#define FARPER 512
+#endif
+constexpr int kKeys = 32 * KPAIRS;  // keys of a workgroup of dkv_kernel
 constexpr float kLog2e = 1.4426950408889634f;
 
 // dQ: the transposed arrangement of the forward kernel.  A lane owns one query; S^T = K
@@ -157,8 +163,8 @@ struct Keys {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
   static constexpr bool kF16 = __is_same(T, f16_t);
-  static constexpr int kPairs = kCols / 32, kNW = 2 * kPairs;
-  static constexpr int kT = Tl::kRow > 256 ? 32 : 64;  // rows of a tile
+  static constexpr int kPairs = kKeys / 32, kNW = 2 * kPairs;
+  static constexpr int kT = Tl::kRow > 256 ? 32 : KTILE;  // rows of a tile
   static constexpr int kTile = kT * Tl::kRow;
   struct Lds {
     __attribute__((aligned(1024))) char tiles[2][2][kTile];      // [stage][Q, dO]
@@ -335,13 +341,13 @@ struct Keys {
 // One past the last tile (of kT rows) of queries that see, through their windows, a key of
 // the block at k0.
 __device__ __host__ __forceinline__ int near_end(const Params& p, int k0, int kT) {
-  const int64_t last = static_cast<int64_t>(k0) + kCols - 1 + p.window - p.q_start;  // one past the last such query
+  const int64_t last = static_cast<int64_t>(k0) + kKeys - 1 + p.window - p.q_start;  // one past the last such query
   const int64_t tiles = (p.Sq + kT - 1) / kT;
   return static_cast<int>(last <= 0 ? 0 : (last + kT - 1) / kT < tiles ? (last + kT - 1) / kT : tiles);
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
+__global__ __launch_bounds__(128 * KPAIRS, 2) void dkv_kernel(Params p) {
   using K = Keys<T, DP>;
   constexpr int kT = K::kT;
   __shared__ typename K::Lds lds;
@@ -354,18 +360,19 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(Params p) {
   w.nq = max(0, min(p.Sq, len - p.q_start));  // queries that exist
   const int tiles = (w.nq + kT - 1) / kT;
   w.part = p.far_blocks ? p.far + static_cast<int64_t>(bh) * p.far_blocks * p.far_stride : nullptr;
-  w.far = at_ < p.far_blocks * p.far_chunks;
+  const int blocks = (p.Sk + kKeys - 1) / kKeys;
+  w.far = at_ >= blocks;  // last: the shortest
   if (w.far) {
     // Chunk ck of the queries that see the 32 sinks from 32 sb through no window.
-    const int sb = at_ / p.far_chunks, ck = at_ % p.far_chunks;
+    const int sb = (at_ - blocks) / p.far_chunks, ck = (at_ - blocks) % p.far_chunks;
     w.kfirst = 32 * sb;
-    w.tbase = near_end(p, w.kfirst / kCols * kCols, kT);
+    w.tbase = near_end(p, w.kfirst / kKeys * kKeys, kT);
     w.tcount = max(0, tiles - w.tbase);
     w.i0 = min(w.tcount * G, ck * p.far_per);
     w.i1 = min(w.tcount * G, w.i0 + p.far_per);
     w.part += sb * p.far_stride + (1 + kT / 32 * ck) * (64 * static_cast<int64_t>(p.D));
   } else {
-    w.kfirst = (at_ - p.far_blocks * p.far_chunks) * kCols;
+    w.kfirst = at_ * kKeys;
     w.tbase = max(0, w.kfirst - p.q_start) / kT;
     const int te = w.kfirst >= len ? 0 : w.kfirst < p.sinks && !w.part ? tiles : min(tiles, near_end(p, w.kfirst, kT));
     w.tcount = max(0, te - w.tbase);
@@ -408,13 +415,13 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 // as many as a block's own tiles, else in chunks of a block's tiles (each of half its
 // work or less).  Fills p's far fields; returns the floats of the shares.
 static int64_t plan_far(Params* p, int row_bytes) {
-  const int kT = row_bytes > 256 ? 32 : 64;
+  const int kT = row_bytes > 256 ? 32 : KTILE;
   const int G = p->H / p->Hkv;
   const int beyond = (p->Sq + kT - 1) / kT - near_end(*p, 0, kT);
-  const int own = (std::min(p->window, p->Sq) + kCols) / kT + 1;
+  const int own = (std::min(p->window, p->Sq) + kKeys) / kT + 1;
   if (p->sinks == 0 || beyond < own) return 0;
   p->far_blocks = (p->sinks + 31) / 32;
-  p->far_per = std::max(8, own * G);
+  p->far_per = FARPER / kT;
   p->far_chunks = (beyond * G + p->far_per - 1) / p->far_per;
   p->far_shares = 1 + kT / 32 * p->far_chunks;
   p->far_stride = static_cast<int64_t>(p->far_shares) * 64 * p->D;
@@ -430,9 +437,9 @@ static int64_t delta_floats(const Params& p) { return (static_cast<int64_t>(p.B)
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
   const dim3 gq(static_cast<unsigned>((p.Sq + kCols - 1) / kCols * p.B * p.H));
-  const dim3 gk(static_cast<unsigned>(((p.Sk + kCols - 1) / kCols + p.far_blocks * p.far_chunks) * p.B * p.Hkv));
+  const dim3 gk(static_cast<unsigned>(((p.Sk + kKeys - 1) / kKeys + p.far_blocks * p.far_chunks) * p.B * p.Hkv));
   if (p.Sq > 0) hipLaunchKernelGGL((dq_kernel<T, DP>), gq, dim3(256), 0, s, p);
-  hipLaunchKernelGGL((dkv_kernel<T, DP>), gk, dim3(512), 0, s, p);
+  hipLaunchKernelGGL((dkv_kernel<T, DP>), gk, dim3(128 * KPAIRS), 0, s, p);
   if (p.far_blocks)
     hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>((p.far_blocks * 64 * (p.D / 4) + 255) / 256) * p.B * p.Hkv),
                        dim3(256), 0, s, p);

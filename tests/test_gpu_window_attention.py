@@ -30,6 +30,11 @@ CASES = [  # (B, H, Hkv, Sq, Sk, q_start, window, sinks, lens)
     (3, 2, 1, 129, 129, 0, 0, 0, (1000, -3, 128)),        # lengths out of range are clamped
     (1, 6, 2, 600, 600, 0, 200, 130, None),       # sinks across the key blocks of the gradient
     (1, 2, 1, 1100, 1100, 0, 256, 4, None),
+    # grids of many workgroups
+    (2, 64, 16, 257, 257, 0, 64, 4, None),
+    (4, 64, 64, 130, 200, 70, 50, 4, (200, 130, 131, 7)),
+    (1, 64, 8, 600, 600, 0, 200, 130, None),
+    (2, 48, 48, 400, 400, 0, 0, 0, (400, 333)),
 ]
 
 
