@@ -154,7 +154,7 @@ struct Tile {
 // Rows of 512 bytes leave registers for fewer.
 template <int ROW, typename F, int N, typename Read, typename Use>
 __device__ __forceinline__ void pipelined(const Read& read, const Use& use) {
-  constexpr int kAhead = ROW > 256 ? 2 : 6, A = N < kAhead ? N : kAhead;
+  constexpr int kAhead = ROW > 256 ? 2 : 4, A = N < kAhead ? N : kAhead;
   F a[A];
 #pragma unroll
   for (int j = 0; j < A; ++j) a[j] = read(j);
@@ -195,6 +195,13 @@ __device__ __forceinline__ void store4(f16_t* p, float a, float b, float c, floa
 __device__ __forceinline__ void dma16(i32x4 rsrc, uint32_t la, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                ::"s"(la), "v"(voff), "s"(rsrc) : "memory", "m0");
+}
+// The same from per-lane addresses, 16 or 4 bytes a lane (LDS address la + lane * 16, * 4).
+__device__ __forceinline__ void load16(const void* p, uint32_t la) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(la), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void load4(const void* p, uint32_t la) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(la), "v"(p) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 

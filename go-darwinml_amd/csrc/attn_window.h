@@ -14,16 +14,27 @@ struct Mat3 {
 struct Params {
   Mat3 q, k, v, o, dout, dq, dk, dv;
   float* lse;        // [B, H, Sq]; forward: written (may be null), gradient: read
-  float* ndelta;     // gradient: minus the row sums of do * o, [B, H, Sq]
-  float* far;        // gradient: shares of the sinks' sums, [B, Hkv, far_blocks][far_shares][dk, dv][32][D]
-  int64_t far_stride;                   // floats of one block's shares
-  int far_blocks, far_chunks, far_per;  // blocks of 32 sinks (0: no shares), chunks a block, tiles a chunk
-  int far_shares;
+  // Gradient, [2][B, H, Sq]: minus the log-sum-exp in base 2 (f16: plus 8), and minus delta,
+  // the row sums of do * o.
+  float* stats;
+  // Gradient: shares of dk and dv that join_kernel adds, of the first share_blocks blocks of
+  // 32 keys: [B, Hkv, share_blocks][shares][dk, dv][32][D].
+  float* share;
+  int64_t share_stride;  // floats of one block's shares
+  int share_blocks, shares, chunks, chunk;  // chunks of so many tiles
+  bool far;  // shares: 0 the block's own workgroup, the others chunks of the queries beyond; else all chunks
   const int32_t* lens;
   int B, H, Hkv, Sq, Sk, D;
   int q_start, window, sinks;
   float scale;
 };
+
+// The workgroups of 32 queries up to which the kernels that share their keys among the waves
+// are taken (measured at the forward kernels' launch): one round of the card, one
+// workgroup a CU (rows of 128 bytes: two); in fp32 nearly four.
+constexpr int64_t few_most(int elem_bytes, int dp) {
+  return elem_bytes == 4 ? 1023 : dp * elem_bytes > 128 ? 256 : 512;
+}
 
 // The tokens of sequence b that exist: lens[b] clamped to [0, Sk].
 __device__ __forceinline__ int length_of(const Params& p, int b) {
@@ -53,6 +64,10 @@ struct Tiles {
   }
   __device__ __forceinline__ int operator()(int i) const { return i < ns ? i : first + i - ns; }
 };
+
+// The (batch, head) that workgroup i of each n works on.  Consecutive workgroups go to the
+// 8 XCDs in turn; neighbouring heads, which share K and V, should share an L2.
+__device__ __forceinline__ int spread(int i, int n) { return n % 8 == 0 ? i % 8 * (n / 8) + i / 8 : i; }
 
 // Bits [0, n) of a word, n clamped to 0 .. 32.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }

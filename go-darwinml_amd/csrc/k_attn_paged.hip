@@ -46,17 +46,6 @@ constexpr int kMinTiles = 2;  // tiles of a worker at least
 // 16 zero bytes: what lanes without a token load.
 __device__ const uint4 kZero[1] = {};
 
-// LDS byte address la + lane * 16 (lane * 4) from per-lane addresses.  m0 is set and used
-// inside one statement; nothing else in these kernels reads it.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load16(const char* p, uint32_t la) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(la), "v"(p) : "memory", "m0");
-}
-__device__ __forceinline__ void load4(const int32_t* p, uint32_t la) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(la), "v"(p) : "memory", "m0");
-}
-#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   static_assert(N < 64, "vmcnt");
@@ -261,7 +250,7 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
     auto token0 = [&](int t) { return t < nst ? t * KT : (seen.lo & ~15) + (t - nst) * KT; };
     auto issue_pages = [&](int t, int slot) {
       const int entry = min((token0(t) + (lane & (KT - 1))) / p.page_size, p.max_pages - 1);
-      load4(table + entry, pa0 + slot * 256);
+      tile::load4(table + entry, pa0 + slot * 256);
     };
     // The DMA of tile t, its page numbers landed; returns its rows that hold a token.
     auto issue = [&](int t, int slot) -> uint64_t {
@@ -278,8 +267,8 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
         const int64_t pg = __shfl(page, r, 64), of = __shfl(off, r, 64);
         const bool there = ((rows >> r) & 1) && ch * 16 < p.D * kEs;
         const char* zero = reinterpret_cast<const char*>(kZero);
-        load16(there ? K + pg * p.k_sp + of * p.k_st + ch * 16 : zero, la + i * 1024);
-        load16(there ? V + pg * p.v_sp + of * p.v_st + ch * 16 : zero, la + kTile + i * 1024);
+        tile::load16(there ? K + pg * p.k_sp + of * p.k_st + ch * 16 : zero, la + i * 1024);
+        tile::load16(there ? V + pg * p.v_sp + of * p.v_st + ch * 16 : zero, la + kTile + i * 1024);
       }
       return rows;
     };

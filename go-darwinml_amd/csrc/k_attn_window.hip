@@ -18,12 +18,12 @@ constexpr float kLazyLog2 = 8.f;  // the reference maximum may trail the true on
 
 // A wave's 32 queries, one a lane (in both halves): S^T = K Q^T and O^T = V^T P^T, so the
 // softmax's running maximum, sum and rescale stay in the lane but for one exchange between
-// the halves a tile of KT keys.
-template <typename T, int DP, int KT>
+// the halves a tile.
+template <typename T, int DP>
 struct Queries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
-  static constexpr int NK = KT / 32, ND = DP / 32;
+  static constexpr int ND = DP / 32;
   F qf[DP / 16];
   f32x16 o[ND];
   float m, l, c;
@@ -31,54 +31,52 @@ struct Queries {
   int len;
   bool live;    // the lane's query exists
 
-  __device__ __forceinline__ void init(const Params& p, int b, int h, int qw, int lane) {
+  __device__ __forceinline__ void place(const Params& p, int b, int qw, int lane) {
     const int qi = qw + (lane & 31);
     len = length_of(p, b);
     pw = p.q_start + qw;
     pos = p.q_start + qi;
     live = qi < p.Sq && pos < len;
-    const T* Q = at<T>(p.q, b, h) + static_cast<int64_t>(qi) * p.q.ss;
+    m = -INFINITY;
+    l = 0.f;
+    c = p.scale * 1.4426950408889634f;
+  }
+  // (Behind the first tile's DMA, so that the two are waited for together.)
+  __device__ __forceinline__ void load(const Params& p, int b, int h, int qw, int lane) {
+    const T* Q = at<T>(p.q, b, h) + static_cast<int64_t>(qw + (lane & 31)) * p.q.ss;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) qf[s] = Tl::frag_global(Q, s, lane >> 5, p.D, live);
     tile::settle(qf);
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[db] = tile::splat(0.f);
-    m = -INFINITY;
-    l = 0.f;
-    c = p.scale * 1.4426950408889634f;
+  }
+  // Whether any of the wave's queries, pw .. pw + 31, sees a key of key0 .. key0 + 31.
+  __device__ __forceinline__ bool sees(const Params& p, int key0) const {
+    return key0 <= pw + 31 && key0 < len && (key0 + 31 > pw - p.window || key0 < p.sinks);
   }
 
-  // Keys key0 .. key0 + KT - 1 from the tiles at sk, sv.
+  // Keys key0 .. key0 + 31 from the tiles at sk, sv.
   __device__ __forceinline__ void step(const Params& p, const char* sk, const char* sv, int key0, int lane) {
-    // The wave's queries pw .. pw + 31 see nothing of this tile.
-    if (key0 > pw + 31 || (key0 + KT - 1 <= pw - p.window && key0 >= p.sinks)) return;
     const int h2 = lane >> 5;
-    f32x16 x[NK];
-#pragma unroll
-    for (int k = 0; k < NK; ++k) x[k] = tile::splat(0.f);
-    tile::pipelined<Tl::kRow, F, NK * DP / 16>(
-        [&](int j) { return Tl::frag_row(sk + (j % NK) * 32 * Tl::kRow, j / NK, lane); },
-        [&](int j, const F& a) {
-          // fp32 products are 16 times as long: those of the padding are left out.
-          if (sizeof(T) == 4 && 16 * (j / NK) >= p.D) return;
-          x[j % NK] = tile::mma<T>(a, qf[j / NK], x[j % NK]);
-        });
-    // x[k][v] is key key0 + 32 k + 4 h2 + kv, kv = 8 (v / 4) + v % 4.
-    if (key0 + KT - 1 > pw || key0 + KT > len || key0 <= pw + 31 - p.window) {
+    f32x16 x = tile::splat(0.f);
+    tile::pipelined<Tl::kRow, F, DP / 16>([&](int s) { return Tl::frag_row(sk, s, lane); },
+                                          [&](int s, const F& a) {
+                                            // fp32 products are 16 times as long: the padding's are left out.
+                                            if (sizeof(T) == 4 && 16 * s >= p.D) return;
+                                            x = tile::mma<T>(a, qf[s], x);
+                                          });
+    // x[v] is key key0 + 4 h2 + 8 (v / 4) + v % 4.
+    if (key0 + 31 > pw || key0 + 32 > len || key0 <= pw + 31 - p.window) {
       asm volatile("");  // a branch: most tiles need no mask
+      const uint32_t w = seen_keys(p, pos, live, len, key0 + 4 * h2);
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        const uint32_t w = seen_keys(p, pos, live, len, key0 + 32 * k + 4 * h2);
-#pragma unroll
-        for (int v = 0; v < 16; ++v) x[k][v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[k][v], -INFINITY);
-      }
+      for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], -INFINITY);
     }
     // The first maximum is the compiler's, which waits for the products' last results;
     // v_max3_f32 directly for the others (fmaxf would quiet every one of them first).
-    float mx = fmaxf(x[0][0], x[NK - 1][15]);
+    float mx = fmaxf(x[0], x[15]);
 #pragma unroll
-    for (int i = 1; i < 16 * NK - 1; i += 2)
-      asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mx) : "v"(x[i / 16][i % 16]), "v"(x[(i + 1) / 16][(i + 1) % 16]));
+    for (int v = 1; v < 15; v += 2) asm("v_max3_f32 %0, %0, %1, %2" : "+v"(mx) : "v"(x[v]), "v"(x[v + 1]));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     // The reference maximum moves only when a tile's exceeds it by more than 2^8.
     if (__builtin_amdgcn_ballot_w64((mx - m) * c > kLazyLog2)) {
@@ -92,25 +90,19 @@ struct Queries {
         for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
     }
     const float nb = m == -INFINITY ? 0.f : -m * c;
-    F pf[2 * NK];
+    float ls = 0.f;
 #pragma unroll
-    for (int k = 0; k < NK; ++k) {
-      float ls = 0.f;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        x[k][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k][v], c, nb));
-        ls += x[k][v];  // the sum takes the weights before they are rounded for P V
-      }
-      l += ls;
-      pf[2 * k] = tile::pack<T>(x[k], 0);
-      pf[2 * k + 1] = tile::pack<T>(x[k], 1);
+    for (int v = 0; v < 16; ++v) {
+      x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nb));
+      ls += x[v];  // the sum takes the weights before they are rounded for P V
     }
-    tile::pipelined<Tl::kRow, F, 2 * NK * ND>(
-        [&](int j) { return Tl::frag_tr(sv + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
-        [&](int j, const F& a) {
-          if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
-          o[j % ND] = tile::mma<T>(a, pf[j / ND], o[j % ND]);
-        });
+    l += ls;
+    const F pf[2] = {tile::pack<T>(x, 0), tile::pack<T>(x, 1)};
+    tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(sv + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+                                         [&](int j, const F& a) {
+                                           if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
+                                           o[j % ND] = tile::mma<T>(a, pf[j / ND], o[j % ND]);
+                                         });
   }
 
   // o[db][v] is d = 32 db + 8 (v / 4) + 4 h2 + v % 4 of the lane's query.
@@ -141,20 +133,20 @@ struct Queries {
 // in flight during a tile.
 constexpr int kBQ = 128;
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(Params p) {
+__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 3)) void fwd_kernel(Params p) {
   using Tl = tile::Tile<T, DP>;
-  constexpr int KT = 64, kTile = KT * Tl::kRow;
+  constexpr int KT = 32, kTile = KT * Tl::kRow;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
   const uint32_t lds0 = tile::lds_addr(smem);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nqb = (p.Sq + kBQ - 1) / kBQ;
   const int nbh = p.B * p.H;
   const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
-  const int bh = blockIdx.x % nbh;
+  const int bh = spread(blockIdx.x % nbh, nbh);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
   const int q0 = qb * kBQ, qw = q0 + wave * 32, p0 = p.q_start + q0;
-  Queries<T, DP, KT> q;
-  q.init(p, b, h, qw, lane);
+  Queries<T, DP> q;
+  q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
   tile::Loader<T, DP, KT, 4> lk, lv;
@@ -172,9 +164,10 @@ __global__ __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) void fwd_kernel(
     constexpr int ST = decltype(st)::value;
     tile::landed_barrier();  // tile i is there, and nobody reads the other stage any more
     if (i + 1 < tl.n) issue(i + 1);
-    q.step(p, smem[ST][0], smem[ST][1], tl(i) * KT, lane);
+    if (q.sees(p, tl(i) * KT)) q.step(p, smem[ST][0], smem[ST][1], tl(i) * KT, lane);
   };
   if (tl.n > 0) issue(0);
+  q.load(p, b, h, qw, lane);
   for (int i = 0; i < tl.n; i += 2) {
     step(std::integral_constant<int, 0>{}, i);
     if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
@@ -196,10 +189,10 @@ __global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t lds0 = tile::lds_addr(smem[wave]);
   const int nbh = p.B * p.H;
-  const int bh = blockIdx.x % nbh, qw = blockIdx.x / nbh * 32;
+  const int bh = spread(blockIdx.x % nbh, nbh), qw = blockIdx.x / nbh * 32;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
-  Queries<T, DP, KT> q;
-  q.init(p, b, h, qw, lane);
+  Queries<T, DP> q;
+  q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
   tile::Loader<T, DP, KT, 1> lk, lv;
@@ -213,6 +206,7 @@ __global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
   };
   int stage = 0;
   if (wave < tl.n) issue(wave, 0);
+  q.load(p, b, h, qw, lane);
   for (int i = wave; i < tl.n; i += 4) {
     if (kStages > 1 && i + 4 < tl.n) {
       issue(i + 4, stage ^ 1);
@@ -220,7 +214,7 @@ __global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    q.step(p, smem[wave][stage][0], smem[wave][stage][1], tl(i) * KT, lane);
+    if (q.sees(p, tl(i) * KT)) q.step(p, smem[wave][stage][0], smem[wave][stage][1], tl(i) * KT, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
     if (kStages > 1) stage ^= 1;
     else if (i + 4 < tl.n) issue(i + 4, 0);
@@ -254,6 +248,7 @@ __global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) a += f[w] * reinterpret_cast<const float*>(smem[w])[(db * 16 + v) * 64 + lane];
       q.o[db][v] = a;
+      if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // a few shares' reads in flight, not all
     }
   q.finish(p, b, h, qw, lane);
 }
@@ -318,7 +313,7 @@ int check_operand(const char* what, const char* name, int dtype, const void* ptr
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
   const int64_t bh = static_cast<int64_t>(p.B) * p.H, few = (p.Sq + 31) / 32 * bh, many = (p.Sq + kBQ - 1) / kBQ * bh;
-  constexpr int64_t kMost = sizeof(T) == 4 ? 1023 : DP * sizeof(T) > 128 ? 256 : 512;
+  constexpr int64_t kMost = few_most(sizeof(T), DP);
   if (few <= kMost)
     hipLaunchKernelGGL((fwd_few_kernel<T, DP>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, p);
   else

@@ -17,45 +17,42 @@ namespace win {
 using tile::f32x16;
 
 constexpr int kCols = 128;  // queries of a workgroup of dq_kernel
-#ifndef KPAIRS
-#define KPAIRS 2
-#define KTILE 32
-#define FARPER 512
-#endif
-constexpr int kKeys = 32 * KPAIRS;  // keys of a workgroup of dkv_kernel
+constexpr int kKeys = 64;   // keys of a workgroup of dkv_kernel
 constexpr float kLog2e = 1.4426950408889634f;
 
-// dQ: the transposed arrangement of the forward kernel.  A lane owns one query; S^T = K
-// Q^T and dP^T = V dO^T come out as columns, dS^T enters dQ^T += K^T dS^T from the
-// registers.  The product's accumulator starts at -delta, and the scale sits in the
-// exponent (P scale = 2^(s c - lse2 + log2 scale)), so an element costs one FMA, one
+// dQ: the transposed arrangement of the forward kernel.  A lane owns one of a wave's 32
+// queries; S^T = K Q^T and dP^T = V dO^T come out as columns, dS^T enters dQ^T += K^T dS^T
+// from the registers.  The product's accumulator starts at -delta, and the scale sits in
+// the exponent (P scale = 2^(s c - lse2 + log2 scale)), so an element costs one FMA, one
 // exponential and one multiplication.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel(Params p) {
+struct Queries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
-  constexpr int kT = 64, kTile = kT * Tl::kRow, kQW = 32;
-  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
-  const uint32_t lds0 = tile::lds_addr(smem);
-
-  const int lane = threadIdx.x & 63, h2 = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nqb = (p.Sq + kCols - 1) / kCols;
-  const int nbh = p.B * p.H;
-  const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
-  const int bh = blockIdx.x % nbh;
-  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
-  const int len = length_of(p, b);
-  const int q0 = qb * kCols, qw = q0 + wave * kQW, qi = qw + (lane & 31);
-  const int pos = p.q_start + qi, pw = p.q_start + qw;
-  const bool live = qi < p.Sq && pos < len;
-
+  static constexpr int ND = DP / 32;
   F qf[DP / 16], gf[DP / 16];
-  float nd = 0.f;  // minus delta
-  {
+  f32x16 dq[ND];
+  float c, nl, nd;  // minus the log-sum-exp in base 2 (plus log2 scale), minus delta
+  int pw, pos;      // positions: the wave's first, the lane's own
+  int len;
+  bool live;        // the lane's query exists
+
+  __device__ __forceinline__ void place(const Params& p, int b, int qw, int lane) {
+    const int qi = qw + (lane & 31);
+    len = length_of(p, b);
+    pw = p.q_start + qw;
+    pos = p.q_start + qi;
+    live = qi < p.Sq && pos < len;
+    c = p.scale * kLog2e;
+  }
+  // (Behind the first tile's DMA, so that the two are waited for together.)  tell: this
+  // wave leaves the queries' statistics for dkv_kernel.
+  __device__ __forceinline__ void load(const Params& p, int b, int h, int qw, int lane, bool tell) {
+    const int qi = qw + (lane & 31), h2 = lane >> 5;
     const T* Q = at<T>(p.q, b, h) + static_cast<int64_t>(qi) * p.q.ss;
     const T* G = at<T>(p.dout, b, h) + static_cast<int64_t>(qi) * p.dout.ss;
     const T* O = at<T>(p.o, b, h) + static_cast<int64_t>(qi) * p.o.ss;
+    nd = 0.f;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       qf[s] = Tl::frag_global(Q, s, h2, p.D, live);
@@ -64,97 +61,186 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
 #pragma unroll
       for (int e = 0; e < 8; ++e) nd -= tile::value<T>(gf[s], e) * tile::value<T>(of, e);
     }
+    nd += __shfl_xor(nd, 32, 64);
+    const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Sq + qi;
+    nl = live ? -p.lse[row] * kLog2e : 0.f;
+    if (tell && qi < p.Sq && h2 == 0) {
+      p.stats[row] = nl + (__is_same(T, f16_t) ? 8.f : 0.f);
+      p.stats[static_cast<int64_t>(p.B) * p.H * p.Sq + row] = nd;
+    }
+    nl += __builtin_amdgcn_logf(p.scale);
+    tile::settle(qf);
+    tile::settle(gf);
+    asm volatile("" : "+v"(nl));
+#pragma unroll
+    for (int db = 0; db < ND; ++db) dq[db] = tile::splat(0.f);
   }
-  nd += __shfl_xor(nd, 32, 64);
-  const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Sq + qi;
-  if (h2 == 0 && qi < p.Sq) p.ndelta[row] = nd;
-  const float c = p.scale * kLog2e;
-  float nl = live ? __builtin_amdgcn_logf(p.scale) - p.lse[row] * kLog2e : 0.f;
-  tile::settle(qf);
-  tile::settle(gf);
-  asm volatile("" : "+v"(nl));
+  // Whether any of the wave's queries, pw .. pw + 31, sees a key of key0 .. key0 + 31.
+  __device__ __forceinline__ bool sees(const Params& p, int key0) const {
+    return key0 <= pw + 31 && key0 < len && (key0 + 31 > pw - p.window || key0 < p.sinks);
+  }
+  // Keys key0 .. key0 + 31 from the tiles at sk, sv.
+  __device__ __forceinline__ void step(const Params& p, const char* sk, const char* sv, int key0, int lane) {
+    f32x16 x = tile::splat(0.f), g = tile::splat(nd);
+    tile::pipelined<Tl::kRow, F, DP / 8>([&](int j) { return Tl::frag_row(j & 1 ? sv : sk, j >> 1, lane); },
+                                         [&](int j, const F& a) {
+                                           // fp32 products are 16 times as long: the padding's are left out.
+                                           if (sizeof(T) == 4 && 16 * (j >> 1) >= p.D) return;
+                                           f32x16& to = j & 1 ? g : x;
+                                           to = tile::mma<T>(a, j & 1 ? gf[j >> 1] : qf[j >> 1], to);
+                                         });
+#pragma unroll
+    for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nl)) * g[v];
+    if (key0 + 31 > pw || key0 + 32 > len || key0 <= pw + 31 - p.window) {
+      asm volatile("");  // a branch: most tiles need no mask
+      const uint32_t w = seen_keys(p, pos, live, len, key0 + 4 * (lane >> 5));
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], 0.f);
+    }
+    const F df[2] = {tile::pack<T>(x, 0), tile::pack<T>(x, 1)};
+    tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(sk + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+                                         [&](int j, const F& a) {
+                                           if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
+                                           dq[j % ND] = tile::mma<T>(a, df[j / ND], dq[j % ND]);
+                                         });
+  }
+  __device__ __forceinline__ void finish(const Params& p, int b, int h, int qw, int lane) {
+    const int qi = qw + (lane & 31), h2 = lane >> 5;
+    if (qi >= p.Sq) return;
+    T* out = at<T>(p.dq, b, h) + static_cast<int64_t>(qi) * p.dq.ss;
+#pragma unroll
+    for (int db = 0; db < ND; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = db * 32 + g * 8 + 4 * h2;
+        if (d >= p.D) continue;
+        float r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = live ? dq[db][4 * g + e] : 0.f;
+        tile::store4(out + d, r[0], r[1], r[2], r[3]);
+      }
+  }
+};
 
-  const tile::Rows K = rows_of<T>(p.k, b, hk, len), V = rows_of<T>(p.v, b, hk, len);
-  tile::Loader<T, DP, kT, 4> lk, lv;
+// Four waves of 32 queries each; K and V stream through two LDS stages.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel(Params p) {
+  using Tl = tile::Tile<T, DP>;
+  constexpr int KT = 64, kTile = KT * Tl::kRow;
+  __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
+  const uint32_t lds0 = tile::lds_addr(smem);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nqb = (p.Sq + kCols - 1) / kCols;
+  const int nbh = p.B * p.H;
+  const int qb = nqb - 1 - static_cast<int>(blockIdx.x / nbh);
+  const int bh = spread(blockIdx.x % nbh, nbh);
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
+  const int q0 = qb * kCols, qw = q0 + wave * 32, p0 = p.q_start + q0;
+  Queries<T, DP> q;
+  q.place(p, b, qw, lane);
+
+  const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
+  tile::Loader<T, DP, KT, 4> lk, lv;
   lk.init(K.step, p.D, wave, lane);
   lv.init(V.step, p.D, wave, lane);
-  const int p0 = p.q_start + q0;
-  const Tiles<kT> tl(p, p0, p0 < len ? min(len, p.q_start + min(q0 + kCols, p.Sq)) : 0);
+  const Tiles<KT> tl(p, p0, p0 < q.len ? min(q.len, p.q_start + min(q0 + kCols, p.Sq)) : 0);
   auto issue = [&](int i) {
     const uint32_t la = lds0 + (i & 1) * (2 * kTile);
-    const int r = tl(i) * kT;
-    lk.issue(K, r, la, wave);
-    lv.issue(V, r, la + kTile, wave);
+    lk.issue(K, tl(i) * KT, la, wave);
+    lv.issue(V, tl(i) * KT, la + kTile, wave);
   };
-
-  f32x16 dq[DP / 32];
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db) dq[db] = tile::splat(0.f);
-
   // Tile i from stage ST, known when compiled.
   auto step = [&](auto st, int i) {
     constexpr int ST = decltype(st)::value;
     tile::landed_barrier();
     if (i + 1 < tl.n) issue(i + 1);
 #pragma unroll
-    for (int kb = 0; kb < kT / 32; ++kb) {
-      const int key0 = tl(i) * kT + 32 * kb;
-      if (key0 > pw + kQW - 1 || key0 >= len || (key0 + 31 <= pw - p.window && key0 >= p.sinks)) continue;
-      const char* sk = smem[ST][0] + 32 * kb * Tl::kRow;
-      const char* sv = smem[ST][1] + 32 * kb * Tl::kRow;
-      f32x16 x = tile::splat(0.f), g = tile::splat(nd);
-      tile::pipelined<Tl::kRow, F, DP / 8>([&](int j) { return Tl::frag_row(j & 1 ? sv : sk, j >> 1, lane); },
-                                 [&](int j, const F& a) {
-                                   f32x16& to = j & 1 ? g : x;
-                                   to = tile::mma<T>(a, j & 1 ? gf[j >> 1] : qf[j >> 1], to);
-                                 });
-#pragma unroll
-      for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, nl)) * g[v];
-      if (key0 + 31 > pw || key0 + 32 > len || key0 <= pw + kQW - 1 - p.window) {
-        asm volatile("");  // a branch: most tiles need no mask
-        const uint32_t w = seen_keys(p, pos, live, len, key0 + 4 * h2);
-#pragma unroll
-        for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], 0.f);
-      }
-      const F df[2] = {tile::pack<T>(x, 0), tile::pack<T>(x, 1)};
-      constexpr int ND = DP / 32;
-      tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(sk + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
-                                 [&](int j, const F& a) { dq[j % ND] = tile::mma<T>(a, df[j / ND], dq[j % ND]); });
+    for (int k = 0; k < KT / 32; ++k) {
+      const int key0 = tl(i) * KT + 32 * k;
+      if (q.sees(p, key0)) q.step(p, smem[ST][0] + 32 * k * Tl::kRow, smem[ST][1] + 32 * k * Tl::kRow, key0, lane);
     }
   };
   if (tl.n > 0) issue(0);
+  q.load(p, b, h, qw, lane, true);
   for (int i = 0; i < tl.n; i += 2) {
     step(std::integral_constant<int, 0>{}, i);
     if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
   }
-  if (qi >= p.Sq) return;
-  T* out = at<T>(p.dq, b, h) + static_cast<int64_t>(qi) * p.dq.ss;
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + g * 8 + 4 * h2;
-      if (d >= p.D) continue;
-      float r[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = live ? dq[db][4 * g + e] : 0.f;
-      tile::store4(out + d, r[0], r[1], r[2], r[3]);
+  q.finish(p, b, h, qw, lane);
+}
+
+// Grids of few workgroups: 32 queries a workgroup, its four waves take the key tiles in
+// turn, each with LDS stages of its own and no barrier; their sums are added through LDS.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void dq_few_kernel(Params p) {
+  using Tl = tile::Tile<T, DP>;
+  constexpr int KT = 32, kTile = KT * Tl::kRow, ND = DP / 32;
+  constexpr int kStages = Tl::kRow > 256 ? 1 : 2;
+  constexpr int kDma = 2 * kTile / 1024;  // DMA instructions of a tile
+  __shared__ __attribute__((aligned(1024))) char smem[4][kStages][2][kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds0 = tile::lds_addr(smem[wave]);
+  const int nbh = p.B * p.H;
+  const int bh = spread(blockIdx.x % nbh, nbh), qw = blockIdx.x / nbh * 32;
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
+  Queries<T, DP> q;
+  q.place(p, b, qw, lane);
+
+  const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
+  tile::Loader<T, DP, KT, 1> lk, lv;
+  lk.init(K.step, p.D, 0, lane);
+  lv.init(V.step, p.D, 0, lane);
+  const Tiles<KT> tl(p, q.pw, q.pw < q.len ? min(q.len, p.q_start + min(qw + 32, p.Sq)) : 0);
+  auto issue = [&](int i, int stage) {
+    const uint32_t la = lds0 + stage * (2 * kTile);
+    lk.issue(K, tl(i) * KT, la, 0);
+    lv.issue(V, tl(i) * KT, la + kTile, 0);
+  };
+  int stage = 0;
+  if (wave < tl.n) issue(wave, 0);
+  q.load(p, b, h, qw, lane, wave == 0);
+  for (int i = wave; i < tl.n; i += 4) {
+    if (kStages > 1 && i + 4 < tl.n) {
+      issue(i + 4, stage ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma < 64 ? kDma : 0) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    if (q.sees(p, tl(i) * KT)) q.step(p, smem[wave][stage][0], smem[wave][stage][1], tl(i) * KT, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
+    if (kStages > 1) stage ^= 1;
+    else if (i + 4 < tl.n) issue(i + 4, 0);
+  }
+
+  float* mine = reinterpret_cast<float*>(smem[wave]);
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mine[(db * 16 + v) * 64 + lane] = q.dq[db][v];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) a += reinterpret_cast<const float*>(smem[w])[(db * 16 + v) * 64 + lane];
+      q.dq[db][v] = a;
+      if (v % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // a few shares' reads in flight, not all
+    }
+  q.finish(p, b, h, qw, lane);
 }
 
 // dK, dV: a lane owns one key; S = Q K^T and dP = dO V^T come out with the lane's key as
 // their column, so P and dS enter dV^T += dO^T P and dK^T += Q^T dS from the registers.
 // Two waves share 32 keys, half of the registers each (K, V and both sums in one wave
 // left one wave a SIMD, which stood waiting 55% of its time): the first holds K and
-// the sum dV, and hands P over through LDS in fp32; the second holds V and the sum dK.
+// the sum dV, and hands P over through LDS in fp32; the second holds V and the sum dK.  (A
+// second wave one tile behind the first, with one barrier a tile but three stages and two
+// P, was no faster at D 128 and 15% slower at 64, where it left room for a workgroup less.)
 // Q and dO stream through two LDS stages, head after head of the group, with each query's
 // log-sum-exp and delta beside them.
-//
-// Every query sees the sinks, so their keys' sums run over the whole sequence, not over a
-// window.  Where that matters (plan_far) the queries behind the window of the sinks' block
-// are left to workgroups of their own, which deal them out in chunks and hold 32 sinks
-// each, every pair of waves another 32 rows of a tile; their fp32 sums and the block's
-// own are added by join_kernel in a fixed order.
 //
 // f16 only: P is at most 1 and of order 1 / window, so it is rounded 2^8 times larger
 // (small weights would be subnormal), and dS is rounded with the scale applied.
@@ -164,19 +250,21 @@ struct Keys {
   using F = typename Tl::F;
   static constexpr bool kF16 = __is_same(T, f16_t);
   static constexpr int kPairs = kKeys / 32, kNW = 2 * kPairs;
-  static constexpr int kT = Tl::kRow > 256 ? 32 : KTILE;  // rows of a tile
+  static constexpr int kT = 32;  // rows of a tile
   static constexpr int kTile = kT * Tl::kRow;
   struct Lds {
-    __attribute__((aligned(1024))) char tiles[2][2][kTile];      // [stage][Q, dO]
-    __attribute__((aligned(16))) float p[kPairs][kT / 32][4][64][4];  // P of a pair's keys, in accumulator order
-    __attribute__((aligned(16))) float stat[2][2][kT];           // [stage][-log-sum-exp in base 2, -delta]
+    __attribute__((aligned(1024))) char tiles[2][2][kTile];    // [stage][Q, dO]
+    __attribute__((aligned(16))) float p[kPairs][4][64][4];  // P of a pair's keys, in accumulator order
+    __attribute__((aligned(16))) float stat[2][2][kT];       // [stage], as Params::stats
   };
   // What a workgroup works on: tiles tbase .. tbase + tcount - 1 of each head of the group
-  // as one list, its entries i0 .. i1 - 1; keys from kfirst on.
+  // as one list, its entries i0 .. i1 - 1; a pair's keys from kfirst on; where its sums go
+  // as a share (null: to the outputs).
   struct Work {
     int b, hk, kfirst, tbase, tcount, i0, i1, nq;
-    bool far;  // the 32 keys from kfirst on, a pair of waves each 32 rows of the tiles
-    float* part;
+    bool idle;  // the pair only helps to load
+    int apart;  // with a share: the keys below this one are the shares', the others go to the outputs
+    float* share;
   };
 
   // ROLE 0: P and dV; 1: dS and dK.
@@ -186,32 +274,23 @@ struct Keys {
     const int lane = threadIdx.x & 63, h2 = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % kPairs;
     const int len = length_of(p, w.b);
-    const int kw = w.far ? w.kfirst : w.kfirst + pair * 32, key = kw + (lane & 31);
+    const int kw = w.kfirst, key = kw + (lane & 31);
     const int G = p.H / p.Hkv;
     const float c = p.scale * kLog2e;
 
-    F kf[DP / 16];  // K (ROLE 0) or V
-    {
-      const Mat3& m = ROLE == 0 ? p.k : p.v;
-      const T* K = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) kf[s] = Tl::frag_global(K, s, h2, p.D, key < len);
-    }
-    tile::settle(kf);
     tile::Loader<T, DP, kT, kNW> lq, lg;
     lq.init(static_cast<uint32_t>(p.q.ss * Tl::kEs), p.D, wave, lane);
     lg.init(static_cast<uint32_t>(p.dout.ss * Tl::kEs), p.D, wave, lane);
-    float st = 0.f;  // this thread's entry of the next tile's statistics
     int tn = w.tbase + w.i0 % max(w.tcount, 1), tc = tn;  // the tile that issue() loads next, the tile worked on
     const int h0 = w.hk * G + w.i0 / max(w.tcount, 1);
     // Its head's rows; the heads of a group follow one another by a head stride.
     tile::Rows Q = rows_of<T>(p.q, w.b, h0, w.nq), dO = rows_of<T>(p.dout, w.b, h0, w.nq);
-    const float* stats = (threadIdx.x < kT ? p.lse : p.ndelta) + (static_cast<int64_t>(w.b) * p.H + h0) * p.Sq;
-    const float sf = threadIdx.x < kT ? -kLog2e : 1.f, sa = kF16 && threadIdx.x < kT ? 8.f : 0.f;
+    // Lanes 0 .. 31: the queries' log-sum-exp, 32 .. 63: their delta.  (Rows past the
+    // queries, which nothing sees, take the last one's.)
+    const float* stats = p.stats + (lane < 32 ? 0 : static_cast<int64_t>(p.B) * p.H * p.Sq) +
+                         (static_cast<int64_t>(w.b) * p.H + h0) * p.Sq;
     auto issue = [&](int stage) {
-      // (Rows past the queries, which nothing sees, take the last one's: a load under a
-      // condition would be waited for at once.)
-      st = stats[min(tn * kT + static_cast<int>(threadIdx.x % kT), w.nq - 1)];
+      if (wave == 0) tile::load4(stats + min(tn * kT + (lane & 31), w.nq - 1), tile::lds_addr(lds.stat[stage]));
       const uint32_t la = lds0 + stage * (2 * kTile);
       lq.issue(Q, tn * kT, la, wave);
       lg.issue(dO, tn * kT, la + kTile, wave);
@@ -222,41 +301,46 @@ struct Keys {
         stats += p.Sq;
       }
     };
-    auto put = [&](int stage) {
-      if (threadIdx.x < 2 * kT) lds.stat[stage][threadIdx.x / kT][threadIdx.x % kT] = __builtin_fmaf(st, sf, sa);
-    };
+    if (w.i0 < w.i1) issue(0);  // (waited for together with the rows below)
 
+    F kf[DP / 16];  // K (ROLE 0) or V
+    {
+      const Mat3& m = ROLE == 0 ? p.k : p.v;
+      const T* K = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) kf[s] = Tl::frag_global(K, s, h2, p.D, key < len);
+    }
+    tile::settle(kf);
     f32x16 sum[DP / 32];  // dV (ROLE 0) or dK
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) sum[db] = tile::splat(0.f);
 
     // Entry i from stage ST, known when compiled.
     auto step = [&](auto stage, int i) {
-      constexpr int ST = decltype(stage)::value;
+      constexpr int ST = decltype(stage)::value, ND = DP / 32;
       tile::landed_barrier();  // the tile is there; nobody reads the other stage or P any more
       if (i + 1 < w.i1) issue(1 - ST);
-      const int t0 = p.q_start + tc * kT;  // the tile's first position
+      const int p0 = p.q_start + tc * kT;  // the tile's first position
       if (++tc == w.tbase + w.tcount) tc = w.tbase;
-      f32x16 x[kT / 32];
-      F pf[kT / 32][2];
-      bool on[kT / 32];
-#pragma unroll
-      for (int rb = 0; rb < kT / 32; ++rb) {
-        const int p0 = t0 + 32 * rb;
-        on[rb] = !(p0 + 31 < kw || (p0 >= kw + 31 + p.window && kw >= p.sinks) || p0 - p.q_start >= w.nq) &&
-                 (!w.far || rb == pair);
-        if (!on[rb]) continue;
-        const char* tl = lds.tiles[ST][ROLE] + 32 * rb * Tl::kRow;
-        const float* ps = &lds.stat[ST][ROLE][32 * rb + 4 * h2];
+      const bool on = !(p0 + 31 < kw || (p0 >= kw + 31 + p.window && kw >= p.sinks) || p0 - p.q_start >= w.nq || w.idle);
+      float4* pp = reinterpret_cast<float4*>(lds.p[pair]);
+      f32x16 x;
+      F pf[2];
+      if (on) {
+        const char* t1 = lds.tiles[ST][ROLE];
+        const float* ps = &lds.stat[ST][ROLE][4 * h2];
         f32x16 stat;
 #pragma unroll
         for (int v = 0; v < 16; ++v) stat[v] = ps[(v >> 2) * 8 + (v & 3)];
-        x[rb] = ROLE == 0 ? tile::splat(0.f) : stat;
-        tile::pipelined<Tl::kRow, F, DP / 16>([&](int s) { return Tl::frag_row(tl, s, lane); },
-                                    [&](int s, const F& a) { x[rb] = tile::mma<T>(a, kf[s], x[rb]); });
+        x = ROLE == 0 ? tile::splat(0.f) : stat;
+        tile::pipelined<Tl::kRow, F, DP / 16>([&](int s) { return Tl::frag_row(t1, s, lane); },
+                                              [&](int s, const F& a) {
+                                                if (sizeof(T) == 4 && 16 * s >= p.D) return;
+                                                x = tile::mma<T>(a, kf[s], x);
+                                              });
         if constexpr (ROLE == 0) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v) x[rb][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[rb][v], c, stat[v]));
+          for (int v = 0; v < 16; ++v) x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], c, stat[v]));
           if (p0 < kw + 31 || p0 + 31 - p.q_start >= w.nq || (p0 + 31 >= kw + p.window && kw + 31 >= p.sinks)) {
             asm volatile("");  // a branch: most tiles need no mask
             // Rows key - p0 .. min(end, key + window) - p0 - 1 see the key.
@@ -264,54 +348,45 @@ struct Keys {
             const int first = key - p0 - 4 * h2, last = (key < p.sinks ? end : min(end, key + p.window)) - p0 - 4 * h2;
             const uint32_t bits = low_bits(last) & ~low_bits(first);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) x[rb][v] = select_bit(bits, (v >> 2) * 8 + (v & 3), x[rb][v], 0.f);
+            for (int v = 0; v < 16; ++v) x[v] = select_bit(bits, (v >> 2) * 8 + (v & 3), x[v], 0.f);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(lds.p[pair][rb][j][lane]) =
-                make_float4(x[rb][4 * j], x[rb][4 * j + 1], x[rb][4 * j + 2], x[rb][4 * j + 3]);
-#pragma unroll
-          for (int s = 0; s < 2; ++s) pf[rb][s] = tile::pack<T>(x[rb], s);
+          for (int j = 0; j < 4; ++j) pp[64 * j + lane] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+          pf[0] = tile::pack<T>(x, 0);
+          pf[1] = tile::pack<T>(x, 1);
         }
       }
       // P is there (the next tile's DMA stays in flight).
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (!on) return;
+      if constexpr (ROLE == 1) {
+        const float f = kF16 ? p.scale * 0x1p-8f : 1.f;
 #pragma unroll
-      for (int rb = 0; rb < kT / 32; ++rb) {
-        if (!on[rb]) continue;
-        if constexpr (ROLE == 1) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 pv = *reinterpret_cast<const float4*>(lds.p[pair][rb][j][lane]);
-            const float f = kF16 ? p.scale * 0x1p-8f : 1.f;
-            x[rb][4 * j] *= kF16 ? pv.x * f : pv.x;
-            x[rb][4 * j + 1] *= kF16 ? pv.y * f : pv.y;
-            x[rb][4 * j + 2] *= kF16 ? pv.z * f : pv.z;
-            x[rb][4 * j + 3] *= kF16 ? pv.w * f : pv.w;
-          }
-#pragma unroll
-          for (int s = 0; s < 2; ++s) pf[rb][s] = tile::pack<T>(x[rb], s);
+        for (int j = 0; j < 4; ++j) {
+          const float4 pv = pp[64 * j + lane];
+          x[4 * j] *= kF16 ? pv.x * f : pv.x;
+          x[4 * j + 1] *= kF16 ? pv.y * f : pv.y;
+          x[4 * j + 2] *= kF16 ? pv.z * f : pv.z;
+          x[4 * j + 3] *= kF16 ? pv.w * f : pv.w;
         }
-        const char* tl = lds.tiles[ST][1 - ROLE] + 32 * rb * Tl::kRow;  // dO for dV, Q for dK
-        constexpr int ND = DP / 32;
-        tile::pipelined<Tl::kRow, F, 2 * ND>(
-            [&](int j) { return Tl::frag_tr(tl + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
-            [&](int j, const F& a) { sum[j % ND] = tile::mma<T>(a, pf[rb][j / ND], sum[j % ND]); });
+        pf[0] = tile::pack<T>(x, 0);
+        pf[1] = tile::pack<T>(x, 1);
       }
-      if (i + 1 < w.i1) put(1 - ST);
+      const char* t2 = lds.tiles[ST][1 - ROLE];  // dO for dV, Q for dK
+      tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(t2 + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
+                                           [&](int j, const F& a) {
+                                             if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
+                                             sum[j % ND] = tile::mma<T>(a, pf[j / ND], sum[j % ND]);
+                                           });
     };
-    if (w.i0 < w.i1) {
-      issue(0);
-      put(0);
-    }
     for (int i = w.i0; i < w.i1; i += 2) {
       step(std::integral_constant<int, 0>{}, i);
       if (i + 1 < w.i1) step(std::integral_constant<int, 1>{}, i + 1);
     }
 
-    if (w.far ? pair < kT / 32 : w.part && kw < p.sinks) {  // shares of sinks' sums: [dk, dv][32 keys][D]
-      const int64_t block = w.far ? 0 : kw / 32 * p.far_stride;
-      float* to = w.part + block + (static_cast<int64_t>(w.far ? pair : 0) * 64 + (ROLE == 0 ? 32 : 0) + (lane & 31)) * p.D;
+    if (w.idle) return;
+    if (w.share) {  // [dk, dv][32 keys][D] in fp32
+      float* to = w.share + ((ROLE == 0 ? 32 : 0) + (lane & 31)) * static_cast<int64_t>(p.D);
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -320,7 +395,7 @@ struct Keys {
           if (d < p.D) tile::store4(to + d, sum[db][4 * g], sum[db][4 * g + 1], sum[db][4 * g + 2], sum[db][4 * g + 3]);
         }
     }
-    if (w.far || (w.part && key < p.sinks) || key >= p.Sk) return;
+    if ((w.share && key < w.apart) || key >= p.Sk) return;
     const Mat3& m = ROLE == 0 ? p.dv : p.dk;
     T* out = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
     const float f = ROLE == 0 ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
@@ -338,67 +413,82 @@ struct Keys {
   }
 };
 
-// One past the last tile (of kT rows) of queries that see, through their windows, a key of
-// the block at k0.
-__device__ __host__ __forceinline__ int near_end(const Params& p, int k0, int kT) {
+// One past the last tile of queries that see, through their windows, a key of the
+// workgroup's at k0.
+constexpr int kT = 32;
+__device__ __host__ __forceinline__ int near_end(const Params& p, int k0) {
   const int64_t last = static_cast<int64_t>(k0) + kKeys - 1 + p.window - p.q_start;  // one past the last such query
   const int64_t tiles = (p.Sq + kT - 1) / kT;
   return static_cast<int>(last <= 0 ? 0 : (last + kT - 1) / kT < tiles ? (last + kT - 1) / kT : tiles);
 }
 
+// A workgroup has 64 keys and every tile of queries that sees any of them, except
+//   * far: every query sees the sinks, so their keys' sums run over the whole sequence, not
+//     over a window; the queries beyond the window of the sinks' workgroup are left to
+//     workgroups of their own, which have 32 sinks and a chunk of those tiles each;
+//   * chunks without far (grids of few workgroups): a chunk of the tiles.
+// What several workgroups sum is joined in fp32, in a fixed order.
 template <typename T, int DP>
-__global__ __launch_bounds__(128 * KPAIRS, 2) void dkv_kernel(Params p) {
+__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128 ? 2 : 4)) void dkv_kernel(Params p) {
   using K = Keys<T, DP>;
-  constexpr int kT = K::kT;
   __shared__ typename K::Lds lds;
   const int nbh = p.B * p.Hkv, G = p.H / p.Hkv;
-  const int bh = blockIdx.x % nbh, at_ = blockIdx.x / nbh;
+  const int bh = spread(blockIdx.x % nbh, nbh), at_ = blockIdx.x / nbh;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % K::kPairs;
   typename K::Work w;
   w.b = bh / p.Hkv;
   w.hk = bh % p.Hkv;
   const int len = length_of(p, w.b);
   w.nq = max(0, min(p.Sq, len - p.q_start));  // queries that exist
   const int tiles = (w.nq + kT - 1) / kT;
-  w.part = p.far_blocks ? p.far + static_cast<int64_t>(bh) * p.far_blocks * p.far_stride : nullptr;
+  const int64_t one = 64 * static_cast<int64_t>(p.D);  // floats of a share
   const int blocks = (p.Sk + kKeys - 1) / kKeys;
-  w.far = at_ >= blocks;  // last: the shortest
-  if (w.far) {
+  float* share = p.share + static_cast<int64_t>(bh) * p.share_blocks * p.share_stride;
+  if (p.far && at_ >= blocks) {
     // Chunk ck of the queries that see the 32 sinks from 32 sb through no window.
-    const int sb = (at_ - blocks) / p.far_chunks, ck = (at_ - blocks) % p.far_chunks;
+    const int sb = (at_ - blocks) / p.chunks, ck = (at_ - blocks) % p.chunks;
     w.kfirst = 32 * sb;
-    w.tbase = near_end(p, w.kfirst / kKeys * kKeys, kT);
+    w.tbase = near_end(p, w.kfirst / kKeys * kKeys);
     w.tcount = max(0, tiles - w.tbase);
-    w.i0 = min(w.tcount * G, ck * p.far_per);
-    w.i1 = min(w.tcount * G, w.i0 + p.far_per);
-    w.part += sb * p.far_stride + (1 + kT / 32 * ck) * (64 * static_cast<int64_t>(p.D));
+    w.i0 = min(w.tcount * G, ck * p.chunk);
+    w.i1 = min(w.tcount * G, w.i0 + p.chunk);
+    w.idle = pair > 0;
+    w.apart = p.Sk;
+    w.share = share + sb * p.share_stride + (1 + ck) * one;
   } else {
-    w.kfirst = at_ * kKeys;
-    w.tbase = max(0, w.kfirst - p.q_start) / kT;
-    const int te = w.kfirst >= len ? 0 : w.kfirst < p.sinks && !w.part ? tiles : min(tiles, near_end(p, w.kfirst, kT));
+    const bool split = !p.far && p.share_blocks > 0;
+    const int kb = split ? at_ / p.chunks : at_, ck = split ? at_ % p.chunks : 0, k0 = kb * kKeys;
+    w.kfirst = k0 + pair * 32;
+    w.tbase = max(0, k0 - p.q_start) / kT;
+    const int te = k0 >= len ? 0 : k0 < p.sinks && !p.far ? tiles : min(tiles, near_end(p, k0));
     w.tcount = max(0, te - w.tbase);
-    w.i0 = 0;
-    w.i1 = w.tcount * G;
+    const int n = w.tcount * G;
+    w.i0 = split ? min(n, ck * p.chunk) : 0;
+    w.i1 = split ? min(n, w.i0 + p.chunk) : n;
+    w.idle = w.kfirst >= p.Sk;
+    w.apart = p.far ? p.sinks : p.Sk;
+    w.share = w.kfirst < 32 * p.share_blocks ? share + w.kfirst / 32 * p.share_stride + ck * one : nullptr;
   }
-  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= K::kPairs) K::template run<1>(p, lds, w);
+  if (wave >= K::kPairs) K::template run<1>(p, lds, w);
   else K::template run<0>(p, lds, w);
 }
 
-// dk, dv of the sinks: the shares of their block and of the chunks, added in that order.
+// dk, dv of keys whose sums several workgroups hold: the shares, added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr bool kF16 = __is_same(T, f16_t);
-  const int vecs = p.D / 4, wgs = (p.far_blocks * 64 * vecs + 255) / 256;  // workgroups of a (batch, kv head)
+  const int vecs = p.D / 4, wgs = (p.share_blocks * 64 * vecs + 255) / 256;  // workgroups of a (batch, kv head)
   const int bh = blockIdx.x / wgs, b = bh / p.Hkv, hk = bh % p.Hkv;
   const int e = blockIdx.x % wgs * 256 + threadIdx.x;
   const int row = e / vecs, d = e % vecs * 4;  // row: block, then [dk, dv], then key
-  const int sb = row / 64, which = row / 32 % 2, key = sb * 32 + row % 32;
-  if (key >= p.sinks || sb >= p.far_blocks) return;
-  const float* part = p.far + (static_cast<int64_t>(bh) * p.far_blocks + sb) * p.far_stride +
+  const int kb = row / 64, which = row / 32 % 2, key = kb * 32 + row % 32;
+  if (kb >= p.share_blocks || key >= (p.far ? p.sinks : p.Sk)) return;
+  const float* part = p.share + (static_cast<int64_t>(bh) * p.share_blocks + kb) * p.share_stride +
                       (which * 32 + row % 32) * static_cast<int64_t>(p.D) + d;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int i = 0; i < p.far_shares; ++i) {
-    const float4 v = *reinterpret_cast<const float4*>(part + i * (2 * 32 * static_cast<int64_t>(p.D)));
+  for (int i = 0; i < p.shares; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(part + i * (64 * static_cast<int64_t>(p.D)));
     a[0] += v.x;
     a[1] += v.y;
     a[2] += v.z;
@@ -411,37 +501,53 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
                live ? a[3] * f : 0.f);
 }
 
-// The workgroups for the queries that see sinks through no window: none unless they are
-// as many as a block's own tiles, else in chunks of a block's tiles (each of half its
-// work or less).  Fills p's far fields; returns the floats of the shares.
-static int64_t plan_far(Params* p, int row_bytes) {
-  const int kT = row_bytes > 256 ? 32 : KTILE;
+// How dkv_kernel's work is dealt out (its comment).  Fills p's share fields; returns the
+// floats of the shares.
+static int64_t plan_shares(Params* p) {
   const int G = p->H / p->Hkv;
-  const int beyond = (p->Sq + kT - 1) / kT - near_end(*p, 0, kT);
-  const int own = (std::min(p->window, p->Sq) + kKeys) / kT + 1;
-  if (p->sinks == 0 || beyond < own) return 0;
-  p->far_blocks = (p->sinks + 31) / 32;
-  p->far_per = FARPER / kT;
-  p->far_chunks = (beyond * G + p->far_per - 1) / p->far_per;
-  p->far_shares = 1 + kT / 32 * p->far_chunks;
-  p->far_stride = static_cast<int64_t>(p->far_shares) * 64 * p->D;
-  return static_cast<int64_t>(p->B) * p->Hkv * p->far_blocks * p->far_stride;
-}
-static int64_t plan_far(Params* p, bool f32) {
-  return plan_far(p, (p->D <= 64 ? 64 : p->D <= 128 ? 128 : 256) * (f32 ? 4 : 2));
+  const int tiles = (p->Sq + kT - 1) / kT;
+  const int beyond = p->sinks > 0 ? tiles - near_end(*p, 0) : 0;
+  // Tiles of the first, and with it of the longest list of a head.
+  const int own = std::min(tiles, (std::min(p->window, p->Sq) + kKeys) / kT + 1);
+  const int64_t grid = static_cast<int64_t>((p->Sk + kKeys - 1) / kKeys) * p->B * p->Hkv;
+  if (beyond >= own) {
+    p->far = true;
+    p->share_blocks = (p->sinks + 31) / 32;
+    p->chunk = 8;
+    p->chunks = (beyond * G + p->chunk - 1) / p->chunk;
+    p->shares = 1 + p->chunks;
+  } else if (grid < 256) {
+    // Few workgroups: chunks of at least 4 tiles, towards 512 workgroups.
+    const int64_t longest = static_cast<int64_t>(p->sinks > 0 ? tiles : own) * G;
+    const int64_t goal = std::min<int64_t>(grid > 0 ? (512 + grid - 1) / grid : 1, longest / 4);
+    if (goal > 1) {
+      p->chunk = static_cast<int>((longest + goal - 1) / goal);
+      p->chunks = static_cast<int>((longest + p->chunk - 1) / p->chunk);
+      p->share_blocks = (p->Sk + 31) / 32;
+      p->shares = p->chunks;
+    }
+  }
+  p->share_stride = static_cast<int64_t>(p->shares) * 64 * p->D;
+  return static_cast<int64_t>(p->B) * p->Hkv * p->share_blocks * p->share_stride;
 }
 
-// Floats of delta, a whole number of 16 bytes.
-static int64_t delta_floats(const Params& p) { return (static_cast<int64_t>(p.B) * p.H * p.Sq + 3) / 4 * 4; }
+// Floats of the statistics, a whole number of 16 bytes.
+static int64_t stats_floats(const Params& p) { return (static_cast<int64_t>(p.B) * p.H * p.Sq * 2 + 3) / 4 * 4; }
 
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
-  const dim3 gq(static_cast<unsigned>((p.Sq + kCols - 1) / kCols * p.B * p.H));
-  const dim3 gk(static_cast<unsigned>(((p.Sk + kKeys - 1) / kKeys + p.far_blocks * p.far_chunks) * p.B * p.Hkv));
-  if (p.Sq > 0) hipLaunchKernelGGL((dq_kernel<T, DP>), gq, dim3(256), 0, s, p);
-  hipLaunchKernelGGL((dkv_kernel<T, DP>), gk, dim3(128 * KPAIRS), 0, s, p);
-  if (p.far_blocks)
-    hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>((p.far_blocks * 64 * (p.D / 4) + 255) / 256) * p.B * p.Hkv),
+  const int nbh = p.B * p.Hkv, blocks = (p.Sk + kKeys - 1) / kKeys;
+  const int wgs = p.far ? blocks + p.share_blocks * p.chunks : p.share_blocks ? blocks * p.chunks : blocks;
+  // dq_few_kernel by the forward kernels' rule.
+  const int64_t bh = static_cast<int64_t>(p.B) * p.H, few = (p.Sq + 31) / 32 * bh;
+  constexpr int64_t kMost = few_most(sizeof(T), DP);
+  if (p.Sq > 0 && few <= kMost)
+    hipLaunchKernelGGL((dq_few_kernel<T, DP>), dim3(static_cast<unsigned>(few)), dim3(256), 0, s, p);
+  else if (p.Sq > 0)
+    hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(static_cast<unsigned>((p.Sq + kCols - 1) / kCols * bh)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(static_cast<unsigned>(wgs) * nbh), dim3(256), 0, s, p);
+  if (p.share_blocks)
+    hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>((p.share_blocks * 64 * (p.D / 4) + 255) / 256) * nbh),
                        dim3(256), 0, s, p);
 }
 template <typename T>
@@ -461,7 +567,7 @@ extern "C" int64_t ghip_sdpa_window_bwd_workspace_bytes(int dtype, int64_t B, in
                                                         int64_t sinks) {
   win::Params p{};
   if (win::check_problem("", dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, 1.f, &p, nullptr)) return 0;
-  return (win::delta_floats(p) + win::plan_far(&p, dtype == GHIP_DTYPE_FLOAT32)) * 4;
+  return (win::stats_floats(p) + win::plan_shares(&p)) * 4;
 }
 
 extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
@@ -498,9 +604,9 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", kWhat);
   p.lse = const_cast<float*>(lse);
-  p.ndelta = static_cast<float*>(workspace);
-  p.far = p.ndelta + win::delta_floats(p);
-  win::plan_far(&p, dtype == GHIP_DTYPE_FLOAT32);
+  p.stats = static_cast<float*>(workspace);
+  p.share = p.stats + win::stats_floats(p);
+  win::plan_shares(&p);
   p.lens = lens;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GHIP_DTYPE_FLOAT32) win::launch<float>(p, s);
