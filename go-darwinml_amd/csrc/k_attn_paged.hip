@@ -67,55 +67,75 @@ struct Seen {
   __device__ __forceinline__ int tiles(int kt) const { return sink_tiles(kt) + (len - (lo & ~15) + kt - 1) / kt; }
 };
 
+// Sum of x over this lane and the lower ones: shifts within the rows of 16 lanes, then the
+// rows' totals broadcast to the rows after them (one VALU instruction a step).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
+  return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
+  x = dpp_add<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+
 // Where the tiles of the sequences lie in the common order (sequence, unit of heads,
-// tile).  A lane counts one sequence; scans over the wave give the places.
+// tile).  A lane counts one sequence of 64; a sequence has fewer than 2^26 tiles (the host
+// checks), so 64 of them fit 32 bits.
 template <int KT>
 struct Order {
-  int64_t total = 0;
+  int64_t total = 0;  // tiles of all sequences and units
   int lane, units;
-  int64_t n0, up0;  // the first 64 sequences' tiles, and their running sums
+  int len0;           // the first 64 sequences: lengths, tiles, running sums
+  uint32_t n0, up0;
   __device__ __forceinline__ Order(const Params& p, int units_) : lane(threadIdx.x & 63), units(units_) {
-    n0 = count(p, lane);
-    up0 = scan(n0);
-    total = __shfl(up0, 63, 64);
-    for (int b0 = 64; b0 < p.B; b0 += 64) total += __shfl(scan(count(p, b0 + lane)), 63, 64);
+    if (units == 0) return;
+    len0 = lane < p.B ? p.lens[lane] : 0;
+    n0 = Seen(p, len0).tiles(KT);
+    up0 = wave_scan(n0);
+    total = lane_of(up0, 63);
+    for (int b0 = 64; b0 < p.B; b0 += 64) total += lane_of(wave_scan(count(p, b0 + lane)), 63);
+    total *= units;
   }
-  __device__ __forceinline__ int64_t count(const Params& p, int b) const {
-    return b < p.B ? static_cast<int64_t>(Seen(p, p.lens[b]).tiles(KT)) * units : 0;
+  __device__ __forceinline__ uint32_t count(const Params& p, int b) const {
+    return b < p.B ? Seen(p, p.lens[b]).tiles(KT) : 0;
   }
-  __device__ __forceinline__ int64_t scan(int64_t x) const {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int64_t y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
-    }
-    return x;
+  __device__ __forceinline__ int length(const Params& p, int b) const {
+    return b < 64 ? static_cast<int>(lane_of(static_cast<uint32_t>(len0), b)) : p.lens[b];
   }
   // The sequence that place `at` < total lies in; *begin: where it begins.
   __device__ __forceinline__ int find(const Params& p, int64_t at, int64_t* begin) const {
     int64_t before = 0;
     for (int b0 = 0;; b0 += 64) {
-      const int64_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? scan(n) + before : up0;
-      const uint64_t over = __builtin_amdgcn_ballot_w64(up > at);
+      const uint32_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? wave_scan(n) : up0;
+      const uint64_t over = __builtin_amdgcn_ballot_w64((before + up) * units > at);
       if (over) {
         const int l = __builtin_ctzll(over);
-        *begin = __shfl(up - n, l, 64);
+        *begin = (before + lane_of(up - n, l)) * units;
         return b0 + l;
       }
-      before = __shfl(up, 63, 64);
+      before += lane_of(up, 63);
     }
   }
   // Where sequence b begins.
   __device__ __forceinline__ int64_t begin(const Params& p, int b) const {
     int64_t before = 0;
     for (int b0 = 0;; b0 += 64) {
-      const int64_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? scan(n) + before : up0;
-      if (b < b0 + 64) return __shfl(up - n, b - b0, 64);
-      before = __shfl(up, 63, 64);
+      const uint32_t n = b0 ? count(p, b0 + lane) : n0, up = b0 ? wave_scan(n) : up0;
+      if (b < b0 + 64) return (before + lane_of(up - n, b - b0)) * units;
+      before += lane_of(up, 63);
     }
   }
   __device__ __forceinline__ int64_t share() const {
-    const int64_t per = (total + kWorkers - 1) / kWorkers;
+    const int64_t per = total <= 0xffffffffLL ? static_cast<uint32_t>(total + kWorkers - 1) / kWorkers
+                                              : (total + kWorkers - 1) / kWorkers;
     return per < kMinTiles ? kMinTiles : per;
   }
 };
@@ -193,7 +213,7 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
 
   int b;
   int64_t at, end, begin;
-  const Order<KT> order(p, units);
+  const Order<KT> order(p, SPLIT ? units : 0);
   if constexpr (SPLIT) {
     const int64_t per = order.share();
     at = blockIdx.x * per;
@@ -208,7 +228,7 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
   const int64_t first = at;
 
   for (;;) {
-    const Seen seen(p, p.lens[b]);
+    const Seen seen(p, SPLIT ? order.length(p, b) : p.lens[b]);
     const int nt = seen.tiles(KT), nst = seen.sink_tiles(KT);
     int unit, ta, te;
     if constexpr (SPLIT) {
@@ -409,24 +429,22 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
 }
 
 // Joins the shares of units that several workers hold: a workgroup a (sequence, head),
-// the shares dealt out over groups of lanes that each hold a row of the output, their
-// sums added in the groups' order.  Sequences without a visible token, which no worker
-// holds, get zeros.
+// the shares dealt out over groups of lanes that each hold a row of the output and a
+// running maximum; the groups are added in order.  Sequences without a visible token,
+// which no worker holds, get zeros.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int KT = 8192 / (DP * static_cast<int>(sizeof(T)));
-  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes;
-  __shared__ float weight[kWorkers];
-  __shared__ float red[4];
+  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes, kAhead = 4;
+  __shared__ float stat[2][kGroups];
   __shared__ __attribute__((aligned(16))) float sums[kGroups][DP];
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = blockIdx.x, b = row / p.H, h = row % p.H, hk = h / G;
   const int unit = hk * blocks + (h - hk * G) / kHeads, hd = (h - hk * G) % kHeads;
   const int d = threadIdx.x % kLanes * 4, grp = threadIdx.x / kLanes;
   T* out = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + d;
   const Order<KT> order(p, units);
-  const int nt = Seen(p, p.lens[b]).tiles(KT);
+  const int nt = Seen(p, order.length(p, b)).tiles(KT);
   if (nt == 0) {
     if (grp == 0 && d < p.D) tile::store4(out, 0.f, 0.f, 0.f, 0.f);
     return;
@@ -438,52 +456,58 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
   auto slot = [&](int i) {
     return (2 * static_cast<int64_t>(w0 + i) + (i == 0 && u0 != w0 * per ? 1 : 0)) * p.unit_heads + hd;
   };
-  float mx = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    weight[i] = p.part_lse[slot(i)];
-    mx = fmaxf(mx, weight[i]);
-  }
-  mx = wave_max(mx);
-  if (lane == 0) red[wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const float ls = weight[i];
-    weight[i] = ls == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls - mx);  // (NaN stays NaN)
-    sum += weight[i];
-  }
-  sum = wave_sum(sum);
-  if (lane == 0) red[wave] = sum;
-  __syncthreads();
-  sum = (red[0] + red[1]) + (red[2] + red[3]);
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
-  if (d < p.D) {
-#pragma unroll 4
-    for (int i = grp; i < n; i += kGroups) {
-      const float f = weight[i];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(i) * p.D + d);
-      a[0] += f * v.x;
-      a[1] += f * v.y;
-      a[2] += f * v.z;
-      a[3] += f * v.w;
-    }
-    *reinterpret_cast<float4*>(&sums[grp][d]) = make_float4(a[0], a[1], a[2], a[3]);
-  }
-  __syncthreads();
-  if (grp == 0 && d < p.D) {
+  float a[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, sum = 0.f;
+  for (int i0 = grp; i0 < n; i0 += kAhead * kGroups) {  // kAhead shares' loads in flight
+    float ls[kAhead];
+    float4 v[kAhead];
 #pragma unroll
-    for (int i = 1; i < kGroups; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(&sums[i][d]);
-      a[0] += v.x;
-      a[1] += v.y;
-      a[2] += v.z;
-      a[3] += v.w;
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * kGroups;
+      ls[j] = i < n ? p.part_lse[slot(i)] : -INFINITY;
+      v[j] = i < n && d < p.D ? *reinterpret_cast<const float4*>(p.part_o + slot(i) * p.D + d) : make_float4(0, 0, 0, 0);
     }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    tile::store4(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
+    float m = mx;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) m = fmaxf(m, ls[j]);
+    const float old = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m);
+    sum *= old;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] *= old;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float f = ls[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls[j] - m);  // (NaN stays NaN)
+      sum += f;
+      a[0] += f * v[j].x;
+      a[1] += f * v[j].y;
+      a[2] += f * v[j].z;
+      a[3] += f * v[j].w;
+    }
+    mx = m;
   }
+  *reinterpret_cast<float4*>(&sums[grp][d]) = make_float4(a[0], a[1], a[2], a[3]);
+  if (threadIdx.x % kLanes == 0) {
+    stat[0][grp] = mx;
+    stat[1][grp] = sum;
+  }
+  __syncthreads();
+  if (grp != 0 || d >= p.D) return;
+  float m = stat[0][0];
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) m = fmaxf(m, stat[0][i]);
+  sum = 0.f;
+  a[0] = a[1] = a[2] = a[3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const float f = stat[0][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[0][i] - m);
+    const float4 v = *reinterpret_cast<const float4*>(&sums[i][d]);
+    sum += f * stat[1][i];
+    a[0] += f * v.x;
+    a[1] += f * v.y;
+    a[2] += f * v.z;
+    a[3] += f * v.w;
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  tile::store4(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
 }
 
 template <typename T, int DP>
@@ -575,8 +599,9 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
     return set_error(err, GHIP_ERR_UNSUPPORTED,
                      "%s: needs a head dim that is a multiple of 8 up to 256 (float32: of 4 up to 128)", kWhat);
   constexpr int64_t kMost = int64_t{1} << 30;
-  if (num_pages > kMost || page_size > kMost || max_pages > kMost || page_size * max_pages > kMost || B * H > kMost)
-    return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: at most 2^30 pages, tokens of a sequence and heads", kWhat);
+  if (num_pages > kMost || page_size > kMost || max_pages > kMost || page_size * max_pages > kMost / 2 ||
+      B > kMost || H > kMost || B * H > kMost)
+    return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: at most 2^30 pages and heads and 2^29 tokens of a sequence", kWhat);
   if (B == 0) return GHIP_OK;
   if (!q || !o || !lens || !q_strides || !k_strides || !v_strides || !o_strides || !k_cache || !v_cache || !block_table)
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: null pointer", kWhat);
