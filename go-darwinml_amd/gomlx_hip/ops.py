@@ -272,10 +272,11 @@ def _launch(dev: torch.device, name: str, stream, *args):
 def _one_device(first: torch.Tensor, *ts) -> torch.device:
     """The device that every tensor lies on."""
     dev = first.device
-    if dev.type != "cuda":
+    if not first.is_cuda:
         raise ValueError("gomlx_hip ops take device tensors")
+    n = dev.index
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != n:  # (-1: the host)
             raise ValueError(f"gomlx_hip: tensors on device {dev} and {t.device}")
     return dev
 
@@ -287,10 +288,9 @@ def _like(what: str, t: torch.Tensor, shape, dtype):
 
 def _ints(what: str, t, n: int):
     """A dense int32 [n] operand (None stays None)."""
-    if t is not None:
+    if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1)):
         _like(what, t, (n,), torch.int32)
-        if n > 1 and t.stride(0) != 1:
-            raise ValueError(f"{what}: must be contiguous")
+        raise ValueError(f"{what}: must be contiguous")
 
 
 _I3 = ctypes.c_int64 * 3
@@ -298,10 +298,10 @@ _I3 = ctypes.c_int64 * 3
 
 def _rows3(what: str, t: torch.Tensor):
     """The strides of a tensor's first three axes; the last one must be contiguous."""
-    st = t.stride()
-    if st[3] != 1 and t.shape[3] != 1:
+    b, h, s, d = t.stride()
+    if d != 1 and t.shape[3] != 1:
         raise ValueError(f"{what}: the head dim must be contiguous")
-    return _I3(st[0], st[1], st[2])
+    return _I3(b, h, s)
 
 
 def _window_shapes(q, k, v, q_start, lens):
@@ -382,16 +382,22 @@ def sdpa_window_grad(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     return dq, dk, dv
 
 
-def _paged_cache(what, k_cache, v_cache, block_table, B):
+def _check_cache(what, k_cache, v_cache, block_table, B, Hkv, D, dtype):
     """(num_pages, page_size, max_pages, table stride) of caches viewed as [page, Hkv, token, D]."""
-    if k_cache.dim() != 4:
+    shape = k_cache.shape
+    if len(shape) != 4:
         raise ValueError(f"{what}: the caches are [pages, Hkv, page_size, D]")
-    _like(f"{what}: v_cache", v_cache, k_cache.shape, k_cache.dtype)
+    pages, heads, size, dim = shape
+    if heads != Hkv or dim != D or k_cache.dtype != dtype:
+        _like(f"{what}: k_cache", k_cache, (pages, Hkv, size, D), dtype)
+    _like(f"{what}: v_cache", v_cache, shape, dtype)
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B:
         raise ValueError(f"{what}: block_table is int32 [{B}, pages of a sequence]")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+    step, one = block_table.stride()
+    per = block_table.shape[1]
+    if per > 1 and one != 1:
         raise ValueError(f"{what}: a sequence's table entries must be contiguous")
-    return k_cache.shape[0], k_cache.shape[2], block_table.shape[1], block_table.stride(0)
+    return pages, size, per, step
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -401,10 +407,12 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     counts[b] (None: S), of the sequences whose pages block_table [B, pages] names.  Wraps
     ghip_kv_append."""
     dev = _one_device(k, v, k_cache, v_cache, block_table, starts, counts)
-    B, Hkv, S, D = k.shape
-    _like("kv_append: v", v, k.shape, k.dtype)
-    pages, size, per, ts = _paged_cache("kv_append", k_cache, v_cache, block_table, B)
-    _like("kv_append: k_cache", k_cache, (pages, Hkv, size, D), k.dtype)
+    shape = k.shape
+    if len(shape) != 4:
+        raise ValueError("kv_append: k / v [B, Hkv, S, D] are needed")
+    B, Hkv, S, D = shape
+    _like("kv_append: v", v, shape, k.dtype)
+    pages, size, per, ts = _check_cache("kv_append", k_cache, v_cache, block_table, B, Hkv, D, k.dtype)
     _ints("kv_append: starts", starts, B)
     _ints("kv_append: counts", counts, B)
     _launch(dev, "ghip_kv_append", stream, k.element_size(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
@@ -428,10 +436,11 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     workspace (`workspace`, or one allocated here), so the sequences' tokens are dealt out
     over the card.  Wraps ghip_sdpa_paged."""
     dev = _one_device(q, k_cache, v_cache, block_table, lens, out, workspace)
+    if q.dim() != 3:
+        raise ValueError("sdpa_paged: q [B, H, D] is needed")
     B, H, D = q.shape
-    pages, size, per, ts = _paged_cache("sdpa_paged", k_cache, v_cache, block_table, B)
-    Hkv = k_cache.shape[1]
-    _like("sdpa_paged: k_cache", k_cache, (pages, Hkv, size, D), q.dtype)
+    Hkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    pages, size, per, ts = _check_cache("sdpa_paged", k_cache, v_cache, block_table, B, Hkv, D, q.dtype)
     _ints("sdpa_paged: lens", lens, B)
     if out is None:
         out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
