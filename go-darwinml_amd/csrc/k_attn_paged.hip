@@ -570,10 +570,19 @@ __global__ __launch_bounds__(256) void append_kernel(Append p) {
 
 using namespace ghip;
 
+// No workspace, so a wave for each unit: caches of at most 4 tiles a sequence, or 12 with
+// 512 units or more.  bf16, 32 heads over 8, us a call split / unsplit: 16 sequences of 128
+// tokens (4 tiles) 11.7 / 10.6, of 192 12.1 / 13.9; 64 sequences of 384 (12 tiles) 30.3 /
+// 28.5, of 512 36.1 / 36.7.  (More units hide the two kernels' latencies, not the second
+// launch.)
 extern "C" int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                    int64_t page_size, int64_t max_pages) {
-  if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || page_size <= 0 || max_pages <= 0) return 0;
-  return 2 * static_cast<int64_t>(paged::kWorkers) * std::min<int64_t>(paged::kHeads, H / Hkv) * (D + 1) * 4;
+  if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 256 || page_size <= 0 || max_pages <= 0) return 0;
+  const int64_t heads = H / Hkv, units = B * Hkv * ((heads + paged::kHeads - 1) / paged::kHeads);
+  const int64_t row = (D <= 64 ? 64 : D <= 128 ? 128 : 256) * (dtype == GHIP_DTYPE_FLOAT32 ? 4 : 2);
+  const double tokens = static_cast<double>(page_size) * static_cast<double>(max_pages);
+  if (tokens * row <= 8192. * (units >= 512 ? 12 : 4)) return 0;
+  return 2 * static_cast<int64_t>(paged::kWorkers) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4;
 }
 
 extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o, int64_t B,
@@ -633,8 +642,8 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
   p.sinks = static_cast<int>(sinks > kMost ? kMost : sinks);
   p.scale = scale;
   p.unit_heads = static_cast<int>(std::min<int64_t>(paged::kHeads, H / Hkv));
-  if (workspace) {
-    const int64_t need = ghip_sdpa_paged_workspace_bytes(dtype, B, H, Hkv, D, page_size, max_pages);
+  const int64_t need = workspace ? ghip_sdpa_paged_workspace_bytes(dtype, B, H, Hkv, D, page_size, max_pages) : 0;
+  if (need > 0) {
     if (workspace_bytes < need)
       return set_error(err, GHIP_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed", kWhat,
                        static_cast<long long>(workspace_bytes), static_cast<long long>(need));
