@@ -329,12 +329,19 @@ struct Keys {
       if (on) {
         const char* t1 = lds.tiles[ST][ROLE];
         const float* ps = &lds.stat[ST][ROLE][4 * h2];
-        f32x16 stat;
+        if constexpr (ROLE == 0) {
+          x = tile::splat(0.f);
+        } else {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) stat[v] = ps[(v >> 2) * 8 + (v & 3)];
-        x = ROLE == 0 ? tile::splat(0.f) : stat;
+          for (int v = 0; v < 16; ++v) x[v] = ps[(v >> 2) * 8 + (v & 3)];
+        }
+        f32x16 stat;
         tile::pipelined<Tl::kRow, F, DP / 16>([&](int s) { return Tl::frag_row(t1, s, lane); },
                                               [&](int s, const F& a) {
+                                                // (The statistics as the last operands leave registers free.)
+                                                if (ROLE == 0 && s == DP / 16 - 2)
+#pragma unroll
+                                                  for (int v = 0; v < 16; ++v) stat[v] = ps[(v >> 2) * 8 + (v & 3)];
                                                 if (sizeof(T) == 4 && 16 * s >= p.D) return;
                                                 x = tile::mma<T>(a, kf[s], x);
                                               });
@@ -429,7 +436,7 @@ __device__ __host__ __forceinline__ int near_end(const Params& p, int k0) {
 //   * chunks without far (grids of few workgroups): a chunk of the tiles.
 // What several workgroups sum is joined in fp32, in a fixed order.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128 ? 2 : 4)) void dkv_kernel(Params p) {
+__global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 128 ? 3 : 4)) void dkv_kernel(Params p) {
   using K = Keys<T, DP>;
   __shared__ typename K::Lds lds;
   const int nbh = p.B * p.Hkv, G = p.H / p.Hkv;
@@ -510,10 +517,14 @@ static int64_t plan_shares(Params* p) {
   // Tiles of the first, and with it of the longest list of a head.
   const int own = std::min(tiles, (std::min(p->window, p->Sq) + kKeys) / kT + 1);
   const int64_t grid = static_cast<int64_t>((p->Sk + kKeys - 1) / kKeys) * p->B * p->Hkv;
-  if (beyond >= own) {
+  if (beyond > 0 && beyond >= own && p->sinks <= 128) {
+    // (More sinks are many workgroups of their own.)  Chunks of 8 tiles, us a call with 4 /
+    // 8 / 16 / 32: padded batch of 12 heads of 64, window 128, 50.5 / 51.9 / 56 / 65; 4 x 16
+    // heads, 2048 tokens, window 512, 200 / 197 / 200 / 209.  The shares take half of q's
+    // memory.
     p->far = true;
     p->share_blocks = (p->sinks + 31) / 32;
-    p->chunk = 8;
+    p->chunk = 8 * p->share_blocks;
     p->chunks = (beyond * G + p->chunk - 1) / p->chunk;
     p->shares = 1 + p->chunks;
   } else if (grid < 256) {
@@ -582,6 +593,8 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
   win::Params p{};
   if (int rc = win::check_problem(kWhat, dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, scale, &p, err)) return rc;
   if (B == 0 || Sk == 0) return GHIP_OK;
+  if ((Sq / 32 + 1) * (H / Hkv) > 0x7fffffffLL)
+    return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   const struct {
     const char* name;
     const void* ptr;

@@ -313,7 +313,8 @@ int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v,
  * tokens starts[b] + i, i < min(S, counts[b]) (counts NULL: S), copied bit for bit; other
  * rows of the cache stay as they are.  Tokens at a negative position, past max_pages or on
  * a page outside [0, num_pages) are skipped.  Two tokens that land in one row race.
- * Elements of 1, 2, 4 or 8 bytes, any alignment of whole elements. */
+ * Elements of 1, 2, 4 or 8 bytes, any alignment of whole elements; at most 65535 sequences
+ * and 2^30 tokens a sequence. */
 int ghip_kv_append(int elem_bytes, const void* k, const void* v, void* k_cache, void* v_cache,
                    int64_t B, int64_t S, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
                    int64_t max_pages, const int32_t* block_table, int64_t table_stride,
@@ -333,8 +334,8 @@ int ghip_kv_append(int elem_bytes, const void* k, const void* v, void* k_cache, 
  * does not depend on the lengths) the tiles of all sequences are dealt out evenly over the
  * card and joined by log-sum-exp in a second kernel, in a fixed order; without one each
  * (sequence, kv head) is one workgroup's.  0 bytes: the cache's sequences are too short to
- * split.  Calls that share a workspace must be ordered (one stream).  No reference op: the
- * reference's decoding reads dense caches. */
+ * split.  Calls that share a workspace must be ordered (one stream).  At most 2^29 tokens a
+ * sequence.  No reference op: the reference's decoding reads dense caches. */
 int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                         int64_t page_size, int64_t max_pages);
 int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,

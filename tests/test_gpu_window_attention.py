@@ -185,6 +185,38 @@ def test_same_bits_and_streams_and_graph(cuda):
         assert all(torch.equal(x, y) for x, y in zip(got, flat(want)))
 
 
+@pytest.mark.parametrize("G", [1, 3])
+@pytest.mark.parametrize("sinks", [1, 33, 64, 128, 129])
+def test_many_sinks(cuda, sinks, G):
+    """The gradient's ways of summing sinks' keys: chunks in one to four blocks of 32, and
+    beyond 128 sinks whole lists; sequences whose queries end before, inside and behind the
+    windows of the sinks' blocks."""
+    for lens in (None, (700, 90, 300)):
+        case = (3, 2 * G, 2, 700, 700, 0, 40, sinks, lens)
+        q, k, v, do = tensors(cuda, case, BF16, 64, seed=sinks)
+        check(cuda, case, q, k, v, do, 0.125, *run_both(q, k, v, do, 0.125, case, lens_of(cuda, case)))
+
+
+def test_a_stream_of_the_callers(cuda):
+    """`stream` given as a handle while torch's current stream is another: the workspace
+    stays the call's until that stream is done with it."""
+    case = (2, 8, 2, 300, 300, 0, 100, 4, None)
+    q, k, v, do = tensors(cuda, case, BF16, 128)
+    o, lse, want = run_both(q, k, v, do, 0.09, case, None)
+    s = torch.cuda.Stream()
+    outs = [torch.empty_like(t) for t in want]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        ops.sdpa_window_grad(do, q, k, v, o, lse, 0.09, 100, 4, q_start=0, outs=outs, stream=s.cuda_stream)
+        junk = [torch.full((1 << 20,), float("nan"), device=cuda) for _ in range(8)]
+        s.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        del junk
+
+
 def test_rows_far_apart(cuda):
     """A slice of K and V over more than 4 GiB: 64-bit offsets."""
     Sk, D, step = 34000, 128, 1 << 16

@@ -88,6 +88,28 @@ def test_nothing_to_do():
     assert _lib.load().ghip_sdpa_paged_workspace_bytes(BF16, 0, 4, 2, 64, 16, 100) == 0
 
 
+def test_workspace_policy():
+    """Paged decoding splits caches of more than 4 tiles a sequence (of 8 KiB a kv head: 32
+    tokens of 128 16-bit values), or 12 with 512 (sequence, kv head, 16 heads) units; the
+    gradient's workspace holds the rows' two statistics and, where sinks' keys or few
+    workgroups are shared out, fp32 shares of at most half of q's bytes a block of sinks."""
+    ws = _lib.load().ghip_sdpa_paged_workspace_bytes
+    assert ws(BF16, 16, 32, 8, 128, 16, 8) == 0 and ws(BF16, 16, 32, 8, 128, 16, 9) == 2 * 1024 * 4 * 129 * 4
+    assert ws(F16, 64, 32, 8, 128, 64, 6) == 0 and ws(F16, 64, 32, 8, 128, 64, 7) > 0
+    assert ws(BF16, 1, 40, 2, 64, 16, 16) == 0 and ws(BF16, 1, 40, 2, 64, 16, 17) == 2 * 1024 * 16 * 65 * 4
+    assert ws(F32, 1, 8, 8, 128, 16, 4) == 0 and ws(F32, 1, 8, 8, 128, 16, 5) == 2 * 1024 * 129 * 4
+    gw = _lib.load().ghip_sdpa_window_bwd_workspace_bytes
+    assert gw(BF16, 4, 16, 16, 2048, 2048, 128, 0, 512, 0) == 2 * 4 * 16 * 2048 * 4
+    rows = 2 * 4 * 16 * 2048 * 4
+    assert 0 < gw(BF16, 4, 16, 16, 2048, 2048, 128, 0, 512, 4) - rows <= 4 * 16 * 2048 * 128
+    assert gw(BF16, 4, 16, 16, 2048, 2048, 128, 0, 512, 300) == rows  # many sinks: no shares
+    assert gw(BF16, 4, 16, 16, 2048, 2048, 128, 0, 0, 4) == rows      # no window: nothing lies beyond it
+    assert gw(BF16, 1, 2, 1, 512, 512, 128, 0, 0, 0) > 2 * 2 * 512 * 4  # 8 workgroups: chunks
+    for sizes in ((0, 5), (1, 1), (0, 0), (1, 700), (3, 3)):  # no or few queries
+        for window, sinks in ((0, 0), (1, 1), (0, 4), (7, 0), (3, 500)):
+            assert gw(F16, 1, 4, 2, *sizes, 64, 0, window, sinks) >= 2 * 4 * sizes[0] * 4
+
+
 def test_reference_gradient_against_differences():
     """attention_ref's formula in float64 against central differences of its forward: with
     h = 2^-16 their own error is about h^2 plus 2^-52 / h, below 1e-8 of values of order 1."""
