@@ -20,6 +20,9 @@
 namespace ghip {
 namespace tile {
 
+// Workgroups of 256 threads that one launch holds (HIP: fewer than 2^32 threads).
+constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -609,8 +609,9 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
                      "%s: needs a head dim that is a multiple of 8 up to 256 (float32: of 4 up to 128)", kWhat);
   constexpr int64_t kMost = int64_t{1} << 30;
   if (num_pages > kMost || page_size > kMost || max_pages > kMost || page_size * max_pages > kMost / 2 ||
-      B > kMost || H > kMost || B * H > kMost)
-    return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: at most 2^30 pages and heads and 2^29 tokens of a sequence", kWhat);
+      B > kMost || H > kMost || B * H > tile::kMostGroups)
+    return set_error(err, GHIP_ERR_UNSUPPORTED,
+                     "%s: at most 2^30 pages, 2^29 tokens of a sequence and fewer than 2^24 heads of all sequences", kWhat);
   if (B == 0) return GHIP_OK;
   if (!q || !o || !lens || !q_strides || !k_strides || !v_strides || !o_strides || !k_cache || !v_cache || !block_table)
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: null pointer", kWhat);
@@ -672,7 +673,7 @@ extern "C" int ghip_kv_append(int elem_bytes, const void* k, const void* v, void
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: bad sizes", kWhat);
   constexpr int64_t kMost = int64_t{1} << 30;
   if (num_pages > kMost || page_size > kMost || max_pages > kMost || page_size * max_pages > kMost || B > 65535 ||
-      S > kMost || Hkv > kMost || S * Hkv > kMost || D > (1 << 20) || S * Hkv * D > (kMost << 6))
+      S > kMost || Hkv > kMost || S * Hkv > kMost || D > (1 << 20))
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   if (B == 0 || S == 0) return GHIP_OK;
   if (!k || !v || !k_cache || !v_cache || !block_table || !starts || !k_strides || !v_strides || !k_cache_strides ||
@@ -705,6 +706,7 @@ extern "C" int ghip_kv_append(int elem_bytes, const void* k, const void* v, void
   p.num_pages = static_cast<int>(num_pages); p.page_size = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
   const int64_t n = S * Hkv * p.chunks;
+  if (n > tile::kMostGroups * 256) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(B));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (unit == 16) hipLaunchKernelGGL((paged::append_kernel<uint4>), grid, dim3(256), 0, s, p);

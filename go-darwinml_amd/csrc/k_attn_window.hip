@@ -295,7 +295,7 @@ int check_operand(const char* what, const char* name, int dtype, const void* ptr
     if (strides[i] < 0 || strides[i] % al != 0)
       return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s needs non-negative strides that are multiples of %d elements",
                        what, name, static_cast<int>(al));
-  if ((64 * strides[2] + 256) * es >= (int64_t{1} << 31))
+  if (strides[2] >= ((int64_t{1} << 31) / es - 256) / 64)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s needs a sequence stride below 32 MiB", what, name);
   if (reinterpret_cast<uintptr_t>(ptr) % (al * es) != 0)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s must be %d-byte aligned", what, name, static_cast<int>(al * es));
@@ -340,6 +340,8 @@ extern "C" int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, con
   win::Params p{};
   if (int rc = win::check_problem(kWhat, dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, scale, &p, err)) return rc;
   if (B == 0 || Sq == 0) return GHIP_OK;
+  if ((Sq + win::kBQ - 1) / win::kBQ * B * H > tile::kMostGroups)
+    return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   if (int rc = win::check_operand(kWhat, "q", dtype, q, q_strides, false, &p.q, err)) return rc;
   if (int rc = win::check_operand(kWhat, "k", dtype, k, k_strides, false, &p.k, err)) return rc;
   if (int rc = win::check_operand(kWhat, "v", dtype, v, v_strides, false, &p.v, err)) return rc;

@@ -508,9 +508,14 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
                live ? a[3] * f : 0.f);
 }
 
-// How dkv_kernel's work is dealt out (its comment).  Fills p's share fields; returns the
-// floats of the shares.
-static int64_t plan_shares(Params* p) {
+// Tiles of a group's heads as one list are counted in 32 bits.
+static bool list_too_long(int64_t Sq, int64_t G) { return (Sq / kT + 1) * G > 0x7fffffffLL; }
+
+// How dkv_kernel's work is dealt out (its comment): fills p's share fields.
+struct Plan {
+  int64_t groups, floats;  // workgroups, floats of the shares
+};
+static Plan plan_shares(Params* p) {
   const int G = p->H / p->Hkv;
   const int tiles = (p->Sq + kT - 1) / kT;
   const int beyond = p->sinks > 0 ? tiles - near_end(*p, 0) : 0;
@@ -539,7 +544,9 @@ static int64_t plan_shares(Params* p) {
     }
   }
   p->share_stride = static_cast<int64_t>(p->shares) * 64 * p->D;
-  return static_cast<int64_t>(p->B) * p->Hkv * p->share_blocks * p->share_stride;
+  const int64_t nbh = static_cast<int64_t>(p->B) * p->Hkv;
+  return {p->far ? grid + nbh * p->share_blocks * p->chunks : p->share_blocks ? grid * p->chunks : grid,
+          nbh * p->share_blocks * p->share_stride};
 }
 
 // Floats of the statistics, a whole number of 16 bytes.
@@ -578,7 +585,8 @@ extern "C" int64_t ghip_sdpa_window_bwd_workspace_bytes(int dtype, int64_t B, in
                                                         int64_t sinks) {
   win::Params p{};
   if (win::check_problem("", dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, 1.f, &p, nullptr)) return 0;
-  return (win::stats_floats(p) + win::plan_shares(&p)) * 4;
+  if (win::list_too_long(Sq, H / Hkv)) return 0;
+  return (win::stats_floats(p) + win::plan_shares(&p).floats) * 4;
 }
 
 extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
@@ -593,7 +601,8 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
   win::Params p{};
   if (int rc = win::check_problem(kWhat, dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, scale, &p, err)) return rc;
   if (B == 0 || Sk == 0) return GHIP_OK;
-  if ((Sq / 32 + 1) * (H / Hkv) > 0x7fffffffLL)
+  if (win::list_too_long(Sq, H / Hkv) || (Sq + win::kCols - 1) / win::kCols * B * H > tile::kMostGroups ||
+      win::plan_shares(&p).groups > tile::kMostGroups)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   const struct {
     const char* name;
@@ -619,7 +628,6 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
   p.lse = const_cast<float*>(lse);
   p.stats = static_cast<float*>(workspace);
   p.share = p.stats + win::stats_floats(p);
-  win::plan_shares(&p);
   p.lens = lens;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GHIP_DTYPE_FLOAT32) win::launch<float>(p, s);

@@ -277,6 +277,13 @@ def _kept(ws, stream):
     return ws
 
 
+def _given(what: str, ws):
+    """A caller's workspace: its bytes must lie one after the other."""
+    if not ws.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous")
+    return ws
+
+
 def _one_device(first: torch.Tensor, *ts) -> torch.device:
     """The device that every tensor lies on."""
     dev = first.device
@@ -381,7 +388,10 @@ def sdpa_window_grad(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
         _like("sdpa_window_grad: dq", dq, q.shape, q.dtype)
         _like("sdpa_window_grad: dk", dk, k.shape, q.dtype)
         _like("sdpa_window_grad: dv", dv, k.shape, q.dtype)
-    ws = _kept(sdpa_window_grad_workspace(q, k, window, sinks, q_start), stream) if workspace is None else workspace
+    if workspace is None:
+        ws = _kept(sdpa_window_grad_workspace(q, k, window, sinks, q_start), stream)
+    else:
+        ws = _given("sdpa_window_grad", workspace)
     _launch(dev, "ghip_sdpa_window_bwd", stream, dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
             o.data_ptr(), d_out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *dims,
             _rows3("q", q), _rows3("k", k), _rows3("v", v), _rows3("o", o), _rows3("d_out", d_out), _rows3("dq", dq),
@@ -458,8 +468,10 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         if t.stride(2) != 1 and D != 1:
             raise ValueError(f"sdpa_paged: {what}'s head dim must be contiguous")
     ws = None
-    if split:
-        ws = _kept(sdpa_paged_workspace(q, k_cache, block_table), stream) if workspace is None else workspace
+    if split and workspace is None:
+        ws = _kept(sdpa_paged_workspace(q, k_cache, block_table), stream)
+    elif split:
+        ws = _given("sdpa_paged", workspace)
     _launch(dev, "ghip_sdpa_paged", stream, dtype_code(q.dtype), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             out.data_ptr(), B, H, Hkv, D, pages, size, per, block_table.data_ptr(), ts, lens.data_ptr(),
             _I3(q.stride(0), q.stride(1)), _rows3("k_cache", k_cache), _rows3("v_cache", v_cache),

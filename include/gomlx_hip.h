@@ -266,8 +266,8 @@ int ghip_sdpa_fwd_masked_ws(int dtype, const void* q, const void* k, const void*
  * sequence's length is padding: o is 0 and lse -inf, and nothing that q, k or v hold at
  * padding reaches another row.  A NaN or an infinity in a token inside the length may
  * reach any row of its sequence.
- * Operands by ELEMENT strides (batch, head, sequence) as in ghip_sdpa_fwd, any of them
- * 0 or shared; BFLOAT16 or FLOAT16 with D a multiple of 8 up to 256, or FLOAT32 with a
+ * Operands by ELEMENT strides (batch, head, sequence) as in ghip_sdpa_fwd, those of the
+ * inputs 0 or shared as they like; outputs overlap nothing; BFLOAT16 or FLOAT16 with D a multiple of 8 up to 256, or FLOAT32 with a
  * multiple of 4 up to 128; strides multiples of 16 bytes (o: 4 elements), rows at
  * strides below 32 MiB, slices of any size.  lse [B, H, Sq] float32, dense, may be NULL.
  * q_start + Sq <= Sk.  Sums and statistics are fp32; the weights are rounded to the
@@ -286,7 +286,8 @@ int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, const void* v,
  *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T d_out
  * dk and dv are summed over the H / Hkv query heads of a kv head.  Sizes, types, strides,
  * lens and the mask as there; padding gets zero gradients (dk, dv for every key, dq for
- * every query) and what d_out and o hold there is not used.  workspace: device memory of
+ * every query) and what d_out and o hold there is not used; an input broadcast by a stride
+ * of 0 gets the gradient of each of its copies.  workspace: device memory of
  * ghip_sdpa_window_bwd_workspace_bytes() bytes, 16-byte aligned, written on `stream`
  * (calls that share one must be ordered).  Sums are fp32 and in a fixed order: the same
  * bits every run.  No reference op (GoMLX differentiates the composite). */
@@ -335,7 +336,8 @@ int ghip_kv_append(int elem_bytes, const void* k, const void* v, void* k_cache, 
  * card and joined by log-sum-exp in a second kernel, in a fixed order; without one each
  * (sequence, kv head) is one workgroup's.  0 bytes: the cache's sequences are too short to
  * split.  Calls that share a workspace must be ordered (one stream).  At most 2^29 tokens a
- * sequence.  No reference op: the reference's decoding reads dense caches. */
+ * sequence and fewer than 2^24 heads of all sequences.  No reference op: the reference's
+ * decoding reads dense caches. */
 int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                         int64_t page_size, int64_t max_pages);
 int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,

@@ -302,6 +302,27 @@ def test_same_bits_on_another_stream(cuda):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("handle", ["own", 0])
+def test_a_stream_of_the_callers(cuda, handle):
+    """`stream` as a handle (0: the default stream) while torch's current stream is another;
+    the workspace stays the call's until that stream is done with it."""
+    kc, vc, table = cache(cuda, 4, 2, 64, 16, 40, BF16)
+    q = torch.randn((4, 8, 64), device=cuda).to(BF16)
+    lens = torch.tensor([640, 3, 0, 500], dtype=torch.int32, device=cuda)
+    want = ops.sdpa_paged(q, kc, vc, table, lens, 0.1)
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        for _ in range(5):
+            got = torch.zeros_like(want)
+            torch.cuda.synchronize()
+            ops.sdpa_paged(q, kc, vc, table, lens, 0.1, out=got, stream=s.cuda_stream if handle == "own" else handle)
+            junk = [torch.full((1 << 20,), float("nan"), device=cuda) for _ in range(8)]
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            del junk
+
+
 def test_refusals_on_the_device(cuda):
     kc, vc, table = cache(cuda, 2, 2, 64, 16, 3, BF16)
     q = torch.randn((2, 4, 64), device=cuda).to(BF16)
@@ -316,6 +337,9 @@ def test_refusals_on_the_device(cuda):
         ops.sdpa_paged(q, kc, vc[:2], table, lens, 0.1)
     with pytest.raises(ValueError, match="k_cache"):
         ops.sdpa_paged(q.half(), kc, vc, table, lens, 0.1)
+    with pytest.raises(ValueError, match="workspace must be contiguous"):
+        ops.sdpa_paged(q, kc, vc, table, lens, 0.1,
+                       workspace=torch.empty(1, dtype=torch.uint8, device=cuda).expand(1 << 20))
     with pytest.raises(BackendError, match="multiple of num_kv_heads"):
         ops.sdpa_paged(q[:, :3], kc, vc, table, lens, 0.1)
     k = torch.randn((2, 2, 1, 64), device=cuda)

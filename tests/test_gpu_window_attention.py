@@ -276,3 +276,6 @@ def test_refusals_on_the_device(cuda):
     lse = torch.zeros((1, 2, 8), device=cuda)
     with pytest.raises(BackendError, match="workspace of"):
         ops.sdpa_window_grad(q, q, q, q, q, lse, 0.1, workspace=torch.empty(16, dtype=torch.uint8, device=cuda))
+    with pytest.raises(ValueError, match="workspace must be contiguous"):
+        ops.sdpa_window_grad(q, q, q, q, q, lse, 0.1,
+                             workspace=torch.empty(1, dtype=torch.uint8, device=cuda).expand(1 << 20))

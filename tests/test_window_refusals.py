@@ -48,7 +48,8 @@ REFUSED = [
     (window, dict(dt=F32, D=66), 2, "head dim"), (window, dict(q=None), 1, "q is null"),
     (window, dict(q=PTR + 8), 2, "aligned"), (window, dict(o=PTR + 4), 2, "aligned"),
     (window, dict(st=(-512, 64, 64)), 2, "strides"), (window, dict(st=(512, 64, 68)), 2, "strides"),
-    (window, dict(st=(512, 64, 1 << 24)), 2, "below 32 MiB"),
+    (window, dict(st=(512, 64, 1 << 24)), 2, "below 32 MiB"), (window, dict(st=(512, 64, 1 << 58)), 2, "below 32 MiB"),
+    (window, dict(B=1 << 16, H=256, Sq=1, Sk=1), 2, "too large"),  # 2^32 threads
     (window, dict(Sq=1, Sk=(1 << 29) + 8, st=(64, 64, 64)), 2, "too large"),
     (window, dict(B=1 << 40, H=1 << 40, Hkv=1), 2, "too large"),
     (grad, dict(D=300), 2, "head dim"), (grad, dict(ws=None), 1, "workspace of"), (grad, dict(nbytes=100), 1, "workspace of"),
@@ -66,7 +67,8 @@ REFUSED = [
     (append, dict(es=3), 2, "elements of"), (append, dict(S=-1), 1, "bad sizes"), (append, dict(k=None), 1, "null"),
     (append, dict(pages=0), 1, "without pages"), (append, dict(k=PTR + 1), 1, "aligned"),
     (append, dict(st=(-1, 64, 64)), 2, "negative strides"), (append, dict(ts=-2), 1, "table stride"),
-    (append, dict(B=70000), 2, "too large"), (append, dict(size=1 << 20, per=1 << 20), 2, "too large"),
+    (paged, dict(B=1 << 14, H=1 << 10), 2, "fewer than 2\\^24 heads"),
+    (append, dict(S=1 << 20, Hkv=64, D=1024), 2, "too large"), (append, dict(B=70000), 2, "too large"), (append, dict(size=1 << 20, per=1 << 20), 2, "too large"),
 ]
 
 
@@ -75,6 +77,18 @@ def test_refused(fn, kw, code, words):
     with pytest.raises(_lib.BackendError, match=words) as e:
         fn(**kw)
     assert e.value.code == code
+
+
+def test_gradient_grids():
+    """More workgroups than a launch holds, of either kernel, and a list of tiles past 32
+    bits: refused, not wrapped around."""
+    s = I3(0, 0, 64)
+    for B, H, Hkv, Sq, Sk in ((1 << 16, 256, 256, 1, 1), (1 << 10, 64, 64, 1, 1 << 14), (1, 1 << 22, 1, 1 << 15, 1 << 15)):
+        with pytest.raises(_lib.BackendError, match="too large") as e:
+            _lib.call("ghip_sdpa_window_bwd", BF16, *[PTR] * 9, B, H, Hkv, Sq, Sk, 64, *[s] * 8, 0, 0, 0, None, 1.0, PTR,
+                      1 << 50, None)
+        assert e.value.code == 2
+    assert _lib.load().ghip_sdpa_window_bwd_workspace_bytes(BF16, 1, 1 << 24, 1, 1 << 15, 1 << 15, 64, 0, 1, 4) == 0
 
 
 def test_nothing_to_do():
