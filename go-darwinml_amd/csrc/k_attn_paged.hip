@@ -298,17 +298,16 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
     for (int db = 0; db < DP / 16; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    // The order of the DMA is pages(j + 1), K and V(j).
+    // The order of the DMA is pages(j + 1), K and V(j) (the first two tiles' pages together).
     const int n = te - ta;
     auto tile_of = [&](int j) { return ta + j; };
     uint64_t rows0 = 0, rows1 = 0;  // of tiles j and j + 1
     if (n > 0) {
       issue_pages(tile_of(0), 0);
-      wait_vm<0>();
       if (n > 1) issue_pages(tile_of(1), 1);
+      wait_vm<0>();
       rows0 = issue(tile_of(0), 0);
       if (n > 1) {
-        wait_vm<2 * kN>();
         if (n > 2) issue_pages(tile_of(2), 0);
         rows1 = issue(tile_of(1), 1);
       }
