@@ -375,6 +375,8 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
           x[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][v], c, nb));
           l += x[i][v];
         }
+        // The weights, at most 2^8, are rounded for the product with V only: half a step of the
+        // type beside V's own rounding; their sum above is not.
         const typename O::P pf = O::pack(x[i]);
 #pragma unroll
         for (int db = 0; db < DP / 16; ++db) {

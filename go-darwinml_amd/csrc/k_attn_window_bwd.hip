@@ -246,6 +246,8 @@ __global__ __launch_bounds__(256, 1) void dq_few_kernel(Params p) {
 // Q and dO stream through two LDS stages, head after head of the group, with each query's
 // log-sum-exp and delta beside them.
 //
+// P and dS are rounded once each, to the operands' type, as they enter the second products
+// (16-bit matrix instructions take nothing wider); dS is formed from P in fp32.
 // f16 only: P is at most 1 and of order 1 / window, so it is rounded 2^8 times larger
 // (small weights would be subnormal), and dS is rounded with the scale applied.
 template <typename T, int DP>
