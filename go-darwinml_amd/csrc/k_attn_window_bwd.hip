@@ -6,10 +6,10 @@
 // evaluate P and dS again, so nothing of size Sq x Sk is stored and no sum depends on
 // the order of atomics: the first owns queries (dQ, and delta for the second), the
 // second keys.
-#include <algorithm>
 #include <type_traits>
 
 #include "attn_window.h"
+#include "attn_window_rules.h"
 
 namespace ghip {
 namespace win {
@@ -17,7 +17,6 @@ namespace win {
 using tile::f32x16;
 
 constexpr int kCols = 128;  // queries of a workgroup of dq_kernel
-constexpr int kKeys = 64;   // keys of a workgroup of dkv_kernel
 constexpr float kLog2e = 1.4426950408889634f;
 
 // dQ: the transposed arrangement of the forward kernel.  A lane owns one of a wave's 32
@@ -256,7 +255,6 @@ struct Keys {
   using F = typename Tl::F;
   static constexpr bool kF16 = __is_same(T, f16_t);
   static constexpr int kPairs = kKeys / 32, kNW = 2 * kPairs;
-  static constexpr int kT = 32;  // rows of a tile
   static constexpr int kTile = kT * Tl::kRow;
   struct Lds {
     __attribute__((aligned(1024))) char tiles[2][2][kTile];    // [stage][Q, dO]
@@ -426,15 +424,6 @@ struct Keys {
   }
 };
 
-// One past the last tile of queries that see, through their windows, a key of the
-// workgroup's at k0.
-constexpr int kT = 32;
-__device__ __host__ __forceinline__ int near_end(const Params& p, int k0) {
-  const int64_t last = static_cast<int64_t>(k0) + kKeys - 1 + p.window - p.q_start;  // one past the last such query
-  const int64_t tiles = (p.Sq + kT - 1) / kT;
-  return static_cast<int>(last <= 0 ? 0 : (last + kT - 1) / kT < tiles ? (last + kT - 1) / kT : tiles);
-}
-
 // Bound by the exchange of P with its two barriers a tile: 4 x 16 heads of 2048 tokens,
 // window 512, sinks, bf16 D 128 100 us (0.61 PFLOP/s of visible pairs), 34% of the cycles in
 // matrix instructions, 28% in vector ones.  Three waves a SIMD instead of two took the whole
@@ -465,7 +454,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 1
     // Chunk ck of the queries that see the 32 sinks from 32 sb through no window.
     const int sb = (at_ - blocks) / p.chunks, ck = (at_ - blocks) % p.chunks;
     w.kfirst = 32 * sb;
-    w.tbase = near_end(p, w.kfirst / kKeys * kKeys);
+    w.tbase = near_end(p.Sq, p.q_start, p.window, w.kfirst / kKeys * kKeys);
     w.tcount = max(0, tiles - w.tbase);
     w.i0 = min(w.tcount * G, ck * p.chunk);
     w.i1 = min(w.tcount * G, w.i0 + p.chunk);
@@ -476,8 +465,8 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 1
     const bool split = !p.far && p.share_blocks > 0;
     const int kb = split ? at_ / p.chunks : at_, ck = split ? at_ % p.chunks : 0, k0 = kb * kKeys;
     w.kfirst = k0 + pair * 32;
-    w.tbase = max(0, k0 - p.q_start) / kT;
-    const int te = k0 >= len ? 0 : k0 < p.sinks && !p.far ? tiles : min(tiles, near_end(p, k0));
+    w.tbase = near_begin(p.q_start, k0);
+    const int te = k0 >= len ? 0 : k0 < p.sinks && !p.far ? tiles : min(tiles, near_end(p.Sq, p.q_start, p.window, k0));
     w.tcount = max(0, te - w.tbase);
     const int n = w.tcount * G;
     w.i0 = split ? min(n, ck * p.chunk) : 0;
@@ -525,38 +514,17 @@ static bool list_too_long(int64_t Sq, int64_t G) { return (Sq / kT + 1) * G > 0x
 struct Plan {
   int64_t groups, floats;  // workgroups, floats of the shares
 };
-static Plan plan_shares(Params* p) {
-  const int G = p->H / p->Hkv;
-  const int tiles = (p->Sq + kT - 1) / kT;
-  const int beyond = p->sinks > 0 ? tiles - near_end(*p, 0) : 0;
-  // Tiles of the first, and with it of the longest list of a head.
-  const int own = std::min(tiles, (std::min(p->window, p->Sq) + kKeys) / kT + 1);
-  const int64_t grid = static_cast<int64_t>((p->Sk + kKeys - 1) / kKeys) * p->B * p->Hkv;
-  if (beyond > 0 && beyond >= own && p->sinks <= 128) {
-    // (More sinks are many workgroups of their own.)  Chunks of 8 tiles, us a call with 4 /
-    // 8 / 16 / 32: padded batch of 12 heads of 64, window 128, 50.5 / 51.9 / 56 / 65; 4 x 16
-    // heads, 2048 tokens, window 512, 200 / 197 / 200 / 209.  The shares take half of q's
-    // memory.
-    p->far = true;
-    p->share_blocks = (p->sinks + 31) / 32;
-    p->chunk = 8 * p->share_blocks;
-    p->chunks = (beyond * G + p->chunk - 1) / p->chunk;
-    p->shares = 1 + p->chunks;
-  } else if (grid < 256) {
-    // Few workgroups: chunks of at least 4 tiles, towards 512 workgroups.
-    const int64_t longest = static_cast<int64_t>(p->sinks > 0 ? tiles : own) * G;
-    const int64_t goal = std::min<int64_t>(grid > 0 ? (512 + grid - 1) / grid : 1, longest / 4);
-    if (goal > 1) {
-      p->chunk = static_cast<int>((longest + goal - 1) / goal);
-      p->chunks = static_cast<int>((longest + p->chunk - 1) / p->chunk);
-      p->share_blocks = (p->Sk + 31) / 32;
-      p->shares = p->chunks;
-    }
-  }
-  p->share_stride = static_cast<int64_t>(p->shares) * 64 * p->D;
+static Plan plan(Params* p) {
   const int64_t nbh = static_cast<int64_t>(p->B) * p->Hkv;
-  return {p->far ? grid + nbh * p->share_blocks * p->chunks : p->share_blocks ? grid * p->chunks : grid,
-          nbh * p->share_blocks * p->share_stride};
+  const SharePlan s = plan_shares(nbh, p->H / p->Hkv, p->Sq, p->Sk, p->q_start, p->window, p->sinks);
+  p->share_blocks = s.blocks;
+  p->shares = s.shares;
+  p->chunks = s.chunks;
+  p->chunk = s.chunk;
+  p->far = s.far;
+  p->share_stride = static_cast<int64_t>(s.shares) * 64 * p->D;
+  const int64_t grid = static_cast<int64_t>((p->Sk + kKeys - 1) / kKeys) * nbh;
+  return {s.far ? grid + nbh * s.blocks * s.chunks : s.blocks ? grid * s.chunks : grid, nbh * s.blocks * p->share_stride};
 }
 
 // Floats of the statistics, a whole number of 16 bytes.
@@ -596,7 +564,7 @@ extern "C" int64_t ghip_sdpa_window_bwd_workspace_bytes(int dtype, int64_t B, in
   win::Params p{};
   if (win::check_problem("", dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, 1.f, &p, nullptr)) return 0;
   if (win::list_too_long(Sq, H / Hkv)) return 0;
-  return (win::stats_floats(p) + win::plan_shares(&p).floats) * 4;
+  return (win::stats_floats(p) + win::plan(&p).floats) * 4;
 }
 
 extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, const void* v, const void* o,
@@ -612,7 +580,7 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
   if (int rc = win::check_problem(kWhat, dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks, scale, &p, err)) return rc;
   if (B == 0 || Sk == 0) return GHIP_OK;
   if (win::list_too_long(Sq, H / Hkv) || (Sq + win::kCols - 1) / win::kCols * B * H > tile::kMostGroups ||
-      win::plan_shares(&p).groups > tile::kMostGroups)
+      win::plan(&p).groups > tile::kMostGroups)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
   const struct {
     const char* name;
