@@ -2,6 +2,10 @@
 
 torch is used only as the allocator of device memory and as the source of the
 current HIP stream; every computation runs in libgomlx_hip.so.
+
+`stream` is a HIP stream's handle.  A call on one that is not torch's current stream orders
+nothing: its inputs, and the outputs and workspace that the caller gives, must be ready there
+(an event, a wait), and so must its outputs be before the current stream reads them.
 """
 from __future__ import annotations
 
@@ -41,6 +45,34 @@ def _stream(stream=None) -> int:
     return int(stream)
 
 
+def _stream_of(handle, device):
+    """torch's stream of a handle (ExternalStream takes 0 for a new stream)."""
+    return torch.cuda.ExternalStream(int(handle), device=device) if int(handle) else torch.cuda.default_stream(device)
+
+
+def _empty(shape, dtype, device, stream=None) -> torch.Tensor:
+    """An output or a workspace of a call on `stream` (a handle; None: the current stream).
+    torch reuses memory in the order of the stream that it was allocated on, so it comes
+    from `stream`'s own: work still queued on the current stream for whoever had the memory
+    before cannot meet the call.  Freed, it waits for the current stream's uses too."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(_stream_of(stream, device)):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
+def _empty_like(x: torch.Tensor, stream=None) -> torch.Tensor:
+    """torch.empty_like as _empty."""
+    if stream is None:
+        return torch.empty_like(x)
+    with torch.cuda.stream(_stream_of(stream, x.device)):
+        t = torch.empty_like(x)
+    t.record_stream(torch.cuda.current_stream(x.device))
+    return t
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -62,7 +94,7 @@ def softmax(x: torch.Tensor, log: bool = False, out=None, stream=None) -> torch.
     """Softmax (log-softmax) over the last axis."""
     _check_dev(x)
     rows, n = _rows(x)
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     call("ghip_softmax_rows", dtype_code(x.dtype), x.data_ptr(), y.data_ptr(), rows, n,
          int(log), _stream(stream))
     return y
@@ -74,7 +106,7 @@ def scale_mask_softmax(x: torch.Tensor, scale: float, causal: bool, bmask=None, 
     _check_dev(x, bmask)
     sq, sk = x.shape[-2], x.shape[-1]
     rows = x.numel() // sk
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     call("ghip_scale_mask_softmax_rows", dtype_code(x.dtype), x.data_ptr(), y.data_ptr(), rows,
          sq, sk, float(scale), int(causal), _ptr(bmask), _stream(stream))
     return y
@@ -83,7 +115,7 @@ def scale_mask_softmax(x: torch.Tensor, scale: float, causal: bool, bmask=None, 
 def rmsnorm(x: torch.Tensor, gamma=None, eps: float = 1e-6, out=None, stream=None):
     _check_dev(x, gamma)
     rows, n = _rows(x)
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     call("ghip_rmsnorm_rows", dtype_code(x.dtype), x.data_ptr(), _ptr(gamma), y.data_ptr(),
          rows, n, float(eps), _stream(stream))
     return y
@@ -92,17 +124,17 @@ def rmsnorm(x: torch.Tensor, gamma=None, eps: float = 1e-6, out=None, stream=Non
 def layernorm(x: torch.Tensor, gamma=None, beta=None, eps: float = 1e-5, out=None, stream=None):
     _check_dev(x, gamma, beta)
     rows, n = _rows(x)
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     call("ghip_layernorm_rows", dtype_code(x.dtype), x.data_ptr(), _ptr(gamma), _ptr(beta),
          y.data_ptr(), rows, n, float(eps), _stream(stream))
     return y
 
 
-def gemm_workspace(a_dtype, out_dtype, B: int, M: int, N: int, K: int, device):
+def gemm_workspace(a_dtype, out_dtype, B: int, M: int, N: int, K: int, device, stream=None):
     """Workspace for ghip_gemm_batched_ws / ghip_gemm_grouped_ws (None when a
-    product of these sizes never splits its contraction)."""
+    product of these sizes never splits its contraction), for calls on `stream`."""
     n = _lib.load().ghip_gemm_workspace_bytes(dtype_code(a_dtype), dtype_code(out_dtype or a_dtype), B, M, N, K)
-    return torch.empty((n,), dtype=torch.uint8, device=device) if n > 0 else None
+    return _empty((n,), torch.uint8, device, stream) if n > 0 else None
 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, out_dtype=None, out=None, stream=None, k_split: bool = True,
@@ -119,10 +151,10 @@ def gemm(a: torch.Tensor, b: torch.Tensor, out_dtype=None, out=None, stream=None
     if K != K2 or (B2 != B and B2 != 1):
         raise ValueError(f"gemm: shapes {tuple(a.shape)} x {tuple(b.shape)}")
     odt = out_dtype or a.dtype
-    c = torch.empty((B, M, N), dtype=odt, device=a.device) if out is None else out.view(B, M, N)
+    c = _empty((B, M, N), odt, a.device, stream) if out is None else out.view(B, M, N)
     sb_b = b3.stride(0) if B2 == B else 0
     if k_split and workspace is None:
-        workspace = gemm_workspace(a.dtype, odt, B, M, N, K, a.device)
+        workspace = gemm_workspace(a.dtype, odt, B, M, N, K, a.device, stream)
     ws_ptr = workspace.data_ptr() if (k_split and workspace is not None) else None
     ws_bytes = workspace.numel() * workspace.element_size() if ws_ptr is not None else 0
     call("ghip_gemm_batched_ws", dtype_code(a.dtype), dtype_code(odt), B, M, N, K,
@@ -143,13 +175,13 @@ def gemm_grouped(a: torch.Tensor, bs, out_dtype=None, outs=None, stream=None, k_
     if K != K2 or any(b.shape != bs[0].shape or b.stride() != bs[0].stride() for b in bs):
         raise ValueError("gemm_grouped: every b must be [K, N] with the same strides")
     odt = out_dtype or a.dtype
-    cs = [torch.empty((M, N), dtype=odt, device=a.device) for _ in bs] if outs is None else list(outs)
+    cs = [_empty((M, N), odt, a.device, stream) for _ in bs] if outs is None else list(outs)
     if any(c.stride() != cs[0].stride() or c.stride(1) != 1 for c in cs):
         raise ValueError("gemm_grouped: outputs need one row stride and unit column stride")
     bp = (ctypes.c_void_p * len(bs))(*[b.data_ptr() for b in bs])
     cp = (ctypes.c_void_p * len(cs))(*[c.data_ptr() for c in cs])
     if k_split and workspace is None:
-        workspace = gemm_workspace(a.dtype, odt, 1, M, N, K, a.device)
+        workspace = gemm_workspace(a.dtype, odt, 1, M, N, K, a.device, stream)
     ws_ptr = workspace.data_ptr() if (k_split and workspace is not None) else None
     ws_bytes = workspace.numel() * workspace.element_size() if ws_ptr is not None else 0
     call("ghip_gemm_grouped_ws", dtype_code(a.dtype), dtype_code(odt), len(bs), M, N, K, a.data_ptr(),
@@ -171,7 +203,7 @@ def softmax_axis(x: torch.Tensor, axis: int, log: bool = False, out=None, stream
     inner = 1
     for d in x.shape[axis + 1:]:
         inner *= d
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     call("ghip_softmax_cols", dtype_code(x.dtype), x.data_ptr(), y.data_ptr(), outer, x.shape[axis], inner,
          int(log), _stream(stream))
     return y
@@ -198,11 +230,12 @@ def _strides3(t: torch.Tensor):
     return (ctypes.c_int64 * 3)(t.stride(0), t.stride(1), t.stride(2))
 
 
-def sdpa_workspace(q: torch.Tensor, Hkv: int, Sk: int, causal: bool):
-    """Workspace for ghip_sdpa_fwd_masked_ws (None when the shape takes no key split)."""
+def sdpa_workspace(q: torch.Tensor, Hkv: int, Sk: int, causal: bool, stream=None):
+    """Workspace for ghip_sdpa_fwd_masked_ws (None when the shape takes no key split), for
+    calls on `stream`."""
     B, H, Sq, D = q.shape
     n = _lib.load().ghip_sdpa_workspace_bytes(dtype_code(q.dtype), B, H, Hkv, Sq, Sk, D, int(causal))
-    return torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
+    return _empty((n,), torch.uint8, q.device, stream) if n > 0 else None
 
 
 def sdpa(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool,
@@ -236,10 +269,10 @@ def sdpa_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask, scale: 
     _check_dev(q, k, v, *([mask] if mask is not None else []))
     B, H, Sq, D = q.shape
     _, Hkv, Sk, _ = k.shape
-    o = torch.empty((B, H, Sq, D), dtype=q.dtype, device=q.device) if out is None else out
+    o = _empty((B, H, Sq, D), q.dtype, q.device, stream) if out is None else out
     mdt = -1 if mask is None else dtype_code(mask.dtype)
     ms = None if mask is None else _mask_strides(mask, B, H, Sq, Sk)
-    ws = (workspace if workspace is not None else sdpa_workspace(q, Hkv, Sk, causal)) if kv_split else None
+    ws = (workspace if workspace is not None else sdpa_workspace(q, Hkv, Sk, causal, stream)) if kv_split else None
     call("ghip_sdpa_fwd_masked_ws", dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
          o.data_ptr(), B, H, Hkv, Sq, Sk, D, _strides3(q), _strides3(k), _strides3(v),
          _strides3(o), _ptr(mask), mdt, ms, float(scale), int(causal), _ptr(ws),
@@ -251,7 +284,7 @@ def scale_mask_softmax_ex(x: torch.Tensor, scale: float, causal: bool, mask=None
     """softmax(x * scale + mask) over the last axis of scores x [B, H, Sq, Sk]."""
     _check_dev(x, mask)
     B, H, Sq, Sk = x.shape
-    y = torch.empty_like(x) if out is None else out
+    y = _empty_like(x, stream) if out is None else out
     mdt = -1 if mask is None else dtype_code(mask.dtype)
     ms = None if mask is None else _mask_strides(mask, B, H, Sq, Sk)
     call("ghip_scale_mask_softmax_rows_ex", dtype_code(x.dtype), x.data_ptr(), y.data_ptr(), B, H, Sq, Sk,
@@ -267,14 +300,6 @@ def _launch(dev: torch.device, name: str, stream, *args):
     else:
         # The current stream's handle alone: a torch.cuda.Stream object costs 3 us.
         call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else int(stream))
-
-
-def _kept(ws, stream):
-    """A workspace allocated here, for a call on `stream`: torch may give its memory away
-    only when that stream is done with it."""
-    if ws is not None and stream is not None:
-        ws.record_stream(torch.cuda.ExternalStream(int(stream), device=ws.device))
-    return ws
 
 
 def _given(what: str, ws):
@@ -341,7 +366,7 @@ def sdpa_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
     dims, start = _window_shapes(q, k, v, q_start, lens)
     B, H, _, Sq, _, D = dims
     if out is None:
-        out = torch.empty((B, H, Sq, D), dtype=q.dtype, device=dev)
+        out = _empty((B, H, Sq, D), q.dtype, dev, stream)
     else:
         _like("sdpa_window: out", out, (B, H, Sq, D), q.dtype)
     if lse is not None:
@@ -349,21 +374,22 @@ def sdpa_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
         if not lse.is_contiguous():
             raise ValueError("sdpa_window: lse must be contiguous")
     elif with_lse:
-        lse = torch.empty((B, H, Sq), dtype=torch.float32, device=dev)
+        lse = _empty((B, H, Sq), torch.float32, dev, stream)
     _launch(dev, "ghip_sdpa_window_fwd", stream, dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
             out.data_ptr(), _ptr(lse), *dims, _rows3("q", q), _rows3("k", k), _rows3("v", v), _rows3("out", out), start,
             int(window), int(sinks), _ptr(lens), float(scale))
     return (out, lse) if with_lse else out
 
 
-def sdpa_window_grad_workspace(q: torch.Tensor, k: torch.Tensor, window: int = 0, sinks: int = 0, q_start=None):
-    """Workspace for sdpa_window_grad at these sizes."""
+def sdpa_window_grad_workspace(q: torch.Tensor, k: torch.Tensor, window: int = 0, sinks: int = 0, q_start=None,
+                               stream=None):
+    """Workspace for sdpa_window_grad at these sizes, for calls on `stream`."""
     B, H, Sq, D = q.shape
     Hkv, Sk = k.shape[1], k.shape[2]
     n = _lib.load().ghip_sdpa_window_bwd_workspace_bytes(dtype_code(q.dtype), B, H, Hkv, Sq, Sk, D,
                                                          Sk - Sq if q_start is None else int(q_start), int(window),
                                                          int(sinks))
-    return torch.empty((n,), dtype=torch.uint8, device=q.device)
+    return _empty((n,), torch.uint8, q.device, stream)
 
 
 def sdpa_window_grad(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
@@ -380,16 +406,16 @@ def sdpa_window_grad(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     if not lse.is_contiguous():
         raise ValueError("sdpa_window_grad: lse must be contiguous")
     if outs is None:
-        dq = torch.empty((B, H, Sq, D), dtype=q.dtype, device=dev)
-        dk = torch.empty((B, Hkv, Sk, D), dtype=q.dtype, device=dev)
-        dv = torch.empty((B, Hkv, Sk, D), dtype=q.dtype, device=dev)
+        dq = _empty((B, H, Sq, D), q.dtype, dev, stream)
+        dk = _empty((B, Hkv, Sk, D), q.dtype, dev, stream)
+        dv = _empty((B, Hkv, Sk, D), q.dtype, dev, stream)
     else:
         dq, dk, dv = outs
         _like("sdpa_window_grad: dq", dq, q.shape, q.dtype)
         _like("sdpa_window_grad: dk", dk, k.shape, q.dtype)
         _like("sdpa_window_grad: dv", dv, k.shape, q.dtype)
     if workspace is None:
-        ws = _kept(sdpa_window_grad_workspace(q, k, window, sinks, q_start), stream)
+        ws = sdpa_window_grad_workspace(q, k, window, sinks, q_start, stream)
     else:
         ws = _given("sdpa_window_grad", workspace)
     _launch(dev, "ghip_sdpa_window_bwd", stream, dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -438,12 +464,13 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             _ptr(counts), _rows3("k", k), _rows3("v", v), _rows3("k_cache", k_cache), _rows3("v_cache", v_cache))
 
 
-def sdpa_paged_workspace(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor):
-    """Workspace for sdpa_paged at these sizes (None when the sequences never split)."""
+def sdpa_paged_workspace(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor, stream=None):
+    """Workspace for sdpa_paged at these sizes (None when the sequences never split), for
+    calls on `stream`."""
     B, H, D = q.shape
     n = _lib.load().ghip_sdpa_paged_workspace_bytes(dtype_code(q.dtype), B, H, k_cache.shape[1], D, k_cache.shape[2],
                                                     block_table.shape[1])
-    return torch.empty((n,), dtype=torch.uint8, device=q.device) if n > 0 else None
+    return _empty((n,), torch.uint8, q.device, stream) if n > 0 else None
 
 
 def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -461,7 +488,7 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     pages, size, per, ts = _check_cache("sdpa_paged", k_cache, v_cache, block_table, B, Hkv, D, q.dtype)
     _ints("sdpa_paged: lens", lens, B)
     if out is None:
-        out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+        out = _empty((B, H, D), q.dtype, dev, stream)
     else:
         _like("sdpa_paged: out", out, (B, H, D), q.dtype)
     for what, t in (("q", q), ("out", out)):
@@ -469,7 +496,7 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             raise ValueError(f"sdpa_paged: {what}'s head dim must be contiguous")
     ws = None
     if split and workspace is None:
-        ws = _kept(sdpa_paged_workspace(q, k_cache, block_table), stream)
+        ws = sdpa_paged_workspace(q, k_cache, block_table, stream)
     elif split:
         ws = _given("sdpa_paged", workspace)
     _launch(dev, "ghip_sdpa_paged", stream, dtype_code(q.dtype), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -487,8 +514,7 @@ def gather_rows(table: torch.Tensor, ids: torch.Tensor, out=None, stream=None):
         raise ValueError("gather_rows: contiguous table and int32 ids required")
     V = table.shape[0]
     row_bytes = table[0].numel() * table.element_size()
-    o = torch.empty((ids.numel(),) + tuple(table.shape[1:]), dtype=table.dtype,
-                    device=table.device) if out is None else out
+    o = _empty((ids.numel(),) + tuple(table.shape[1:]), table.dtype, table.device, stream) if out is None else out
     call("ghip_gather_rows", table.data_ptr(), V, row_bytes, ids.data_ptr(), ids.numel(),
          o.data_ptr(), _stream(stream))
     return o.view(tuple(ids.shape) + tuple(table.shape[1:])) if out is None else o
@@ -506,15 +532,14 @@ def argminmax(x: torch.Tensor, axis: int, is_min: bool = False, out_dtype=torch.
     inner = 1
     for d in x.shape[ax + 1:]:
         inner *= d
-    o = torch.empty(tuple(x.shape[:ax]) + tuple(x.shape[ax + 1:]), dtype=out_dtype,
-                    device=x.device)
+    o = _empty(tuple(x.shape[:ax]) + tuple(x.shape[ax + 1:]), out_dtype, x.device, stream)
     call("ghip_argminmax", dtype_code(x.dtype), x.data_ptr(), outer, x.shape[ax], inner,
          int(is_min), dtype_code(out_dtype), o.data_ptr(), _stream(stream))
     return o
 
 
 def iota(shape, axis: int, dtype=torch.int32, device="cuda", stream=None):
-    o = torch.empty(tuple(shape), dtype=dtype, device=device)
+    o = _empty(tuple(shape), dtype, device, stream)
     ax = axis % len(shape)
     outer = 1
     for d in shape[:ax]:
