@@ -14,7 +14,7 @@ struct Mat3 {
 struct Params {
   Mat3 q, k, v, o, dout, dq, dk, dv;
   float* lse;        // [B, H, Sq]; forward: written (may be null), gradient: read
-  // Gradient, [2][B, H, Sq]: minus the log-sum-exp in base 2 (f16: plus 8), and minus delta,
+  // Gradient, [2][B, H, Sq]: minus the log-sum-exp in base 2 (f16: plus 15), and minus delta,
   // the row sums of do * o.
   float* stats;
   // Gradient: shares of dk and dv that join_kernel adds, of the first share_blocks blocks of

@@ -19,6 +19,39 @@ using tile::f32x16;
 constexpr int kCols = 128;  // queries of a workgroup of dq_kernel
 constexpr float kLog2e = 1.4426950408889634f;
 
+// f16 (5 bits of exponent): P, at most 1 and of order 1 / window, is rounded 2^15 times larger,
+// and dS, whose size follows d_out's and the window's, times a power of two 2^e that each
+// column (a lane's query in dq, its key in dk) finds as its running maximum does in a
+// softmax: from kFirst, where all that could reach an f16 result is inside the range, e falls
+// when a tile's values pass 2^15, so that they end below 2^7 and leave 2^8 for later tiles.  A
+// value then keeps all its bits down to 2^-20 of the largest, and none overflows.  The sums
+// follow, and lose 2^e at the end, in fp32.  The whole gradient, with a fixed factor / so: 4 x
+// 16 heads of 2048 tokens, D 128, window 512 179 / 185 us, padded batch of 12 heads of 64 52.4 /
+// 54.4, D 256 (2 x 8 heads of 2048) 111 / 136, where the sums' registers move for the rare branch.
+constexpr int kPUp = 15;
+__device__ __forceinline__ int first_exponent(float scale) {
+  return 60 - max(0, static_cast<int>(__builtin_amdgcn_logf(scale)));  // (P scale 2^e: at most 2^61)
+}
+// x holds values times 2^e: returns by how much e has to change (0: x and the sums stay).
+template <int ND>
+__device__ __forceinline__ int make_room(f32x16& x, f32x16 (&sum)[ND]) {
+  float mx = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; v += 2) mx = fmaxf(fmaxf(fabsf(x[v]), fabsf(x[v + 1])), mx);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const bool over = mx > 0x1p15f;
+  if (!__builtin_amdgcn_ballot_w64(over)) return 0;
+  const int d = over ? min(0, 7 - __builtin_amdgcn_frexp_expf(mx)) : 0;
+  const float f = __builtin_amdgcn_ldexpf(1.f, d);
+#pragma unroll
+  for (int v = 0; v < 16; ++v) x[v] *= f;
+#pragma unroll
+  for (int db = 0; db < ND; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) sum[db][v] *= f;
+  return d;
+}
+
 // dQ: the transposed arrangement of the forward kernel.  A lane owns one of a wave's 32
 // queries; S^T = K Q^T and dP^T = V dO^T come out as columns, dS^T enters dQ^T += K^T dS^T
 // from the registers.  The product's accumulator starts at -delta, and the scale sits in
@@ -28,10 +61,12 @@ template <typename T, int DP>
 struct Queries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
+  static constexpr bool kF16 = __is_same(T, f16_t);
   static constexpr int ND = DP / 32;
   F qf[DP / 16], gf[DP / 16];
   f32x16 dq[ND];
-  float c, nl, nd;  // minus the log-sum-exp in base 2 (plus log2 scale), minus delta
+  float c, nl, nd;  // minus the log-sum-exp in base 2 (plus log2 scale, f16: plus e), minus delta
+  int e;            // f16: dS and dq are held times 2^e
   int pw, pos;      // positions: the wave's first, the lane's own
   int len;
   bool live;        // the lane's query exists
@@ -64,10 +99,14 @@ struct Queries {
     const int64_t row = (static_cast<int64_t>(b) * p.H + h) * p.Sq + qi;
     nl = live ? -p.lse[row] * kLog2e : 0.f;
     if (tell && qi < p.Sq && h2 == 0) {
-      p.stats[row] = nl + (__is_same(T, f16_t) ? 8.f : 0.f);
+      p.stats[row] = nl + (kF16 ? static_cast<float>(kPUp) : 0.f);
       p.stats[static_cast<int64_t>(p.B) * p.H * p.Sq + row] = nd;
     }
     nl += __builtin_amdgcn_logf(p.scale);
+    if constexpr (kF16) {
+      e = first_exponent(p.scale);
+      nl += e;
+    }
     tile::settle(qf);
     tile::settle(gf);
     asm volatile("" : "+v"(nl));
@@ -96,12 +135,27 @@ struct Queries {
 #pragma unroll
       for (int v = 0; v < 16; ++v) x[v] = select_bit(w, (v >> 2) * 8 + (v & 3), x[v], 0.f);
     }
+    if constexpr (kF16) {
+      const int d = make_room(x, dq);
+      e += d;
+      nl += d;
+    }
     const F df[2] = {tile::pack<T>(x, 0), tile::pack<T>(x, 1)};
     tile::pipelined<Tl::kRow, F, 2 * ND>([&](int j) { return Tl::frag_tr(sk + 16 * (j / ND) * Tl::kRow, j % ND, lane); },
                                          [&](int j, const F& a) {
                                            if (sizeof(T) == 4 && 32 * (j % ND) >= p.D) return;
                                            dq[j % ND] = tile::mma<T>(a, df[j / ND], dq[j % ND]);
                                          });
+  }
+  // dq without 2^e.
+  __device__ __forceinline__ void settle_sums() {
+    if constexpr (kF16) {
+      const float f = __builtin_amdgcn_ldexpf(1.f, -e);
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) dq[db][v] *= f;
+    }
   }
   __device__ __forceinline__ void finish(const Params& p, int b, int h, int qw, int lane) {
     const int qi = qw + (lane & 31), h2 = lane >> 5;
@@ -169,6 +223,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
     step(std::integral_constant<int, 0>{}, i);
     if (i + 1 < tl.n) step(std::integral_constant<int, 1>{}, i + 1);
   }
+  q.settle_sums();
   q.finish(p, b, h, qw, lane);
 }
 
@@ -215,6 +270,7 @@ __global__ __launch_bounds__(256, 1) void dq_few_kernel(Params p) {
     else if (i + 4 < tl.n) issue(i + 4, 0);
   }
 
+  q.settle_sums();
   float* mine = reinterpret_cast<float*>(smem[wave]);
 #pragma unroll
   for (int db = 0; db < ND; ++db)
@@ -246,9 +302,8 @@ __global__ __launch_bounds__(256, 1) void dq_few_kernel(Params p) {
 // log-sum-exp and delta beside them.
 //
 // P and dS are rounded once each, to the operands' type, as they enter the second products
-// (16-bit matrix instructions take nothing wider); dS is formed from P in fp32.
-// f16 only: P is at most 1 and of order 1 / window, so it is rounded 2^8 times larger
-// (small weights would be subnormal), and dS is rounded with the scale applied.
+// (16-bit matrix instructions take nothing wider; f16: raised, see kPUp); dS is formed from P
+// in fp32.
 template <typename T, int DP>
 struct Keys {
   using Tl = tile::Tile<T, DP>;
@@ -318,6 +373,7 @@ struct Keys {
     f32x16 sum[DP / 32];  // dV (ROLE 0) or dK
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) sum[db] = tile::splat(0.f);
+    int e = kF16 && ROLE == 1 ? first_exponent(p.scale) : 0;
 
     // Entry i from stage ST, known when compiled.
     auto step = [&](auto stage, int i) {
@@ -371,7 +427,7 @@ struct Keys {
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (!on) return;
       if constexpr (ROLE == 1) {
-        const float f = kF16 ? p.scale * 0x1p-8f : 1.f;
+        const float f = kF16 ? __builtin_amdgcn_ldexpf(p.scale, e - kPUp) : 1.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float4 pv = pp[64 * j + lane];
@@ -380,6 +436,7 @@ struct Keys {
           x[4 * j + 2] *= kF16 ? pv.z * f : pv.z;
           x[4 * j + 3] *= kF16 ? pv.w * f : pv.w;
         }
+        if constexpr (kF16) e += make_room(x, sum);
         pf[0] = tile::pack<T>(x, 0);
         pf[1] = tile::pack<T>(x, 1);
       }
@@ -396,6 +453,13 @@ struct Keys {
     }
 
     if (w.idle) return;
+    if constexpr (kF16 && ROLE == 1) {
+      const float f = __builtin_amdgcn_ldexpf(1.f, -e);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum[db][v] *= f;
+    }
     if (w.share) {  // [dk, dv][32 keys][D] in fp32
       float* to = w.share + ((ROLE == 0 ? 32 : 0) + (lane & 31)) * static_cast<int64_t>(p.D);
 #pragma unroll
@@ -409,7 +473,7 @@ struct Keys {
     if ((w.share && key < w.apart) || key >= p.Sk) return;
     const Mat3& m = ROLE == 0 ? p.dv : p.dk;
     T* out = at<T>(m, w.b, w.hk) + static_cast<int64_t>(key) * m.ss;
-    const float f = ROLE == 0 ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
+    const float f = ROLE == 0 ? (kF16 ? 1.f / (1 << kPUp) : 1.f) : (kF16 ? 1.f : p.scale);
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -500,7 +564,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     a[2] += v.z;
     a[3] += v.w;
   }
-  const float f = which ? (kF16 ? 0x1p-8f : 1.f) : (kF16 ? 1.f : p.scale);
+  const float f = which ? (kF16 ? 1.f / (1 << kPUp) : 1.f) : (kF16 ? 1.f : p.scale);
   const Mat3& m = which ? p.dv : p.dk;
   const bool live = key < length_of(p, b);
   tile::store4(at<T>(m, b, hk) + key * m.ss + d, live ? a[0] * f : 0.f, live ? a[1] * f : 0.f, live ? a[2] * f : 0.f,

@@ -287,7 +287,9 @@ int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, const void* v,
  * dk and dv are summed over the H / Hkv query heads of a kv head.  Sizes, types, strides,
  * lens and the mask as there; padding gets zero gradients (dk, dv for every key, dq for
  * every query) and what d_out and o hold there is not used; an input broadcast by a stride
- * of 0 gets the gradient of each of its copies.  workspace: device memory of
+ * of 0 gets the gradient of each of its copies.  P and dS are rounded to the operands' type
+ * for the products that make dv, dk and dq; in FLOAT16 times powers of two, taken out again in
+ * fp32, so that d_out of any size keeps its bits.  workspace: device memory of
  * ghip_sdpa_window_bwd_workspace_bytes() bytes, 16-byte aligned, written on `stream`
  * (calls that share one must be ordered).  Sums are fp32 and in a fixed order: the same
  * bits every run.  No reference op (GoMLX differentiates the composite). */
