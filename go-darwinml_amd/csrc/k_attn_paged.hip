@@ -207,6 +207,9 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
   constexpr int KT = 8192 / kRow;              // 64, 32 or 16 tokens: 8 KiB of K and of V
   constexpr int kN = 8, kPer = 1024 / kRow;    // DMA instructions of a K (V) tile, rows of one
   constexpr int kTile = 8192;
+  // f16 weights (and their sum, in every share alike) are raised by 2^7: beside a token that
+  // takes nearly all of the softmax the others keep all their bits down to 2^-21 of it.
+  constexpr float kUpLog2 = __is_same(T, f16_t) ? 7.f : 0.f;
   using O = Op<T>;
   using F = typename tile::Frag<T>::type;
   __shared__ __attribute__((aligned(1024))) char smem[2][2][kTile];
@@ -367,7 +370,7 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[db][v] *= alpha;
       }
-      const float nb = m == -INFINITY ? 0.f : -m * c;
+      const float nb = m == -INFINITY ? 0.f : kUpLog2 - m * c;
 #pragma unroll
       for (int i = 0; i < KT / 16; ++i) {
 #pragma unroll
@@ -375,8 +378,8 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
           x[i][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][v], c, nb));
           l += x[i][v];
         }
-        // The weights, at most 2^8, are rounded for the product with V only: half a step of the
-        // type beside V's own rounding; their sum above is not.
+        // The weights, at most 2^8 (f16: 2^15), are rounded for the product with V only: half a
+        // step of the type beside V's own rounding; their sum above is not.
         const typename O::P pf = O::pack(x[i]);
 #pragma unroll
         for (int db = 0; db < DP / 16; ++db) {

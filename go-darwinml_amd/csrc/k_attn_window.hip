@@ -15,6 +15,10 @@ namespace win {
 using tile::f32x16;
 
 constexpr float kLazyLog2 = 8.f;  // the reference maximum may trail the true one by 2^8
+// f16 weights (and their sum) are raised by 2^7, so to 2^15 at most: beside a key that takes
+// nearly all of the softmax the others keep all their bits down to 2^-21 of it.
+template <typename T>
+constexpr float kUpLog2 = __is_same(T, f16_t) ? 7.f : 0.f;
 
 // A wave's 32 queries, one a lane (in both halves): S^T = K Q^T and O^T = V^T P^T, so the
 // softmax's running maximum, sum and rescale stay in the lane but for one exchange between
@@ -89,7 +93,7 @@ struct Queries {
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
     }
-    const float nb = m == -INFINITY ? 0.f : -m * c;
+    const float nb = m == -INFINITY ? 0.f : kUpLog2<T> - m * c;
     float ls = 0.f;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
@@ -125,7 +129,7 @@ struct Queries {
       }
     if (p.lse && h2 == 0)
       p.lse[(static_cast<int64_t>(b) * p.H + h) * p.Sq + qi] =
-          live ? (m * c + __builtin_amdgcn_logf(lt)) * 0.6931471805599453f : -INFINITY;
+          live ? (m * c + (__builtin_amdgcn_logf(lt) - kUpLog2<T>)) * 0.6931471805599453f : -INFINITY;
   }
 };
 
