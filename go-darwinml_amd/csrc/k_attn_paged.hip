@@ -9,6 +9,7 @@
 // ghip_sdpa_fwd_masked_ws reads); bound by the bytes of K and V.
 #include <algorithm>
 
+#include "attn_paged_rules.h"
 #include "attn_tile.h"
 
 namespace ghip {
@@ -38,11 +39,6 @@ struct Params {
 
 // Heads of one kv head's group that a unit of work holds: the columns of a 16-wide MFMA.
 constexpr int kHeads = 16;
-// The workers that share the tiles of all sequences: one wave each, four a CU with 32 KiB
-// of LDS tiles, most of it in flight.  (268 MB: 65 us; with 1280, 1536, 2048 or 4096 workers,
-// which do not all run at once, 85, 77, 68 and 75.)
-constexpr int kWorkers = 1024;
-constexpr int kMinTiles = 2;  // tiles of a worker at least
 
 // 16 zero bytes: what lanes without a token load.
 __device__ const uint4 kZero[1] = {};
@@ -134,11 +130,7 @@ struct Order {
       before += lane_of(up, 63);
     }
   }
-  __device__ __forceinline__ int64_t share() const {
-    const int64_t per = total <= 0xffffffffLL ? static_cast<uint32_t>(total + kWorkers - 1) / kWorkers
-                                              : (total + kWorkers - 1) / kWorkers;
-    return per < kMinTiles ? kMinTiles : per;
-  }
+  __device__ __forceinline__ int64_t share() const { return share_of(total); }
 };
 
 // a / b of non-negative values, in 32 bits where they fit.
