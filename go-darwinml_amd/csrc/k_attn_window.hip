@@ -24,7 +24,7 @@ constexpr float kUpLog2 = __is_same(T, f16_t) ? 7.f : 0.f;
 // softmax's running maximum, sum and rescale stay in the lane but for one exchange between
 // the halves a tile.
 template <typename T, int DP>
-struct Queries {
+struct FwdQueries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
   static constexpr int ND = DP / 32;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 3)) void fwd_kerne
   const int bh = spread(blockIdx.x % nbh, nbh);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
   const int q0 = qb * kBQ, qw = q0 + wave * 32, p0 = p.q_start + q0;
-  Queries<T, DP> q;
+  FwdQueries<T, DP> q;
   q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, 1) void fwd_few_kernel(Params p) {
   const int nbh = p.B * p.H;
   const int bh = spread(blockIdx.x % nbh, nbh), qw = blockIdx.x / nbh * 32;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
-  Queries<T, DP> q;
+  FwdQueries<T, DP> q;
   q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);

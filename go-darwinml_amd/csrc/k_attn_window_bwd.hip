@@ -58,7 +58,7 @@ __device__ __forceinline__ int make_room(f32x16& x, f32x16 (&sum)[ND]) {
 // the exponent (P scale = 2^(s c - lse2 + log2 scale)), so an element costs one FMA, one
 // exponential and one multiplication.
 template <typename T, int DP>
-struct Queries {
+struct GradQueries {
   using Tl = tile::Tile<T, DP>;
   using F = typename Tl::F;
   static constexpr bool kF16 = __is_same(T, f16_t);
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 2)) void dq_kernel
   const int bh = spread(blockIdx.x % nbh, nbh);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
   const int q0 = qb * kCols, qw = q0 + wave * 32, p0 = p.q_start + q0;
-  Queries<T, DP> q;
+  GradQueries<T, DP> q;
   q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, 1) void dq_few_kernel(Params p) {
   const int nbh = p.B * p.H;
   const int bh = spread(blockIdx.x % nbh, nbh), qw = blockIdx.x / nbh * 32;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hkv);
-  Queries<T, DP> q;
+  GradQueries<T, DP> q;
   q.place(p, b, qw, lane);
 
   const tile::Rows K = rows_of<T>(p.k, b, hk, q.len), V = rows_of<T>(p.v, b, hk, q.len);
