@@ -85,9 +85,10 @@ __device__ __forceinline__ float select_bit(uint32_t word, int bit, float x, flo
 // The problem's sizes and types; fills p.  Returns GHIP_OK or the error.
 int check_problem(const char* what, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
                   int64_t q_start, int64_t window, int64_t sinks, float scale, Params* p, GHipError* err);
-// One operand: its strides and alignment (out: 8-byte rows of 16-bit values suffice).
-int check_operand(const char* what, const char* name, int dtype, const void* ptr, const int64_t* strides, bool out,
-                  Mat3* m, GHipError* err);
+// One operand of p's batch, `heads` heads, `rows` rows: its strides (an axis of one entry may
+// have any that is not negative) and alignment (out: 8-byte rows of 16-bit values suffice).
+int check_operand(const char* what, const char* name, int dtype, const void* ptr, const int64_t* strides,
+                  const Params& p, int heads, int rows, bool out, Mat3* m, GHipError* err);
 
 }  // namespace win
 }  // namespace ghip

@@ -626,10 +626,11 @@ extern "C" int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, co
   const int64_t es = f32 ? 4 : 2;
   auto al = [](const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>(ptr) & (a - 1)) == 0; };
   bool ok = al(q, 16) && al(k_cache, 16) && al(v_cache, 16) && al(o, 4 * es);
-  for (int i = 0; i < 3; ++i)
-    ok = ok && k_strides[i] >= 0 && v_strides[i] >= 0 && k_strides[i] * es % 16 == 0 && v_strides[i] * es % 16 == 0;
-  for (int i = 0; i < 2; ++i)
-    ok = ok && q_strides[i] >= 0 && o_strides[i] >= 0 && q_strides[i] * es % 16 == 0 && o_strides[i] % 4 == 0;
+  // (An axis of one entry may have any stride that is not negative.)
+  auto whole = [](int64_t stride, int64_t n, int64_t of) { return stride >= 0 && (n <= 1 || stride % of == 0); };
+  const int64_t cache[3] = {num_pages, Hkv, page_size}, rows[2] = {B, H};
+  for (int i = 0; i < 3; ++i) ok = ok && whole(k_strides[i], cache[i], 16 / es) && whole(v_strides[i], cache[i], 16 / es);
+  for (int i = 0; i < 2; ++i) ok = ok && whole(q_strides[i], rows[i], 16 / es) && whole(o_strides[i], rows[i], 4);
   if (!ok)
     return set_error(err, GHIP_ERR_UNSUPPORTED,
                      "%s: q and the caches must be 16-byte aligned with non-negative strides of whole 16 bytes, o "
@@ -687,13 +688,14 @@ extern "C" int ghip_kv_append(int elem_bytes, const void* k, const void* v, void
   if (num_pages == 0 || max_pages == 0)
     return set_error(err, GHIP_ERR_INVALID_ARG, "%s: a cache without pages", kWhat);
   if (table_stride < 0) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: negative table stride", kWhat);
-  // The widest unit that every row and stride is a multiple of.
+  // The widest unit that every row and stride (of an axis of several entries) is a multiple of.
   uint64_t bits = reinterpret_cast<uint64_t>(k) | reinterpret_cast<uint64_t>(v) | reinterpret_cast<uint64_t>(k_cache) |
                   reinterpret_cast<uint64_t>(v_cache) | static_cast<uint64_t>(D * elem_bytes);
+  const int64_t fresh[3] = {B, Hkv, S}, cache[3] = {num_pages, Hkv, page_size};
   for (const int64_t* s : {k_strides, v_strides, k_cache_strides, v_cache_strides})
     for (int i = 0; i < 3; ++i) {
       if (s[i] < 0) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: negative strides", kWhat);
-      bits |= static_cast<uint64_t>(s[i] * elem_bytes);
+      if ((s == k_strides || s == v_strides ? fresh : cache)[i] > 1) bits |= static_cast<uint64_t>(s[i] * elem_bytes);
     }
   if (bits % elem_bytes) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: pointers are not aligned to elements", kWhat);
   const int unit = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;

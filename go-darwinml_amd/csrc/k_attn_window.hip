@@ -297,20 +297,22 @@ int check_problem(const char* what, int dtype, int64_t B, int64_t H, int64_t Hkv
   return GHIP_OK;
 }
 
-int check_operand(const char* what, const char* name, int dtype, const void* ptr, const int64_t* strides, bool out,
-                  Mat3* m, GHipError* err) {
+int check_operand(const char* what, const char* name, int dtype, const void* ptr, const int64_t* strides,
+                  const Params& p, int heads, int rows, bool out, Mat3* m, GHipError* err) {
   if (!ptr || !strides) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: %s is null", what, name);
   const int64_t es = dtype == GHIP_DTYPE_FLOAT32 ? 4 : 2;
   const int64_t al = out ? 4 : 16 / es;
+  const int n[3] = {p.B, heads, rows};
   for (int i = 0; i < 3; ++i)
-    if (strides[i] < 0 || strides[i] % al != 0)
+    if (strides[i] < 0 || (n[i] > 1 && strides[i] % al != 0))
       return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s needs non-negative strides that are multiples of %d elements",
                        what, name, static_cast<int>(al));
-  if (strides[2] >= ((int64_t{1} << 31) / es - 256) / 64)
+  if (rows > 1 && strides[2] >= ((int64_t{1} << 31) / es - 256) / 64)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s needs a sequence stride below 32 MiB", what, name);
   if (reinterpret_cast<uintptr_t>(ptr) % (al * es) != 0)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: %s must be %d-byte aligned", what, name, static_cast<int>(al * es));
-  *m = Mat3{ptr, strides[0], strides[1], strides[2]};
+  // (A tile's rows behind the only one lie behind it, so past the descriptor's end.)
+  *m = Mat3{ptr, p.B > 1 ? strides[0] : 0, heads > 1 ? strides[1] : 0, rows > 1 ? strides[2] : p.D};
   return GHIP_OK;
 }
 
@@ -353,10 +355,10 @@ extern "C" int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, con
   if (B == 0 || Sq == 0) return GHIP_OK;
   if ((Sq + win::kBQ - 1) / win::kBQ * B * H > tile::kMostGroups)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
-  if (int rc = win::check_operand(kWhat, "q", dtype, q, q_strides, false, &p.q, err)) return rc;
-  if (int rc = win::check_operand(kWhat, "k", dtype, k, k_strides, false, &p.k, err)) return rc;
-  if (int rc = win::check_operand(kWhat, "v", dtype, v, v_strides, false, &p.v, err)) return rc;
-  if (int rc = win::check_operand(kWhat, "o", dtype, o, o_strides, true, &p.o, err)) return rc;
+  if (int rc = win::check_operand(kWhat, "q", dtype, q, q_strides, p, p.H, p.Sq, false, &p.q, err)) return rc;
+  if (int rc = win::check_operand(kWhat, "k", dtype, k, k_strides, p, p.Hkv, p.Sk, false, &p.k, err)) return rc;
+  if (int rc = win::check_operand(kWhat, "v", dtype, v, v_strides, p, p.Hkv, p.Sk, false, &p.v, err)) return rc;
+  if (int rc = win::check_operand(kWhat, "o", dtype, o, o_strides, p, p.H, p.Sq, true, &p.o, err)) return rc;
   p.lse = lse;
   p.lens = lens;
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -657,8 +657,11 @@ extern "C" int ghip_sdpa_window_bwd(int dtype, const void* q, const void* k, con
                   {"do", d_out, d_out_strides, false, &p.dout}, {"dq", dq, dq_strides, true, &p.dq},
                   {"dk", dk, dk_strides, true, &p.dk},       {"dv", dv, dv_strides, true, &p.dv}};
   for (const auto& x : operands) {
-    if (Sq == 0 && x.to != &p.k && x.to != &p.v && x.to != &p.dk && x.to != &p.dv) continue;  // empty operands
-    if (int rc = win::check_operand(kWhat, x.name, dtype, x.ptr, x.strides, x.out, x.to, err)) return rc;
+    const bool kv = x.to == &p.k || x.to == &p.v || x.to == &p.dk || x.to == &p.dv;
+    if (Sq == 0 && !kv) continue;  // empty operands
+    if (int rc = win::check_operand(kWhat, x.name, dtype, x.ptr, x.strides, p, kv ? p.Hkv : p.H, kv ? p.Sk : p.Sq, x.out,
+                                    x.to, err))
+      return rc;
   }
   if (!lse && Sq > 0) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: lse is null", kWhat);
   const int64_t need = ghip_sdpa_window_bwd_workspace_bytes(dtype, B, H, Hkv, Sq, Sk, D, q_start, window, sinks);

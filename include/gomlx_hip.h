@@ -267,13 +267,14 @@ int ghip_sdpa_fwd_masked_ws(int dtype, const void* q, const void* k, const void*
  * padding reaches another row.  A NaN or an infinity in a token inside the length may
  * reach any row of its sequence.
  * Operands by ELEMENT strides (batch, head, sequence) as in ghip_sdpa_fwd, those of the
- * inputs 0 or shared as they like; outputs overlap nothing; BFLOAT16 or FLOAT16 with D a multiple of 8 up to 256, or FLOAT32 with a
- * multiple of 4 up to 128; strides multiples of 16 bytes (o: 4 elements), rows at
- * strides below 32 MiB, slices of any size.  lse [B, H, Sq] float32, dense, may be NULL.
- * q_start + Sq <= Sk.  Sums and statistics are fp32; the weights are rounded to the
- * operands' type for the product with v only.  No reference op: it stands beside
- * FusedScaledDotProductAttention (function.go:2669-2907), whose mask operand reads
- * Sq x Sk values and computes every key tile. */
+ * inputs 0 or shared as they like; outputs overlap nothing; BFLOAT16 or FLOAT16 with D a
+ * multiple of 8 up to 256, or FLOAT32 with a multiple of 4 up to 128; strides multiples of 16
+ * bytes (o: 4 elements), rows at strides below 32 MiB (an axis of one entry: any stride that is
+ * not negative), slices of any size.  lse [B, H, Sq] float32, dense, may be NULL.
+ * q_start + Sq <= Sk; scale positive and finite (below 1e30).  Sums and statistics are fp32;
+ * the weights are rounded to the operands' type for the product with v only.  No reference
+ * op: it stands beside FusedScaledDotProductAttention (function.go:2669-2907), whose mask
+ * operand reads Sq x Sk values and computes every key tile. */
 int ghip_sdpa_window_fwd(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
                          int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -331,8 +332,9 @@ int ghip_kv_append(int elem_bytes, const void* k, const void* v, void* k_cache, 
  * [B, H, D] (strides batch, head).  lens is clamped to [0, max_pages * page_size]; a sequence
  * of length 0 gets zeros, and tokens on a page outside [0, num_pages) are not seen.  Rows
  * of the cache that are not seen are never used, whatever they hold.  Types and head dims as
- * ghip_sdpa_window_fwd; q and the caches 16-byte aligned with strides of whole 16
- * bytes, o of whole 4 elements.
+ * ghip_sdpa_window_fwd; q and the caches 16-byte aligned with strides of whole 16 bytes, o of
+ * whole 4 elements (an axis of one entry: any stride that is not negative); scale positive and
+ * finite (below 1e30).
  * With a workspace of ghip_sdpa_paged_workspace_bytes() bytes (16-byte aligned; its size
  * does not depend on the lengths) the tiles of all sequences are dealt out evenly over the
  * card and joined by log-sum-exp in a second kernel, in a fixed order; without one each
