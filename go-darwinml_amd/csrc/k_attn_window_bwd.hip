@@ -543,11 +543,14 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : DP * sizeof(T) > 1
   else K::template run<0>(p, lds, w);
 }
 
+// join_kernel's workgroups of a (batch, kv head).
+__device__ __host__ __forceinline__ int join_groups(const Params& p) { return (p.share_blocks * 64 * (p.D / 4) + 255) / 256; }
+
 // dk, dv of keys whose sums several workgroups hold: the shares, added in order.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr bool kF16 = __is_same(T, f16_t);
-  const int vecs = p.D / 4, wgs = (p.share_blocks * 64 * vecs + 255) / 256;  // workgroups of a (batch, kv head)
+  const int vecs = p.D / 4, wgs = join_groups(p);
   const int bh = blockIdx.x / wgs, b = bh / p.Hkv, hk = bh % p.Hkv;
   const int e = blockIdx.x % wgs * 256 + threadIdx.x;
   const int row = e / vecs, d = e % vecs * 4;  // row: block, then [dk, dv], then key
@@ -576,7 +579,7 @@ static bool list_too_long(int64_t Sq, int64_t G) { return (Sq / kT + 1) * G > 0x
 
 // How dkv_kernel's work is dealt out (its comment): fills p's share fields.
 struct Plan {
-  int64_t groups, floats;  // workgroups, floats of the shares
+  int64_t groups, floats;  // workgroups of dkv_kernel or, if they are more, of join_kernel; floats of the shares
 };
 static Plan plan(Params* p) {
   const int64_t nbh = static_cast<int64_t>(p->B) * p->Hkv;
@@ -588,7 +591,8 @@ static Plan plan(Params* p) {
   p->far = s.far;
   p->share_stride = static_cast<int64_t>(s.shares) * 64 * p->D;
   const int64_t grid = static_cast<int64_t>((p->Sk + kKeys - 1) / kKeys) * nbh;
-  return {s.far ? grid + nbh * s.blocks * s.chunks : s.blocks ? grid * s.chunks : grid, nbh * s.blocks * p->share_stride};
+  const int64_t dkv = s.far ? grid + nbh * s.blocks * s.chunks : s.blocks ? grid * s.chunks : grid;
+  return {std::max(dkv, nbh * join_groups(*p)), nbh * s.blocks * p->share_stride};
 }
 
 // Floats of the statistics, a whole number of 16 bytes.
@@ -607,8 +611,7 @@ static void launch_d(const Params& p, hipStream_t s) {
     hipLaunchKernelGGL((dq_kernel<T, DP>), dim3(static_cast<unsigned>((p.Sq + kCols - 1) / kCols * bh)), dim3(256), 0, s, p);
   hipLaunchKernelGGL((dkv_kernel<T, DP>), dim3(static_cast<unsigned>(wgs) * nbh), dim3(256), 0, s, p);
   if (p.share_blocks)
-    hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>((p.share_blocks * 64 * (p.D / 4) + 255) / 256) * nbh),
-                       dim3(256), 0, s, p);
+    hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>(join_groups(p)) * nbh), dim3(256), 0, s, p);
 }
 template <typename T>
 static void launch(const Params& p, hipStream_t s) {
