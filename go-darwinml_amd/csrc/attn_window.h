@@ -31,9 +31,9 @@ struct Params {
 
 // The workgroups of 32 queries up to which the kernels that share their keys among the waves
 // are taken (measured at the forward kernels' launch): one round of the card, one
-// workgroup a CU (rows of 128 bytes: two); in fp32 nearly four.
+// workgroup a CU (rows of 128 bytes: two); in fp32 three.
 constexpr int64_t few_most(int elem_bytes, int dp) {
-  return elem_bytes == 4 ? 1023 : dp * elem_bytes > 128 ? 256 : 512;
+  return elem_bytes == 4 ? 768 : dp * elem_bytes > 128 ? 256 : 512;
 }
 
 // The tokens of sequence b that exist: lens[b] clamped to [0, Sk].

@@ -576,10 +576,16 @@ __global__ __launch_bounds__(256) void append_kernel(Append p) {
 using namespace ghip;
 
 // No workspace, so a wave for each unit: caches of at most 4 tiles a sequence, or 12 with
-// 512 units or more.  bf16, 32 heads over 8, us a call split / unsplit: 16 sequences of 128
-// tokens (4 tiles) 11.7 / 10.6, of 192 12.1 / 13.9; 64 sequences of 384 (12 tiles) 30.3 /
-// 28.5, of 512 36.1 / 36.7.  (More units hide the two kernels' latencies, not the second
-// launch.)
+// 512 units or more.  (More units hide the two kernels' latencies, not the second launch.)
+// bf16 D 128, sequences of one length, us a call in a graph, split / unsplit:
+//   units      4 tiles      6           8           12          16          24
+//   64         11.0 / 10.3  11.3 / 13.7  11.3 / 17.2  11.7 / 23.8
+//   256        12.9 / 10.4  13.8 / 13.9  14.7 / 18.3  19.1 / 25.5
+//   512        16.6 / 11.7  21.1 / 16.2  24.3 / 20.4  30.2 / 28.4  35.9 / 36.5  46.9 / 52.5
+//   1024       26.7 / 15.7  32.2 / 21.3  38.2 / 26.6  49.7 / 37.6  60.4 / 46.9  97.8 / 81.9
+// (As many units as workers and more fill the card unsplit when the lengths are alike; the
+// rule, which does not know them, splits from 13 tiles on: one sequence of the whole cache
+// among short ones would keep the others waiting.)
 extern "C" int64_t ghip_sdpa_paged_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                    int64_t page_size, int64_t max_pages) {
   if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 256 || page_size <= 0 || max_pages <= 0) return 0;

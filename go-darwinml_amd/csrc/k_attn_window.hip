@@ -317,12 +317,19 @@ int check_operand(const char* what, const char* name, int dtype, const void* ptr
 }
 
 // Which kernel: fwd_few_kernel while its workgroups, four times as many, run at once (one
-// a CU, rows of 128 bytes two), us a call: bf16 D 128, 64 queries of 32 heads over a window
-// of 1024 (64 workgroups) 18.0 against 25.5, 512 queries of 16 heads, window 128 (256) 9.6
-// against 11.5, of 32 heads without one (512) 20.5 against 14.9; f16 D 64 the same (512)
-// 9.4 against 11.5.  In fp32, where a tile's products take 16 times as long, up to fewer
-// than 1024: 64 queries, window 1024 52 against 165, 512 of 32 heads (512) 42 against 78, 1024
-// of 32 heads, window 2048 (1024) 349 against 320.
+// a CU, rows of 128 bytes two).  32 heads over 8, windows of 128 / 1024, us a call in a graph,
+// fwd_few_kernel against fwd_kernel at so many workgroups of 32 queries:
+//   bf16 D 128, 256: 9.9 / 18.6 against 11.6 / 31.3; 288: 17.6 / 33.2 against 11.7 / 31.1
+//   bf16 D 256, 256: 19.4 / 37.5 against 22.0 / 56.6; 288: 35.6 / 68.9 against 22.2 / 56.6
+//   f16 D 64, 512: 7.7 / 15.4 against 9.4 / 25.5; 544: 11.8 / 23.3 against 9.5 / 25.6
+// In fp32, where a tile's products take 16 times as long, a third round still breaks even:
+//   D 64, 512: 21.4 / 55.8 against 23.9 / 88.0; 768: 30.4 / 81.8 against 24.4 / 88.0; 896: 38.9
+//   / 108 against 24.6 / 88.5;  D 128, 768: 50.8 / 144 against 44.7 / 166; 896: 66.7 / 190
+//   against 45.6 / 167
+// (768, windows of 192 to 512: within 5% either way at D 128, 3 to 13% behind at D 64; a
+// window of 2048: a quarter ahead.)  The gradient's dq_few_kernel goes by the same rule: whole
+// gradients bf16 D 128, 256: 37.3 / 49.8 against 39.1 / 63.6; 288: 46.9 / 68.3 against 40.2 /
+// 66.8; fp32 D 64, 768: 103 / 339 against 95 / 346; 896: 116 / 412 against 95 / 383.
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
   const int64_t bh = static_cast<int64_t>(p.B) * p.H, few = (p.Sq + 31) / 32 * bh, many = (p.Sq + kBQ - 1) / kBQ * bh;
