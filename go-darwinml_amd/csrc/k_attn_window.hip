@@ -137,7 +137,7 @@ struct FwdQueries {
 // in flight during a tile.  Bound by a SIMD's matrix and vector cycles, which add up: of a
 // 32 x 32 tile at D 128, 512 and about 530.  32-key tiles leave registers for three waves a
 // SIMD, each computing in another's waits.  bf16, D 128, counting visible pairs: 32 heads of
-// 8192 tokens causal 542 us (1.01 PFLOP/s), with a window of 2048 256 us (0.94; that sum at
+// 8192 tokens causal 550 us (1.00 PFLOP/s), with a window of 2048 266 us (0.91; that sum at
 // the 1.9 GHz it runs at: 246 us); 4 x 16 heads of 2048 tokens, window 512, 60 us (0.50),
 // where 4 workgroups a CU run as three and one.  No faster: three LDS stages (1% at D 128, 4% slower at 256),
 // windows walked so that neighbours meet at the same tiles (half the L2 misses, 2% faster

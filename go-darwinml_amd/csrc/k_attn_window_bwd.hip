@@ -491,7 +491,7 @@ struct Keys {
 // Bound by the exchange of P with its two barriers a tile: 4 x 16 heads of 2048 tokens,
 // window 512, sinks, bf16 D 128 100 us (0.61 PFLOP/s of visible pairs), 34% of the cycles in
 // matrix instructions, 28% in vector ones.  Three waves a SIMD instead of two took the whole
-// gradient from 187 to 178 us.
+// gradient from 187 to 178 us (184 on another card).
 // A workgroup has 64 keys and every tile of queries that sees any of them, except
 //   * far: every query sees the sinks, so their keys' sums run over the whole sequence, not
 //     over a window; the queries beyond the window of the sinks' workgroup are left to
