@@ -139,9 +139,9 @@ struct FwdQueries {
 // SIMD, each computing in another's waits.  bf16, D 128, counting visible pairs: 32 heads of
 // 8192 tokens causal 550 us (1.00 PFLOP/s), with a window of 2048 266 us (0.91; that sum at
 // the 1.9 GHz it runs at: 246 us); 4 x 16 heads of 2048 tokens, window 512, 60 us (0.50),
-// where 4 workgroups a CU run as three and one.  No faster: three LDS stages (1% at D 128, 4% slower at 256),
-// windows walked so that neighbours meet at the same tiles (half the L2 misses, 2% faster
-// there, 3-5% slower on windows of 128 and in fp32).
+// where 4 workgroups a CU run as three and one.  No faster: three LDS stages (1% at D 128, 4%
+// slower at 256), windows walked so that neighbours meet at the same tiles (half the L2 misses,
+// 2% faster there, 3-5% slower on windows of 128 and in fp32).
 constexpr int kBQ = 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) > 256 ? 1 : 3)) void fwd_kernel(Params p) {

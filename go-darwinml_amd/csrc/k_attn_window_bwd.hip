@@ -22,8 +22,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // f16 (5 bits of exponent): P, at most 1 and of order 1 / window, is rounded 2^15 times larger,
 // and dS, whose size follows d_out's and the window's, times a power of two 2^e that each
 // column (a lane's query in dq, its key in dk) finds as its running maximum does in a
-// softmax: from kFirst, where all that could reach an f16 result is inside the range, e falls
-// when a tile's values pass 2^15, so that they end below 2^7 and leave 2^8 for later tiles.  A
+// softmax: from first_exponent(), where all that could reach an f16 result is inside the range, e
+// falls when a tile's values pass 2^15, so that they end below 2^7 and leave 2^8 for later tiles.  A
 // value then keeps all its bits down to 2^-20 of the largest, and none overflows.  The sums
 // follow, and lose 2^e at the end, in fp32.  The whole gradient, with a fixed factor / so: 4 x
 // 16 heads of 2048 tokens, D 128, window 512 179 / 185 us, padded batch of 12 heads of 64 52.4 /
@@ -491,7 +491,7 @@ struct Keys {
 // Bound by the exchange of P with its two barriers a tile: 4 x 16 heads of 2048 tokens,
 // window 512, sinks, bf16 D 128 100 us (0.61 PFLOP/s of visible pairs), 34% of the cycles in
 // matrix instructions, 28% in vector ones.  Three waves a SIMD instead of two took the whole
-// gradient from 187 to 178 us (184 on another card).
+// gradient from 187 to 178-184 us.
 // A workgroup has 64 keys and every tile of queries that sees any of them, except
 //   * far: every query sees the sinks, so their keys' sums run over the whole sequence, not
 //     over a window; the queries beyond the window of the sinks' workgroup are left to
