@@ -12,9 +12,9 @@ constexpr int kWorkers = 1024;
 constexpr int kMinTiles = 2;  // tiles of a worker at least
 
 // Tiles of a worker, of `total` in all.  (A division in 32 bits where the dividend fits.)
-constexpr int64_t share_of(int64_t total) {
-  const int64_t up = total + kWorkers - 1;
-  const int64_t per = up <= 0xffffffffLL ? static_cast<uint32_t>(up) / kWorkers : up / kWorkers;
+constexpr int64_t share_of(int64_t total, int workers = kWorkers) {
+  const int64_t up = total + workers - 1;
+  const int64_t per = up <= 0xffffffffLL ? static_cast<uint32_t>(up) / static_cast<uint32_t>(workers) : up / workers;
   return per < kMinTiles ? kMinTiles : per;
 }
 

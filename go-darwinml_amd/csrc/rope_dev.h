@@ -1,0 +1,53 @@
+// Rotary positions on the device: the angles of a workgroup's tokens, and the rotation.
+#pragma once
+
+#include "common.h"
+
+namespace ghip {
+namespace rope {
+
+constexpr int kMostAxes = 4;
+constexpr int kMostHalf = 128;  // pairs of a row
+
+// Which angle turns which pair: pair i of token (b, s) by positions[axis(i)][b][s] * freqs[i].
+struct Angles {
+  const int32_t* positions;  // nullptr: starts[b] + s
+  const int32_t* starts;
+  const float* freqs;
+  int64_t p_sa, p_sb, p_ss;  // element strides of axis, sequence, token
+  int half;                  // pairs of a row
+  int ends[kMostAxes];       // where each axis' pairs end
+  int neighbours;            // pairs (2i, 2i + 1); 0: (i, i + half)
+  int inverse;
+};
+
+// The position that turns pair i of token (b, s).
+__device__ __forceinline__ double position(const Angles& a, int b, int s, int i) {
+  if (!a.positions) return static_cast<double>(static_cast<int64_t>(a.starts[b]) + s);
+  const int axis = (i >= a.ends[0]) + (i >= a.ends[1]) + (i >= a.ends[2]);
+  return static_cast<double>(a.positions[axis * a.p_sa + b * a.p_sb + s * a.p_ss]);
+}
+
+// (cos, sin) of pos * freq.  The angle is a product in 64 bits, reduced by whole turns in two
+// steps (2 pi as the sum of two doubles), so positions of any size keep 2^-52 of a turn;
+// each of the two is rounded to fp32 once.  (An fp32 angle of 10^5 is off by 2^-8.)
+__device__ __forceinline__ float2 turn(double pos, float freq, int inverse) {
+  const double a = pos * static_cast<double>(freq);
+  const double k = rint(a * 0.15915494309189535);
+  double r = fma(-k, 6.283185307179586, a);
+  r = fma(-k, 2.4492935982947064e-16, r);
+  double s, c;
+  sincos(r, &s, &c);
+  return make_float2(static_cast<float>(c), static_cast<float>(inverse ? -s : s));
+}
+
+// (x, y) turned.  Each product is rounded by itself: left to be fused with the sum, which of
+// them is would depend on the kernel, and a key's code in a 4-bit cache with it.
+__device__ __forceinline__ float2 turned(float x, float y, float2 cs) {
+#pragma clang fp contract(off)
+  const float xc = x * cs.x, ys = y * cs.y, xs = x * cs.y, yc = y * cs.x;
+  return make_float2(xc - ys, xs + yc);
+}
+
+}  // namespace rope
+}  // namespace ghip

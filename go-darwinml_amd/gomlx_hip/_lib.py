@@ -38,6 +38,21 @@ _vp = ctypes.c_void_p
 _f32 = ctypes.c_float
 _errp = ctypes.POINTER(GHipError)
 
+class Rope(ctypes.Structure):
+    """GHipRope."""
+    _fields_ = [("positions", _vp), ("position_strides", _i64 * 3), ("axes", _i64), ("sections", _i64 * 4),
+                ("freqs", _vp), ("rotary_dim", _i64), ("interleaved", _i64)]
+
+
+class Kv4(ctypes.Structure):
+    """GHipKv4."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("code_strides", _i64 * 3), ("scale_strides", _i64 * 3)]
+
+
+_i64p = ctypes.POINTER(_i64)
+_ropep = ctypes.POINTER(Rope)
+_kv4p = ctypes.POINTER(Kv4)
+
 # name -> argtypes (every entry point returns int except where noted).
 SIGNATURES = {
     "ghip_softmax_rows": [_int, _vp, _vp, _i64, _i64, _int, _vp, _errp],
@@ -81,6 +96,15 @@ SIGNATURES = {
                       + [_vp, _errp],
     "ghip_sdpa_paged": [_int] + [_vp] * 4 + [_i64] * 7 + [_vp, _i64, _vp] + [ctypes.POINTER(_i64)] * 4
                        + [_i64, _i64, _f32, _vp, _i64, _vp, _errp],
+    "ghip_rope": [_int, _vp, _vp] + [_i64] * 4 + [_i64p, _i64p, _ropep, _int, _vp, _errp],
+    "ghip_kv_append_rope": [_int] + [_vp] * 6 + [_i64] * 8 + [_vp, _i64, _vp, _vp] + [_i64p] * 6 + [_ropep, _vp, _errp],
+    "ghip_kv4_append_rope": [_int] + [_vp] * 4 + [_kv4p] * 2 + [_i64] * 8 + [_vp, _i64, _vp, _vp] + [_i64p] * 4
+                            + [_ropep, _vp, _errp],
+    "ghip_kv4_read": [_int, _kv4p, _kv4p, _vp, _vp] + [_i64] * 7 + [_vp, _i64, _vp, _i64p, _i64p, _vp, _errp],
+    "ghip_sdpa_paged_kv4": [_int, _vp, _kv4p, _kv4p, _vp] + [_i64] * 7 + [_vp, _i64, _vp, _i64p, _i64p, _i64, _i64, _f32,
+                                                                          _vp, _i64, _vp, _errp],
+    "ghip_token_logprobs": [_int, _vp, _i64, _vp] + [_i64] * 3 + [_f32] + [_vp] * 6 + [_i64, _vp, _errp],
+    "ghip_token_logprobs_grad": [_int, _vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _vp, _i64, _vp, _errp],
 }
 
 # name -> argtypes of the entry points that return int64_t.
@@ -89,6 +113,8 @@ SIGNATURES_I64 = {
     "ghip_gemm_workspace_bytes": [_int, _int, _i64, _i64, _i64, _i64],
     "ghip_sdpa_window_bwd_workspace_bytes": [_int] + [_i64] * 9,
     "ghip_sdpa_paged_workspace_bytes": [_int] + [_i64] * 6,
+    "ghip_sdpa_paged_kv4_workspace_bytes": [_i64] * 6,
+    "ghip_token_logprobs_workspace_bytes": [_int] + [_i64] * 3,
 }
 
 _lib = None

@@ -507,6 +507,275 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     return out
 
 
+_I4 = ctypes.c_int64 * 4
+
+
+def _rope(what: str, freqs, positions, sections, interleaved, B: int, S: int, D: int):
+    """The GHipRope of a call on B sequences of S tokens (None: nothing is turned)."""
+    if freqs is None:
+        if positions is not None or sections is not None:
+            raise ValueError(f"{what}: positions and sections go with freqs")
+        return None
+    if freqs.dtype != torch.float32 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError(f"{what}: freqs is a contiguous float32 vector, one value a pair")
+    pairs, axes, step = freqs.shape[0], 1, (0, 0, 0)
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.dim() not in (2, 3) or positions.shape[-2:] != (B, S):
+            raise ValueError(f"{what}: positions is int32 [{B}, {S}] or [axes, {B}, {S}]")
+        axes = positions.shape[0] if positions.dim() == 3 else 1
+        step = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
+    sections = [pairs] if sections is None else list(sections)
+    if len(sections) != axes or axes > 4:
+        raise ValueError(f"{what}: {len(sections)} sections for {axes} axes of positions (1 to 4)")
+    return _lib.Rope(_ptr(positions), _I3(*step), axes, _I4(*sections), freqs.data_ptr(), 2 * pairs, int(interleaved))
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections=None, interleaved: bool = False,
+         inverse: bool = False, out=None, stream=None) -> torch.Tensor:
+    """Rotary positions: pair i of each row of x [B, H, S, D] (any strides with a contiguous head
+    dim) turned by positions * freqs[i]; positions int32 [B, S], or [axes, B, S] with `sections`,
+    the number of pairs that each axis turns.  freqs: float32 [rotary_dim / 2]; interleaved: pairs
+    are neighbours, else half a rotary_dim apart.  inverse: turned back, the gradient of x from
+    that of the output.  out may be x.  Wraps ghip_rope."""
+    dev = _one_device(x, positions, freqs, out)
+    if x.dim() != 4:
+        raise ValueError("rope: x [B, H, S, D] is needed")
+    B, H, S, D = x.shape
+    if positions is None or freqs is None:
+        raise ValueError("rope: positions and freqs are needed")
+    r = _rope("rope", freqs, positions, sections, interleaved, B, S, D)
+    if out is None:
+        out = _empty((B, H, S, D), x.dtype, dev, stream)
+    else:
+        _like("rope: out", out, x.shape, x.dtype)
+    _launch(dev, "ghip_rope", stream, dtype_code(x.dtype), x.data_ptr(), out.data_ptr(), B, H, S, D, _rows3("x", x),
+            _rows3("out", out), ctypes.byref(r), int(inverse))
+    return out
+
+
+def _new_tokens(what, q, k, v, q_out, stream, dev):
+    """(B, H, Hkv, S, D), q_out and the strides of an append's operands."""
+    if k.dim() != 4 or (q is not None and q.dim() != 4):
+        raise ValueError(f"{what}: q [B, H, S, D] and k / v [B, Hkv, S, D] are needed")
+    B, Hkv, S, D = k.shape
+    _like(f"{what}: v", v, k.shape, k.dtype)
+    if q is None:
+        if q_out is not None:
+            raise ValueError(f"{what}: q_out goes with q")
+        return (B, 0, Hkv, S, D), None, (None, None, _rows3("k", k), _rows3("v", v))
+    H = q.shape[1]
+    _like(f"{what}: q", q, (B, H, S, D), k.dtype)
+    if q_out is None:
+        q_out = _empty((B, H, S, D), q.dtype, dev, stream)
+    else:
+        _like(f"{what}: q_out", q_out, q.shape, q.dtype)
+    return (B, H, Hkv, S, D), q_out, (_rows3("q", q), _rows3("q_out", q_out), _rows3("k", k), _rows3("v", v))
+
+
+def kv_append_rope(q, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_table: torch.Tensor, starts: torch.Tensor, freqs, counts=None, positions=None, sections=None,
+                   interleaved: bool = False, q_out=None, stream=None):
+    """kv_append with rotary positions on the way: k is turned as rope does and v copied into the
+    pages, q [B, H, S, D] (None: none) is turned into q_out, which is returned (it may be q).
+    positions None: token i of sequence b is at starts[b] + i; freqs None: nothing is turned.
+    Wraps ghip_kv_append_rope."""
+    what = "kv_append_rope"
+    dev = _one_device(k, q, v, k_cache, v_cache, block_table, starts, freqs, counts, positions, q_out)
+    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream, dev)
+    pages, size, per, ts = _check_cache(what, k_cache, v_cache, block_table, B, Hkv, D, k.dtype)
+    _ints(f"{what}: starts", starts, B)
+    _ints(f"{what}: counts", counts, B)
+    r = _rope(what, freqs, positions, sections, interleaved, B, S, D)
+    _launch(dev, "ghip_kv_append_rope", stream, dtype_code(k.dtype), _ptr(q), _ptr(q_out), k.data_ptr(), v.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), B, H, Hkv, S, D, pages, size, per, block_table.data_ptr(), ts,
+            starts.data_ptr(), _ptr(counts), *steps, _rows3("k_cache", k_cache), _rows3("v_cache", v_cache), r)
+    return q_out
+
+
+def kv4_cache(num_pages: int, page_size: int, Hkv: int, D: int, device="cuda"):
+    """A paged cache's storage for keys (or values) in 4 bits: (codes [num_pages, Hkv, page_size,
+    D / 2], scales [num_pages, Hkv, page_size, 4 ceil(D / 128)]), uint8, all zeros."""
+    return (torch.zeros((num_pages, Hkv, page_size, D // 2), dtype=torch.uint8, device=device),
+            torch.zeros((num_pages, Hkv, page_size, (D + 127) // 128 * 4), dtype=torch.uint8, device=device))
+
+
+def _kv4(what, k_cache, v_cache, block_table, B, Hkv, D):
+    """The two GHipKv4 of caches (codes, scales) viewed as [page, Hkv, token, ...], and
+    (num_pages, page_size, max_pages, table stride)."""
+    made = []
+    shape = k_cache[0].shape
+    for name, (codes, scales) in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if codes.dim() != 4 or codes.shape != shape or codes.shape[1] != Hkv or codes.shape[3] * 2 != D or codes.dtype != torch.uint8:
+            raise ValueError(f"{what}: {name}'s codes are uint8 [pages, {Hkv}, page_size, {D // 2}], both alike")
+        _like(f"{what}: {name}'s scales", scales, (*shape[:3], (D + 127) // 128 * 4), torch.uint8)
+        made.append(_lib.Kv4(codes.data_ptr(), scales.data_ptr(), _rows3(f"{name}'s codes", codes),
+                             _rows3(f"{name}'s scales", scales)))
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B:
+        raise ValueError(f"{what}: block_table is int32 [{B}, pages of a sequence]")
+    step, one = block_table.stride()
+    per = block_table.shape[1]
+    if per > 1 and one != 1:
+        raise ValueError(f"{what}: a sequence's table entries must be contiguous")
+    return made, (shape[0], shape[2], per, step)
+
+
+def kv4_append_rope(q, k: torch.Tensor, v: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor,
+                    starts: torch.Tensor, freqs, counts=None, positions=None, sections=None, interleaved: bool = False,
+                    q_out=None, stream=None):
+    """kv_append_rope into caches of 4 bits, (codes, scales) as kv4_cache makes them: E2M1 values
+    and a power of two for each 32.  D: a multiple of 32.  Wraps ghip_kv4_append_rope."""
+    what = "kv4_append_rope"
+    dev = _one_device(k, q, v, *k_cache, *v_cache, block_table, starts, freqs, counts, positions, q_out)
+    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream, dev)
+    (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
+    _ints(f"{what}: starts", starts, B)
+    _ints(f"{what}: counts", counts, B)
+    r = _rope(what, freqs, positions, sections, interleaved, B, S, D)
+    _launch(dev, "ghip_kv4_append_rope", stream, dtype_code(k.dtype), _ptr(q), _ptr(q_out), k.data_ptr(), v.data_ptr(),
+            kc, vc, B, H, Hkv, S, D, pages, size, per, block_table.data_ptr(), ts, starts.data_ptr(), _ptr(counts), *steps, r)
+    return q_out
+
+
+def kv4_read(k_cache, v_cache, block_table: torch.Tensor, tokens: int, lens=None, dtype=torch.bfloat16, outs=None,
+             stream=None):
+    """(k, v) [B, Hkv, tokens, D]: each sequence's first tokens out of caches of 4 bits, as the
+    values they hold; zeros past lens[b] (int32 [B]; None: none) and on pages out of range.
+    What sdpa_window takes for a later chunk of a prompt.  Wraps ghip_kv4_read."""
+    what = "kv4_read"
+    dev = _one_device(*k_cache, *v_cache, block_table, lens, *(outs or ()))
+    B = block_table.shape[0]
+    if k_cache[0].dim() != 4:
+        raise ValueError(f"{what}: the caches are [pages, Hkv, page_size, ...]")
+    Hkv, D = k_cache[0].shape[1], 2 * k_cache[0].shape[3]
+    (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
+    _ints(f"{what}: lens", lens, B)
+    shape = (B, Hkv, int(tokens), D)
+    k, v = outs if outs is not None else (_empty(shape, dtype, dev, stream), _empty(shape, dtype, dev, stream))
+    _like(f"{what}: k", k, shape, k.dtype)
+    _like(f"{what}: v", v, shape, k.dtype)
+    _launch(dev, "ghip_kv4_read", stream, dtype_code(k.dtype), kc, vc, k.data_ptr(), v.data_ptr(), B, Hkv, int(tokens), D,
+            pages, size, per, block_table.data_ptr(), ts, _ptr(lens), _rows3("k", k), _rows3("v", v))
+    return k, v
+
+
+def sdpa_paged_kv4_workspace(q: torch.Tensor, k_cache, block_table: torch.Tensor, stream=None):
+    """Workspace for sdpa_paged_kv4 at these sizes (None when the sequences never split), for
+    calls on `stream`."""
+    B, H, D = q.shape
+    n = _lib.load().ghip_sdpa_paged_kv4_workspace_bytes(B, H, k_cache[0].shape[1], D, k_cache[0].shape[2],
+                                                        block_table.shape[1])
+    return _empty((n,), torch.uint8, q.device, stream) if n > 0 else None
+
+
+def sdpa_paged_kv4(q: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor, lens: torch.Tensor, scale: float,
+                   window: int = 0, sinks: int = 0, out=None, stream=None, split: bool = True, workspace=None):
+    """sdpa_paged over caches of 4 bits, (codes, scales) each, as kv4_append_rope wrote them.
+    Wraps ghip_sdpa_paged_kv4."""
+    what = "sdpa_paged_kv4"
+    dev = _one_device(q, *k_cache, *v_cache, block_table, lens, out, workspace)
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q [B, H, D] is needed")
+    B, H, D = q.shape
+    Hkv = k_cache[0].shape[1] if k_cache[0].dim() == 4 else 0
+    (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
+    _ints(f"{what}: lens", lens, B)
+    if out is None:
+        out = _empty((B, H, D), q.dtype, dev, stream)
+    else:
+        _like(f"{what}: out", out, (B, H, D), q.dtype)
+    for name, t in (("q", q), ("out", out)):
+        if t.stride(2) != 1 and D != 1:
+            raise ValueError(f"{what}: {name}'s head dim must be contiguous")
+    ws = None
+    if split and workspace is None:
+        ws = sdpa_paged_kv4_workspace(q, k_cache, block_table, stream)
+    elif split:
+        ws = _given(what, workspace)
+    _launch(dev, "ghip_sdpa_paged_kv4", stream, dtype_code(q.dtype), q.data_ptr(), kc, vc, out.data_ptr(), B, H, Hkv, D,
+            pages, size, per, block_table.data_ptr(), ts, lens.data_ptr(), _I3(q.stride(0), q.stride(1)),
+            _I3(out.stride(0), out.stride(1)), int(window), int(sinks), float(scale), _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size())
+    return out
+
+
+def _logits(what: str, logits, ids):
+    """The row stride of logits [N, V] beside ids [N]."""
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: logits [N, V] are needed")
+    if logits.stride(1) != 1 and logits.shape[1] != 1:
+        raise ValueError(f"{what}: a row's logits must be contiguous")
+    _ints(f"{what}: ids", ids, logits.shape[0])
+    return logits.stride(0)
+
+
+def token_logprobs_workspace(logits: torch.Tensor, top: int = 0, stream=None):
+    """Workspace for token_logprobs at these sizes (None where a row is never shared), for calls
+    on `stream`."""
+    n = _lib.load().ghip_token_logprobs_workspace_bytes(dtype_code(logits.dtype), *logits.shape, int(top))
+    return _empty((n,), torch.uint8, logits.device, stream) if n > 0 else None
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, scale: float = 1.0, outs=None, stream=None,
+                   split: bool = True, workspace=None):
+    """(logp, entropy, lse, top_logps, top_ids) of rows of logits [N, V] times scale (1 /
+    temperature): the log probability of each row's token ids [N] (int32; outside [0, V): 0),
+    the entropy and the log-sum-exp of the row (float32 [N]), and the log probabilities and
+    indices of the `top` largest logits, larger first, equal ones by index ([N, top]; None
+    where top is 0).  outs: the five tensors to write.  split: with a workspace (`workspace`, or
+    one allocated here), so few rows are shared out over the card.  Wraps ghip_token_logprobs."""
+    what = "token_logprobs"
+    dev = _one_device(logits, ids, workspace, *(outs or ()))
+    step = _logits(what, logits, ids)
+    N, V = logits.shape
+    top = int(top)
+    shapes = ((N,), torch.float32), ((N,), torch.float32), ((N,), torch.float32), ((N, top), torch.float32), ((N, top), torch.int32)
+    if outs is None:
+        outs = [_empty(shape, dt, dev, stream) if i < 3 or top > 0 else None for i, (shape, dt) in enumerate(shapes)]
+    else:
+        for i, (t, (shape, dt)) in enumerate(zip(outs, shapes, strict=True)):
+            if t is None and (i < 3 or top > 0):
+                raise ValueError(f"{what}: five outputs are needed (the last two may be None where top is 0)")
+            if t is not None:
+                _like(f"{what}: output {i}", t, shape, dt)
+                if not t.is_contiguous():
+                    raise ValueError(f"{what}: outputs must be contiguous")
+    ws = None
+    if split and workspace is None:
+        ws = token_logprobs_workspace(logits, top, stream)
+    elif split:
+        ws = _given(what, workspace)
+    _launch(dev, "ghip_token_logprobs", stream, dtype_code(logits.dtype), logits.data_ptr(), step, ids.data_ptr(), N, V, top,
+            float(scale), *(_ptr(t) for t in outs), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size())
+    return tuple(outs)
+
+
+def token_logprobs_grad(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, d_logp, entropy=None, d_entropy=None,
+                        scale: float = 1.0, out=None, stream=None) -> torch.Tensor:
+    """The gradient of logits from those of token_logprobs' logp and entropy (float32 [N]; one of
+    them may be None), with the lse and, beside d_entropy, the entropy that it gave.  out may be
+    logits.  Wraps ghip_token_logprobs_grad."""
+    what = "token_logprobs_grad"
+    dev = _one_device(logits, ids, lse, d_logp, entropy, d_entropy, out)
+    step = _logits(what, logits, ids)
+    N, V = logits.shape
+    if lse is None or (d_logp is None and d_entropy is None) or (d_entropy is not None and entropy is None):
+        raise ValueError(f"{what}: lse and d_logp or d_entropy (with entropy) are needed")
+    for name, t in (("lse", lse), ("d_logp", d_logp), ("entropy", entropy), ("d_entropy", d_entropy)):
+        if t is not None:
+            _like(f"{what}: {name}", t, (N,), torch.float32)
+            if not t.is_contiguous():
+                raise ValueError(f"{what}: {name} must be contiguous")
+    if out is None:
+        out = _empty((N, V), logits.dtype, dev, stream)
+    else:
+        _like(f"{what}: out", out, (N, V), logits.dtype)
+        if out.stride(1) != 1 and V != 1:
+            raise ValueError(f"{what}: a row of out must be contiguous")
+    _launch(dev, "ghip_token_logprobs_grad", stream, dtype_code(logits.dtype), logits.data_ptr(), step, ids.data_ptr(),
+            lse.data_ptr(), _ptr(entropy), _ptr(d_logp), _ptr(d_entropy), N, V, float(scale), out.data_ptr(), out.stride(0))
+    return out
+
+
 def gather_rows(table: torch.Tensor, ids: torch.Tensor, out=None, stream=None):
     """out[i] = table[clamp(ids[i])] for an embedding table [V, ...]."""
     _check_dev(table, ids)

@@ -351,6 +351,127 @@ int ghip_sdpa_paged(int dtype, const void* q, const void* k_cache, const void* v
                     const int64_t* v_strides, const int64_t* o_strides, int64_t window, int64_t sinks,
                     float scale, void* workspace, int64_t workspace_bytes, void* stream, GHipError* err);
 
+/* Rotary positions.  A row of D values at token (b, s) is turned pair by pair, pair i < rotary_dim / 2
+ * by the angle a = position * freqs[i] (a product in 64 bits):
+ *   (x, y) -> (x cos a - y sin a, x sin a + y cos a)
+ * Pair i is values (i, i + rotary_dim / 2) of the row, interleaved != 0: (2 i, 2 i + 1); values from
+ * rotary_dim on stay as they are.  positions: int32, read at [axis][b][s] by ELEMENT strides (0
+ * allowed), any sign; axis 0 turns the first sections[0] pairs, axis 1 the next sections[1], ...
+ * (text: one axis; images and video: time, height, width), and the sections hold all pairs. */
+typedef struct {
+  const int32_t* positions;
+  int64_t position_strides[3];
+  int64_t axes;        /* 1 .. 4 */
+  int64_t sections[4];
+  const float* freqs;  /* [rotary_dim / 2], on the device */
+  int64_t rotary_dim;  /* even, at most D; 0: nothing is turned */
+  int64_t interleaved;
+} GHipRope;
+
+/* out[b, h, s] = x[b, h, s] turned; inverse != 0: by -a, which is the gradient of x from the
+ * gradient of out.  [B, H, S, D] by ELEMENT strides (batch, head, sequence) with the head dim
+ * contiguous, D up to 256; out may be x itself (the same strides), else they overlap nothing.
+ * cos and sin are taken in 64 bits and rounded to fp32, products and sums are fp32, rounded
+ * once.  16-byte vectors where pointers, strides and half of rotary_dim allow them, single
+ * values elsewhere.  No reference op (GoMLX composes it of primitives). */
+int ghip_rope(int dtype, const void* x, void* out, int64_t B, int64_t H, int64_t S, int64_t D,
+              const int64_t* x_strides, const int64_t* out_strides, const GHipRope* rope, int inverse,
+              void* stream, GHipError* err);
+
+/* ghip_kv_append with the rotation on the way: k [B, Hkv, S, D] is turned and v copied into the
+ * pages, and q [B, H, S, D] (H = 0: none) is turned into q_out (which may be q itself).  Without
+ * rope->positions token (b, i) is at position starts[b] + i; rope NULL: nothing is turned.
+ * counts, skipped tokens and pages as there; every row of q is turned, also of tokens that are
+ * not appended.  Two tokens that land in one row race. */
+int ghip_kv_append_rope(int dtype, const void* q, void* q_out, const void* k, const void* v, void* k_cache,
+                        void* v_cache, int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D,
+                        int64_t num_pages, int64_t page_size, int64_t max_pages, const int32_t* block_table,
+                        int64_t table_stride, const int32_t* starts, const int32_t* counts,
+                        const int64_t* q_strides, const int64_t* q_out_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, const int64_t* k_cache_strides,
+                        const int64_t* v_cache_strides, const GHipRope* rope, void* stream, GHipError* err);
+
+/* Rows of a paged cache in 4 bits (a quarter of the bytes of 16): [page, kv head, token] rows of
+ * D values, D a multiple of 32 up to 256.  codes: D / 2 bytes a row, value 2 i in the low half of
+ * byte i and 2 i + 1 in the high one, each a sign bit and one of {0, 1/2, 1, 3/2, 2, 3, 4, 6}
+ * (E2M1); scales: a byte for each 32 consecutive values, which are multiplied by
+ * 2^(byte - 127) (255: they are NaN), in rows of 4 * ceil(D / 128) bytes whose last ones may
+ * not be used (the Open Compute Project's MX format of 4 bits).  BYTE strides of page, head,
+ * token; codes 16-byte aligned with strides of whole 16, scales 4-byte aligned with strides
+ * of whole 4 (an axis of one entry: any that is not negative). */
+typedef struct {
+  void* codes;
+  void* scales;
+  int64_t code_strides[3];
+  int64_t scale_strides[3];
+} GHipKv4;
+
+/* ghip_kv_append_rope into a cache of 4 bits.  The scale of 32 values is the least power of two
+ * from 2^-126 to 2^125 of which they are at most 6 (so none is clipped but fp32 values above
+ * 6 * 2^125), the codes are rounded to nearest, ties to the even code, from the turned fp32
+ * values; 32 values one of which is NaN or infinite become NaN. */
+int ghip_kv4_append_rope(int dtype, const void* q, void* q_out, const void* k, const void* v,
+                         const GHipKv4* k_cache, const GHipKv4* v_cache, int64_t B, int64_t H, int64_t Hkv,
+                         int64_t S, int64_t D, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                         const int32_t* block_table, int64_t table_stride, const int32_t* starts,
+                         const int32_t* counts, const int64_t* q_strides, const int64_t* q_out_strides,
+                         const int64_t* k_strides, const int64_t* v_strides, const GHipRope* rope,
+                         void* stream, GHipError* err);
+
+/* Tokens 0 .. S - 1 of each sequence out of a cache of 4 bits, as the values it holds (exact in
+ * BFLOAT16 and FLOAT32 within their range): k / v [B, Hkv, S, D], 16-byte aligned with strides of
+ * whole 16 bytes; what a later chunk of a prompt gives ghip_sdpa_window_fwd.  Tokens from
+ * lens[b] on (lens NULL: none) and those on a page outside [0, num_pages) are zeros.  At most
+ * 65535 sequences. */
+int ghip_kv4_read(int dtype, const GHipKv4* k_cache, const GHipKv4* v_cache, void* k, void* v, int64_t B,
+                  int64_t Hkv, int64_t S, int64_t D, int64_t num_pages, int64_t page_size,
+                  int64_t max_pages, const int32_t* block_table, int64_t table_stride, const int32_t* lens,
+                  const int64_t* k_strides, const int64_t* v_strides, void* stream, GHipError* err);
+
+/* ghip_sdpa_paged over a cache of 4 bits: the same tokens, window and sinks, workspace (of
+ * ghip_sdpa_paged_kv4_workspace_bytes()) and limits, D a multiple of 32 up to 256 for every type
+ * of q.  The cache's values enter the products exactly; q as the sum of one, two or three
+ * bf16 values (BFLOAT16, FLOAT16, FLOAT32: all its bits), the weights as the sum of two, two or
+ * three (16 or 24 bits).  Sums and statistics are fp32. */
+int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                            int64_t page_size, int64_t max_pages);
+int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_cache, const GHipKv4* v_cache, void* o,
+                        int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                        int64_t max_pages, const int32_t* block_table, int64_t table_stride,
+                        const int32_t* lens, const int64_t* q_strides, const int64_t* o_strides,
+                        int64_t window, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes,
+                        void* stream, GHipError* err);
+
+/* Log probabilities of given tokens.  Row r of logits [N, V] (ELEMENT stride row_stride, V
+ * contiguous), times scale (1 / temperature; positive and finite), is x:
+ *   lse = log sum_v exp x_v,  logp = x_id - lse,  entropy = -sum_v p_v log p_v,  p = exp(x - lse)
+ * and the `top` (0 .. 32, at most V) largest logits: top_ids by value, then by index (a NaN
+ * is above all numbers, -0 equals 0), top_logps their log probabilities.  ids: int32 [N]; logp of
+ * an id outside [0, V) is 0.  Outputs [N] and [N, top], dense, float32 and int32; entropy, lse,
+ * top_logps and top_ids may be NULL (top = 0: the last two are not used).
+ * Logits of -infinity are tokens that cannot be (p = 0, log p = -infinity); a row of nothing
+ * else has lse -infinity, entropy 0, log probabilities -infinity.  A row that holds a NaN or
+ * +infinity gets NaN (its top_ids stay as defined).  Sums are fp32, in a fixed order.
+ * workspace: ghip_token_logprobs_workspace_bytes() bytes (0: none needed), 16-byte aligned,
+ * written on `stream`; NULL: a row is one workgroup's.  Beside FusedSoftmax's log form
+ * (function.go:2276-2286), whose output has V values a row. */
+int64_t ghip_token_logprobs_workspace_bytes(int dtype, int64_t N, int64_t V, int64_t top);
+int ghip_token_logprobs(int dtype, const void* logits, int64_t row_stride, const int32_t* ids, int64_t N,
+                        int64_t V, int64_t top, float scale, float* logp, float* entropy, float* lse,
+                        float* top_logps, int32_t* top_ids, void* workspace, int64_t workspace_bytes,
+                        void* stream, GHipError* err);
+
+/* Gradient of the logits from those of logp and entropy (each [N] float32, one of them may be
+ * NULL), the lse and (where d_entropy is given) the entropy that ghip_token_logprobs gave:
+ *   d_logits_v = scale (d_logp ([v = id] - p_v) - d_entropy p_v (log p_v + entropy))
+ * A row whose id is outside [0, V) has no logp (d_logp is not used there); rows of lse -infinity
+ * get zeros.  d_logits [N, V] in the logits' type with a row stride of its own; it may be the
+ * logits themselves (the same stride), else they overlap nothing. */
+int ghip_token_logprobs_grad(int dtype, const void* logits, int64_t row_stride, const int32_t* ids,
+                             const float* lse, const float* entropy, const float* d_logp,
+                             const float* d_entropy, int64_t N, int64_t V, float scale, void* d_logits,
+                             int64_t d_row_stride, void* stream, GHipError* err);
+
 /* Embedding lookup: out[i, :] = table[clamp(ids[i], 0, V-1), :] (row_bytes per
  * row, copied bit-exactly).  Replaces the gather fast path
  * (gather.go:61-203 -> mpsgraph_gather_along_axis, bridge.m:764-782). */
