@@ -130,9 +130,9 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 // running maximum; the groups are added in order.  Sequences without a visible token,
 // which no worker holds, get zeros.
 // Bound by the latency of lengths, then shares: 4.8 us for 8 x 32 heads, 6 us for 64 x 32.
-template <typename T, int DP, int KT, int WORKERS>
-__global__ __launch_bounds__(256) void join_kernel(Common p) {
-  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes, kAhead = 4;
+template <typename T, int DP, int KT, int WORKERS, int NT = 256>
+__global__ __launch_bounds__(NT) void join_kernel(Common p) {
+  constexpr int kLanes = DP / 4, kGroups = NT / kLanes, kAhead = 4;
   __shared__ float stat[2][kGroups];
   __shared__ __attribute__((aligned(16))) float sums[kGroups][DP];
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;

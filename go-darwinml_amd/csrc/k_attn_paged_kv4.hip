@@ -27,20 +27,32 @@ using paged::wait_vm;
 struct Rows {
   const char* codes;
   const char* scales;
-  int64_t sp, sh, st;     // byte strides of page, head, token of the codes
-  int64_t ssp, ssh, sst;  // and of the scales
+  uint32_t sp, st;    // byte strides of page and token of the codes
+  uint32_t ssp, sst;  // and of the scales
+  int64_t sh, ssh;    // of the heads
 };
 
 struct Params : Common {
   Rows k, v;
+  uint32_t page_mul;  // a token's page: page_of()
+  int page_shift;
 };
+
+// n / page_size of 0 <= n < 2^31, by the product with a 33-bit reciprocal: with shift =
+// ceil(log2 d) and mul = floor(2^32 (2^shift - d) / d) + 1 the quotient is exact (Granlund and
+// Montgomery).  A division costs 25 instructions, two of them a tile of 64 tokens 7% of it.
+__device__ __forceinline__ int page_of(const Params& p, int n) {
+  const uint32_t t = __umulhi(p.page_mul, static_cast<uint32_t>(n));
+  return static_cast<int>((t + ((static_cast<uint32_t>(n) - t) >> min(p.page_shift, 1))) >> max(p.page_shift - 1, 0));
+}
 
 constexpr int kTile = 64;  // tokens of a tile
 
 // Waves that share the tiles of all sequences: eight a CU, four with rows of 128 bytes.
 constexpr int workers(int DP) { return DP == 256 ? 1024 : 2048; }
 
-__device__ const uint4 kZero4[1] = {};
+// A row of zeros: what lanes without a token load.
+__device__ const uint4 kZero4[8] = {};
 
 template <typename T> struct Parts;
 // bf16 parts of the queries, and of the weights: their rounding stays below that of the output.
@@ -73,9 +85,27 @@ __device__ __forceinline__ f32x4 mma(const tile::bf16x8& a, const tile::bf16x8& 
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// Another lane's pointer.
+__device__ __forceinline__ const char* from_lane(const char* x, int lane) {
+  const uint64_t u = reinterpret_cast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * lane, static_cast<int>(u));
+  const uint32_t hi = __builtin_amdgcn_ds_bpermute(4 * lane, static_cast<int>(u >> 32));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The bytes of a row that hold N values, a lane's share of V.
+template <int N> struct Word;
+template <> struct Word<4> { using type = uint16_t; };
+template <> struct Word<8> { using type = uint32_t; };
+template <> struct Word<16> { using type = uint2; };
+
 template <int B>
-__device__ __forceinline__ uint32_t decode_byte(uint64_t w, float s) {
-  return kv4::decode2<(B & 3)>(static_cast<uint32_t>(w >> (32 * (B >> 2))), s);
+__device__ __forceinline__ uint32_t decode_byte(uint32_t w, float s) {
+  return kv4::decode2<B>(w, s);
+}
+template <int B>
+__device__ __forceinline__ uint32_t decode_byte(uint2 w, float s) {
+  return kv4::decode2<(B & 3)>(B < 4 ? w.x : w.y, s);
 }
 
 // A wave works alone on tiles of 64 tokens: codes and scales come by per-lane DMA into two
@@ -97,6 +127,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
   constexpr int kAll = 2 * kDma + 2 * kPlanes;          // DMA instructions of a tile
   constexpr int kWords = kRow / 16;                     // words of a quarter of a row
   constexpr int kVals = DP / 16;                        // values of V a lane holds of a token
+  constexpr int kQuarterGroups = DP == 256 ? 2 : 1;     // scales of a quarter of a row
   __shared__ __attribute__((aligned(1024))) char smem[2][kStage];
   __shared__ __attribute__((aligned(16))) int32_t page_lds[2][64];
 
@@ -104,17 +135,27 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
   const uint32_t la0 = tile::lds_addr(smem), pa0 = tile::lds_addr(page_lds);
   const float c = p.scale * 1.4426950408889634f;
-  // Groups past the head dim count as zeros, whatever their bytes hold.
   const int groups = p.D / kv4::kGroup;
+  // A scale's byte as an fp32 power of two; groups past the head dim have none, whatever lies there.
+  auto scale_of = [&](uint32_t byte, int group) {
+    return __uint_as_float(__umul24(byte, group < groups ? 1u << 23 : 0u));
+  };
   auto slot_of = [](int r) { return (r & ~15) | ((r & 3) << 2) | ((r >> 2) & 3); };  // (its own inverse)
-  auto swz = [](int s) { return s / (256 / kRow) % kCh; };
+  auto swz = [](int s) { return s / (256 / kRow) % kCh; };  // (the same for slots 16 apart)
+  const int kslot = slot_of(col);
 
   int b;
   int64_t at, end, begin;
   const Order<kTile, workers(DP)> order(p, SPLIT ? units : 0);
+  int worker = 0;
   if constexpr (SPLIT) {
+    // Workgroups go to the eight XCDs in turn; each XCD takes neighbouring workers, so that heads
+    // whose rows share cache lines meet in one L2.
     const int64_t per = order.share();
-    at = blockIdx.x * per;
+    const int used = static_cast<int>((order.total + per - 1) / per), each = (used + 7) >> 3;
+    worker = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3);
+    if (static_cast<int>(blockIdx.x >> 3) >= each) return;
+    at = worker * per;
     end = min(order.total, at + per);
     if (at >= end) return;
     b = order.find(p, at, &begin);
@@ -141,6 +182,62 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     const int hk = unit / blocks, h0 = hk * G + (unit % blocks) * kHeads;
     const int heads = min(kHeads, (hk + 1) * G - h0);
 
+    const int32_t* table = p.table + b * p.table_stride;
+    const char* kc = p.k.codes + hk * p.k.sh;
+    const char* vc = p.v.codes + hk * p.v.sh;
+    const char* ks = p.k.scales + hk * p.k.ssh;
+    const char* vs = p.v.scales + hk * p.v.ssh;
+    const char* zero = reinterpret_cast<const char*>(kZero4);
+
+    auto token0 = [&](int t) { return t < nst ? t * kTile : (seen.lo & ~15) + (t - nst) * kTile; };
+    auto issue_pages = [&](int t, int slot) {
+      const int entry = min(page_of(p, token0(t) + lane), p.max_pages - 1);
+      tile::load4(table + entry, pa0 + slot * 256);
+    };
+    // The DMA of tile t, its page numbers landed; returns its rows that hold a token.  A lane finds
+    // the addresses of its token's rows, those that load them fetch them from it.
+    auto issue = [&](int t, int slot) -> uint64_t {
+      const int tok = token0(t) + lane;
+      const int page = page_lds[slot][lane];
+      const uint32_t off = tok - page_of(p, tok) * p.page_size;
+      const bool ok = (t < nst ? tok < seen.ns : tok >= seen.lo && tok < seen.len) && page >= 0 && page < p.num_pages;
+      const uint32_t la = la0 + slot * kStage, pg = ok ? page : 0;
+      auto row = [&](const char* base, uint32_t sp, uint32_t st) {
+        const char* at = base + static_cast<uint64_t>(pg) * sp + static_cast<uint64_t>(off) * st;
+        return ok ? at : zero;
+      };
+      const char* krow = row(kc, p.k.sp, p.k.st);
+      const char* vrow = row(vc, p.v.sp, p.v.st);
+#pragma unroll
+      for (int i = 0; i < kDma; ++i) {
+        const int s = i * kPer + lane / kCh, r = slot_of(s);
+        // (Past the head dim: any bytes of the row; their scales count as 2^-127 and q as 0.)
+        const int ch = min((lane % kCh) ^ swz(s), groups - 1) * 16;
+        tile::load16(from_lane(krow, r) + ch, la + i * 1024);
+        tile::load16(from_lane(vrow, r) + ch, la + kCodes + i * 1024);
+      }
+      const char* kscale = row(ks, p.k.ssp, p.k.sst);
+      const char* vscale = row(vs, p.v.ssp, p.v.sst);
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) {
+        tile::load4(kscale + 4 * i, la + 2 * kCodes + i * 256);
+        tile::load4(vscale + 4 * i, la + 2 * kCodes + (kPlanes + i) * 256);
+      }
+      return __builtin_amdgcn_ballot_w64(ok);
+    };
+
+    f32x4 o[kVals];
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    // The order of the DMA is pages 0, 1, tile 0, pages 2, tile 1, pages 3, tile 2, ..
+    const int n = te - ta;
+    uint64_t rows0 = 0, rows1 = 0;  // of tiles j and j + 1
+    if (n > 0) {
+      issue_pages(ta, 0);
+      if (n > 1) issue_pages(ta + 1, 1);
+    }
     tile::bf16x8 qf[kVals / 2][kQ];  // [step][part]
     {
       const T* Q = static_cast<const T*>(p.q) + b * p.q_sb + (h0 + col) * p.q_sh;
@@ -157,55 +254,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
 #pragma unroll
       for (int s = 0; s < kVals / 2; ++s) tile::settle(qf[s]);
     }
-    const int32_t* table = p.table + b * p.table_stride;
-    const char* kc = p.k.codes + hk * p.k.sh;
-    const char* vc = p.v.codes + hk * p.v.sh;
-    const char* ks = p.k.scales + hk * p.k.ssh;
-    const char* vs = p.v.scales + hk * p.v.ssh;
-    const char* zero = reinterpret_cast<const char*>(kZero4);
-
-    auto token0 = [&](int t) { return t < nst ? t * kTile : (seen.lo & ~15) + (t - nst) * kTile; };
-    auto issue_pages = [&](int t, int slot) {
-      const int entry = min((token0(t) + lane) / p.page_size, p.max_pages - 1);
-      tile::load4(table + entry, pa0 + slot * 256);
-    };
-    // The DMA of tile t, its page numbers landed; returns its rows that hold a token.
-    auto issue = [&](int t, int slot) -> uint64_t {
-      const int tok = token0(t) + lane;
-      const int page = page_lds[slot][lane];
-      const int off = tok % p.page_size;
-      const bool ok = (t < nst ? tok < seen.ns : tok >= seen.lo && tok < seen.len) && page >= 0 && page < p.num_pages;
-      const uint64_t rows = __builtin_amdgcn_ballot_w64(ok);
-      const uint32_t la = la0 + slot * kStage;
-#pragma unroll
-      for (int i = 0; i < kDma; ++i) {
-        const int s = i * kPer + lane / kCh, r = slot_of(s);
-        const int ch = (lane % kCh) ^ swz(s);
-        const int64_t pg = __shfl(page, r, 64), of = __shfl(off, r, 64);
-        const bool there = ((rows >> r) & 1) && ch * 32 < p.D;
-        tile::load16(there ? kc + pg * p.k.sp + of * p.k.st + ch * 16 : zero, la + i * 1024);
-        tile::load16(there ? vc + pg * p.v.sp + of * p.v.st + ch * 16 : zero, la + kCodes + i * 1024);
-      }
-#pragma unroll
-      for (int i = 0; i < kPlanes; ++i) {
-        const bool there = ok && i * 128 < p.D;
-        tile::load4(there ? ks + page * p.k.ssp + off * p.k.sst + 4 * i : zero, la + 2 * kCodes + i * 256);
-        tile::load4(there ? vs + page * p.v.ssp + off * p.v.sst + 4 * i : zero, la + 2 * kCodes + (kPlanes + i) * 256);
-      }
-      return rows;
-    };
-
-    f32x4 o[kVals];
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
-    // The order of the DMA is pages(j + 1), tile(j) (the first two tiles' pages together).
-    const int n = te - ta;
-    uint64_t rows0 = 0, rows1 = 0;  // of tiles j and j + 1
     if (n > 0) {
-      issue_pages(ta, 0);
-      if (n > 1) issue_pages(ta + 1, 1);
       wait_vm<0>();
       rows0 = issue(ta, 0);
       if (n > 1) {
@@ -214,48 +263,74 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
       }
     }
     for (int j = 0; j < n; ++j) {
-      // Everything older than tile j + 1's own DMA has landed (and its successor's pages).
-      if (j + 2 < n) wait_vm<kAll + 1>();
-      else if (j + 1 < n) wait_vm<kAll>();
+      // Everything older than tile j + 1's own DMA has landed, its successor's pages among it.
+      if (j + 1 < n) wait_vm<kAll>();
       else wait_vm<0>();
+      // All of the tile into registers, so that its stage takes tile j + 2 while this one is computed.
       const char* sk = smem[j & 1];
       const char* sv = sk + kCodes;
       const uint8_t* ssk = reinterpret_cast<const uint8_t*>(sk + 2 * kCodes);
       const uint8_t* ssv = ssk + kPlanes * 256;
-      f32x4 x[4];
+      uint32_t kw[4][kWords];
+      float kscale[4][kQuarterGroups];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int r = 16 * i + col, s = slot_of(r);
-        uint32_t w[kWords];
+        const char* row = sk + i * 16 * kRow + kslot * kRow;  // token 16 i + col
         if constexpr (kWords == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(sk + s * kRow + (((g >> 1) ^ swz(s)) << 4) + (g & 1) * 8);
-          w[0] = v.x;
-          w[1] = v.y;
+          const uint2 v = *reinterpret_cast<const uint2*>(row + (((g >> 1) ^ swz(kslot)) << 4) + (g & 1) * 8);
+          kw[i][0] = v.x;
+          kw[i][1] = v.y;
         } else {
 #pragma unroll
           for (int u = 0; u < kWords / 4; ++u) {
-            const uint4 v = *reinterpret_cast<const uint4*>(sk + s * kRow + ((((kWords / 4) * g + u) ^ swz(s)) << 4));
-            w[4 * u] = v.x;
-            w[4 * u + 1] = v.y;
-            w[4 * u + 2] = v.z;
-            w[4 * u + 3] = v.w;
+            const uint4 v = *reinterpret_cast<const uint4*>(row + ((((kWords / 4) * g + u) ^ swz(kslot)) << 4));
+            kw[i][4 * u] = v.x;
+            kw[i][4 * u + 1] = v.y;
+            kw[i][4 * u + 2] = v.z;
+            kw[i][4 * u + 3] = v.w;
           }
         }
 #pragma unroll
-        for (int u = 0; u < kWords; ++u) {
-          const int group = (g * (DP / 4) + 8 * u) / kv4::kGroup;
-          const uint32_t byte = group < groups ? ssk[(group >> 2) * 256 + 4 * r + (group & 3)] : 0u;
-          const tile::bf16x8 kf = __builtin_bit_cast(tile::bf16x8, kv4::decode8(w[u], kv4::scale_f32(byte)));
+        for (int u = 0; u < kQuarterGroups; ++u) {
+          const int group = g * (DP / 4) / kv4::kGroup + u;
+          kscale[i][u] = scale_of(ssk[64 * i + 4 * col + (group >> 2) * 256 + (group & 3)], group);
+        }
+      }
+      typename Word<kVals>::type vw[2][8];
+      float vscale[2][8];
+      const int vgroup = col * kVals / kv4::kGroup;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // token 32 t + 16 (e / 4) + 4 g + e % 4, in slot .. + 4 (e % 4) + g
+          const int s = 4 * (e & 3) + g, byte = col * (kVals / 2);
+          vw[t][e] = *reinterpret_cast<const typename Word<kVals>::type*>(
+              sv + (32 * t + 16 * (e >> 2) + 4 * (e & 3)) * kRow + g * kRow + (((byte >> 4) ^ swz(s)) << 4) + (byte & 15));
+          vscale[t][e] = scale_of(ssv[4 * (32 * t + 16 * (e >> 2) + (e & 3)) + 16 * g + (vgroup >> 2) * 256 + (vgroup & 3)], vgroup);
+        }
+      const uint64_t rows = rows0;
+      rows0 = rows1;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + 2 < n) {
+        if (j + 3 < n) issue_pages(ta + j + 3, (j + 1) & 1);
+        rows1 = issue(ta + j + 2, j & 1);
+      }
+      f32x4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < kWords; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const tile::bf16x8 kf = __builtin_bit_cast(tile::bf16x8, kv4::decode8(kw[i][u], kscale[i][u * kQuarterGroups / kWords]));
 #pragma unroll
           for (int q = 0; q < kQ; ++q) x[i] = mma(kf, qf[u][q], x[i]);
         }
-      }
       // x[i][v]: token 16 i + 4 g + v, head col.
-      if (rows0 != ~0ull) {
+      if (rows != ~0ull) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t bits = static_cast<uint32_t>(rows0 >> (16 * i + 4 * g));
+          const uint32_t bits = static_cast<uint32_t>(rows >> (16 * i + 4 * g));
 #pragma unroll
           for (int v = 0; v < 4; ++v) x[i][v] = (bits >> v) & 1 ? x[i][v] : -INFINITY;
         }
@@ -263,9 +338,9 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])), mx);
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       if (__builtin_amdgcn_ballot_w64((mx - m) * c > 8.f)) {  // the maximum may trail by 2^8
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float mnew = fmaxf(m, mx);
         const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mnew) * c);
         m = mnew;
@@ -288,24 +363,11 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
         }
         tile::bf16x8 pf[kP];
         split8<kP>(w8, pf);
-        uint64_t words[8];
-        float scales[8];
-        const int group = col * kVals / kv4::kGroup;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int r = 32 * t + 4 * g + (e & 3) + 16 * (e >> 2), s = slot_of(r);
-          const int byte = col * (kVals / 2);
-          const char* a = sv + s * kRow + (((byte >> 4) ^ swz(s)) << 4) + (byte & 15);
-          if constexpr (kVals == 4) words[e] = *reinterpret_cast<const uint16_t*>(a);
-          else if constexpr (kVals == 8) words[e] = *reinterpret_cast<const uint32_t*>(a);
-          else words[e] = *reinterpret_cast<const uint64_t*>(a);
-          scales[e] = kv4::scale_f32(group < groups ? ssv[(group >> 2) * 256 + 4 * r + (group & 3)] : 0u);
-        }
         auto product = [&](auto B) {
           constexpr int kB = decltype(B)::value;
           uint32_t pair[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) pair[e] = decode_byte<kB>(words[e], scales[e]);
+          for (int e = 0; e < 8; ++e) pair[e] = decode_byte<kB>(vw[t][e], vscale[t][e]);
           uint32_t lo[4], hi[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -333,13 +395,6 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
           product(std::integral_constant<int, 7>{});
         }
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
-      rows0 = rows1;
-      if (j + 2 < n) {
-        wait_vm<kAll>();  // its page numbers
-        if (j + 3 < n) issue_pages(ta + j + 3, (j + 1) & 1);
-        rows1 = issue(ta + j + 2, j & 1);
-      }
     }
 
     // o[j][v] is d = kVals (4 g + v) + j of head col.
@@ -348,7 +403,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no token seen: zeros
     if (col < heads) {
       const bool whole = ta == 0 && te == nt;
-      const int64_t r = (2 * static_cast<int64_t>(blockIdx.x) + (at == first ? 0 : 1)) * p.unit_heads + col;
+      const int64_t r = (2 * static_cast<int64_t>(worker) + (at == first ? 0 : 1)) * p.unit_heads + col;
       T* out = static_cast<T*>(p.o) + b * p.o_sb + (h0 + col) * p.o_sh;
       float* part = SPLIT ? p.part_o + r * p.D : nullptr;
 #pragma unroll
@@ -379,8 +434,11 @@ static void launch_d(const Params& p, hipStream_t s) {
   const int G = p.H / p.Hkv, units = p.Hkv * ((G + kHeads - 1) / kHeads);
   if (p.part_o) {
     hipLaunchKernelGGL((attend4_kernel<T, DP, true>), dim3(workers(DP)), dim3(64), 0, s, p);
-    hipLaunchKernelGGL((paged::join_kernel<T, DP, kTile, workers(DP)>), dim3(static_cast<unsigned>(p.B * p.H)), dim3(256), 0, s,
-                       static_cast<const Common&>(p));
+    // (Few rows have many shares each: 256 of 32 heads' one long sequence, 8.8 us with 256 threads.)
+    const dim3 rows(static_cast<unsigned>(p.B * p.H));
+    const Common& c = p;
+    if (p.B * p.H <= 256) hipLaunchKernelGGL((paged::join_kernel<T, DP, kTile, workers(DP), 1024>), rows, dim3(1024), 0, s, c);
+    else hipLaunchKernelGGL((paged::join_kernel<T, DP, kTile, workers(DP)>), rows, dim3(256), 0, s, c);
   } else {
     hipLaunchKernelGGL((attend4_kernel<T, DP, false>), dim3(static_cast<unsigned>(p.B * units)), dim3(64), 0, s, p);
   }
@@ -456,18 +514,25 @@ extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_ca
   paged4::Params p{};
   paged4::Rows* to[2] = {&p.k, &p.v};
   const GHipKv4* from[2] = {k_cache, v_cache};
+  bool near = true;
   for (int j = 0; j < 2; ++j) {
     const GHipKv4& f = *from[j];
     ok = ok && al(f.codes, 16) && al(f.scales, 4);
     for (int i = 0; i < 3; ++i) ok = ok && whole(f.code_strides[i], cache[i], 16) && whole(f.scale_strides[i], cache[i], 4);
+    // (A cache of one page, or pages of one token: that stride is not used.)
+    const int64_t steps[4] = {num_pages > 1 ? f.code_strides[0] : 0, page_size > 1 ? f.code_strides[2] : 0,
+                              num_pages > 1 ? f.scale_strides[0] : 0, page_size > 1 ? f.scale_strides[2] : 0};
+    for (const int64_t t : steps) near = near && t <= 0xffffffffLL;
     *to[j] = paged4::Rows{static_cast<const char*>(f.codes), static_cast<const char*>(f.scales),
-                          f.code_strides[0], f.code_strides[1], f.code_strides[2],
-                          f.scale_strides[0], f.scale_strides[1], f.scale_strides[2]};
+                          static_cast<uint32_t>(steps[0]), static_cast<uint32_t>(steps[1]),
+                          static_cast<uint32_t>(steps[2]), static_cast<uint32_t>(steps[3]),
+                          f.code_strides[1], f.scale_strides[1]};
   }
   if (!ok)
     return set_error(err, GHIP_ERR_UNSUPPORTED,
                      "%s: codes must be 16-byte aligned with non-negative strides of whole 16 bytes, scales 4-byte aligned "
                      "with strides of whole 4", kWhat);
+  if (!near) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: pages and tokens at strides of 4 GiB and more", kWhat);
   p.q = q; p.o = o;
   p.table = block_table; p.lens = lens;
   p.q_sb = q_strides[0]; p.q_sh = q_strides[1]; p.o_sb = o_strides[0]; p.o_sh = o_strides[1];
@@ -478,6 +543,8 @@ extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_ca
   p.window = static_cast<int>(window == 0 || window > kMost ? kMost : window);
   p.sinks = static_cast<int>(sinks > kMost ? kMost : sinks);
   p.scale = scale;
+  while (int64_t{1} << p.page_shift < page_size) ++p.page_shift;
+  p.page_mul = static_cast<uint32_t>(((static_cast<uint64_t>((int64_t{1} << p.page_shift) - page_size)) << 32) / static_cast<uint64_t>(page_size) + 1);
   p.unit_heads = static_cast<int>(std::min<int64_t>(paged::kHeads, H / Hkv));
   const int64_t need = workspace ? ghip_sdpa_paged_kv4_workspace_bytes(B, H, Hkv, D, page_size, max_pages) : 0;
   if (need > 0) {
