@@ -455,15 +455,24 @@ static void launch(const Params& p, hipStream_t s) {
 
 using namespace ghip;
 
-// No workspace, so a wave for each unit: caches of at most 4 tiles a sequence, or 12 with
-// 512 units or more.
+// No workspace, so a wave for each unit: caches of at most 6 tiles a sequence, 12 with 512 units
+// or more, 24 with 1024.  (The second kernel costs 5-7 us; a wave alone takes 1.5 us a tile.)
+// bf16 D 128, 32 heads over 8, sequences of one length, us a call in a graph, split / unsplit:
+//   units      4 tiles      6           8           12          16          24          32
+//   8          12.8 / 9.4   12.9 / 12.4 12.8 / 15.4 12.9 / 21.2 12.9 / 27.0 13.0 / 38.6
+//   256        13.3 / 9.8   13.9 / 12.6 14.4 / 15.8 17.1 / 21.6 18.5 / 27.8 23.4 / 39.7
+//   512        16.1 / 10.1  18.5 / 13.0 20.0 / 16.8 24.8 / 22.9 27.9 / 29.0 34.1 / 41.3
+//   1024       24.9 / 12.1  29.2 / 16.0 32.6 / 19.1 37.7 / 25.2 42.7 / 31.0 52.8 / 43.1 63.1 / 55.9
+//   2048       40.5 / 19.6  46.6 / 24.8 51.3 / 29.6 61.4 / 39.9 72.1 / 50.5  105 / 84.2  129 / 108
+// (Beyond, sequences of one length would still run faster unsplit with 1024 units and more; the
+// rule does not know the lengths, and one long sequence would keep the others waiting.)
 extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page_size,
                                                        int64_t max_pages) {
   if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 256 || page_size <= 0 || max_pages <= 0) return 0;
   const int64_t heads = H / Hkv;
   const double units = static_cast<double>(B) * static_cast<double>(Hkv) * static_cast<double>((heads + paged::kHeads - 1) / paged::kHeads);
   const double tokens = static_cast<double>(page_size) * static_cast<double>(max_pages);
-  if (tokens <= paged4::kTile * (units >= 512 ? 12. : 4.)) return 0;
+  if (tokens <= paged4::kTile * (units >= 1024 ? 24. : units >= 512 ? 12. : 6.)) return 0;
   return 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4;
 }
 

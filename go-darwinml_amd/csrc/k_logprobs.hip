@@ -6,6 +6,7 @@
 // No reference op (GoMLX composes it of FusedSoftmax and primitives); beside the log-softmax
 // rows, which write V values a row.  Bound by the bytes of the logits, read once.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -19,6 +20,7 @@ namespace logprobs {
 constexpr int kMostTop = 32;
 constexpr int kMostSlices = 64;
 constexpr int kRun = 4;      // vectors a lane takes at a time
+constexpr int kSlots = 16;   // runs of a lane whose maxima are kept apart
 constexpr int kQueue = 256;  // candidates a wave holds
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 constexpr float kFar = -200.f;  // 2^kFar is 0: what stands for log 0 in a product with a weight of 0
@@ -58,30 +60,11 @@ struct Stats {
     s += o.s;
     e += o.e;
   }
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float most, float c) {
-    move(fmaxf(m, most * c));
-    const float base = m == -INFINITY ? 0.f : m;
-    float s2 = 0.f, e2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float u = __builtin_fmaf(x[i], c, -base), w = __builtin_amdgcn_exp2f(u);
-      s2 += w;
-      e2 = __builtin_fmaf(w, fmaxf(u, kFar), e2);  // (-inf: 0, not 0 times -inf; NaN stays in w)
-    }
-    s += s2;
-    e += e2;
-  }
 };
+// The lanes' sums beside their wave's one maximum.
 __device__ __forceinline__ Stats wave_join(Stats a) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    Stats b;
-    b.m = __shfl_xor(a.m, d, 64);
-    b.s = __shfl_xor(a.s, d, 64);
-    b.e = __shfl_xor(a.e, d, 64);
-    a.join(b);
-  }
+  a.s = wave_sum(a.s);
+  a.e = wave_sum(a.e);
   return a;
 }
 
@@ -99,18 +82,37 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
   return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~i);
 }
 
+// Sum of x over this lane and the lower ones: shifts within the rows of 16 lanes, then the rows'
+// totals broadcast to the rows after them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
+  return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = dpp_add<0x111, 0xf>(x);
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  x = dpp_add<0x143, 0xc>(x);
+  return x;
+}
 __device__ __forceinline__ int rank_in(uint64_t mask) {  // set bits below this lane's
   return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
-// The largest number of BITS leading bits (the others 0) that at least k lanes' values reach.
-template <typename U, int BITS>
-__device__ __forceinline__ U kth_bound(U v, int k) {
+// The largest number of BITS leading bits (the others 0) that at least k of the lanes' M values reach.
+template <typename U, int BITS, int M>
+__device__ __forceinline__ U kth_bound(const U (&v)[M], int k) {
   U cur = 0;
   constexpr int kWidth = 8 * static_cast<int>(sizeof(U));
+#pragma unroll
   for (int bit = kWidth - 1; bit >= kWidth - BITS; --bit) {
     const U next = cur | static_cast<U>(1) << bit;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= next)) >= k) cur = next;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= next));
+    if (n >= k) cur = next;
   }
   return cur;
 }
@@ -122,8 +124,11 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A wave's candidates for the largest keys: every key above `tau`, a bound that k keys of the
-// row reach.  The bound comes from the lanes' own maxima: k lanes hold k different logits.
+// The largest keys of rows where many logits are equal (constant rows, masks of the lowest value
+// or -infinity, fewer tokens than `top`): a wave's second pass over its part, in the order of
+// the indices.  Every key above `tau`, a bound that k keys of the row reach, is a candidate;
+// the bound comes from the lanes' own maxima (k lanes hold k different logits) and, when
+// candidates are many, from the k-th of them.
 struct Queue {
   uint64_t* q;  // [kQueue] in LDS
   int n = 0, k;
@@ -131,15 +136,13 @@ struct Queue {
   float tau_x = -INFINITY;  // logits below it are no candidates
   float best = -INFINITY;   // the lane's largest logit so far
   __device__ __forceinline__ Queue(uint64_t* lds, int k_) : q(lds), k(k_) {}
-  __device__ __forceinline__ void raise(uint64_t to) {
-    if (to > tau) {
-      tau = to;
-      tau_x = value_of(static_cast<uint32_t>(to >> 32));
-    }
-  }
-  __device__ __forceinline__ void bound(uint32_t order) {  // logits of this order and above are candidates
-    if (order) raise((static_cast<uint64_t>(order) << 32) - 1);
-    if (order) tau_x = fmaxf(tau_x, value_of(order));
+  // Logits of this order and above are candidates (0: all); whether that is news.
+  __device__ __forceinline__ bool bound(uint32_t order) {
+    const uint64_t to = (static_cast<uint64_t>(order) << 32) - 1;
+    if (order == 0 || to <= tau) return false;
+    tau = to;
+    tau_x = value_of(order);
+    return true;
   }
   // Keeps the k largest.
   __device__ __forceinline__ void compact() {
@@ -162,7 +165,10 @@ struct Queue {
       if (lane + 64 * i < n && above[i] < k) q[above[i]] = mine[i];
     n = min(n, k);
     wave_sync();
-    if (n == k) raise(q[k - 1]);
+    if (n == k && q[k - 1] > tau) {
+      tau = q[k - 1];
+      tau_x = value_of(static_cast<uint32_t>(tau >> 32));
+    }
   }
   __device__ __forceinline__ void push(uint64_t key) {  // 0: none
     const uint64_t mask = __builtin_amdgcn_ballot_w64(key > tau);
@@ -180,11 +186,15 @@ struct Queue {
 template <int NT, typename Out>
 __device__ __forceinline__ void select(const uint64_t* list, int n, int k, const Out& out) {
   const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  for (int i = t; i < n; i += NT) {
-    const uint64_t mine = list[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += list[j] > mine;
-    if (above < k) out(above, mine);
+  for (int i0 = 0; i0 < n; i0 += NT) {
+    const uint64_t mine = i0 + t < n ? list[i0 + t] : ~0ull;
+    int above = 0, j = 0;
+    for (; j + 8 <= n; j += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) above += list[j + u] > mine;
+    }
+    for (; j < n; ++j) above += list[j] > mine;
+    if (i0 + t < n && above < k) out(above, mine);
   }
 }
 
@@ -193,32 +203,39 @@ __device__ __forceinline__ float logit(const Params& p, int64_t row, uint32_t i)
   return Elem<T>::load1(reinterpret_cast<const T*>(p.x + row * p.stride) + i);
 }
 
+// The row's token and its logit; one thread, ahead of the row's pass.
+struct Given {
+  bool there = false;
+  float x = 0.f;
+  template <typename T>
+  __device__ __forceinline__ void load(const Params& p, int64_t row) {
+    const int id = p.ids[row];
+    there = id >= 0 && id < p.V;
+    if (there) x = logit<T>(p, row, id);
+  }
+};
+
 // What a row's statistics give; one thread.
-template <typename T>
-__device__ __forceinline__ void finish(const Params& p, int64_t row, const Stats& a) {
+__device__ __forceinline__ void finish(const Params& p, int64_t row, const Stats& a, const Given& id) {
   const float log_s = a.s == 0.f ? -INFINITY : __builtin_amdgcn_logf(a.s);
   const bool none = a.m == -INFINITY && a.s == a.s;
-  const int id = p.ids[row];
-  const bool there = id >= 0 && id < p.V;
   float lp = 0.f;
-  if (there) lp = none ? -INFINITY : kLn2 * (__builtin_fmaf(logit<T>(p, row, id), p.c, -a.m) - log_s);
+  if (id.there) lp = none ? -INFINITY : kLn2 * (__builtin_fmaf(id.x, p.c, -a.m) - log_s);
   p.logp[row] = lp;
   if (p.entropy) p.entropy[row] = none ? 0.f : kLn2 * (log_s - a.e / a.s);
   if (p.lse) p.lse[row] = none ? -INFINITY : kLn2 * (a.m + log_s);
 }
-template <typename T>
 __device__ __forceinline__ void finish_top(const Params& p, int64_t row, const Stats& a, int rank, uint64_t key) {
-  const uint32_t i = ~static_cast<uint32_t>(key);
-  p.top_ids[row * p.top + rank] = static_cast<int32_t>(i);
+  p.top_ids[row * p.top + rank] = static_cast<int32_t>(~static_cast<uint32_t>(key));
   const bool none = a.m == -INFINITY && a.s == a.s;
-  p.top_logps[row * p.top + rank] =
-      none ? -INFINITY : kLn2 * (__builtin_fmaf(logit<T>(p, row, i), p.c, -a.m) - __builtin_amdgcn_logf(a.s));
+  const float x = value_of(static_cast<uint32_t>(key >> 32));
+  p.top_logps[row * p.top + rank] = none ? -INFINITY : kLn2 * (__builtin_fmaf(x, p.c, -a.m) - __builtin_amdgcn_logf(a.s));
 }
 
 // Rows that hold a NaN or +infinity (their sum is NaN, which the bounds above do not see): the
 // largest keys one after the other, a pass over the row for each.  Every thread of NT calls it.
 template <typename T, int NT>
-__device__ __noinline__ void top_of_nan_row(const Params& p, int64_t row, const Stats& a, uint64_t* lds) {
+__device__ __forceinline__ void top_of_nan_row(const Params& p, int64_t row, const Stats& a, uint64_t* lds) {
   const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
   uint64_t last = ~0ull;
   for (int r = 0; r < p.top; ++r) {
@@ -239,150 +256,530 @@ __device__ __noinline__ void top_of_nan_row(const Params& p, int64_t row, const 
       for (int w = 0; w < NT / 64; ++w) best = lds[w] > best ? lds[w] : best;
     }
     last = best;
-    if (t == 0) finish_top<T>(p, row, a, r, best);
+    if (t == 0) finish_top(p, row, a, r, best);
   }
 }
 
-// A row, or a slice of one, by WAVES waves.  The lanes keep a running softmax each, joined at
-// the end; the waves collect candidates for the largest logits above a bound that they share.
-// Per logit: one conversion, half a maximum, a multiply-add, an exponential, two sums.
-template <typename T, int WAVES, bool TOP>
-__global__ __launch_bounds__(256) void stats_kernel(Params p) {
-  constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
-  __shared__ uint64_t queues[TOP ? 4 : 1][TOP ? kQueue : 1];
-  __shared__ uint64_t list[TOP ? 4 * kQueue : 4];
-  __shared__ float parts[3][4];
-  __shared__ uint32_t shared_tau;
-  __shared__ int listed;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = WAVES == 1 ? 0 : wave;
-  const int64_t unit = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
-  if (WAVES == 1 && unit >= p.N) return;
-  const int64_t row = WAVES == 1 ? unit : unit / p.slices;
-  const int slice = WAVES == 1 ? 0 : static_cast<int>(unit - row * p.slices);
-  const char* base = p.x + row * p.stride;
-  const T* X = reinterpret_cast<const T*>(base);
-  // The row's elements before and after its 16-byte vectors.
-  const int head = min(static_cast<int>((-reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T)), p.V);
-  const int nv = (p.V - head) / VEC, rest = p.V - nv * VEC;
-  const int v0 = slice * p.per, v1 = WAVES == 1 ? nv : min(nv, v0 + p.per);
-  const uint4* body = reinterpret_cast<const uint4*>(X + head);
+// The largest of three, without the two instructions that quiet a signalling NaN in each (rows
+// with a NaN are found by their sums).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
-  if constexpr (TOP && WAVES > 1) {
-    if (threadIdx.x == 0) shared_tau = 0, listed = 0;
-    __syncthreads();
-  }
-  Stats a;
-  Queue q(queues[TOP ? wave : 0], p.top);
-  uint4 next[kRun];
-  auto fetch = [&](int v) {
+// The order of a lane's largest logit, 0 if there is none above -infinity: the lanes' k-th bounds the
+// row's, since k lanes hold k different logits.
+__device__ __forceinline__ uint32_t order_of_best(float best) { return best == -INFINITY ? 0u : order_of(best); }
+__device__ __forceinline__ uint32_t bound_of(float best, int k) {
+  const uint32_t v[1] = {order_of_best(best)};
+  return kth_bound<uint32_t, 16>(v, k);
+}
+// The same of four waves' lanes, from the upper halves of their orders; in the order's upper half.
+__device__ __forceinline__ uint32_t bound_of(const uint16_t (&bests)[256], int lane, int k) {
+  const uint2 v = reinterpret_cast<const uint2*>(bests)[lane];
+  const uint32_t four[4] = {v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u};
+  return kth_bound<uint32_t, 16>(four, k);
+}
+
+// A wave's candidates by Queue: vectors [v0, v1) of the row, one a lane at a time.
+template <typename T>
+__device__ __forceinline__ void scan(Queue& q, const T* body, int head, int first, int step, int v0, int v1) {
+  constexpr int VEC = Elem<T>::kVec;
+  const int lane = threadIdx.x & 63;
+  for (int v = v0 + first; v < v1; v += step) {
+    const int at = v + lane;
+    float x[VEC], most = -INFINITY;
+    if (at < v1) load_vec(body + static_cast<int64_t>(at) * VEC, x);
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const int at = v + NT * j + 64 * part + lane;
-      if (at < v1) next[j] = body[at];
+    for (int i = 0; i < VEC; ++i) {
+      if (at >= v1) x[i] = -INFINITY;
+      most = fmaxf(most, x[i]);
+    }
+    q.best = fmaxf(q.best, most);
+    if (__builtin_amdgcn_ballot_w64(most >= q.tau_x && at < v1) == 0) continue;
+    q.bound(bound_of(q.best, q.k));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const bool in = at < v1 && x[i] >= q.tau_x;
+      if (__builtin_amdgcn_ballot_w64(in)) q.push(in ? key_of(x[i], head + at * VEC + i) : 0);
+    }
+  }
+}
+
+// Where a row, or a slice of one, lies.
+template <typename T>
+struct Part {
+  static constexpr int VEC = Elem<T>::kVec;
+  int64_t row;
+  int slice, head, rest, v0, v1;  // rest: elements before (head) and after the row's 16-byte vectors
+  const T* x;
+  const uint4* body;
+  __device__ __forceinline__ Part(const Params& p, int64_t unit) {
+    row = p.slices == 1 ? unit : unit / p.slices;
+    slice = static_cast<int>(unit - row * p.slices);
+    const char* base = p.x + row * p.stride;
+    x = reinterpret_cast<const T*>(base);
+    head = min(static_cast<int>((-reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T)), p.V);
+    const int nv = (p.V - head) / VEC;
+    rest = p.V - nv * VEC;
+    v0 = min(slice * p.per, nv);
+    v1 = min(nv, v0 + p.per);
+    body = reinterpret_cast<const uint4*>(x + head);
+    if (slice != 0) rest = 0;  // (the first slice's)
+  }
+  __device__ __forceinline__ int single(const Params& p, int lane) const { return lane < head ? lane : p.V - rest + lane; }
+};
+
+// Thread t's vector of those from `v` on: the address of the workgroup's in scalar registers, the
+// lane's in one.
+__device__ __forceinline__ uint4 vector_at(const uint4* body, int v, int t) {
+  return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(body + v) + 16u * static_cast<uint32_t>(t));
+}
+
+// A run of kRun vectors a lane, NT lanes: from vector v on, thread t's.
+template <int NT>
+__device__ __forceinline__ void fetch(uint4 (&next)[kRun], const uint4* body, int v, int t, int v1) {
+  if (v + NT * kRun <= v1) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) next[j] = vector_at(body, v + NT * j, t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      if (v + NT * j + t < v1) next[j] = vector_at(body, v + NT * j, t);
+  }
+}
+template <int N>
+__device__ __forceinline__ float most_of(const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i + 1 < N; i += 2) m = max3(m, x[i], x[i + 1]);
+  return N % 2 == 0 ? max3(m, x[N - 1], x[N - 1]) : m;
+}
+// Vector j of a run, widened; -infinity where there is none.
+template <typename T, int NT>
+struct Run {
+  static constexpr bool kFromMemory = false;
+  const uint4 (&raw)[kRun];
+  int v, t, v1;
+  __device__ __forceinline__ bool there(int j) const { return v + NT * j + t < v1; }
+  // FRESH: widened once more; left alone, the compiler keeps a whole run's values for a second use.
+  template <bool FRESH = false>
+  __device__ __forceinline__ void get(int j, float (&x)[Elem<T>::kVec]) const {
+    uint4 r = raw[j];
+    if constexpr (FRESH) asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
+    load_vec(reinterpret_cast<const T*>(&r), x);
+    if (v + NT * kRun > v1) {
+#pragma unroll
+      for (int i = 0; i < Elem<T>::kVec; ++i) x[i] = there(j) ? x[i] : -INFINITY;
+    }
+  }
+};
+// The same of a run that streams: as soon as a vector is widened, that of the next run loads into its
+// registers (past its end: the last one once more).  A second look reads memory again (it is
+// rare, and a run's copy costs 16 registers).  FULL: every lane has all of its vectors.
+template <typename T, int NT, bool FULL>
+struct Streamed {
+  static constexpr bool kFromMemory = true;
+  uint4 (&raw)[kRun];
+  const uint4* body;
+  int v, t, v1;
+  const uint4* then;  // the next run's
+  int nv, nv1;
+  template <bool AGAIN = false>
+  __device__ __forceinline__ void get(int j, float (&x)[Elem<T>::kVec]) const {
+    const bool there = FULL || v + NT * j + t < v1;
+    if constexpr (AGAIN) {
+      uint4 r{};
+      if (there) r = vector_at(body, 0, v + NT * j + t);
+      load_vec(reinterpret_cast<const T*>(&r), x);
+    } else {
+      // (Kept apart, or the compiler widens all vectors ahead of the branch between the two forms.)
+      if constexpr (FULL) asm volatile("; whole run" : "+v"(raw[j].x), "+v"(raw[j].y), "+v"(raw[j].z), "+v"(raw[j].w));
+      else asm volatile("; last run" : "+v"(raw[j].x), "+v"(raw[j].y), "+v"(raw[j].z), "+v"(raw[j].w));
+      load_vec(reinterpret_cast<const T*>(&raw[j]), x);
+      raw[j] = vector_at(then, 0, min(nv + NT * j + t, nv1 - 1));
+    }
+    if constexpr (!FULL) {
+#pragma unroll
+      for (int i = 0; i < Elem<T>::kVec; ++i) x[i] = there ? x[i] : -INFINITY;
+    }
+  }
+};
+struct Single {
+  static constexpr bool kFromMemory = false;
+  float value;
+  template <bool FRESH = false>
+  __device__ __forceinline__ void get(int j, float (&x)[1]) const { x[0] = j == 0 ? value : -INFINITY; }
+};
+
+// What stands before is computed before what follows.
+__device__ __forceinline__ void here(float (&x)[2], float (&y)[2]) {
+  asm volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(y[0]), "+v"(y[1]));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The first run's maximum, ahead of its sums, which would be taken twice without it.
+template <typename T, int NT>
+__device__ __forceinline__ void look(Stats& a, const uint4 (&raw)[kRun], int v, int t, int v1, float c) {
+  float most = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    float x[Elem<T>::kVec];
+    load_vec(reinterpret_cast<const T*>(&raw[j]), x);
+    const float m = most_of(x);
+    most = v + NT * j + t < v1 ? fmaxf(most, m) : most;
+  }
+  a.move(fmaxf(a.m, wave_max(most) * c));
+}
+
+// A run's sums into the lane's; a.m is the wave's maximum, and moves only where a run's weights say
+// that it has grown (kGrown).  Per logit: a conversion, a multiply-add, an exponential (four issue
+// slots), two sums.  Returns the lane's largest of the run, with MOST at half an instruction a
+// logit.
+template <int M, bool MOST, typename Values>
+__device__ __forceinline__ float add_run(Stats& a, const Values& values, float c) {
+  constexpr float kGrown = 256.f;
+  float most = -INFINITY, s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f}, shift = a.m == -INFINITY ? 0.f : -a.m;
+  auto weigh = [&](auto again, int j) {
+    float x[M];
+    values.template get<decltype(again)::value>(j, x);
+    if constexpr (MOST && !decltype(again)::value) {
+      if constexpr (M == 1) most = fmaxf(most, x[0]);
+      else most = max3(most, most_of(x), most);
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const float u = __builtin_fmaf(x[i], c, shift), w = __builtin_amdgcn_exp2f(u);
+      s[i & 1] += w;
+      e[i & 1] = __builtin_fmaf(w, decltype(again)::value ? fmaxf(u, kFar) : u, e[i & 1]);
     }
   };
-  fetch(v0);
-  if (slice == 0 && part == 0) {  // the single elements, one a lane
-    const int i = lane < head ? lane : p.V - rest + lane;
-    const bool there = lane < rest;
-    float x[1] = {there ? Elem<T>::load1(X + i) : -INFINITY};
-    a.add(x, x[0], p.c);
-    if constexpr (TOP) q.push(there ? key_of(x[0], i) : 0);
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    weigh(std::integral_constant<bool, false>{}, j);
+    here(s, e);  // (all vectors at once take 32 registers more)
   }
-  for (int v = v0; v < v1; v += NT * kRun) {
-    float x[kRun][VEC], most[kRun];
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const bool there = v + NT * j + 64 * part + lane < v1;
-      load_vec(reinterpret_cast<const T*>(&next[j]), x[j]);
-      most[j] = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        x[j][i] = there ? x[j][i] : -INFINITY;
-        most[j] = fmaxf(most[j], x[j][i]);
-      }
-    }
-    fetch(v + NT * kRun);
-    float all = most[0];
-#pragma unroll
-    for (int j = 1; j < kRun; ++j) all = fmaxf(all, most[j]);
-    a.add(*reinterpret_cast<const float(*)[kRun * VEC]>(&x), all, p.c);
-    if constexpr (TOP) {
-      q.best = fmaxf(q.best, all);
-      if constexpr (WAVES > 1) q.bound(*static_cast<volatile uint32_t*>(&shared_tau));
-      if (__builtin_amdgcn_ballot_w64(all >= q.tau_x)) {
-        const uint32_t order = kth_bound<uint32_t, 16>(q.best == -INFINITY ? 0u : order_of(q.best), p.top);
-        q.bound(order);
-        if constexpr (WAVES > 1)
-          if (lane == 0 && order) atomicMax(&shared_tau, order);
+  // A maximum that has grown, NaN, infinities: once more beside the run's own maximum, and with
+  // 0 for 0 times -infinity.
+  if (__builtin_amdgcn_ballot_w64(!(s[0] + s[1] < kGrown) || e[0] + e[1] != e[0] + e[1]) || a.m == -INFINITY) {
+    auto each = [&](auto f) {
+      if constexpr (Values::kFromMemory) {
+#pragma unroll 1
+        for (int j = 0; j < kRun; ++j) f(j);
+      } else {
 #pragma unroll
         for (int j = 0; j < kRun; ++j) {
-          const int at = v + NT * j + 64 * part + lane;
-          if (__builtin_amdgcn_ballot_w64(most[j] >= q.tau_x && at < v1) == 0) continue;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            q.push(at < v1 && x[j][i] >= q.tau_x ? key_of(x[j][i], head + at * VEC + i) : 0);
+          f(j);
+          here(s, e);
         }
       }
-    }
-  }
-  a = wave_join(a);
-  if constexpr (WAVES == 1) {
-    if (lane == 0) finish<T>(p, row, a);
-    if constexpr (TOP) {
-      if (a.s != a.s) {
-        top_of_nan_row<T, 64>(p, row, a, nullptr);
-      } else {
-        wave_sync();
-        select<64>(q.q, q.n, p.top, [&](int rank, uint64_t key) { finish_top<T>(p, row, a, rank, key); });
-      }
-    }
-  } else {
-    if (lane == 0) parts[0][wave] = a.m, parts[1][wave] = a.s, parts[2][wave] = a.e;
-    __syncthreads();
-    a = Stats();
+    };
+    if constexpr (!MOST) {
+      each([&](int j) {
+        float x[M];
+        values.template get<true>(j, x);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      Stats o;
-      o.m = parts[0][w];
-      o.s = parts[1][w];
-      o.e = parts[2][w];
-      a.join(o);
+        for (int i = 0; i < M; ++i) most = fmaxf(most, x[i]);
+      });
     }
-    const bool whole = p.slices == 1;
-    if (threadIdx.x == 0) {
-      if (whole) finish<T>(p, row, a);
-      else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+    a.move(fmaxf(a.m, wave_max(most) * c));
+    shift = a.m == -INFINITY ? 0.f : -a.m;
+    s[0] = s[1] = e[0] = e[1] = 0.f;
+    each([&](int j) { weigh(std::integral_constant<bool, true>{}, j); });
+  }
+  const float ss = s[0] + s[1], es = e[0] + e[1];
+  a.s += ss;
+  a.e += es;
+  return most;
+}
+// Joins the four waves' statistics.
+__device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
+  Stats a;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    Stats o;
+    o.m = parts[0][w];
+    o.s = parts[1][w];
+    o.e = parts[2][w];
+    a.join(o);
+  }
+  return a;
+}
+// Rows (WAVES = 1: a wave a row) and slices (4) of one run a lane: the logits stay in registers, so
+// candidates are taken from there.  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
+// in 16 slices each 9 us, and 5 for their join.
+template <typename T, int WAVES, bool TOP>
+__global__ __launch_bounds__(256) void run_kernel(Params p) {
+  constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
+  constexpr int kKeys = WAVES * kQueue;
+  __shared__ uint64_t lists[TOP ? 4 * kQueue : 1];
+  __shared__ uint64_t queues[TOP ? 4 * kQueue : 1];
+  __shared__ __attribute__((aligned(16))) uint16_t bests[256];
+  __shared__ float parts[3][4];
+  __shared__ int counts[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, own = WAVES == 1 ? wave : 0;
+  const int t = WAVES == 1 ? lane : threadIdx.x;  // among the part's threads
+  const int64_t unit = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + wave : blockIdx.x;
+  if (WAVES == 1 && unit >= p.N) return;
+  auto sync = [] {
+    if constexpr (WAVES == 1) wave_sync();
+    else __syncthreads();
+  };
+  const Part<T> at(p, unit);
+  const bool whole = p.slices == 1;
+  uint4 raw[kRun];
+  fetch<NT>(raw, at.body, at.v0, t, at.v1);
+  Given given;
+  if (t == 0 && whole) given.load<T>(p, at.row);
+  Stats a;
+  float single = -INFINITY, best;
+  const bool alone = t < at.rest;
+  if (at.rest > 0 && (WAVES == 1 || wave == 0)) {
+    if (alone) single = Elem<T>::load1(at.x + at.single(p, t));
+    add_run<1, true>(a, Single{single}, p.c);
+  }
+  const Run<T, NT> values{raw, at.v0, t, at.v1};
+  look<T, NT>(a, raw, at.v0, t, at.v1, p.c);
+  best = fmaxf(add_run<VEC, TOP>(a, values, p.c), single);
+  a = wave_join(a);
+  uint32_t tau = 0;  // logits of this order and above are candidates (0: all)
+  if constexpr (WAVES > 1) {
+    if (lane == 0) parts[0][wave] = a.m, parts[1][wave] = a.s, parts[2][wave] = a.e;
+    if (threadIdx.x == 0) counts[0] = 0;
+    if constexpr (TOP) bests[t] = static_cast<uint16_t>(order_of_best(best) >> 16);
+    __syncthreads();
+    a = waves_join(parts);
+    if constexpr (TOP) tau = bound_of(bests, lane, p.top);
+  } else if constexpr (TOP) {
+    tau = bound_of(best, p.top);
+  }
+  if (t == 0) {
+    if (whole) finish(p, at.row, a, given);
+    else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+  }
+  if constexpr (TOP) {
+    uint64_t* list = lists + own * kQueue;
+    if (whole && a.s != a.s) {
+      top_of_nan_row<T, NT>(p, at.row, a, lists);
+      return;
     }
-    if constexpr (TOP) {
-      if (whole && a.s != a.s) {
-        top_of_nan_row<T, NT>(p, row, a, list);
-        return;
-      }
-      // The waves' candidates that all their bounds leave.
-      const uint64_t tau = shared_tau ? (static_cast<uint64_t>(shared_tau) << 32) - 1 : 0;
-      for (int i = lane; i < q.n; i += 64)
-        if (q.q[i] > tau) list[atomicAdd(&listed, 1)] = q.q[i];
-      __syncthreads();
-      const int n = listed;
-      if (whole) {
-        select<NT>(list, n, p.top, [&](int rank, uint64_t key) { finish_top<T>(p, row, a, rank, key); });
-      } else {
-        uint64_t* out = p.keys + unit * p.top;
-        select<NT>(list, n, p.top, [&](int rank, uint64_t key) { out[rank] = key; });
-        for (int i = n + threadIdx.x; i < p.top; i += NT) out[i] = 0;
-      }
+    const float tau_x = tau ? value_of(tau) : -INFINITY;
+    // A lane marks its candidates (a bit each, the single element last), then writes them behind those
+    // of the lanes before it, each looked up once more by its index.
+    constexpr int kBits = kRun * VEC;
+    uint64_t marks = static_cast<uint64_t>(alone && single >= tau_x) << kBits;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const bool there = values.there(j);
+      float x[VEC];
+      values.template get<true>(j, x);
+      if (__builtin_amdgcn_ballot_w64(there && most_of(x) >= tau_x) == 0) continue;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) bits |= x[i] >= tau_x ? 1u << i : 0u;
+      marks |= static_cast<uint64_t>(there ? bits : 0u) << (VEC * j);
+    }
+    const int mine = __builtin_popcountll(marks), upto = static_cast<int>(wave_scan(static_cast<uint32_t>(mine)));
+    int n = __builtin_amdgcn_readlane(upto, 63), to = upto - mine;
+    if constexpr (WAVES > 1) {
+      int first = 0;
+      if (lane == 0) first = atomicAdd(&counts[0], n);
+      to += __builtin_amdgcn_readfirstlane(first);
+    }
+    while (marks) {
+      const int i = __builtin_ctzll(marks);
+      marks &= marks - 1;
+      const int at_i = i == kBits ? at.single(p, t) : at.head + (at.v0 + NT * (i / VEC) + t) * VEC + i % VEC;
+      if (to < kKeys) list[to] = key_of(Elem<T>::load1(at.x + at_i), at_i);
+      ++to;
+    }
+    sync();
+    if constexpr (WAVES > 1) n = counts[0];
+    if (n > kKeys) {
+      Queue q(queues + wave * kQueue, p.top);
+      q.bound(tau);
+      q.best = single;
+      if (WAVES == 1 || wave == 0) q.push(alone && single >= q.tau_x ? key_of(single, at.single(p, t)) : 0);
+      scan<T>(q, at.x + at.head, at.head, WAVES == 1 ? 0 : 64 * wave, NT, at.v0, at.v1);
+      sync();
+      if (t == 0) counts[own] = 0;
+      sync();
+      for (int i = lane; i < q.n; i += 64) list[atomicAdd(&counts[own], 1)] = q.q[i];
+      sync();
+      n = counts[own];
+    }
+    if (whole) {
+      select<NT>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, a, rank, key); });
+    } else {
+      uint64_t* out = p.keys + unit * p.top;
+      select<NT>(list, n, p.top, [&](int rank, uint64_t key) { out[rank] = key; });
+      for (int i = n + t; i < p.top; i += NT) out[i] = 0;
     }
   }
 }
 
-// Joins a row's slices; a wave a row.
+// Longer rows and slices: workgroups that stay, four waves that stream one part after the other and,
+// with a top, a fifth that picks each part's largest logits while the next one streams.  A lane
+// keeps the largest of each of its runs (half an instruction a logit), as the upper half of its
+// order; the k-th largest of a wave's lanes bounds the k-th of the part, and the runs that reach
+// the bound, few more than `top`, are read again.
+// Bound by the bytes: 4096 rows of 131072 bf16 logits 191 us without a top (5.6 TB/s).
+template <typename T, bool TOP>
+__global__ __launch_bounds__(TOP ? 320 : 256) void stream_kernel(Params p, int64_t parts_n) {
+  constexpr int VEC = Elem<T>::kVec, NT = 256, kStep = NT * kRun;
+  constexpr int kKeys = 512, kPicks = 512;
+  __shared__ __attribute__((aligned(16))) uint16_t slots[TOP ? 2 : 1][TOP ? kSlots : 1][NT];
+  __shared__ uint64_t list[TOP ? kKeys : 1];
+  __shared__ uint64_t queue[TOP ? kQueue : 1];
+  __shared__ uint16_t picks[TOP ? kPicks : 1];
+  __shared__ __attribute__((aligned(16))) uint16_t bests[2][256];
+  __shared__ float parts[2][3][4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = threadIdx.x;
+  int parity = 0;
+  if (!TOP || wave < 4) {
+    int64_t unit = blockIdx.x;
+    if (unit >= parts_n) return;
+    uint4 raw[kRun];
+    {
+      const Part<T> at(p, unit);
+      fetch<NT>(raw, at.body, at.v0, t, at.v1);
+    }
+    for (; unit < parts_n; unit += gridDim.x, parity ^= 1) {
+      const Part<T> at(p, unit);
+      const bool more = unit + gridDim.x < parts_n;
+      const Part<T> after(p, more ? unit + gridDim.x : unit);
+      Stats a;
+      float best = -INFINITY;
+      if (at.rest > 0 && wave == 0) {
+        best = lane < at.rest ? Elem<T>::load1(at.x + at.single(p, lane)) : -INFINITY;
+        add_run<1, true>(a, Single{best}, p.c);
+      }
+      int run = 0;
+      if (at.v0 < at.v1) look<T, NT>(a, raw, at.v0, t, at.v1, p.c);
+      for (int v = at.v0; v < at.v1; v += kStep, ++run) {
+        // (The next part's first run loads while this part ends; without one, a single vector.)
+        const bool last = v + kStep >= at.v1;
+        const uint4* then = last ? after.body : at.body;
+        const int nv = last ? after.v0 : v + kStep, nv1 = !last ? at.v1 : more ? after.v1 : after.v0 + 1;
+        const float most = v + kStep <= at.v1
+                               ? add_run<VEC, TOP>(a, Streamed<T, NT, true>{raw, at.body, v, t, at.v1, then, nv, nv1}, p.c)
+                               : add_run<VEC, TOP>(a, Streamed<T, NT, false>{raw, at.body, v, t, at.v1, then, nv, nv1}, p.c);
+        if constexpr (TOP) {
+          best = fmaxf(best, most);
+          const uint32_t held = v + t < at.v1 ? order_of(most) >> 16 : 0u;  // 0: no vector
+          uint16_t* slot = &slots[parity][run % kSlots][t];
+          *slot = static_cast<uint16_t>(run < kSlots ? held : max(held, static_cast<uint32_t>(*slot)));
+        }
+      }
+      a = wave_join(a);
+      if (lane == 0) parts[parity][0][wave] = a.m, parts[parity][1][wave] = a.s, parts[parity][2][wave] = a.e;
+      if constexpr (TOP) bests[parity][t] = static_cast<uint16_t>(order_of_best(best) >> 16);
+      __syncthreads();
+      if (!TOP && t == 0) {
+        a = waves_join(parts[parity]);
+        Given given;
+        if (p.slices == 1) given.load<T>(p, at.row), finish(p, at.row, a, given);
+        else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+      }
+    }
+  } else if constexpr (TOP) {
+    for (int64_t unit = blockIdx.x; unit < parts_n; unit += gridDim.x, parity ^= 1) {
+      const Part<T> at(p, unit);
+      const bool whole = p.slices == 1;
+      Given given;
+      if (whole && lane == 0) given.load<T>(p, at.row);
+      const bool alone = lane < at.rest;
+      const float single = alone ? Elem<T>::load1(at.x + at.single(p, lane)) : -INFINITY;
+      __syncthreads();  // the part has been streamed
+      const Stats a = waves_join(parts[parity]);
+      if (lane == 0) {
+        if (whole) finish(p, at.row, a, given);
+        else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+      }
+      if (whole && a.s != a.s) {
+        top_of_nan_row<T, 64>(p, at.row, a, nullptr);
+        continue;
+      }
+      const uint32_t tau = bound_of(bests[parity], lane, p.top);
+      const float tau_x = tau ? value_of(tau) : -INFINITY;
+      int n = 0, runs = 0;
+      auto add = [&](bool in, float value, int i) {
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+        if (mask == 0) return;
+        const int to = n + rank_in(mask);
+        if (in && to < kKeys) list[to] = key_of(value, i);
+        n += __builtin_popcountll(mask);
+      };
+      add(alone && single >= tau_x, single, at.single(p, lane));
+      const int held = min(kSlots, (at.v1 - at.v0 + kStep - 1) / kStep);
+      const uint32_t least = max(tau >> 16, 1u);
+      for (int k = 0; k < held; ++k) {
+        const uint2 four = reinterpret_cast<const uint2*>(slots[parity][k])[lane];
+        const uint32_t order[4] = {four.x & 0xffff, four.x >> 16, four.y & 0xffff, four.y >> 16};
+        if (__builtin_amdgcn_ballot_w64(max(max(order[0], order[1]), max(order[2], order[3])) >= least) == 0) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t mask = __builtin_amdgcn_ballot_w64(order[j] >= least);
+          const int to = runs + rank_in(mask);
+          if (order[j] >= least && to < kPicks) picks[to] = static_cast<uint16_t>(k * NT + 4 * lane + j);
+          runs += __builtin_popcountll(mask);
+        }
+      }
+      wave_sync();
+      for (int i0 = 0; i0 < runs && runs <= kPicks; i0 += 64) {
+        const bool mine = i0 + lane < runs;
+        const int pick = mine ? picks[i0 + lane] : 0;
+        for (int v0 = at.v0; v0 < at.v1; v0 += kSlots * kStep) {  // (runs of one slot)
+          const int v = v0 + pick / NT * kStep + pick % NT;
+          uint4 raw[kRun];
+#pragma unroll
+          for (int j = 0; j < kRun; ++j)
+            if (mine && v + NT * j < at.v1) raw[j] = at.body[v + NT * j];
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) {
+            float x[VEC];
+            load_vec(reinterpret_cast<const T*>(&raw[j]), x);
+            const bool there = mine && v + NT * j < at.v1;
+            if (__builtin_amdgcn_ballot_w64(there && most_of(x) >= tau_x) == 0) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) add(there && x[i] >= tau_x, x[i], at.head + (v + NT * j) * VEC + i);
+          }
+        }
+      }
+      if (runs > kPicks || n > kKeys) {
+        Queue q(queue, p.top);
+        q.bound(tau);
+        q.best = single;
+        q.push(alone && single >= q.tau_x ? key_of(single, at.single(p, lane)) : 0);
+        scan<T>(q, at.x + at.head, at.head, 0, 64, at.v0, at.v1);
+        wave_sync();
+        for (int i = lane; i < q.n; i += 64) list[i] = q.q[i];
+        n = q.n;
+      }
+      wave_sync();
+      if (whole) {
+        select<64>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, a, rank, key); });
+      } else {
+        uint64_t* out = p.keys + unit * p.top;
+        select<64>(list, n, p.top, [&](int rank, uint64_t key) { out[rank] = key; });
+        for (int i = n + lane; i < p.top; i += 64) out[i] = 0;
+      }
+      wave_sync();
+    }
+  }
+}
+
+// Joins a row's slices; a wave a row.  Bound by the chain of its loads: 5 us for 16 rows.
 template <typename T>
 __global__ __launch_bounds__(64) void join_kernel(Params p) {
+  constexpr int kHeld = 8;  // keys of a lane in registers
   __shared__ uint64_t list[kMostSlices * kMostTop];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
   Stats a;
+  Given given;
+  if (lane == 0) given.load<T>(p, row);
   if (lane < p.slices) {
     const float4 s = p.stats[row * p.slices + lane];
     a.m = s.x;
@@ -391,26 +788,34 @@ __global__ __launch_bounds__(64) void join_kernel(Params p) {
   }
   const int n = p.slices * p.top;
   const uint64_t* keys = p.keys + row * n;
-  uint64_t best = 0;
-  for (int i = lane; i < n; i += 64) best = keys[i] > best ? keys[i] : best;
+  uint64_t best = 0, held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
+  a.move(wave_max(a.m));
   a = wave_join(a);
-  if (lane == 0) finish<T>(p, row, a);
+  if (lane == 0) finish(p, row, a, given);
   if (p.top == 0) return;
   if (a.s != a.s) {
     top_of_nan_row<T, 64>(p, row, a, nullptr);
     return;
   }
-  const uint64_t bound = kth_bound<uint64_t, 64>(best, p.top);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) best = held[i] > best ? held[i] : best;
+  for (int i = lane + 64 * kHeld; i < n; i += 64) best = keys[i] > best ? keys[i] : best;
+  const uint32_t high[1] = {static_cast<uint32_t>(best >> 32)};
+  const uint64_t bound = static_cast<uint64_t>(kth_bound<uint32_t, 32>(high, p.top)) << 32;
   int count = 0;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const uint64_t key = i0 + lane < n ? keys[i0 + lane] : 0;
+  auto take = [&](uint64_t key) {
     const bool in = key != 0 && key >= bound;
     const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
     if (in) list[count + rank_in(mask)] = key;
     count += __builtin_popcountll(mask);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) take(held[i]);
+  for (int i0 = 64 * kHeld; i0 < n; i0 += 64) take(i0 + lane < n ? keys[i0 + lane] : 0);
   wave_sync();
-  select<64>(list, count, p.top, [&](int rank, uint64_t key) { finish_top<T>(p, row, a, rank, key); });
+  select<64>(list, count, p.top, [&](int rank, uint64_t key) { finish_top(p, row, a, rank, key); });
 }
 
 // ---------------------------------------------------------------- gradient
@@ -490,12 +895,17 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   }
 }
 
-// Waves of a row: one where that wave takes it in one run or two, four beyond.
-static bool short_rows(int64_t V, int64_t es) { return V * es <= 2 * 64 * 16 * kRun; }
+constexpr int kCus = 256, kStay = 4;  // of an MI355X; workgroups of stream_kernel on each
+
+// Logits of a run of `waves` waves.
+constexpr int64_t run_of(int64_t es, int waves) { return waves * 64 * kRun * 16 / es; }
+
+// A wave takes a row alone where one run (the gradient: two) holds it.
+static bool short_rows(int64_t V, int64_t es, int runs = 1) { return V <= runs * run_of(es, 1); }
 
 // Workgroups that share a row: so many that about 1024 run, each with a full run at least.
 static int64_t slices_of(int64_t N, int64_t V, int64_t es) {
-  const int64_t run = 256 * 16 / es * kRun;
+  const int64_t run = run_of(es, 4);
   return std::max<int64_t>(1, std::min<int64_t>({(V + run - 1) / run, 1024 / std::max<int64_t>(N, 1), kMostSlices}));
 }
 
@@ -503,13 +913,22 @@ template <typename T>
 static void launch(const Params& p, hipStream_t s) {
   if (short_rows(p.V, sizeof(T))) {
     const dim3 grid(static_cast<unsigned>((p.N + 3) / 4));
-    if (p.top) hipLaunchKernelGGL((stats_kernel<T, 1, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((stats_kernel<T, 1, false>), grid, dim3(256), 0, s, p);
+    if (p.top) hipLaunchKernelGGL((run_kernel<T, 1, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((run_kernel<T, 1, false>), grid, dim3(256), 0, s, p);
     return;
   }
-  const dim3 grid(static_cast<unsigned>(p.N * p.slices));
-  if (p.top) hipLaunchKernelGGL((stats_kernel<T, 4, true>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((stats_kernel<T, 4, false>), grid, dim3(256), 0, s, p);
+  const int64_t parts = p.N * p.slices;
+  if (p.per <= 256 * kRun) {
+    const dim3 grid(static_cast<unsigned>(parts));
+    if (p.top) hipLaunchKernelGGL((run_kernel<T, 4, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((run_kernel<T, 4, false>), grid, dim3(256), 0, s, p);
+  } else {
+    // Workgroups that stay, as many as run at once, with as many parts each as can be alike.
+    const int64_t most = kCus * kStay, turns = (parts + most - 1) / most;
+    const dim3 grid(static_cast<unsigned>(p.top ? (parts + turns - 1) / turns : parts));
+    if (p.top) hipLaunchKernelGGL((stream_kernel<T, true>), grid, dim3(320), 0, s, p, parts);
+    else hipLaunchKernelGGL((stream_kernel<T, false>), grid, dim3(256), 0, s, p, parts);
+  }
   if (p.slices > 1) hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>(p.N)), dim3(64), 0, s, p);
 }
 
@@ -517,7 +936,7 @@ template <typename T>
 static int launch_grad(Grad& p, hipStream_t s, GHipError* err, const char* what) {
   const bool wide = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.d)) % 16 == 0 &&
                     (p.N <= 1 || (p.x_stride - p.d_stride) % 16 == 0);
-  const bool one = short_rows(p.V, sizeof(T));
+  const bool one = short_rows(p.V, sizeof(T), 2);
   const int64_t run = 256 * (wide ? static_cast<int64_t>(Elem<T>::kVec) * kRun : 8);
   p.runs = one ? 1 : static_cast<int>((p.V + run - 1) / run);
   const int64_t blocks = one ? (p.N + 3) / 4 : p.N * p.runs;
