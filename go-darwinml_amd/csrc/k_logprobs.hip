@@ -626,7 +626,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
 // the bound, few more than `top`, are read again.
 // Bound by the bytes: 4096 rows of 131072 bf16 logits 191 us without a top (5.6 TB/s).
 template <typename T, bool TOP>
-__global__ __launch_bounds__(TOP ? 320 : 256) void stream_kernel(Params p, int64_t parts_n) {
+__global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Params p, int64_t parts_n) {
   constexpr int VEC = Elem<T>::kVec, NT = 256, kStep = NT * kRun;
   constexpr int kKeys = 512, kPicks = 512;
   __shared__ __attribute__((aligned(16))) uint16_t slots[TOP ? 2 : 1][TOP ? kSlots : 1][NT];
@@ -895,7 +895,7 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   }
 }
 
-constexpr int kCus = 256, kStay = 4;  // of an MI355X; workgroups of stream_kernel on each
+constexpr int kCus = 256, kStay = 5;  // of an MI355X; workgroups of stream_kernel on each
 
 // Logits of a run of `waves` waves.
 constexpr int64_t run_of(int64_t es, int waves) { return waves * 64 * kRun * 16 / es; }

@@ -36,6 +36,7 @@ struct Params {
   int64_t tokens;  // B S
   int S, H, Hkv, D, R, num_pages, page_size, max_pages;
   int block_tokens, splits, splits4;  // tokens of a workgroup; workgroups that share their rows
+  int both;                           // 4 bits: the one workgroup of a token takes its rows of both kinds
   int units, units4;                  // threads of a row
 };
 
@@ -188,9 +189,34 @@ __device__ __forceinline__ void row_unit4(const Params& p, const T* src, char* c
   if ((u & 3) == 0) scales[u >> 2] = static_cast<char>(scale);
 }
 
+// A slot of a workgroup (the threads of a row) and the rows that it takes: (token, head) of `n`
+// tokens and `nh` heads, one slot after the other.
+struct Slots {
+  int u, t, h, dt, dh, nh;
+  bool any;
+  __device__ __forceinline__ Slots(int units, int nh_) : nh(nh_) {
+    const int slots = kThreads / units, slot = threadIdx.x / units;
+    u = threadIdx.x - slot * units;
+    any = slot < slots && nh > 0;
+    if (!any) return;
+    dt = slots / nh;
+    dh = slots - dt * nh;
+    t = slot / nh;
+    h = slot - t * nh;
+  }
+  __device__ __forceinline__ void next() {
+    t += dt;
+    h += dh;
+    if (h >= nh) {
+      h -= nh;
+      ++t;
+    }
+  }
+};
+
 // A workgroup takes some tokens and all their rows, or, where the tokens are few, a share of
 // one token's rows: the angles are computed once for all of its heads.  FOUR: the rows of
-// keys and values go into 4 bits, in workgroups of their own.
+// keys and values go into 4 bits, by threads of their own share of a row.
 // Bound by the bytes of the rows, then, for a few tokens, by the chain position - angle - row.
 template <typename T, int N, bool FOUR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
@@ -200,63 +226,43 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
   const int split = blockIdx.x - static_cast<int>(block) * splits;
   const int64_t first = block * p.block_tokens;
   const int n = static_cast<int>(min(static_cast<int64_t>(p.block_tokens), p.tokens - first));
-  const bool four = FOUR && split >= p.splits;
   prepare(p, sh, first, n, p.R > 0);
-  // The rows of this workgroup: heads [h0, h1) of each token, a row in each slot.
-  const int units = four ? p.units4 : p.units, slots = kThreads / units;
-  const int slot = threadIdx.x / units, u = threadIdx.x - slot * units;
-  const int heads = four ? 2 * p.Hkv : FOUR ? p.H : p.H + 2 * p.Hkv;
-  const int part = four ? split - p.splits : split, parts = four ? p.splits4 : p.splits;
-  const int per = (heads + parts - 1) / parts, h0 = part * per, nh = min(per, heads - h0);
-  if (nh <= 0 || slot >= slots) return;
-  const int dt = slots / nh, dh = slots - dt * nh;  // the next row of a slot
-  int t = slot / nh, h = slot - t * nh;
-  while (t < n) {
-    const int b = sh.b[t], s = sh.s[t], page = sh.page[t];
-    const int64_t at = sh.at[t];
-    const float2* cs = sh.cs[t];
-    const int head = h0 + h;
-    if constexpr (FOUR) {
-      if (four) {
-        const bool key = head < p.Hkv;
-        const int hk = key ? head : head - p.Hkv;
+  if (split < p.splits) {
+    const int heads = FOUR ? p.H : p.H + 2 * p.Hkv, per = (heads + p.splits - 1) / p.splits, h0 = split * per;
+    Slots at(p.units, min(per, heads - h0));
+    for (; at.any && at.t < n; at.next()) {
+      const int b = sh.b[at.t], s = sh.s[at.t], head = h0 + at.h;
+      if (FOUR || head < p.H) {
+        row_unit<T, N>(p, reinterpret_cast<const T*>(p.q.p + b * p.q.sb + head * p.q.sh + s * p.q.ss),
+                       reinterpret_cast<T*>(p.qo.p + b * p.qo.sb + head * p.qo.sh + s * p.qo.ss), sh.cs[at.t], at.u, p.R > 0);
+      } else if (const int page = sh.page[at.t]; page >= 0) {
+        const bool key = head < p.H + p.Hkv;
+        const int hk = head - p.H - (key ? 0 : p.Hkv);
         const Rows& r = key ? p.k : p.v;
         const Cache& c = key ? p.kc : p.vc;
-        const Cache& w = key ? p.ks : p.vs;
-        if (page >= 0)
-          row_unit4<T, WIDE>(p, reinterpret_cast<const T*>(r.p + b * r.sb + hk * r.sh + s * r.ss),
-                             c.p + page * c.sp + hk * c.sh + at * c.st, w.p + page * w.sp + hk * w.sh + at * w.st, cs, u,
-                             key && p.R > 0);
-        t += dt;
-        h += dh;
-        if (h >= nh) {
-          h -= nh;
-          ++t;
-        }
-        continue;
+        row_unit<T, N>(p, reinterpret_cast<const T*>(r.p + b * r.sb + hk * r.sh + s * r.ss),
+                       reinterpret_cast<T*>(c.p + page * c.sp + hk * c.sh + static_cast<int64_t>(sh.at[at.t]) * c.st),
+                       sh.cs[at.t], at.u, key && p.R > 0);
       }
     }
-    const T* src;
-    T* dst;
-    bool there = true;
-    if (head < p.H) {
-      src = reinterpret_cast<const T*>(p.q.p + b * p.q.sb + head * p.q.sh + s * p.q.ss);
-      dst = reinterpret_cast<T*>(p.qo.p + b * p.qo.sb + head * p.qo.sh + s * p.qo.ss);
-    } else {
-      const bool key = head < p.H + p.Hkv;
-      const int hk = head - p.H - (key ? 0 : p.Hkv);
+  }
+  if constexpr (FOUR) {
+    const int part = split - (p.both ? 0 : p.splits);  // (both: this workgroup takes all rows)
+    if (part < 0) return;
+    const int parts = p.both ? 1 : p.splits4, heads = 2 * p.Hkv, per = (heads + parts - 1) / parts, h0 = part * per;
+    Slots at(p.units4, min(per, heads - h0));
+    for (; at.any && at.t < n; at.next()) {
+      const int b = sh.b[at.t], s = sh.s[at.t], head = h0 + at.h, page = sh.page[at.t];
+      if (page < 0) continue;
+      const bool key = head < p.Hkv;
+      const int hk = key ? head : head - p.Hkv;
+      const int64_t row = sh.at[at.t];
       const Rows& r = key ? p.k : p.v;
       const Cache& c = key ? p.kc : p.vc;
-      there = page >= 0;
-      src = reinterpret_cast<const T*>(r.p + b * r.sb + hk * r.sh + s * r.ss);
-      dst = reinterpret_cast<T*>(c.p + page * c.sp + hk * c.sh + at * c.st);
-    }
-    if (there) row_unit<T, N>(p, src, dst, cs, u, p.R > 0 && head < p.H + p.Hkv);
-    t += dt;
-    h += dh;
-    if (h >= nh) {
-      h -= nh;
-      ++t;
+      const Cache& w = key ? p.ks : p.vs;
+      row_unit4<T, WIDE>(p, reinterpret_cast<const T*>(r.p + b * r.sb + hk * r.sh + s * r.ss),
+                         c.p + page * c.sp + hk * c.sh + row * c.st, w.p + page * w.sp + hk * w.sh + row * w.st, sh.cs[at.t],
+                         at.u, key && p.R > 0);
     }
   }
 }
@@ -271,54 +277,62 @@ struct Read {
   int S, Hkv, units, num_pages, page_size;
 };
 
-// A thread widens 8 values of a token's key and of its value; rows past a sequence's length
-// and on no page get zeros.  Bound by the bytes written.
+// A thread widens 8 values of a token's key and of its value; a workgroup takes neighbouring
+// tokens of one head, and rows past a sequence's length and on no page get zeros.
+// Bound by the bytes written: 8 x 1280 tokens, 8 heads of 128, to bf16 10.6 us (5.0 TB/s; two heads a
+// thread 11.5, four 12.2).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void read4_kernel(Read p) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t row = e / p.units;
-  const int u = static_cast<int>(e - row * p.units);
-  const int64_t hs = row / p.S;
-  const int s = static_cast<int>(row - hs * p.S), h = static_cast<int>(hs);
-  const int64_t b = blockIdx.y;
-  if (hs >= p.Hkv) return;
+  const int slots = kThreads / p.units, slot = threadIdx.x / p.units, u = threadIdx.x - slot * p.units;
+  const int s = blockIdx.x * slots + slot, b = blockIdx.y, h = blockIdx.z;
+  if (slot >= slots || s >= p.S) return;
   const int entry = s / p.page_size, at = s - entry * p.page_size;
   int page = -1;
   if (!p.lens || s < p.lens[b]) page = p.table[b * p.table_stride + entry];
-  float x[2][8] = {};
+  uint32_t codes[2] = {0, 0}, scales[2] = {0, 0};
   if (page >= 0 && page < p.num_pages) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const Cache& c = j ? p.vc : p.kc;
       const Cache& w = j ? p.vs : p.ks;
-      const uint32_t codes = *reinterpret_cast<const uint32_t*>(c.p + page * c.sp + h * c.sh + at * c.st + 4 * u);
-      const uint32_t scale = *reinterpret_cast<const uint8_t*>(w.p + page * w.sp + h * w.sh + at * w.st + (u >> 2));
-      const uint4 d = kv4::decode8(codes, kv4::scale_f32(scale));
-      const uint32_t words[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[j][2 * i] = __uint_as_float(words[i] << 16);
-        x[j][2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
-      }
+      codes[j] = *reinterpret_cast<const uint32_t*>(c.p + page * c.sp + h * c.sh + at * c.st + 4 * u);
+      scales[j] = *reinterpret_cast<const uint8_t*>(w.p + page * w.sp + h * w.sh + at * w.st + (u >> 2));
     }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const Rows& r = j ? p.v : p.k;
     T* out = reinterpret_cast<T*>(r.p + b * r.sb + h * r.sh + s * r.ss) + 8 * u;
-    constexpr int V = Elem<T>::kVec;
+    const uint4 d = kv4::decode8(codes[j], kv4::scale_f32(scales[j]));
+    if constexpr (__is_same(T, bf16_t)) {
+      *reinterpret_cast<uint4*>(out) = d;
+    } else {
+      const uint32_t words[4] = {d.x, d.y, d.z, d.w};
+      float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += V) store_vec(out + i, x[j] + i);
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(words[e] << 16);
+        x[2 * e + 1] = __uint_as_float(words[e] & 0xffff0000u);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += Elem<T>::kVec) store_vec(out + e, x + e);
+    }
   }
 }
 
-// How the rows are dealt out: about 1024 workgroups (four a CU) before any of them takes
-// more than a row in each slot, then up to twelve, so that a token's angles serve many rows.
+// How the rows are dealt out: a row in each slot until 1024 workgroups (four a CU) run, then two,
+// beyond eight times as many three, so that a token's angles serve many rows and workgroups still follow each other.
+// us with 1, 2, 3, 4, 6, 12 rows a slot (one: a token a workgroup, whose slots its rows may not fill):
+//   rope, 16 heads of 128, bf16, 2048 tokens       7.5   6.1   7.2   7.0   8.4  10.8
+//   the same, 4 x 2048                            20.2  13.5  15.0  13.9  15.2  15.8
+//   the same, 8 x 8192                             151  94.0  98.5  98.8   104   111
+//   into 16 bits, 32 heads and 8, f16, 8 x 1024   54.2  37.7  35.2  35.2  35.4  36.3
+//   into 4 bits, the same in bf16                 52.0  36.4  36.4  37.8  40.8  51.6
 static void plan(Params& p, bool four) {
   const int64_t rows = p.H + (four ? 0 : 2 * p.Hkv), rows4 = four ? 2 * p.Hkv : 0;
   const int64_t slots = kThreads / p.units, slots4 = four ? kThreads / p.units4 : 1;
   const int64_t all = p.tokens * (rows * p.units + rows4 * (four ? p.units4 : 0));
-  const int64_t each = std::min<int64_t>(12, std::max<int64_t>(1, all / (kThreads * 1024)));
+  const int64_t filled = all / (kThreads * 1024), each = filled < 1 ? 1 : filled < 8 ? 2 : 3;
   p.block_tokens = 1;
   auto parts = [&](int64_t r, int64_t s) { return static_cast<int>(r ? std::max<int64_t>(1, (r + s * each - 1) / (s * each)) : 0); };
   p.splits = parts(rows, slots);
@@ -327,6 +341,11 @@ static void plan(Params& p, bool four) {
     const int64_t by = rows ? std::max<int64_t>(1, slots * each / rows) : kMostTokens;
     const int64_t by4 = rows4 ? std::max<int64_t>(1, slots4 * each / rows4) : kMostTokens;
     p.block_tokens = static_cast<int>(std::min<int64_t>({by, by4, kMostTokens}));
+    // Enough tokens for every slot of either kind: the angles are computed once for both.
+    if (four && p.H > 0) {
+      p.both = 1;
+      p.splits4 = 0;
+    }
   }
 }
 
@@ -596,10 +615,10 @@ extern "C" int ghip_kv4_read(int dtype, const GHipKv4* k_cache, const GHipKv4* v
   p.table_stride = table_stride;
   p.S = static_cast<int>(S); p.Hkv = static_cast<int>(Hkv); p.units = static_cast<int>(D / 8);
   p.num_pages = static_cast<int>(num_pages); p.page_size = static_cast<int>(page_size);
-  const int64_t blocks = (S * Hkv * p.units + rope::kThreads - 1) / rope::kThreads;
-  if (B > 65535 || blocks > rope::kMostGroups)
+  const int64_t slots = rope::kThreads / p.units, blocks = (S + slots - 1) / slots;
+  if (B > 65535 || Hkv > 65535 || blocks > rope::kMostGroups)
     return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", kWhat);
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(B));
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(B), static_cast<unsigned>(Hkv));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == GHIP_DTYPE_FLOAT32) hipLaunchKernelGGL((rope::read4_kernel<float>), grid, dim3(rope::kThreads), 0, s, p);
   else if (dtype == GHIP_DTYPE_FLOAT16) hipLaunchKernelGGL((rope::read4_kernel<f16_t>), grid, dim3(rope::kThreads), 0, s, p);

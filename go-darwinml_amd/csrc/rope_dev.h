@@ -28,17 +28,33 @@ __device__ __forceinline__ double position(const Angles& a, int b, int s, int i)
   return static_cast<double>(a.positions[axis * a.p_sa + b * a.p_sb + s * a.p_ss]);
 }
 
-// (cos, sin) of pos * freq.  The angle is a product in 64 bits, reduced by whole turns in two
-// steps (2 pi as the sum of two doubles), so positions of any size keep 2^-52 of a turn;
-// each of the two is rounded to fp32 once.  (An fp32 angle of 10^5 is off by 2^-8.)
+// (cos, sin) of pos * freq.  The angle is a product in 64 bits, reduced by whole quarter turns in two
+// steps (pi / 2 as the sum of two doubles) to |r| <= pi / 4, so positions of any size keep 2^-52
+// of the angle; there the Taylor sums to r^11 and r^12 are off by less than 2^-36, and each of the
+// two is rounded to fp32 once.  (An fp32 angle of 10^5 is off by 2^-8.  The library's sincos,
+// good to 2^-52, takes four times the instructions: a batch of prompts into 4 bits was bound by it.)
 __device__ __forceinline__ float2 turn(double pos, float freq, int inverse) {
   const double a = pos * static_cast<double>(freq);
-  const double k = rint(a * 0.15915494309189535);
-  double r = fma(-k, 6.283185307179586, a);
-  r = fma(-k, 2.4492935982947064e-16, r);
-  double s, c;
-  sincos(r, &s, &c);
-  return make_float2(static_cast<float>(c), static_cast<float>(inverse ? -s : s));
+  const double k = rint(a * 0.6366197723675814);  // 2 / pi
+  double r = fma(-k, 1.5707963267948966, a);
+  r = fma(-k, 6.123233995736766e-17, r);
+  const double z = r * r;
+  double s = fma(z, -1. / 39916800., 1. / 362880.);
+  s = fma(z, s, -1. / 5040.);
+  s = fma(z, s, 1. / 120.);
+  s = fma(z, s, -1. / 6.);
+  s = fma(z * r, s, r);
+  double c = fma(z, 1. / 479001600., -1. / 3628800.);
+  c = fma(z, c, 1. / 40320.);
+  c = fma(z, c, -1. / 720.);
+  c = fma(z, c, 1. / 24.);
+  c = fma(z, c, -0.5);
+  c = fma(z, c, 1.);
+  const int quarter = static_cast<int>(fma(floor(k * 0.25), -4., k));  // 0 .. 3
+  const float sf = static_cast<float>(s), cf = static_cast<float>(c);
+  const float sn = quarter & 1 ? cf : sf, cs = quarter & 1 ? sf : cf;
+  const float si = quarter & 2 ? -sn : sn;
+  return make_float2(((quarter + 1) & 2) ? -cs : cs, inverse ? -si : si);
 }
 
 // (x, y) turned.  Each product is rounded by itself: left to be fused with the sum, which of

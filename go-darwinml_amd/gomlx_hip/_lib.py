@@ -38,15 +38,17 @@ _vp = ctypes.c_void_p
 _f32 = ctypes.c_float
 _errp = ctypes.POINTER(GHipError)
 
+# The arrays of these two are spelled out: a structure of scalars is made in a third of the time.
 class Rope(ctypes.Structure):
     """GHipRope."""
-    _fields_ = [("positions", _vp), ("position_strides", _i64 * 3), ("axes", _i64), ("sections", _i64 * 4),
-                ("freqs", _vp), ("rotary_dim", _i64), ("interleaved", _i64)]
+    _fields_ = ([("positions", _vp)] + [(f"position_stride{i}", _i64) for i in range(3)] + [("axes", _i64)]
+                + [(f"section{i}", _i64) for i in range(4)] + [("freqs", _vp), ("rotary_dim", _i64), ("interleaved", _i64)])
 
 
 class Kv4(ctypes.Structure):
     """GHipKv4."""
-    _fields_ = [("codes", _vp), ("scales", _vp), ("code_strides", _i64 * 3), ("scale_strides", _i64 * 3)]
+    _fields_ = ([("codes", _vp), ("scales", _vp)] + [(f"code_stride{i}", _i64) for i in range(3)]
+                + [(f"scale_stride{i}", _i64) for i in range(3)])
 
 
 _i64p = ctypes.POINTER(_i64)

@@ -507,7 +507,11 @@ def sdpa_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     return out
 
 
-_I4 = ctypes.c_int64 * 4
+def _new(like: torch.Tensor, shape, stream, dtype=None) -> torch.Tensor:
+    """_empty on the device (and of the type) of another tensor."""
+    if stream is None:
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+    return _empty(shape, dtype or like.dtype, like.device, stream)
 
 
 def _rope(what: str, freqs, positions, sections, interleaved, B: int, S: int, D: int):
@@ -518,16 +522,20 @@ def _rope(what: str, freqs, positions, sections, interleaved, B: int, S: int, D:
         return None
     if freqs.dtype != torch.float32 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError(f"{what}: freqs is a contiguous float32 vector, one value a pair")
-    pairs, axes, step = freqs.shape[0], 1, (0, 0, 0)
+    pairs, axes, at, step = freqs.shape[0], 1, None, (0, 0, 0)
     if positions is not None:
         if positions.dtype != torch.int32 or positions.dim() not in (2, 3) or positions.shape[-2:] != (B, S):
             raise ValueError(f"{what}: positions is int32 [{B}, {S}] or [axes, {B}, {S}]")
-        axes = positions.shape[0] if positions.dim() == 3 else 1
-        step = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    sections = [pairs] if sections is None else list(sections)
+        at, step = positions.data_ptr(), positions.stride()
+        if len(step) == 3:
+            axes = positions.shape[0]
+        else:
+            step = (0, *step)
+    if sections is None:
+        sections = (pairs,)
     if len(sections) != axes or axes > 4:
         raise ValueError(f"{what}: {len(sections)} sections for {axes} axes of positions (1 to 4)")
-    return _lib.Rope(_ptr(positions), _I3(*step), axes, _I4(*sections), freqs.data_ptr(), 2 * pairs, int(interleaved))
+    return _lib.Rope(at, *step, axes, *sections, *(0,) * (4 - axes), freqs.data_ptr(), 2 * pairs, interleaved)
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections=None, interleaved: bool = False,
@@ -545,15 +553,15 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections
         raise ValueError("rope: positions and freqs are needed")
     r = _rope("rope", freqs, positions, sections, interleaved, B, S, D)
     if out is None:
-        out = _empty((B, H, S, D), x.dtype, dev, stream)
+        out = _new(x, (B, H, S, D), stream)
     else:
         _like("rope: out", out, x.shape, x.dtype)
     _launch(dev, "ghip_rope", stream, dtype_code(x.dtype), x.data_ptr(), out.data_ptr(), B, H, S, D, _rows3("x", x),
-            _rows3("out", out), ctypes.byref(r), int(inverse))
+            _rows3("out", out), r, inverse)
     return out
 
 
-def _new_tokens(what, q, k, v, q_out, stream, dev):
+def _new_tokens(what, q, k, v, q_out, stream):
     """(B, H, Hkv, S, D), q_out and the strides of an append's operands."""
     if k.dim() != 4 or (q is not None and q.dim() != 4):
         raise ValueError(f"{what}: q [B, H, S, D] and k / v [B, Hkv, S, D] are needed")
@@ -566,7 +574,7 @@ def _new_tokens(what, q, k, v, q_out, stream, dev):
     H = q.shape[1]
     _like(f"{what}: q", q, (B, H, S, D), k.dtype)
     if q_out is None:
-        q_out = _empty((B, H, S, D), q.dtype, dev, stream)
+        q_out = _new(q, (B, H, S, D), stream)
     else:
         _like(f"{what}: q_out", q_out, q.shape, q.dtype)
     return (B, H, Hkv, S, D), q_out, (_rows3("q", q), _rows3("q_out", q_out), _rows3("k", k), _rows3("v", v))
@@ -581,7 +589,7 @@ def kv_append_rope(q, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     Wraps ghip_kv_append_rope."""
     what = "kv_append_rope"
     dev = _one_device(k, q, v, k_cache, v_cache, block_table, starts, freqs, counts, positions, q_out)
-    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream, dev)
+    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream)
     pages, size, per, ts = _check_cache(what, k_cache, v_cache, block_table, B, Hkv, D, k.dtype)
     _ints(f"{what}: starts", starts, B)
     _ints(f"{what}: counts", counts, B)
@@ -602,21 +610,28 @@ def kv4_cache(num_pages: int, page_size: int, Hkv: int, D: int, device="cuda"):
 def _kv4(what, k_cache, v_cache, block_table, B, Hkv, D):
     """The two GHipKv4 of caches (codes, scales) viewed as [page, Hkv, token, ...], and
     (num_pages, page_size, max_pages, table stride)."""
-    made = []
     shape = k_cache[0].shape
+    if len(shape) != 4 or shape[1] != Hkv or shape[3] * 2 != D:
+        raise ValueError(f"{what}: codes are [pages, {Hkv}, page_size, {D // 2}]")
+    pages, _, size, half = shape
+    wide = pages, Hkv, size, (D + 127) // 128 * 4
+    made = []
     for name, (codes, scales) in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if codes.dim() != 4 or codes.shape != shape or codes.shape[1] != Hkv or codes.shape[3] * 2 != D or codes.dtype != torch.uint8:
-            raise ValueError(f"{what}: {name}'s codes are uint8 [pages, {Hkv}, page_size, {D // 2}], both alike")
-        _like(f"{what}: {name}'s scales", scales, (*shape[:3], (D + 127) // 128 * 4), torch.uint8)
-        made.append(_lib.Kv4(codes.data_ptr(), scales.data_ptr(), _rows3(f"{name}'s codes", codes),
-                             _rows3(f"{name}'s scales", scales)))
+        if codes.shape != shape or scales.shape != wide or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            _like(f"{what}: {name}'s codes", codes, shape, torch.uint8)
+            _like(f"{what}: {name}'s scales", scales, wide, torch.uint8)
+        a, b, c, one = codes.stride()
+        e, f, g, uno = scales.stride()
+        if (one != 1 and half != 1) or uno != 1:
+            raise ValueError(f"{what}: a row's codes and scales must be contiguous")
+        made.append(_lib.Kv4(codes.data_ptr(), scales.data_ptr(), a, b, c, e, f, g))
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B:
         raise ValueError(f"{what}: block_table is int32 [{B}, pages of a sequence]")
     step, one = block_table.stride()
     per = block_table.shape[1]
     if per > 1 and one != 1:
         raise ValueError(f"{what}: a sequence's table entries must be contiguous")
-    return made, (shape[0], shape[2], per, step)
+    return made, (pages, size, per, step)
 
 
 def kv4_append_rope(q, k: torch.Tensor, v: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor,
@@ -626,13 +641,14 @@ def kv4_append_rope(q, k: torch.Tensor, v: torch.Tensor, k_cache, v_cache, block
     and a power of two for each 32.  D: a multiple of 32.  Wraps ghip_kv4_append_rope."""
     what = "kv4_append_rope"
     dev = _one_device(k, q, v, *k_cache, *v_cache, block_table, starts, freqs, counts, positions, q_out)
-    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream, dev)
+    (B, H, Hkv, S, D), q_out, steps = _new_tokens(what, q, k, v, q_out, stream)
     (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
     _ints(f"{what}: starts", starts, B)
     _ints(f"{what}: counts", counts, B)
     r = _rope(what, freqs, positions, sections, interleaved, B, S, D)
     _launch(dev, "ghip_kv4_append_rope", stream, dtype_code(k.dtype), _ptr(q), _ptr(q_out), k.data_ptr(), v.data_ptr(),
-            kc, vc, B, H, Hkv, S, D, pages, size, per, block_table.data_ptr(), ts, starts.data_ptr(), _ptr(counts), *steps, r)
+            kc, vc, B, H, Hkv, S, D, pages, size, per, block_table.data_ptr(), ts, starts.data_ptr(), _ptr(counts),
+            *steps, r)
     return q_out
 
 
@@ -650,11 +666,14 @@ def kv4_read(k_cache, v_cache, block_table: torch.Tensor, tokens: int, lens=None
     (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
     _ints(f"{what}: lens", lens, B)
     shape = (B, Hkv, int(tokens), D)
-    k, v = outs if outs is not None else (_empty(shape, dtype, dev, stream), _empty(shape, dtype, dev, stream))
-    _like(f"{what}: k", k, shape, k.dtype)
-    _like(f"{what}: v", v, shape, k.dtype)
-    _launch(dev, "ghip_kv4_read", stream, dtype_code(k.dtype), kc, vc, k.data_ptr(), v.data_ptr(), B, Hkv, int(tokens), D,
-            pages, size, per, block_table.data_ptr(), ts, _ptr(lens), _rows3("k", k), _rows3("v", v))
+    if outs is None:
+        k, v = _new(k_cache[0], shape, stream, dtype), _new(k_cache[0], shape, stream, dtype)
+    else:
+        k, v = outs
+        _like(f"{what}: k", k, shape, k.dtype)
+        _like(f"{what}: v", v, shape, k.dtype)
+    _launch(dev, "ghip_kv4_read", stream, dtype_code(k.dtype), kc, vc, k.data_ptr(), v.data_ptr(), B, Hkv, int(tokens),
+            D, pages, size, per, block_table.data_ptr(), ts, _ptr(lens), _rows3("k", k), _rows3("v", v))
     return k, v
 
 
@@ -680,21 +699,20 @@ def sdpa_paged_kv4(q: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor,
     (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
     _ints(f"{what}: lens", lens, B)
     if out is None:
-        out = _empty((B, H, D), q.dtype, dev, stream)
+        out = _new(q, (B, H, D), stream)
     else:
         _like(f"{what}: out", out, (B, H, D), q.dtype)
-    for name, t in (("q", q), ("out", out)):
-        if t.stride(2) != 1 and D != 1:
-            raise ValueError(f"{what}: {name}'s head dim must be contiguous")
+    (qb, qh, qd), (ob, oh, od) = q.stride(), out.stride()
+    if (qd != 1 or od != 1) and D != 1:
+        raise ValueError(f"{what}: the head dim of q and out must be contiguous")
     ws = None
     if split and workspace is None:
         ws = sdpa_paged_kv4_workspace(q, k_cache, block_table, stream)
     elif split:
         ws = _given(what, workspace)
     _launch(dev, "ghip_sdpa_paged_kv4", stream, dtype_code(q.dtype), q.data_ptr(), kc, vc, out.data_ptr(), B, H, Hkv, D,
-            pages, size, per, block_table.data_ptr(), ts, lens.data_ptr(), _I3(q.stride(0), q.stride(1)),
-            _I3(out.stride(0), out.stride(1)), int(window), int(sinks), float(scale), _ptr(ws),
-            0 if ws is None else ws.numel() * ws.element_size())
+            pages, size, per, block_table.data_ptr(), ts, lens.data_ptr(), _I3(qb, qh), _I3(ob, oh), int(window), int(sinks),
+            float(scale), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size())
     return out
 
 
@@ -728,15 +746,17 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, scale:
     step = _logits(what, logits, ids)
     N, V = logits.shape
     top = int(top)
-    shapes = ((N,), torch.float32), ((N,), torch.float32), ((N,), torch.float32), ((N, top), torch.float32), ((N, top), torch.int32)
     if outs is None:
-        outs = [_empty(shape, dt, dev, stream) if i < 3 or top > 0 else None for i, (shape, dt) in enumerate(shapes)]
+        f32 = torch.float32
+        outs = (_new(ids, (N,), stream, f32), _new(ids, (N,), stream, f32), _new(ids, (N,), stream, f32),
+                _new(ids, (N, top), stream, f32) if top > 0 else None, _new(ids, (N, top), stream) if top > 0 else None)
     else:
-        for i, (t, (shape, dt)) in enumerate(zip(outs, shapes, strict=True)):
+        outs = tuple(outs)
+        for i, (t, shape) in enumerate(zip(outs, ((N,), (N,), (N,), (N, top), (N, top)), strict=True)):
             if t is None and (i < 3 or top > 0):
                 raise ValueError(f"{what}: five outputs are needed (the last two may be None where top is 0)")
             if t is not None:
-                _like(f"{what}: output {i}", t, shape, dt)
+                _like(f"{what}: output {i}", t, shape, torch.int32 if i == 4 else torch.float32)
                 if not t.is_contiguous():
                     raise ValueError(f"{what}: outputs must be contiguous")
     ws = None
@@ -745,8 +765,9 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, scale:
     elif split:
         ws = _given(what, workspace)
     _launch(dev, "ghip_token_logprobs", stream, dtype_code(logits.dtype), logits.data_ptr(), step, ids.data_ptr(), N, V, top,
-            float(scale), *(_ptr(t) for t in outs), _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size())
-    return tuple(outs)
+            float(scale), outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr(), _ptr(outs[3]), _ptr(outs[4]), _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size())
+    return outs
 
 
 def token_logprobs_grad(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tensor, d_logp, entropy=None, d_entropy=None,
@@ -766,7 +787,7 @@ def token_logprobs_grad(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tens
             if not t.is_contiguous():
                 raise ValueError(f"{what}: {name} must be contiguous")
     if out is None:
-        out = _empty((N, V), logits.dtype, dev, stream)
+        out = _new(logits, (N, V), stream)
     else:
         _like(f"{what}: out", out, (N, V), logits.dtype)
         if out.stride(1) != 1 and V != 1:

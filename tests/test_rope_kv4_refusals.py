@@ -8,13 +8,13 @@ import torch
 import rope_kv4_ref as ref
 from gomlx_hip import _lib, ops
 
-I3, I4 = ctypes.c_int64 * 3, ctypes.c_int64 * 4
+I3 = ctypes.c_int64 * 3
 BF16, F16, F32 = _lib.DT_BFLOAT16, _lib.DT_FLOAT16, _lib.DT_FLOAT32
 PTR = 1 << 20  # never dereferenced: every call here is refused
 
 
 def plan(R=64, axes=1, sections=(32, 0, 0, 0), positions=PTR, freqs=PTR, steps=(0, 8, 1), interleaved=0):
-    return _lib.Rope(positions, I3(*steps), axes, I4(*sections), freqs, R, interleaved)
+    return _lib.Rope(positions, *steps, axes, *sections, freqs, R, interleaved)
 
 
 def rope(dt=BF16, B=1, H=4, S=8, D=64, x=PTR, st=None, r=None, **kw):
@@ -29,7 +29,7 @@ def append(dt=BF16, B=1, H=4, Hkv=2, S=2, D=64, pages=4, size=16, per=2, q=PTR, 
 
 
 def cache(codes=PTR, scales=PTR, cst=(1 << 12, 512, 32), sst=(64, 64, 4)):
-    return _lib.Kv4(codes, scales, I3(*cst), I3(*sst))
+    return _lib.Kv4(codes, scales, *cst, *sst)
 
 
 def append4(dt=BF16, B=1, H=4, Hkv=2, S=2, D=64, pages=4, size=16, per=2, k=PTR, ts=2, kc=None, vc=None, **kw):
