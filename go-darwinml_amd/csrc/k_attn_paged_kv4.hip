@@ -108,8 +108,9 @@ __device__ __forceinline__ uint32_t decode_byte(uint2 w, float s) {
   return kv4::decode2<(B & 3)>(B < 4 ? w.x : w.y, s);
 }
 
-// A wave works alone on tiles of 64 tokens: codes and scales come by per-lane DMA into two
-// LDS stages, page numbers one tile further ahead.  S^T = K Q^T, 16 tokens x 16 heads a
+// A wave works alone on tiles of 64 tokens: codes and scales come by per-lane DMA into LDS, from
+// there all of the tile goes to registers, and the next tile's DMA runs while it is computed; page
+// numbers come one tile further ahead.  S^T = K Q^T, 16 tokens x 16 heads a
 // product: lane (c, g) has a quarter g of token c's row, so the contraction runs over d in the
 // order quarter, word, value.  O^T += V^T P^T: lane (c, g) has DP / 16 consecutive values of
 // tokens 4 g .. 4 g + 3 and 16 more; a conversion makes two of one token, a byte permute
@@ -124,11 +125,10 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
   constexpr int kPlanes = DP == 256 ? 2 : 1;            // words of a row's scales
   constexpr int kDma = kTile * kRow / 1024, kPer = 64 / kCh;  // DMA instructions of K's codes, rows of one
   constexpr int kCodes = kTile * kRow, kStage = 2 * kCodes + 2 * kPlanes * 4 * kTile;
-  constexpr int kAll = 2 * kDma + 2 * kPlanes;          // DMA instructions of a tile
   constexpr int kWords = kRow / 16;                     // words of a quarter of a row
   constexpr int kVals = DP / 16;                        // values of V a lane holds of a token
   constexpr int kQuarterGroups = DP == 256 ? 2 : 1;     // scales of a quarter of a row
-  __shared__ __attribute__((aligned(1024))) char smem[2][kStage];
+  __shared__ __attribute__((aligned(1024))) char smem[kStage];
   __shared__ __attribute__((aligned(16))) int32_t page_lds[2][64];
 
   const int lane = threadIdx.x, g = lane >> 4, col = lane & 15;
@@ -196,15 +196,19 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     };
     // The DMA of tile t, its page numbers landed; returns its rows that hold a token.  A lane finds
     // the addresses of its token's rows, those that load them fetch them from it.
-    auto issue = [&](int t, int slot) -> uint64_t {
+    auto issue = [&](int t, int slot) -> uint64_t {  // (page numbers from `slot`)
       const int tok = token0(t) + lane;
       const int page = page_lds[slot][lane];
       const uint32_t off = tok - page_of(p, tok) * p.page_size;
-      const bool ok = (t < nst ? tok < seen.ns : tok >= seen.lo && tok < seen.len) && page >= 0 && page < p.num_pages;
-      const uint32_t la = la0 + slot * kStage, pg = ok ? page : 0;
+      // No branches here: where lanes part, the compiler has put copies of registers in front of the
+      // instruction that brings all lanes back, and those of the lanes that had left were lost.
+      const int from = t < nst ? 0 : seen.lo, to = t < nst ? seen.ns : seen.len;
+      const bool ok = (tok >= from) & (tok < to) & (page >= 0) & (page < p.num_pages);
+      const uint32_t pg = ok ? page : 0;
       auto row = [&](const char* base, uint32_t sp, uint32_t st) {
-        const char* at = base + static_cast<uint64_t>(pg) * sp + static_cast<uint64_t>(off) * st;
-        return ok ? at : zero;
+        uint64_t at = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(pg) * sp + static_cast<uint64_t>(off) * st;
+        asm volatile("" : "+v"(at));  // (computed for all lanes, then selected)
+        return ok ? reinterpret_cast<const char*>(at) : zero;
       };
       const char* krow = row(kc, p.k.sp, p.k.st);
       const char* vrow = row(vc, p.v.sp, p.v.st);
@@ -213,15 +217,15 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
         const int s = i * kPer + lane / kCh, r = slot_of(s);
         // (Past the head dim: any bytes of the row; their scales count as 2^-127 and q as 0.)
         const int ch = min((lane % kCh) ^ swz(s), groups - 1) * 16;
-        tile::load16(from_lane(krow, r) + ch, la + i * 1024);
-        tile::load16(from_lane(vrow, r) + ch, la + kCodes + i * 1024);
+        tile::load16(from_lane(krow, r) + ch, la0 + i * 1024);
+        tile::load16(from_lane(vrow, r) + ch, la0 + kCodes + i * 1024);
       }
       const char* kscale = row(ks, p.k.ssp, p.k.sst);
       const char* vscale = row(vs, p.v.ssp, p.v.sst);
 #pragma unroll
       for (int i = 0; i < kPlanes; ++i) {
-        tile::load4(kscale + 4 * i, la + 2 * kCodes + i * 256);
-        tile::load4(vscale + 4 * i, la + 2 * kCodes + (kPlanes + i) * 256);
+        tile::load4(kscale + 4 * i, la0 + 2 * kCodes + i * 256);
+        tile::load4(vscale + 4 * i, la0 + 2 * kCodes + (kPlanes + i) * 256);
       }
       return __builtin_amdgcn_ballot_w64(ok);
     };
@@ -231,43 +235,40 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     for (int j = 0; j < kVals; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    // The order of the DMA is pages 0, 1, tile 0, pages 2, tile 1, pages 3, tile 2, ..
     const int n = te - ta;
-    uint64_t rows0 = 0, rows1 = 0;  // of tiles j and j + 1
+    uint64_t next = 0;  // the rows of the tile under way
     if (n > 0) {
       issue_pages(ta, 0);
       if (n > 1) issue_pages(ta + 1, 1);
     }
     tile::bf16x8 qf[kVals / 2][kQ];  // [step][part]
     {
-      const T* Q = static_cast<const T*>(p.q) + b * p.q_sb + (h0 + col) * p.q_sh;
+      // (Without branches, so that the loads are under way at once; columns without a head load the last.)
+      const T* Q = static_cast<const T*>(p.q) + b * p.q_sb + (h0 + min(col, heads - 1)) * p.q_sh;
+      float x[kVals / 2][8];
 #pragma unroll
       for (int s = 0; s < kVals / 2; ++s) {
         const int d = g * (DP / 4) + 8 * s;
-        float x[8] = {};
-        if (col < heads && d < p.D) {
 #pragma unroll
-          for (int i = 0; i < 8; i += Elem<T>::kVec) load_vec(Q + d + i, x + i);
-        }
-        split8<kQ>(x, qf[s]);
+        for (int i = 0; i < 8; i += Elem<T>::kVec) load_vec(Q + (d < p.D ? d : 0) + i, x[s] + i);
+      }
+#pragma unroll
+      for (int s = 0; s < kVals / 2; ++s) {
+        const bool in = (col < heads) & (g * (DP / 4) + 8 * s < p.D);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = in ? x[s][e] : 0.f;
+        split8<kQ>(x[s], qf[s]);
       }
 #pragma unroll
       for (int s = 0; s < kVals / 2; ++s) tile::settle(qf[s]);
     }
     if (n > 0) {
       wait_vm<0>();
-      rows0 = issue(ta, 0);
-      if (n > 1) {
-        if (n > 2) issue_pages(ta + 2, 0);
-        rows1 = issue(ta + 1, 1);
-      }
+      next = issue(ta, 0);
     }
     for (int j = 0; j < n; ++j) {
-      // Everything older than tile j + 1's own DMA has landed, its successor's pages among it.
-      if (j + 1 < n) wait_vm<kAll>();
-      else wait_vm<0>();
-      // All of the tile into registers, so that its stage takes tile j + 2 while this one is computed.
-      const char* sk = smem[j & 1];
+      wait_vm<0>();  // tile j, and the pages of j + 1
+      const char* sk = smem;
       const char* sv = sk + kCodes;
       const uint8_t* ssk = reinterpret_cast<const uint8_t*>(sk + 2 * kCodes);
       const uint8_t* ssv = ssk + kPlanes * 256;
@@ -308,12 +309,11 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
               sv + (32 * t + 16 * (e >> 2) + 4 * (e & 3)) * kRow + g * kRow + (((byte >> 4) ^ swz(s)) << 4) + (byte & 15));
           vscale[t][e] = scale_of(ssv[4 * (32 * t + 16 * (e >> 2) + (e & 3)) + 16 * g + (vgroup >> 2) * 256 + (vgroup & 3)], vgroup);
         }
-      const uint64_t rows = rows0;
-      rows0 = rows1;
+      const uint64_t rows = next;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (j + 2 < n) {
-        if (j + 3 < n) issue_pages(ta + j + 3, (j + 1) & 1);
-        rows1 = issue(ta + j + 2, j & 1);
+      if (j + 1 < n) {
+        if (j + 2 < n) issue_pages(ta + j + 2, j & 1);
+        next = issue(ta + j + 1, (j + 1) & 1);
       }
       f32x4 x[4];
 #pragma unroll
@@ -456,14 +456,14 @@ static void launch(const Params& p, hipStream_t s) {
 using namespace ghip;
 
 // No workspace, so a wave for each unit: caches of at most 6 tiles a sequence, 12 with 512 units
-// or more, 24 with 1024.  (The second kernel costs 5-7 us; a wave alone takes 1.5 us a tile.)
+// or more, 24 with 1024.  (The second kernel costs 5-7 us; a wave alone takes 1.4 us a tile.)
 // bf16 D 128, 32 heads over 8, sequences of one length, us a call in a graph, split / unsplit:
 //   units      4 tiles      6           8           12          16          24          32
-//   8          12.8 / 9.4   12.9 / 12.4 12.8 / 15.4 12.9 / 21.2 12.9 / 27.0 13.0 / 38.6
-//   256        13.3 / 9.8   13.9 / 12.6 14.4 / 15.8 17.1 / 21.6 18.5 / 27.8 23.4 / 39.7
-//   512        16.1 / 10.1  18.5 / 13.0 20.0 / 16.8 24.8 / 22.9 27.9 / 29.0 34.1 / 41.3
-//   1024       24.9 / 12.1  29.2 / 16.0 32.6 / 19.1 37.7 / 25.2 42.7 / 31.0 52.8 / 43.1 63.1 / 55.9
-//   2048       40.5 / 19.6  46.6 / 24.8 51.3 / 29.6 61.4 / 39.9 72.1 / 50.5  105 / 84.2  129 / 108
+//   8          12.1 / 8.8   12.2 / 11.7 12.1 / 14.3 12.3 / 19.9 12.2 / 25.2 12.3 / 35.9 12.4 / 46.9
+//   256        12.6 / 9.3   13.2 / 12.0 13.7 / 14.8 16.5 / 20.4 17.7 / 26.3 20.9 / 37.2 23.4 / 48.0
+//   512        15.6 / 9.7   18.0 / 12.5 19.1 / 16.2 22.5 / 21.7 25.0 / 27.2 30.4 / 39.0 34.7 / 49.4
+//   1024       24.1 / 11.6  27.2 / 14.7 29.7 / 17.5 34.3 / 23.3 39.3 / 29.0 48.9 / 40.5 59.9 / 52.3
+//   2048       38.4 / 17.1  42.9 / 21.9 47.6 / 26.7 57.7 / 37.3 67.4 / 47.2 101 / 80.6  127 / 105
 // (Beyond, sequences of one length would still run faster unsplit with 1024 units and more; the
 // rule does not know the lengths, and one long sequence would keep the others waiting.)
 extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page_size,
