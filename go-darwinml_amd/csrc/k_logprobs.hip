@@ -32,7 +32,7 @@ struct Params {
   const int32_t* ids;
   int64_t N;
   int V, top, slices, per;  // per: vectors of a slice
-  float c;                  // scale * log2 e
+  float c, scale;           // c: scale * log2 e
   float* logp;
   float* entropy;
   float* lse;
@@ -43,12 +43,15 @@ struct Params {
 };
 
 // A running softmax in powers of two: m = max of x c, s = sum of w, e = sum of w u, where
-// u = x c - m and w = 2^u.
+// u = x c - m and w = 2^u.  m begins at -kLarge, below which weights are 0: the rounding of a
+// larger maximum's product with c would reach the weights.  A row that has nothing above, or a
+// maximum beyond kLarge, is summed by exact_sums.
+constexpr float kLarge = 1048576.f;
 struct Stats {
-  float m = -INFINITY, s = 0.f, e = 0.f;
+  float m = -kLarge, s = 0.f, e = 0.f;
   // The same sums beside another maximum.
   __device__ __forceinline__ void move(float to) {
-    const float base = to == -INFINITY ? 0.f : to, d = m - base, f = __builtin_amdgcn_exp2f(d);
+    const float d = m - to, f = __builtin_amdgcn_exp2f(d);
     e = f * __builtin_fmaf(fmaxf(d, kFar), s, e);
     s *= f;
     m = to;
@@ -215,27 +218,63 @@ struct Given {
   }
 };
 
-// What a row's statistics give; one thread.
-__device__ __forceinline__ void finish(const Params& p, int64_t row, const Stats& a, const Given& id) {
-  const float log_s = a.s == 0.f ? -INFINITY : __builtin_amdgcn_logf(a.s);
-  const bool none = a.m == -INFINITY && a.s == a.s;
-  float lp = 0.f;
-  if (id.there) lp = none ? -INFINITY : kLn2 * (__builtin_fmaf(id.x, p.c, -a.m) - log_s);
-  p.logp[row] = lp;
-  if (p.entropy) p.entropy[row] = none ? 0.f : kLn2 * (log_s - a.e / a.s);
-  if (p.lse) p.lse[row] = none ? -INFINITY : kLn2 * (a.m + log_s);
+// A row's sums: u = (x - x0) c - m.
+struct Sums : Stats {
+  float x0 = 0.f;
+  bool none = false;  // nothing but -infinity
+  __device__ __forceinline__ float exponent(float x, float c) const { return __builtin_fmaf(x - x0, c, -m); }
+  __device__ __forceinline__ bool usual() const { return fabsf(m) < kLarge && s > 0.f && s < INFINITY; }
+};
+// Rows of one mask, -infinity, 1e10 or a type's lowest number, and rows with a NaN or infinity: the
+// largest logit itself, then u = (x - x0) c.  Every lane of a wave calls it.
+template <typename T>
+__device__ __forceinline__ Sums exact_sums(const Params& p, int64_t row) {
+  const int lane = threadIdx.x & 63;
+  Sums a;
+  float most = -INFINITY;
+  for (int i = lane; i < p.V; i += 64) most = fmaxf(most, logit<T>(p, row, i));
+  a.x0 = wave_max(most);
+  a.m = 0.f;
+  a.none = a.x0 == -INFINITY;
+  if (a.none) a.x0 = 0.f;
+  for (int i = lane; i < p.V; i += 64) {
+    const float u = a.exponent(logit<T>(p, row, i), p.c), w = __builtin_amdgcn_exp2f(u);
+    a.s += w;
+    a.e = __builtin_fmaf(w, fmaxf(u, kFar), a.e);
+  }
+  a.s = wave_sum(a.s);
+  a.e = wave_sum(a.e);
+  if (a.s != a.s) a.none = false;  // nothing but -infinity and NaN
+  return a;
 }
-__device__ __forceinline__ void finish_top(const Params& p, int64_t row, const Stats& a, int rank, uint64_t key) {
+template <typename T>
+__device__ __forceinline__ Sums sums_of(const Params& p, int64_t row, const Stats& a) {
+  Sums r;
+  r.m = a.m;
+  r.s = a.s;
+  r.e = a.e;
+  return r.usual() ? r : exact_sums<T>(p, row);
+}
+
+// What a row's sums give; one thread.
+__device__ __forceinline__ void finish(const Params& p, int64_t row, const Sums& a, const Given& id) {
+  const float log_s = __builtin_amdgcn_logf(a.s);
+  float lp = 0.f;
+  if (id.there) lp = a.none ? -INFINITY : kLn2 * (a.exponent(id.x, p.c) - log_s);
+  p.logp[row] = lp;
+  if (p.entropy) p.entropy[row] = a.none ? 0.f : kLn2 * (log_s - a.e / a.s);
+  if (p.lse) p.lse[row] = a.none ? -INFINITY : __builtin_fmaf(a.x0, p.scale, kLn2 * (a.m + log_s));
+}
+__device__ __forceinline__ void finish_top(const Params& p, int64_t row, const Sums& a, int rank, uint64_t key) {
   p.top_ids[row * p.top + rank] = static_cast<int32_t>(~static_cast<uint32_t>(key));
-  const bool none = a.m == -INFINITY && a.s == a.s;
   const float x = value_of(static_cast<uint32_t>(key >> 32));
-  p.top_logps[row * p.top + rank] = none ? -INFINITY : kLn2 * (__builtin_fmaf(x, p.c, -a.m) - __builtin_amdgcn_logf(a.s));
+  p.top_logps[row * p.top + rank] = a.none ? -INFINITY : kLn2 * (a.exponent(x, p.c) - __builtin_amdgcn_logf(a.s));
 }
 
 // Rows that hold a NaN or +infinity (their sum is NaN, which the bounds above do not see): the
 // largest keys one after the other, a pass over the row for each.  Every thread of NT calls it.
 template <typename T, int NT>
-__device__ __forceinline__ void top_of_nan_row(const Params& p, int64_t row, const Stats& a, uint64_t* lds) {
+__device__ __forceinline__ void top_of_nan_row(const Params& p, int64_t row, const Sums& a, uint64_t* lds) {
   const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
   uint64_t last = ~0ull;
   for (int r = 0; r < p.top; ++r) {
@@ -440,7 +479,7 @@ __device__ __forceinline__ void look(Stats& a, const uint4 (&raw)[kRun], int v, 
 template <int M, bool MOST, typename Values>
 __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c) {
   constexpr float kGrown = 256.f;
-  float most = -INFINITY, s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f}, shift = a.m == -INFINITY ? 0.f : -a.m;
+  float most = -INFINITY, s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f}, shift = -a.m;
   auto weigh = [&](auto again, int j) {
     float x[M];
     values.template get<decltype(again)::value>(j, x);
@@ -462,7 +501,7 @@ __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c
   }
   // A maximum that has grown, NaN, infinities: once more beside the run's own maximum, and with
   // 0 for 0 times -infinity.
-  if (__builtin_amdgcn_ballot_w64(!(s[0] + s[1] < kGrown) || e[0] + e[1] != e[0] + e[1]) || a.m == -INFINITY) {
+  if (__builtin_amdgcn_ballot_w64(!(s[0] + s[1] < kGrown) || e[0] + e[1] != e[0] + e[1])) {
     auto each = [&](auto f) {
       if constexpr (Values::kFromMemory) {
 #pragma unroll 1
@@ -484,7 +523,7 @@ __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c
       });
     }
     a.move(fmaxf(a.m, wave_max(most) * c));
-    shift = a.m == -INFINITY ? 0.f : -a.m;
+    shift = -a.m;
     s[0] = s[1] = e[0] = e[1] = 0.f;
     each([&](int j) { weigh(std::integral_constant<bool, true>{}, j); });
   }
@@ -508,7 +547,7 @@ __device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
 }
 // Rows (WAVES = 1: a wave a row) and slices (4) of one run a lane: the logits stay in registers, so
 // candidates are taken from there.  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
-// in 16 slices each 9 us, and 5 for their join.
+// in 16 slices each 6.7 us, and 4.0 for their join.
 template <typename T, int WAVES, bool TOP>
 __global__ __launch_bounds__(256) void run_kernel(Params p) {
   constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
@@ -554,14 +593,16 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
   } else if constexpr (TOP) {
     tau = bound_of(best, p.top);
   }
+  Sums row;
+  if (whole) row = sums_of<T>(p, at.row, a);
   if (t == 0) {
-    if (whole) finish(p, at.row, a, given);
+    if (whole) finish(p, at.row, row, given);
     else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
   }
   if constexpr (TOP) {
     uint64_t* list = lists + own * kQueue;
-    if (whole && a.s != a.s) {
-      top_of_nan_row<T, NT>(p, at.row, a, lists);
+    if (whole && row.s != row.s) {
+      top_of_nan_row<T, NT>(p, at.row, row, lists);
       return;
     }
     const float tau_x = tau ? value_of(tau) : -INFINITY;
@@ -610,7 +651,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
       n = counts[own];
     }
     if (whole) {
-      select<NT>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, a, rank, key); });
+      select<NT>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, row, rank, key); });
     } else {
       uint64_t* out = p.keys + unit * p.top;
       select<NT>(list, n, p.top, [&](int rank, uint64_t key) { out[rank] = key; });
@@ -624,7 +665,11 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
 // keeps the largest of each of its runs (half an instruction a logit), as the upper half of its
 // order; the k-th largest of a wave's lanes bounds the k-th of the part, and the runs that reach
 // the bound, few more than `top`, are read again.
-// Bound by the bytes: 4096 rows of 131072 bf16 logits 191 us without a top (5.6 TB/s).
+// Bound by the bytes: 4096 rows of 131072 bf16 logits 187 us without a top (5.75 TB/s), 198 with one
+// of 5.  That the fifth wave picks is what hides it: candidates queued by the waves that stream
+// 287 us, a part's end in these waves 260.  Five workgroups a CU, in the registers of seven waves
+// a SIMD; four, without that bound, 209 us, six in the registers of eight 243.
+// Rows of which most is masked with -infinity take 340: their runs are weighed twice.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Params p, int64_t parts_n) {
   constexpr int VEC = Elem<T>::kVec, NT = 256, kStep = NT * kRun;
@@ -676,11 +721,15 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       if (lane == 0) parts[parity][0][wave] = a.m, parts[parity][1][wave] = a.s, parts[parity][2][wave] = a.e;
       if constexpr (TOP) bests[parity][t] = static_cast<uint16_t>(order_of_best(best) >> 16);
       __syncthreads();
-      if (!TOP && t == 0) {
+      if (!TOP && wave == 0) {
         a = waves_join(parts[parity]);
-        Given given;
-        if (p.slices == 1) given.load<T>(p, at.row), finish(p, at.row, a, given);
-        else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+        if (p.slices == 1) {
+          const Sums row = sums_of<T>(p, at.row, a);
+          Given given;
+          if (t == 0) given.load<T>(p, at.row), finish(p, at.row, row, given);
+        } else if (t == 0) {
+          p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
+        }
       }
     }
   } else if constexpr (TOP) {
@@ -693,12 +742,14 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       const float single = alone ? Elem<T>::load1(at.x + at.single(p, lane)) : -INFINITY;
       __syncthreads();  // the part has been streamed
       const Stats a = waves_join(parts[parity]);
+      Sums row;
+      if (whole) row = sums_of<T>(p, at.row, a);
       if (lane == 0) {
-        if (whole) finish(p, at.row, a, given);
+        if (whole) finish(p, at.row, row, given);
         else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
       }
-      if (whole && a.s != a.s) {
-        top_of_nan_row<T, 64>(p, at.row, a, nullptr);
+      if (whole && row.s != row.s) {
+        top_of_nan_row<T, 64>(p, at.row, row, nullptr);
         continue;
       }
       const uint32_t tau = bound_of(bests[parity], lane, p.top);
@@ -759,7 +810,7 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       }
       wave_sync();
       if (whole) {
-        select<64>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, a, rank, key); });
+        select<64>(list, n, p.top, [&](int rank, uint64_t key) { finish_top(p, at.row, row, rank, key); });
       } else {
         uint64_t* out = p.keys + unit * p.top;
         select<64>(list, n, p.top, [&](int rank, uint64_t key) { out[rank] = key; });
@@ -770,7 +821,7 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
   }
 }
 
-// Joins a row's slices; a wave a row.  Bound by the chain of its loads: 5 us for 16 rows.
+// Joins a row's slices; a wave a row.  Bound by the chain of its loads: 4 us for 16 rows.
 template <typename T>
 __global__ __launch_bounds__(64) void join_kernel(Params p) {
   constexpr int kHeld = 8;  // keys of a lane in registers
@@ -792,11 +843,11 @@ __global__ __launch_bounds__(64) void join_kernel(Params p) {
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) held[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
   a.move(wave_max(a.m));
-  a = wave_join(a);
-  if (lane == 0) finish(p, row, a, given);
+  const Sums sums = sums_of<T>(p, row, wave_join(a));
+  if (lane == 0) finish(p, row, sums, given);
   if (p.top == 0) return;
-  if (a.s != a.s) {
-    top_of_nan_row<T, 64>(p, row, a, nullptr);
+  if (sums.s != sums.s) {
+    top_of_nan_row<T, 64>(p, row, sums, nullptr);
     return;
   }
 #pragma unroll
@@ -815,7 +866,7 @@ __global__ __launch_bounds__(64) void join_kernel(Params p) {
   for (int i = 0; i < kHeld; ++i) take(held[i]);
   for (int i0 = 64 * kHeld; i0 < n; i0 += 64) take(i0 + lane < n ? keys[i0 + lane] : 0);
   wave_sync();
-  select<64>(list, count, p.top, [&](int rank, uint64_t key) { finish_top(p, row, a, rank, key); });
+  select<64>(list, count, p.top, [&](int rank, uint64_t key) { finish_top(p, row, sums, rank, key); });
 }
 
 // ---------------------------------------------------------------- gradient
@@ -1000,6 +1051,7 @@ extern "C" int ghip_token_logprobs(int dtype, const void* logits, int64_t row_st
   p.V = static_cast<int>(V);
   p.top = static_cast<int>(top);
   p.c = scale * logprobs::kLog2e;
+  p.scale = scale;
   p.logp = logp; p.entropy = entropy; p.lse = lse; p.top_logps = top_logps; p.top_ids = top_ids;
   p.slices = 1;
   const int64_t need = workspace ? ghip_token_logprobs_workspace_bytes(dtype, N, V, top) : 0;

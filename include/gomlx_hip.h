@@ -422,7 +422,7 @@ int ghip_kv4_append_rope(int dtype, const void* q, void* q_out, const void* k, c
  * BFLOAT16 and FLOAT32 within their range): k / v [B, Hkv, S, D], 16-byte aligned with strides of
  * whole 16 bytes; what a later chunk of a prompt gives ghip_sdpa_window_fwd.  Tokens from
  * lens[b] on (lens NULL: none) and those on a page outside [0, num_pages) are zeros.  At most
- * 65535 sequences. */
+ * 65535 sequences and as many heads. */
 int ghip_kv4_read(int dtype, const GHipKv4* k_cache, const GHipKv4* v_cache, void* k, void* v, int64_t B,
                   int64_t Hkv, int64_t S, int64_t D, int64_t num_pages, int64_t page_size,
                   int64_t max_pages, const int32_t* block_table, int64_t table_stride, const int32_t* lens,
@@ -430,7 +430,7 @@ int ghip_kv4_read(int dtype, const GHipKv4* k_cache, const GHipKv4* v_cache, voi
 
 /* ghip_sdpa_paged over a cache of 4 bits: the same tokens, window and sinks, workspace (of
  * ghip_sdpa_paged_kv4_workspace_bytes()) and limits, D a multiple of 32 up to 256 for every type
- * of q.  The cache's values enter the products exactly; q as the sum of one, two or three
+ * of q, strides of page and token below 4 GiB.  The cache's values enter the products exactly; q as the sum of one, two or three
  * bf16 values (BFLOAT16, FLOAT16, FLOAT32: all its bits), the weights as the sum of two, two or
  * three (16 or 24 bits).  Sums and statistics are fp32. */
 int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D,
@@ -465,7 +465,8 @@ int ghip_token_logprobs(int dtype, const void* logits, int64_t row_stride, const
  * NULL), the lse and (where d_entropy is given) the entropy that ghip_token_logprobs gave:
  *   d_logits_v = scale (d_logp ([v = id] - p_v) - d_entropy p_v (log p_v + entropy))
  * A row whose id is outside [0, V) has no logp (d_logp is not used there); rows of lse -infinity
- * get zeros.  d_logits [N, V] in the logits' type with a row stride of its own; it may be the
+ * get zeros.  (p is taken beside the lse that is given: from 2^24 on, as in rows of nothing but
+ * a large mask, it has no bits of log V, and p is 1.)  d_logits [N, V] in the logits' type with a row stride of its own; it may be the
  * logits themselves (the same stride), else they overlap nothing. */
 int ghip_token_logprobs_grad(int dtype, const void* logits, int64_t row_stride, const int32_t* ids,
                              const float* lse, const float* entropy, const float* d_logp,

@@ -267,3 +267,47 @@ def test_refusals_on_the_device(cuda):
     with pytest.raises(ValueError, match="out"):
         ops.token_logprobs_grad(x, ids, f, f, out=x[:2])
     assert ops.token_logprobs(x[:0], ids[:0], top=2)[4].shape == (0, 2)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("V", [300, 3001, 60001])
+@pytest.mark.parametrize("split", [True, False])
+def test_large_numbers_as_masks(cuda, dt, V, split):
+    """Rows of nothing but one large number, up to the type's lowest and largest, are even, as any
+    constant row (exponents of 0, a sum of V ones, exact below 2^24; its logarithm in base 2 and
+    the product with ln 2 are within 4 roundings); beside a lower one the largest has all of the
+    weight, and so has an ordinary one beside a large mask."""
+    low, high = torch.finfo(dt).min, torch.finfo(dt).max
+    fills = [low, high, -1e5, -1e10, -1e30, 3e20]
+    x = torch.empty((len(fills) + 2, V), device=cuda, dtype=dt)
+    for r, fill in enumerate(fills):
+        x[r] = fill
+    x[6], x[7] = low, -1e20
+    x[6, V // 3], x[7, V - 1] = high, 2.0
+    ids = torch.tensor([V - 1, 0, 1, V // 2, 5, 7, V // 3, V - 1], dtype=torch.int32, device=cuda)
+    logp, entropy, lse, top_logps, top_ids = ops.token_logprobs(x, ids, top=2, split=split)
+    even = torch.log(torch.tensor([V] * len(fills) + [1, 1], dtype=torch.float64))
+    near = 4 * 2.0 ** -24 * even
+    assert ((entropy.cpu().double() - even).abs() <= near).all()
+    assert ((logp.cpu().double() + even).abs() <= near).all()
+    assert ((top_logps[:, 0].cpu().double() + even).abs() <= near).all()
+    assert top_ids[:, 0].tolist() == [0] * len(fills) + [V // 3, V - 1]
+    most = x.double().amax(1).cpu()
+    assert ((lse.cpu().double() - (most + even)).abs() <= 4 * 2.0 ** -24 * (most.abs() + even)).all()
+
+
+@pytest.mark.parametrize("split", [True, False])
+@pytest.mark.parametrize("V", [600011, 1100003])
+def test_long_rows(cuda, V, split):
+    """Slices of several runs, and more runs than a lane has maxima apart: random, few values,
+    rising and falling rows, one token left, two equal tokens at the ends, a constant."""
+    at = torch.arange(V, device=cuda)
+    x, ids = logits_of(cuda, 7, V, BF16)
+    x[1] = (at * 7 % 5).to(BF16)
+    x[2], x[3] = (at.float() / V * 30).to(BF16), (at.float() / V * -30).to(BF16)
+    x[4], x[5], x[6] = -float("inf"), torch.finfo(BF16).min, -1.5
+    x[4, V // 2], x[5, 0], x[5, V - 1] = 1.0, 1.0, 1.0
+    ids[4], ids[5] = V // 2, V - 1
+    for top in (0, 1, 32):
+        check(x, ids, top, split=split)
+        check(x[:1], ids[:1], top, split=split)
