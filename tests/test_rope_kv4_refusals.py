@@ -88,6 +88,9 @@ REFUSED = [
     (paged4, dict(vc=cache(scales=PTR + 1)), 2, "codes must be"), (paged4, dict(kc=cache(scales=None)), 1, "null"),
     (paged4, dict(ts=-1), 1, "table stride"), (paged4, dict(size=1 << 20, per=1 << 20), 2, "at most"),
     (paged4, dict(B=1 << 14, H=1 << 10), 2, "fewer than 2\\^24 heads"),
+    (paged4, dict(kc=cache(cst=(1 << 32, 512, 32))), 2, "4 GiB"), (paged4, dict(vc=cache(cst=(4096, 512, 1 << 33))), 2, "4 GiB"),
+    (paged4, dict(vc=cache(sst=(1 << 32, 64, 4))), 2, "4 GiB"), (paged4, dict(kc=cache(sst=(64, 64, 1 << 32))), 2, "4 GiB"),
+    (read4, dict(Hkv=65536), 2, "too large"), (read4, dict(S=1 << 31, size=1 << 20, per=1 << 10), 2, "too large"),
     (paged4, dict(size=64, per=1024, ws=PTR, nbytes=64), 1, "workspace of"),
     (paged4, dict(size=64, per=1024, ws=PTR + 8, nbytes=1 << 30), 1, "workspace must be"),
     (logprobs, dict(dt=_lib.DT_FLOAT64), 2, "needs float32"), (logprobs, dict(V=0), 1, "bad sizes"), (logprobs, dict(N=-1), 1, "bad sizes"),
