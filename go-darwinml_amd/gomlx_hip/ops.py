@@ -514,6 +514,13 @@ def _new(like: torch.Tensor, shape, stream, dtype=None) -> torch.Tensor:
     return _empty(shape, dtype or like.dtype, like.device, stream)
 
 
+def _new_like(t: torch.Tensor, stream, dtype=None) -> torch.Tensor:
+    """_new of another tensor's shape, contiguous (at two thirds of its cost)."""
+    if stream is None:
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+    return _empty(t.shape, dtype or t.dtype, t.device, stream)
+
+
 def _rope(what: str, freqs, positions, sections, interleaved, B: int, S: int, D: int):
     """The GHipRope of a call on B sequences of S tokens (None: nothing is turned)."""
     if freqs is None:
@@ -553,7 +560,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections
         raise ValueError("rope: positions and freqs are needed")
     r = _rope("rope", freqs, positions, sections, interleaved, B, S, D)
     if out is None:
-        out = _new(x, (B, H, S, D), stream)
+        out = _new_like(x, stream)
     else:
         _like("rope: out", out, x.shape, x.dtype)
     _launch(dev, "ghip_rope", stream, dtype_code(x.dtype), x.data_ptr(), out.data_ptr(), B, H, S, D, _rows3("x", x),
@@ -574,7 +581,7 @@ def _new_tokens(what, q, k, v, q_out, stream):
     H = q.shape[1]
     _like(f"{what}: q", q, (B, H, S, D), k.dtype)
     if q_out is None:
-        q_out = _new(q, (B, H, S, D), stream)
+        q_out = _new_like(q, stream)
     else:
         _like(f"{what}: q_out", q_out, q.shape, q.dtype)
     return (B, H, Hkv, S, D), q_out, (_rows3("q", q), _rows3("q_out", q_out), _rows3("k", k), _rows3("v", v))
@@ -667,7 +674,8 @@ def kv4_read(k_cache, v_cache, block_table: torch.Tensor, tokens: int, lens=None
     _ints(f"{what}: lens", lens, B)
     shape = (B, Hkv, int(tokens), D)
     if outs is None:
-        k, v = _new(k_cache[0], shape, stream, dtype), _new(k_cache[0], shape, stream, dtype)
+        k = _new(k_cache[0], shape, stream, dtype)
+        v = _new_like(k, stream)
     else:
         k, v = outs
         _like(f"{what}: k", k, shape, k.dtype)
@@ -699,7 +707,7 @@ def sdpa_paged_kv4(q: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor,
     (kc, vc), (pages, size, per, ts) = _kv4(what, k_cache, v_cache, block_table, B, Hkv, D)
     _ints(f"{what}: lens", lens, B)
     if out is None:
-        out = _new(q, (B, H, D), stream)
+        out = _new_like(q, stream)
     else:
         _like(f"{what}: out", out, (B, H, D), q.dtype)
     (qb, qh, qd), (ob, oh, od) = q.stride(), out.stride()
@@ -747,9 +755,10 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, scale:
     N, V = logits.shape
     top = int(top)
     if outs is None:
-        f32 = torch.float32
-        outs = (_new(ids, (N,), stream, f32), _new(ids, (N,), stream, f32), _new(ids, (N,), stream, f32),
-                _new(ids, (N, top), stream, f32) if top > 0 else None, _new(ids, (N, top), stream) if top > 0 else None)
+        logp = _new_like(ids, stream, torch.float32)
+        best = _new(logp, (N, top), stream) if top > 0 else None
+        outs = (logp, _new_like(logp, stream), _new_like(logp, stream), best,
+                None if best is None else _new_like(best, stream, torch.int32))
     else:
         outs = tuple(outs)
         for i, (t, shape) in enumerate(zip(outs, ((N,), (N,), (N,), (N, top), (N, top)), strict=True)):
@@ -787,7 +796,7 @@ def token_logprobs_grad(logits: torch.Tensor, ids: torch.Tensor, lse: torch.Tens
             if not t.is_contiguous():
                 raise ValueError(f"{what}: {name} must be contiguous")
     if out is None:
-        out = _new(logits, (N, V), stream)
+        out = _new_like(logits, stream)
     else:
         _like(f"{what}: out", out, (N, V), logits.dtype)
         if out.stride(1) != 1 and V != 1:
