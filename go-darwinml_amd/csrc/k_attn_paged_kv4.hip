@@ -48,7 +48,7 @@ __device__ __forceinline__ int page_of(const Params& p, int n) {
 
 constexpr int kTile = 64;  // tokens of a tile
 
-// Waves that share the tiles of all sequences: eight a CU, four with rows of 128 bytes.
+// Waves that share the tiles of all sequences: eight a CU, four with rows of 128 bytes (registers).
 constexpr int workers(int DP) { return DP == 256 ? 1024 : 2048; }
 
 // A row of zeros: what lanes without a token load.
@@ -118,6 +118,12 @@ __device__ __forceinline__ uint32_t decode_byte(uint2 w, float s) {
 // LDS: 16 rows lie in the order 0, 4, 8, 12, 1, ..: the four that one read of V touches
 // are neighbours; their 16-byte chunks are exchanged so that a read of K by 16 lanes meets
 // every bank once.
+// Bound by the bytes and by what comes before and after them: bf16 D 128, 32 heads over 8, 64
+// sequences of up to 8192 tokens (291 MB) 66-71 us; a thousand tokens more each cost their bytes at
+// 5.7 TB/s, the rest, 12 us, is the launch, the chain lengths - pages - rows on cold caches
+// and the last tiles.  A tile is 500 instructions (66k of 120k cycles of a CU) beside 25k cycles
+// of matrix instructions.  Two LDS stages instead of one: 4% slower; three and four waves a
+// SIMD: 1% and 55% slower (their registers spill).
 template <typename T, int DP, bool SPLIT>
 __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p) {
   constexpr int kQ = Parts<T>::kQ, kP = Parts<T>::kP;
@@ -150,7 +156,8 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
   int worker = 0;
   if constexpr (SPLIT) {
     // Workgroups go to the eight XCDs in turn; each XCD takes neighbouring workers, so that heads
-    // whose rows share cache lines meet in one L2.
+    // whose rows share cache lines meet in one L2.  (Rows of all heads side by side, 64 x 8192
+    // tokens: 197 to 164 us by that alone; a head's rows side by side took the same either way.)
     const int64_t per = order.share();
     const int used = static_cast<int>((order.total + per - 1) / per), each = (used + 7) >> 3;
     worker = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3);

@@ -217,7 +217,10 @@ struct Slots {
 // A workgroup takes some tokens and all their rows, or, where the tokens are few, a share of
 // one token's rows: the angles are computed once for all of its heads.  FOUR: the rows of
 // keys and values go into 4 bits, by threads of their own share of a row.
-// Bound by the bytes of the rows, then, for a few tokens, by the chain position - angle - row.
+// Bound by the bytes of the rows, then, for a few tokens, by the chain position - angle - row:
+// 8192 tokens of 16 heads of 128 in bf16 (67 MB) 12.8 us, 8 prompts of 1024 tokens, 32 heads and
+// 8, into 16 bits (172 MB) 35.7 us, into 4 bits 38; 16 tokens 4.3 and 5.9.  Two rows of a thread
+// under way at once: 59 us for 35.7 (88 registers).
 template <typename T, int N, bool FOUR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
   __shared__ Shared sh;
