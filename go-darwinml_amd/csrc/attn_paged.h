@@ -70,25 +70,26 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
 }
 
 // Where the tiles of the sequences lie in the common order (sequence, unit of heads,
-// tile).  A lane counts one sequence of 64; a sequence has fewer than 2^26 tiles (the host
+// tile), with AHEAD places without a tile before each unit's.  A lane counts one sequence of 64; a sequence has fewer than 2^26 tiles (the host
 // checks), so 64 of them fit 32 bits.
-template <int KT, int WORKERS = kWorkers>
+template <int KT, int AHEAD = 0>
 struct Order {
-  int64_t total = 0;  // tiles of all sequences and units
+  int64_t total = 0;  // places of all sequences and units
   int lane, units;
   int len0;           // the first 64 sequences: lengths, tiles, running sums
   uint32_t n0, up0;
   __device__ __forceinline__ Order(const Common& p, int units_) : lane(threadIdx.x & 63), units(units_) {
     if (units == 0) return;
     len0 = lane < p.B ? p.lens[lane] : 0;
-    n0 = Seen(p, len0).tiles(KT);
+    n0 = places(Seen(p, len0).tiles(KT));
     up0 = wave_scan(n0);
     total = lane_of(up0, 63);
     for (int b0 = 64; b0 < p.B; b0 += 64) total += lane_of(wave_scan(count(p, b0 + lane)), 63);
     total *= units;
   }
+  static __device__ __forceinline__ uint32_t places(int tiles) { return AHEAD == 0 || tiles > 0 ? tiles + AHEAD : 0; }
   __device__ __forceinline__ uint32_t count(const Common& p, int b) const {
-    return b < p.B ? Seen(p, p.lens[b]).tiles(KT) : 0;
+    return b < p.B ? places(Seen(p, p.lens[b]).tiles(KT)) : 0;
   }
   __device__ __forceinline__ int length(const Common& p, int b) const {
     return b < 64 ? static_cast<int>(lane_of(static_cast<uint32_t>(len0), b)) : p.lens[b];
@@ -116,7 +117,7 @@ struct Order {
       before += lane_of(up, 63);
     }
   }
-  __device__ __forceinline__ int64_t share() const { return share_of(total, WORKERS); }
+  __device__ __forceinline__ int64_t share() const { return share_of(total); }
 };
 
 // a / b of non-negative values, in 32 bits where they fit.
@@ -125,53 +126,41 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return a / b;
 }
 
-// Joins the shares of units that several workers hold: a workgroup a (sequence, head),
-// the shares dealt out over groups of lanes that each hold a row of the output and a
-// running maximum; the groups are added in order.  Sequences without a visible token,
-// which no worker holds, get zeros.
-// Bound by the latency of lengths, then shares: 4.8 us for 8 x 32 heads, 6 us for 64 x 32.
-template <typename T, int DP, int KT, int WORKERS, int NT = 256>
-__global__ __launch_bounds__(NT) void join_kernel(Common p) {
-  constexpr int kLanes = DP / 4, kGroups = NT / kLanes, kAhead = 4;
+// A row of the output (PARTS = 1; else columns of it, by the workgroup's number) from its n
+// shares, share i in slot(i): they are dealt out over groups of lanes that each hold the columns
+// and a running maximum; the groups are added in order.
+template <typename T, int DP, int NT, int PARTS, int AHEAD, typename Slot>
+__device__ __forceinline__ void join_shares(const Common& p, T* row, int n, const Slot& slot) {
+  constexpr int kCols = DP / PARTS, kLanes = kCols / 4, kGroups = NT / kLanes;
   __shared__ float stat[2][kGroups];
-  __shared__ __attribute__((aligned(16))) float sums[kGroups][DP];
-  const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
-  const int row = blockIdx.x, b = row / p.H, h = row % p.H, hk = h / G;
-  const int unit = hk * blocks + (h - hk * G) / kHeads, hd = (h - hk * G) % kHeads;
-  const int d = threadIdx.x % kLanes * 4, grp = threadIdx.x / kLanes;
-  T* out = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh + d;
-  const Order<KT, WORKERS> order(p, units);
-  const int nt = Seen(p, order.length(p, b)).tiles(KT);
-  if (nt == 0) {
+  __shared__ __attribute__((aligned(16))) float sums[kGroups][kCols];
+  const int col = threadIdx.x % kLanes * 4, grp = threadIdx.x / kLanes;
+  const int d = PARTS == 1 ? col : static_cast<int>(blockIdx.x % PARTS) * kCols + col;
+  T* out = row + d;
+  if (n == 0) {
     if (grp == 0 && d < p.D) tile::store4(out, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  const int64_t per = order.share(), u0 = order.begin(p, b) + static_cast<int64_t>(unit) * nt;
-  const int w0 = static_cast<int>(quotient(u0, per)), n = static_cast<int>(quotient(u0 + nt - 1, per)) - w0 + 1;
   if (n == 1) return;
-  // The unit's share in worker w0 + i: its first piece, but for a worker that began before.
-  auto slot = [&](int i) {
-    return (2 * static_cast<int64_t>(w0 + i) + (i == 0 && u0 != w0 * per ? 1 : 0)) * p.unit_heads + hd;
-  };
   float a[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, sum = 0.f;
-  for (int i0 = grp; i0 < n; i0 += kAhead * kGroups) {  // kAhead shares' loads in flight
-    float ls[kAhead];
-    float4 v[kAhead];
+  for (int i0 = grp; i0 < n; i0 += AHEAD * kGroups) {  // AHEAD shares' loads in flight
+    float ls[AHEAD];
+    float4 v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
+    for (int j = 0; j < AHEAD; ++j) {
       const int i = i0 + j * kGroups;
       ls[j] = i < n ? p.part_lse[slot(i)] : -INFINITY;
       v[j] = i < n && d < p.D ? *reinterpret_cast<const float4*>(p.part_o + slot(i) * p.D + d) : make_float4(0, 0, 0, 0);
     }
     float m = mx;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) m = fmaxf(m, ls[j]);
+    for (int j = 0; j < AHEAD; ++j) m = fmaxf(m, ls[j]);
     const float old = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - m);
     sum *= old;
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] *= old;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
+    for (int j = 0; j < AHEAD; ++j) {
       const float f = ls[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ls[j] - m);  // (NaN stays NaN)
       sum += f;
       a[0] += f * v[j].x;
@@ -181,7 +170,7 @@ __global__ __launch_bounds__(NT) void join_kernel(Common p) {
     }
     mx = m;
   }
-  *reinterpret_cast<float4*>(&sums[grp][d]) = make_float4(a[0], a[1], a[2], a[3]);
+  *reinterpret_cast<float4*>(&sums[grp][col]) = make_float4(a[0], a[1], a[2], a[3]);
   if (threadIdx.x % kLanes == 0) {
     stat[0][grp] = mx;
     stat[1][grp] = sum;
@@ -196,7 +185,7 @@ __global__ __launch_bounds__(NT) void join_kernel(Common p) {
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const float f = stat[0][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[0][i] - m);
-    const float4 v = *reinterpret_cast<const float4*>(&sums[i][d]);
+    const float4 v = *reinterpret_cast<const float4*>(&sums[i][col]);
     sum += f * stat[1][i];
     a[0] += f * v.x;
     a[1] += f * v.y;

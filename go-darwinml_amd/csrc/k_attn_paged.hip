@@ -317,13 +317,32 @@ __global__ __launch_bounds__(64, 1) void attend_kernel(Params p) {
   }
 }
 
+// Joins the shares of units that several workers hold; a workgroup a (sequence, head).
+// Sequences without a visible token, which no worker holds, get zeros.
+// Bound by the latency of lengths, then shares: 4.8 us for 8 x 32 heads, 6 us for 64 x 32.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void join_kernel(Params p) {
+  constexpr int KT = 8192 / (DP * static_cast<int>(sizeof(T)));
+  const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
+  const int row = blockIdx.x, b = row / p.H, h = row % p.H, hk = h / G;
+  const int unit = hk * blocks + (h - hk * G) / kHeads, hd = (h - hk * G) % kHeads;
+  const Order<KT> order(p, units);
+  const int nt = Seen(p, order.length(p, b)).tiles(KT);
+  const int64_t per = order.share(), u0 = order.begin(p, b) + static_cast<int64_t>(unit) * nt;
+  const int w0 = static_cast<int>(quotient(u0, per));
+  const int n = nt == 0 ? 0 : static_cast<int>(quotient(u0 + nt - 1, per)) - w0 + 1;
+  // The unit's share in worker w0 + i: its first piece, but for a worker that began before.
+  join_shares<T, DP, 256, 1, 4>(p, static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh, n, [&](int i) {
+    return (2 * static_cast<int64_t>(w0 + i) + (i == 0 && u0 != w0 * per ? 1 : 0)) * p.unit_heads + hd;
+  });
+}
+
 template <typename T, int DP>
 static void launch_d(const Params& p, hipStream_t s) {
-  constexpr int KT = 8192 / (DP * static_cast<int>(sizeof(T)));
   const int G = p.H / p.Hkv, units = p.Hkv * ((G + kHeads - 1) / kHeads);
   if (p.part_o) {
     hipLaunchKernelGGL((attend_kernel<T, DP, true>), dim3(kWorkers), dim3(64), 0, s, p);
-    hipLaunchKernelGGL((join_kernel<T, DP, KT, kWorkers>), dim3(static_cast<unsigned>(p.B * p.H)), dim3(256), 0, s, static_cast<const Common&>(p));
+    hipLaunchKernelGGL((join_kernel<T, DP>), dim3(static_cast<unsigned>(p.B * p.H)), dim3(256), 0, s, p);
   } else {
     hipLaunchKernelGGL((attend_kernel<T, DP, false>), dim3(static_cast<unsigned>(p.B * units)), dim3(64), 0, s, p);
   }

@@ -34,17 +34,9 @@ struct Rows {
 
 struct Params : Common {
   Rows k, v;
-  uint32_t page_mul;  // a token's page: page_of()
-  int page_shift;
+  Pages pages;  // of page_size tokens
+  int2* held;   // [B][units]: slot of a unit's first share, number of its shares
 };
-
-// n / page_size of 0 <= n < 2^31, by the product with a 33-bit reciprocal: with shift =
-// ceil(log2 d) and mul = floor(2^32 (2^shift - d) / d) + 1 the quotient is exact (Granlund and
-// Montgomery).  A division costs 25 instructions, two of them a tile of 64 tokens 7% of it.
-__device__ __forceinline__ int page_of(const Params& p, int n) {
-  const uint32_t t = __umulhi(p.page_mul, static_cast<uint32_t>(n));
-  return static_cast<int>((t + ((static_cast<uint32_t>(n) - t) >> min(p.page_shift, 1))) >> max(p.page_shift - 1, 0));
-}
 
 constexpr int kTile = 64;  // tokens of a tile
 
@@ -152,19 +144,18 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
 
   int b;
   int64_t at, end, begin;
-  const Order<kTile, workers(DP)> order(p, SPLIT ? units : 0);
-  int worker = 0;
+  const Order<kTile, kBegin> order(p, SPLIT ? units : 0);
+  int worker = 0, used = 0;
   if constexpr (SPLIT) {
     // Workgroups go to the eight XCDs in turn; each XCD takes neighbouring workers, so that heads
     // whose rows share cache lines meet in one L2.  (Rows of all heads side by side, 64 x 8192
     // tokens: 197 to 164 us by that alone; a head's rows side by side took the same either way.)
-    const int64_t per = order.share();
-    const int used = static_cast<int>((order.total + per - 1) / per), each = (used + 7) >> 3;
+    used = used_of(order.total, workers(DP));
+    const int each = (used + 7) >> 3;
     worker = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3);
-    if (static_cast<int>(blockIdx.x >> 3) >= each) return;
-    at = worker * per;
-    end = min(order.total, at + per);
-    if (at >= end) return;
+    if (static_cast<int>(blockIdx.x >> 3) >= each || worker >= used || order.total == 0) return;
+    at = first_of<workers(DP)>(worker, order.total, used);
+    end = first_of<workers(DP)>(worker + 1, order.total, used);
     b = order.find(p, at, &begin);
   } else {
     b = blockIdx.x / units;
@@ -176,11 +167,16 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
   for (;;) {
     const Seen seen(p, SPLIT ? order.length(p, b) : p.lens[b]);
     const int nt = seen.tiles(kTile), nst = seen.sink_tiles(kTile);
-    int unit, ta, te;
+    int unit, ta, te, taken = 0;
     if constexpr (SPLIT) {
-      unit = static_cast<int>(quotient(at - begin, nt));
-      ta = static_cast<int>(at - begin - static_cast<int64_t>(unit) * nt);
-      te = static_cast<int>(min(static_cast<int64_t>(nt), ta + (end - at)));
+      const int nv = nt + kBegin;
+      unit = static_cast<int>(quotient(at - begin, nv));
+      const int from = static_cast<int>(at - begin - static_cast<int64_t>(unit) * nv);
+      const int to = static_cast<int>(min(static_cast<int64_t>(nv), from + (end - at)));
+      taken = to - from;
+      ta = max(0, from - kBegin);
+      te = to - kBegin;
+      if (te <= 0) return;  // (nothing but the unit's beginning: the end of this worker's part)
     } else {
       unit = blockIdx.x % units;
       ta = 0;
@@ -188,6 +184,14 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     }
     const int hk = unit / blocks, h0 = hk * G + (unit % blocks) * kHeads;
     const int heads = min(kHeads, (hk + 1) * G - h0);
+    if constexpr (SPLIT) {
+      // (For the join, which would else have to find the unit's place among all sequences.)
+      if (ta == 0 && lane == 0) {
+        const int64_t last = begin + static_cast<int64_t>(unit + 1) * (nt + kBegin) - 1;
+        const int n = worker_of(last, order.total, used) - worker + 1;
+        p.held[static_cast<int64_t>(b) * units + unit] = make_int2(2 * worker + (at == first ? 0 : 1), n);
+      }
+    }
 
     const int32_t* table = p.table + b * p.table_stride;
     const char* kc = p.k.codes + hk * p.k.sh;
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
 
     auto token0 = [&](int t) { return t < nst ? t * kTile : (seen.lo & ~15) + (t - nst) * kTile; };
     auto issue_pages = [&](int t, int slot) {
-      const int entry = min(page_of(p, token0(t) + lane), p.max_pages - 1);
+      const int entry = min(p.pages.quotient(token0(t) + lane), p.max_pages - 1);
       tile::load4(table + entry, pa0 + slot * 256);
     };
     // The DMA of tile t, its page numbers landed; returns its rows that hold a token.  A lane finds
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     auto issue = [&](int t, int slot) -> uint64_t {  // (page numbers from `slot`)
       const int tok = token0(t) + lane;
       const int page = page_lds[slot][lane];
-      const uint32_t off = tok - page_of(p, tok) * p.page_size;
+      const uint32_t off = tok - p.pages.quotient(tok) * p.page_size;
       // No branches here: where lanes part, the compiler has put copies of registers in front of the
       // instruction that brings all lanes back, and those of the lanes that had left were lost.
       const int from = t < nst ? 0 : seen.lo, to = t < nst ? seen.ns : seen.len;
@@ -429,11 +433,29 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
     if constexpr (!SPLIT) {
       return;
     } else {
-      at += te - ta;
+      at += taken;
       if (at >= end) return;
-      if (at - begin >= static_cast<int64_t>(nt) * units) b = order.find(p, at, &begin);
+      if (at - begin >= static_cast<int64_t>(nt + kBegin) * units) b = order.find(p, at, &begin);
     }
   }
+}
+
+// Joins the shares of units that several workers hold: a workgroup a (sequence, head) and one of
+// PARTS column ranges.  Sequences without a visible token, which no worker holds, get zeros.
+// Bound by the latency of a unit's place, then of its shares.
+template <typename T, int DP, int PARTS, int AHEAD>
+__global__ __launch_bounds__(256) void join4_kernel(Params p) {
+  const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
+  const int row = blockIdx.x / PARTS, b = row / p.H, h = row % p.H, hk = h / G;
+  const int unit = hk * blocks + (h - hk * G) / kHeads, hd = (h - hk * G) % kHeads;
+  const int len = p.lens[b];
+  const int2 held = p.held[static_cast<int64_t>(b) * units + unit];
+  // The first share is where the worker that began the unit says, the others are in the first slots
+  // of the workers after it.
+  paged::join_shares<T, DP, 256, PARTS, AHEAD>(
+      p, static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh, Seen(p, len).tiles(kTile) == 0 ? 0 : held.y, [&](int i) {
+        return static_cast<int64_t>(i == 0 ? held.x : (held.x & ~1) + 2 * i) * p.unit_heads + hd;
+      });
 }
 
 template <typename T, int DP>
@@ -441,11 +463,10 @@ static void launch_d(const Params& p, hipStream_t s) {
   const int G = p.H / p.Hkv, units = p.Hkv * ((G + kHeads - 1) / kHeads);
   if (p.part_o) {
     hipLaunchKernelGGL((attend4_kernel<T, DP, true>), dim3(workers(DP)), dim3(64), 0, s, p);
-    // (Few rows have many shares each: 256 of 32 heads' one long sequence, 8.8 us with 256 threads.)
-    const dim3 rows(static_cast<unsigned>(p.B * p.H));
-    const Common& c = p;
-    if (p.B * p.H <= 256) hipLaunchKernelGGL((paged::join_kernel<T, DP, kTile, workers(DP), 1024>), rows, dim3(1024), 0, s, c);
-    else hipLaunchKernelGGL((paged::join_kernel<T, DP, kTile, workers(DP)>), rows, dim3(256), 0, s, c);
+    const unsigned rows = static_cast<unsigned>(p.B * p.H);
+    constexpr int kParts = DP / 32;
+    if (rows <= 128) hipLaunchKernelGGL((join4_kernel<T, DP, kParts, 8>), dim3(rows * kParts), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((join4_kernel<T, DP, 1, 4>), dim3(rows), dim3(256), 0, s, p);
   } else {
     hipLaunchKernelGGL((attend4_kernel<T, DP, false>), dim3(static_cast<unsigned>(p.B * units)), dim3(64), 0, s, p);
   }
@@ -480,7 +501,8 @@ extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int
   const double units = static_cast<double>(B) * static_cast<double>(Hkv) * static_cast<double>((heads + paged::kHeads - 1) / paged::kHeads);
   const double tokens = static_cast<double>(page_size) * static_cast<double>(max_pages);
   if (tokens <= paged4::kTile * (units >= 1024 ? 24. : units >= 512 ? 12. : 6.)) return 0;
-  return 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4;
+  return 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4 +
+         8 * B * Hkv * ((heads + paged::kHeads - 1) / paged::kHeads);
 }
 
 extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_cache, const GHipKv4* v_cache, void* o,
@@ -559,8 +581,7 @@ extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_ca
   p.window = static_cast<int>(window == 0 || window > kMost ? kMost : window);
   p.sinks = static_cast<int>(sinks > kMost ? kMost : sinks);
   p.scale = scale;
-  while (int64_t{1} << p.page_shift < page_size) ++p.page_shift;
-  p.page_mul = static_cast<uint32_t>(((static_cast<uint64_t>((int64_t{1} << p.page_shift) - page_size)) << 32) / static_cast<uint64_t>(page_size) + 1);
+  p.pages = paged4::Pages(page_size);
   p.unit_heads = static_cast<int>(std::min<int64_t>(paged::kHeads, H / Hkv));
   const int64_t need = workspace ? ghip_sdpa_paged_kv4_workspace_bytes(B, H, Hkv, D, page_size, max_pages) : 0;
   if (need > 0) {
@@ -569,7 +590,9 @@ extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_ca
                        static_cast<long long>(workspace_bytes), static_cast<long long>(need));
     if (!al(workspace, 16)) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", kWhat);
     p.part_o = static_cast<float*>(workspace);
-    p.part_lse = p.part_o + 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * p.unit_heads * D;
+    const int64_t shares = 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * p.unit_heads;
+    p.part_lse = p.part_o + shares * D;
+    p.held = reinterpret_cast<int2*>(p.part_lse + shares);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (f32) paged4::launch<float>(p, s);

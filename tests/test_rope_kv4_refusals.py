@@ -133,10 +133,10 @@ def test_workspaces():
     assert ws(BF16, 1024, 131072, 20) == 0 and ws(BF16, 1, 2000, 5) == 0 and ws(BF16, 1, 131072, 33) == 0
     assert ws(BF16, 1, 1 << 30, 1) == 64 * 24 and ws(BF16, 0, 131072, 1) == 0
     ws = L.ghip_sdpa_paged_kv4_workspace_bytes
-    assert ws(16, 32, 8, 128, 64, 6) == 0 and ws(16, 32, 8, 128, 64, 7) == 2 * 2048 * 4 * 129 * 4
+    assert ws(16, 32, 8, 128, 64, 6) == 0 and ws(16, 32, 8, 128, 64, 7) == 2 * 2048 * 4 * 129 * 4 + 16 * 8 * 8
     assert ws(64, 32, 8, 128, 64, 12) == 0 and ws(64, 32, 8, 128, 64, 13) > 0
     assert ws(128, 32, 8, 128, 64, 24) == 0 and ws(128, 32, 8, 128, 64, 25) > 0
-    assert ws(0, 32, 8, 128, 64, 100) == 0 and ws(1, 8, 8, 256, 64, 100) == 2 * 1024 * 257 * 4
+    assert ws(0, 32, 8, 128, 64, 100) == 0 and ws(1, 8, 8, 256, 64, 100) == 2 * 1024 * 257 * 4 + 8 * 8
 
 
 def test_host_tensors_are_refused():
