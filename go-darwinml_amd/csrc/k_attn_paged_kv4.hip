@@ -111,9 +111,9 @@ __device__ __forceinline__ uint32_t decode_byte(uint2 w, float s) {
 // are neighbours; their 16-byte chunks are exchanged so that a read of K by 16 lanes meets
 // every bank once.
 // Bound by the bytes and by what comes before and after them: bf16 D 128, 32 heads over 8, 64
-// sequences of up to 8192 tokens (291 MB) 66-71 us; a thousand tokens more each cost their bytes at
-// 5.7 TB/s, the rest, 12 us, is the launch, the chain lengths - pages - rows on cold caches
-// and the last tiles.  A tile is 500 instructions (66k of 120k cycles of a CU) beside 25k cycles
+// sequences of up to 8192 tokens (291 MB) 62 us; a thousand tokens more each cost their bytes at
+// 5.6 TB/s, the rest, 10 us, is the launch, the chain lengths - pages - rows on cold caches
+// and the last tiles.  A tile is 500 instructions (67k of 119k cycles of a CU) beside 25k cycles
 // of matrix instructions.  Two LDS stages instead of one: 4% slower; three and four waves a
 // SIMD: 1% and 55% slower (their registers spill).
 template <typename T, int DP, bool SPLIT>
@@ -442,7 +442,8 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
 
 // Joins the shares of units that several workers hold: a workgroup a (sequence, head) and one of
 // PARTS column ranges.  Sequences without a visible token, which no worker holds, get zeros.
-// Bound by the latency of a unit's place, then of its shares.
+// Bound by the latency of a unit's place, then of its shares: 5.2 us for 64 x 32 rows.  Few rows have
+// many shares each: 32 of one long sequence, 256 each, 4.9 us in four parts, 10 in one.
 template <typename T, int DP, int PARTS, int AHEAD>
 __global__ __launch_bounds__(256) void join4_kernel(Params p) {
   const int G = p.H / p.Hkv, blocks = (G + kHeads - 1) / kHeads, units = p.Hkv * blocks;
@@ -487,11 +488,11 @@ using namespace ghip;
 // or more, 24 with 1024.  (The second kernel costs 5-7 us; a wave alone takes 1.4 us a tile.)
 // bf16 D 128, 32 heads over 8, sequences of one length, us a call in a graph, split / unsplit:
 //   units      4 tiles      6           8           12          16          24          32
-//   8          12.1 / 8.8   12.2 / 11.7 12.1 / 14.3 12.3 / 19.9 12.2 / 25.2 12.3 / 35.9 12.4 / 46.9
-//   256        12.6 / 9.3   13.2 / 12.0 13.7 / 14.8 16.5 / 20.4 17.7 / 26.3 20.9 / 37.2 23.4 / 48.0
-//   512        15.6 / 9.7   18.0 / 12.5 19.1 / 16.2 22.5 / 21.7 25.0 / 27.2 30.4 / 39.0 34.7 / 49.4
-//   1024       24.1 / 11.6  27.2 / 14.7 29.7 / 17.5 34.3 / 23.3 39.3 / 29.0 48.9 / 40.5 59.9 / 52.3
-//   2048       38.4 / 17.1  42.9 / 21.9 47.6 / 26.7 57.7 / 37.3 67.4 / 47.2 101 / 80.6  127 / 105
+//   8          11.8 / 8.8   11.8 / 11.6 11.9 / 14.3 11.9 / 19.9 11.8 / 25.3 12.0 / 36.1 11.9 / 46.8
+//   256        12.3 / 9.2   12.9 / 11.8 15.1 / 14.8 16.4 / 20.2 18.9 / 26.1 22.5 / 36.9 24.7 / 47.7
+//   512        16.3 / 9.6   17.4 / 12.3 19.8 / 16.1 23.0 / 21.9 25.7 / 27.3 31.1 / 39.0 35.2 / 49.4
+//   1024       22.7 / 11.7  26.0 / 14.7 28.6 / 17.5 33.1 / 23.4 38.1 / 28.9 47.8 / 40.2 59.2 / 52.4
+//   2048       30.3 / 17.2  34.4 / 21.7 39.6 / 26.5 48.8 / 36.4 59.6 / 47.3 93.5 / 81.0 119 / 105
 // (Beyond, sequences of one length would still run faster unsplit with 1024 units and more; the
 // rule does not know the lengths, and one long sequence would keep the others waiting.)
 extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page_size,
