@@ -76,15 +76,31 @@ __device__ __forceinline__ void prepare(const Params& p, Shared& sh, int64_t fir
   __syncthreads();
 }
 
+// N elements, aligned to N.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Few {
+  T v[N];
+};
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
-  if constexpr (N == 1) x[0] = Elem<T>::load1(p);
-  else load_vec(p, x);
+  if constexpr (N == Elem<T>::kVec) {
+    load_vec(p, x);
+  } else {
+    const Few<T, N> few = *reinterpret_cast<const Few<T, N>*>(p);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = Elem<T>::load1(&few.v[e]);
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
-  if constexpr (N == 1) Elem<T>::store1(p, x[0]);
-  else store_vec(p, x);
+  if constexpr (N == Elem<T>::kVec) {
+    store_vec(p, x);
+  } else {
+    Few<T, N> few;
+#pragma unroll
+    for (int e = 0; e < N; ++e) Elem<T>::store1(&few.v[e], x[e]);
+    *reinterpret_cast<Few<T, N>*>(p) = few;
+  }
 }
 
 // Rows of whole elements.  A thread holds N pairs of a row, as two runs of N elements: run
@@ -352,10 +368,19 @@ static void plan(Params& p, bool four) {
   }
 }
 
+// Elements that a thread takes at a time: 16 bytes or the most that alignment and half of the pairs
+// allow.  (bf16, 4 x 16 heads of 80, 40 of them turned: 33 us one by one, 14 four by four.)
+static int width(const Params& p, uint64_t bits, int most, int64_t es) {
+  int n = most;
+  while (n > 1 && (bits % static_cast<uint64_t>(n * es) || p.D % n || p.a.half % n)) n /= 2;
+  return n;
+}
+
 template <typename T, bool FOUR>
-static int launch(Params& p, bool wide, bool wide4, hipStream_t s, GHipError* err, const char* what) {
+static int launch(Params& p, uint64_t bits, bool wide4, hipStream_t s, GHipError* err, const char* what) {
   constexpr int V = Elem<T>::kVec;
-  const int n = wide ? V : 1;
+  int n = width(p, bits, V, sizeof(T));
+  if (FOUR && n < V) n = 1;
   p.units = (p.D + 2 * n - 1) / (2 * n);  // (half a row's pairs are a multiple of n)
   p.units4 = p.D / 8;
   plan(p, FOUR);
@@ -363,12 +388,14 @@ static int launch(Params& p, bool wide, bool wide4, hipStream_t s, GHipError* er
   if (blocks > kMostGroups) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", what);
   const dim3 grid(static_cast<unsigned>(blocks));
   if constexpr (FOUR) {
-    if (wide && wide4) hipLaunchKernelGGL((rope_kernel<T, V, true, true>), grid, dim3(kThreads), 0, s, p);
-    else if (wide) hipLaunchKernelGGL((rope_kernel<T, V, true, false>), grid, dim3(kThreads), 0, s, p);
+    if (n == V && wide4) hipLaunchKernelGGL((rope_kernel<T, V, true, true>), grid, dim3(kThreads), 0, s, p);
+    else if (n == V) hipLaunchKernelGGL((rope_kernel<T, V, true, false>), grid, dim3(kThreads), 0, s, p);
     else if (wide4) hipLaunchKernelGGL((rope_kernel<T, 1, true, true>), grid, dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL((rope_kernel<T, 1, true, false>), grid, dim3(kThreads), 0, s, p);
   } else {
-    if (wide) hipLaunchKernelGGL((rope_kernel<T, V, false, false>), grid, dim3(kThreads), 0, s, p);
+    if (n == V) hipLaunchKernelGGL((rope_kernel<T, V, false, false>), grid, dim3(kThreads), 0, s, p);
+    else if (V == 8 && n == 4) hipLaunchKernelGGL((rope_kernel<T, V / 2, false, false>), grid, dim3(kThreads), 0, s, p);
+    else if (n == 2) hipLaunchKernelGGL((rope_kernel<T, 2, false, false>), grid, dim3(kThreads), 0, s, p);
     else hipLaunchKernelGGL((rope_kernel<T, 1, false, false>), grid, dim3(kThreads), 0, s, p);
   }
   GHIP_CHECK(hipGetLastError(), err);
@@ -463,15 +490,14 @@ bool take(R& r, const void* ptr, const int64_t* st, const int64_t (&n)[3], int64
 
 int launch_rope(int dtype, rope::Params& p, uint64_t bits, uint64_t bits4, bool four, hipStream_t s, GHipError* err,
                 const char* what) {
-  const int64_t es = elem(dtype), V = 16 / es;
+  const int64_t es = elem(dtype);
   if ((bits | bits4) % es) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: pointers are not aligned to elements", what);
-  const bool wide = bits % 16 == 0 && p.D % V == 0 && p.a.half % V == 0;
   const bool wide4 = bits4 % 16 == 0 && (p.a.neighbours ? p.R % 8 == 0 : p.a.half % 8 == 0);
   if (dtype == GHIP_DTYPE_FLOAT32)
-    return four ? rope::launch<float, true>(p, wide, wide4, s, err, what) : rope::launch<float, false>(p, wide, false, s, err, what);
+    return four ? rope::launch<float, true>(p, bits, wide4, s, err, what) : rope::launch<float, false>(p, bits, false, s, err, what);
   if (dtype == GHIP_DTYPE_FLOAT16)
-    return four ? rope::launch<f16_t, true>(p, wide, wide4, s, err, what) : rope::launch<f16_t, false>(p, wide, false, s, err, what);
-  return four ? rope::launch<bf16_t, true>(p, wide, wide4, s, err, what) : rope::launch<bf16_t, false>(p, wide, false, s, err, what);
+    return four ? rope::launch<f16_t, true>(p, bits, wide4, s, err, what) : rope::launch<f16_t, false>(p, bits, false, s, err, what);
+  return four ? rope::launch<bf16_t, true>(p, bits, wide4, s, err, what) : rope::launch<bf16_t, false>(p, bits, false, s, err, what);
 }
 
 // A 4-bit cache's tensors; false and the error set if they are not as the kernels read them.

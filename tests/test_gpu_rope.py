@@ -132,3 +132,26 @@ def test_refusals_on_the_device(cuda):
     with pytest.raises(BackendError, match="rotary_dim"):
         ops.rope(x, pos, freqs_of(33, cuda))
     assert ops.rope(x[:, :, :0], pos[:, :0], freqs).shape == (2, 4, 0, 64)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("D,R", [(64, 64), (80, 40), (36, 36), (20, 8), (12, 4)])
+def test_every_width(cuda, dt, D, R):
+    """Rows and outputs that begin 0, 1, 2, 4 and 8 elements into their memory, at strides of as many
+    more than D: the same bits however many elements a thread takes, nothing else written."""
+    B, H, S = 2, 3, 5
+    x, pos, freqs = rand(cuda, B, H, S, D, dt=dt), positions_of(cuda, 1, B, S), freqs_of(R // 2, cuda)
+    for inter in (False, True):
+        want, bound = ref.rotate(x, pos, freqs, None, inter)
+        first = None
+        for a in (0, 1, 2, 4, 8):
+            for b in (0, 1, 2, 4, 8):
+                source, room = (torch.full((B * H * S * (D + n) + n,), 7.0, dtype=dt, device=cuda) for n in (a, b))
+                rows = source[a:].view(B, H, S, D + a)[..., :D]
+                rows.copy_(x)
+                out = room[b:].view(B, H, S, D + b)[..., :D]
+                ops.rope(rows, pos, freqs, interleaved=inter, out=out)
+                first = out.clone() if first is None else first
+                assert torch.equal(out, first), (a, b)
+                assert (room[:b] == 7.0).all() and (room[b:].view(B, H, S, D + b)[..., D:] == 7.0).all()
+        attention_ref.within(first, want, bound)
