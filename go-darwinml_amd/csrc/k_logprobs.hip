@@ -887,7 +887,7 @@ struct Grad {
 // d_v = p_v (A + B t_v) + [v = id] C with t = x - lse, p = e^t, A = -scale (g + h entropy),
 // B = -scale h, C = scale g.  WAVES = 4: a workgroup takes a run of a row; 1: a wave a row.
 // Bound by the bytes: 8192 rows of 32000 bf16 logits (1.05 GB) 190 us, 5.5 TB/s.
-template <typename T, int WAVES, bool WIDE>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
   const int wave = threadIdx.x >> 6, t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -909,41 +909,36 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
     const float u = __builtin_fmaf(x, p.scale, -lse), w = __builtin_amdgcn_exp2f(u * kLog2e);
     return none ? 0.f : w * __builtin_fmaf(B, fmaxf(u, kFar), A);
   };
-  if constexpr (!WIDE) {
-    for (int i = run * NT * 8 + t, end = min(p.V, WAVES == 1 ? p.V : (run + 1) * NT * 8); i < end; i += NT) {
-      const float d = value(Elem<T>::load1(X + i));
-      Elem<T>::store1(D + i, i == id && !none ? d + C : d);
-    }
-  } else {
-    const int head = min(static_cast<int>((-reinterpret_cast<uintptr_t>(xb) & 15) / sizeof(T)), p.V);
-    const int nv = (p.V - head) / VEC, rest = p.V - nv * VEC;
-    if (run == 0 && t < rest) {
-      const int i = t < head ? t : p.V - rest + t;
-      const float d = value(Elem<T>::load1(X + i));
-      Elem<T>::store1(D + i, i == id && !none ? d + C : d);
-    }
-    const int at_id = id >= head && !none ? id - head : -1;
-    for (int v0 = run * NT * kRun; v0 < nv; v0 += NT * kRun) {
-      uint4 raw[kRun];
+  // (Vectors as the gradient's row lies; the logits' may lie otherwise: a load of 16 bytes needs no
+  // alignment.  2048 rows of 32003 bf16 logits, 32064 apart: 70 us one by one, 41.5 so.)
+  const int head = min(static_cast<int>((-reinterpret_cast<uintptr_t>(db) & 15) / sizeof(T)), p.V);
+  const int nv = (p.V - head) / VEC, rest = p.V - nv * VEC;
+  if (run == 0 && t < rest) {
+    const int i = t < head ? t : p.V - rest + t;
+    const float d = value(Elem<T>::load1(X + i));
+    Elem<T>::store1(D + i, i == id && !none ? d + C : d);
+  }
+  const int at_id = id >= head && !none ? id - head : -1;
+  for (int v0 = run * NT * kRun; v0 < nv; v0 += NT * kRun) {
+    uint4 raw[kRun];
 #pragma unroll
-      for (int j = 0; j < kRun; ++j)
-        if (v0 + NT * j + t < nv) raw[j] = reinterpret_cast<const uint4*>(X + head)[v0 + NT * j + t];
+    for (int j = 0; j < kRun; ++j)
+      if (v0 + NT * j + t < nv) __builtin_memcpy(&raw[j], X + head + static_cast<int64_t>(v0 + NT * j + t) * VEC, 16);
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const int v = v0 + NT * j + t;
-        if (v >= nv) break;
-        float x[VEC];
-        load_vec(reinterpret_cast<const T*>(&raw[j]), x);
+    for (int j = 0; j < kRun; ++j) {
+      const int v = v0 + NT * j + t;
+      if (v >= nv) break;
+      float x[VEC];
+      load_vec(reinterpret_cast<const T*>(&raw[j]), x);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] = value(x[i]);
-        if (at_id >= 0 && at_id / VEC == v) {
+      for (int i = 0; i < VEC; ++i) x[i] = value(x[i]);
+      if (at_id >= 0 && at_id / VEC == v) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) x[i] += i == at_id % VEC ? C : 0.f;
-        }
-        store_vec(D + head + v * VEC, x);
+        for (int i = 0; i < VEC; ++i) x[i] += i == at_id % VEC ? C : 0.f;
       }
-      if (WAVES > 1) break;
+      store_vec(D + head + v * VEC, x);
     }
+    if (WAVES > 1) break;
   }
 }
 
@@ -986,18 +981,14 @@ static void launch(const Params& p, hipStream_t s) {
 
 template <typename T>
 static int launch_grad(Grad& p, hipStream_t s, GHipError* err, const char* what) {
-  const bool wide = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.d)) % 16 == 0 &&
-                    (p.N <= 1 || (p.x_stride - p.d_stride) % 16 == 0);
   const bool one = short_rows(p.V, sizeof(T), 2);
-  const int64_t run = 256 * (wide ? static_cast<int64_t>(Elem<T>::kVec) * kRun : 8);
+  const int64_t run = run_of(sizeof(T), 4);
   p.runs = one ? 1 : static_cast<int>((p.V + run - 1) / run);
   const int64_t blocks = one ? (p.N + 3) / 4 : p.N * p.runs;
   if (blocks > kMostGroups) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", what);
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (one && wide) hipLaunchKernelGGL((grad_kernel<T, 1, true>), grid, dim3(256), 0, s, p);
-  else if (one) hipLaunchKernelGGL((grad_kernel<T, 1, false>), grid, dim3(256), 0, s, p);
-  else if (wide) hipLaunchKernelGGL((grad_kernel<T, 4, true>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((grad_kernel<T, 4, false>), grid, dim3(256), 0, s, p);
+  if (one) hipLaunchKernelGGL((grad_kernel<T, 1>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((grad_kernel<T, 4>), grid, dim3(256), 0, s, p);
   GHIP_CHECK(hipGetLastError(), err);
   return GHIP_OK;
 }

@@ -76,31 +76,32 @@ __device__ __forceinline__ void prepare(const Params& p, Shared& sh, int64_t fir
   __syncthreads();
 }
 
-// N elements, aligned to N.
+// N elements at any element's alignment: loads and stores of up to 16 bytes need none.
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Few {
   T v[N];
 };
 template <typename T, int N>
-__device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
+__device__ __forceinline__ void load_n(const T* p, float* x) {
+  Few<T, N> few;
+  __builtin_memcpy(&few, p, sizeof(few));
   if constexpr (N == Elem<T>::kVec) {
-    load_vec(p, x);
+    load_vec(few.v, x);
   } else {
-    const Few<T, N> few = *reinterpret_cast<const Few<T, N>*>(p);
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = Elem<T>::load1(&few.v[e]);
   }
 }
 template <typename T, int N>
-__device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
+__device__ __forceinline__ void store_n(T* p, const float* x) {
+  Few<T, N> few;
   if constexpr (N == Elem<T>::kVec) {
-    store_vec(p, x);
+    store_vec(few.v, x);
   } else {
-    Few<T, N> few;
 #pragma unroll
     for (int e = 0; e < N; ++e) Elem<T>::store1(&few.v[e], x[e]);
-    *reinterpret_cast<Few<T, N>*>(p) = few;
   }
+  __builtin_memcpy(p, &few, sizeof(few));
 }
 
 // Rows of whole elements.  A thread holds N pairs of a row, as two runs of N elements: run
@@ -112,8 +113,8 @@ __device__ __forceinline__ void row_unit(const Params& p, const T* src, T* dst, 
   float x[N], y[N];
   if (u < pairs) {
     const int a = p.a.neighbours ? 2 * N * u : N * u, c = p.a.neighbours ? a + N : p.a.half + a;
-    load_n(src + a, x);
-    load_n(src + c, y);
+    load_n<T, N>(src + a, x);
+    load_n<T, N>(src + c, y);
     if (!p.a.neighbours) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -136,15 +137,15 @@ __device__ __forceinline__ void row_unit(const Params& p, const T* src, T* dst, 
         y[e + 1] = w.y;
       }
     }
-    store_n(dst + a, x);
-    store_n(dst + c, y);
+    store_n<T, N>(dst + a, x);
+    store_n<T, N>(dst + c, y);
   } else {
     const int a = R + 2 * N * (u - pairs);
     const bool two = a + N < p.D;
-    load_n(src + a, x);
-    if (two) load_n(src + a + N, y);
-    store_n(dst + a, x);
-    if (two) store_n(dst + a + N, y);
+    load_n<T, N>(src + a, x);
+    if (two) load_n<T, N>(src + a + N, y);
+    store_n<T, N>(dst + a, x);
+    if (two) store_n<T, N>(dst + a + N, y);
   }
 }
 
@@ -159,7 +160,7 @@ __device__ __forceinline__ void row_unit4(const Params& p, const T* src, char* c
     constexpr int V = Elem<T>::kVec;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += V) load_vec(src + d + i, x + i);
+    for (int i = 0; i < 8; i += V) load_n<T, V>(src + d + i, x + i);
     if (d < R) {
       if (p.a.neighbours) {
 #pragma unroll
@@ -172,7 +173,7 @@ __device__ __forceinline__ void row_unit4(const Params& p, const T* src, char* c
         const bool low = d < p.a.half;
         const int other = low ? d + p.a.half : d - p.a.half, i0 = low ? d : other;
 #pragma unroll
-        for (int i = 0; i < 8; i += V) load_vec(src + other + i, y + i);
+        for (int i = 0; i < 8; i += V) load_n<T, V>(src + other + i, y + i);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float2 r = low ? turned(x[e], y[e], cs[i0 + e]) : turned(y[e], x[e], cs[i0 + e]);
@@ -368,18 +369,18 @@ static void plan(Params& p, bool four) {
   }
 }
 
-// Elements that a thread takes at a time: 16 bytes or the most that alignment and half of the pairs
-// allow.  (bf16, 4 x 16 heads of 80, 40 of them turned: 33 us one by one, 14 four by four.)
-static int width(const Params& p, uint64_t bits, int most, int64_t es) {
+// Elements that a thread takes at a time: 16 bytes, or the most that divide the row and half of what
+// turns of it.  (bf16, 4 x 16 heads of 80, 40 of them turned: 33 us one by one, 14 four by four.)
+static int width(const Params& p, int most) {
   int n = most;
-  while (n > 1 && (bits % static_cast<uint64_t>(n * es) || p.D % n || p.a.half % n)) n /= 2;
+  while (n > 1 && (p.D % n || p.a.half % n)) n /= 2;
   return n;
 }
 
 template <typename T, bool FOUR>
-static int launch(Params& p, uint64_t bits, bool wide4, hipStream_t s, GHipError* err, const char* what) {
+static int launch(Params& p, bool wide4, hipStream_t s, GHipError* err, const char* what) {
   constexpr int V = Elem<T>::kVec;
-  int n = width(p, bits, V, sizeof(T));
+  int n = width(p, V);
   if (FOUR && n < V) n = 1;
   p.units = (p.D + 2 * n - 1) / (2 * n);  // (half a row's pairs are a multiple of n)
   p.units4 = p.D / 8;
@@ -492,12 +493,12 @@ int launch_rope(int dtype, rope::Params& p, uint64_t bits, uint64_t bits4, bool 
                 const char* what) {
   const int64_t es = elem(dtype);
   if ((bits | bits4) % es) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: pointers are not aligned to elements", what);
-  const bool wide4 = bits4 % 16 == 0 && (p.a.neighbours ? p.R % 8 == 0 : p.a.half % 8 == 0);
+  const bool wide4 = p.a.neighbours ? p.R % 8 == 0 : p.a.half % 8 == 0;
   if (dtype == GHIP_DTYPE_FLOAT32)
-    return four ? rope::launch<float, true>(p, bits, wide4, s, err, what) : rope::launch<float, false>(p, bits, false, s, err, what);
+    return four ? rope::launch<float, true>(p, wide4, s, err, what) : rope::launch<float, false>(p, false, s, err, what);
   if (dtype == GHIP_DTYPE_FLOAT16)
-    return four ? rope::launch<f16_t, true>(p, bits, wide4, s, err, what) : rope::launch<f16_t, false>(p, bits, false, s, err, what);
-  return four ? rope::launch<bf16_t, true>(p, bits, wide4, s, err, what) : rope::launch<bf16_t, false>(p, bits, false, s, err, what);
+    return four ? rope::launch<f16_t, true>(p, wide4, s, err, what) : rope::launch<f16_t, false>(p, false, s, err, what);
+  return four ? rope::launch<bf16_t, true>(p, wide4, s, err, what) : rope::launch<bf16_t, false>(p, false, s, err, what);
 }
 
 // A 4-bit cache's tensors; false and the error set if they are not as the kernels read them.
