@@ -376,15 +376,15 @@ __device__ __forceinline__ uint4 vector_at(const uint4* body, int v, int t) {
   return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(body + v) + 16u * static_cast<uint32_t>(t));
 }
 
-// A run of kRun vectors a lane, NT lanes: from vector v on, thread t's.
-template <int NT>
-__device__ __forceinline__ void fetch(uint4 (&next)[kRun], const uint4* body, int v, int t, int v1) {
-  if (v + NT * kRun <= v1) {
+// A run of R vectors a lane, NT lanes: from vector v on, thread t's.
+template <int NT, int R>
+__device__ __forceinline__ void fetch(uint4 (&next)[R], const uint4* body, int v, int t, int v1) {
+  if (v + NT * R <= v1) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) next[j] = vector_at(body, v + NT * j, t);
+    for (int j = 0; j < R; ++j) next[j] = vector_at(body, v + NT * j, t);
   } else {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j)
+    for (int j = 0; j < R; ++j)
       if (v + NT * j + t < v1) next[j] = vector_at(body, v + NT * j, t);
   }
 }
@@ -396,10 +396,11 @@ __device__ __forceinline__ float most_of(const float (&x)[N]) {
   return N % 2 == 0 ? max3(m, x[N - 1], x[N - 1]) : m;
 }
 // Vector j of a run, widened; -infinity where there is none.
-template <typename T, int NT>
+template <typename T, int NT, int R>
 struct Run {
   static constexpr bool kFromMemory = false;
-  const uint4 (&raw)[kRun];
+  static constexpr int kVectors = R;
+  const uint4 (&raw)[R];
   int v, t, v1;
   __device__ __forceinline__ bool there(int j) const { return v + NT * j + t < v1; }
   // FRESH: widened once more; left alone, the compiler keeps a whole run's values for a second use.
@@ -408,7 +409,7 @@ struct Run {
     uint4 r = raw[j];
     if constexpr (FRESH) asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
     load_vec(reinterpret_cast<const T*>(&r), x);
-    if (v + NT * kRun > v1) {
+    if (v + NT * R > v1) {
 #pragma unroll
       for (int i = 0; i < Elem<T>::kVec; ++i) x[i] = there(j) ? x[i] : -INFINITY;
     }
@@ -420,6 +421,7 @@ struct Run {
 template <typename T, int NT, bool FULL>
 struct Streamed {
   static constexpr bool kFromMemory = true;
+  static constexpr int kVectors = kRun;
   uint4 (&raw)[kRun];
   const uint4* body;
   int v, t, v1;
@@ -447,9 +449,10 @@ struct Streamed {
 };
 struct Single {
   static constexpr bool kFromMemory = false;
+  static constexpr int kVectors = 1;
   float value;
   template <bool FRESH = false>
-  __device__ __forceinline__ void get(int j, float (&x)[1]) const { x[0] = j == 0 ? value : -INFINITY; }
+  __device__ __forceinline__ void get(int, float (&x)[1]) const { x[0] = value; }
 };
 
 // What stands before is computed before what follows.
@@ -459,11 +462,11 @@ __device__ __forceinline__ void here(float (&x)[2], float (&y)[2]) {
 }
 
 // The first run's maximum, ahead of its sums, which would be taken twice without it.
-template <typename T, int NT>
-__device__ __forceinline__ void look(Stats& a, const uint4 (&raw)[kRun], int v, int t, int v1, float c) {
+template <typename T, int NT, int R>
+__device__ __forceinline__ void look(Stats& a, const uint4 (&raw)[R], int v, int t, int v1, float c) {
   float most = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
+  for (int j = 0; j < R; ++j) {
     float x[Elem<T>::kVec];
     load_vec(reinterpret_cast<const T*>(&raw[j]), x);
     const float m = most_of(x);
@@ -479,6 +482,7 @@ __device__ __forceinline__ void look(Stats& a, const uint4 (&raw)[kRun], int v, 
 template <int M, bool MOST, typename Values>
 __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c) {
   constexpr float kGrown = 256.f;
+  constexpr int kVectors = Values::kVectors;
   float most = -INFINITY, s[2] = {0.f, 0.f}, e[2] = {0.f, 0.f}, shift = -a.m;
   auto weigh = [&](auto again, int j) {
     float x[M];
@@ -495,7 +499,7 @@ __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c
     }
   };
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
+  for (int j = 0; j < kVectors; ++j) {
     weigh(std::integral_constant<bool, false>{}, j);
     here(s, e);  // (all vectors at once take 32 registers more)
   }
@@ -505,10 +509,10 @@ __device__ __forceinline__ float add_run(Stats& a, const Values& values, float c
     auto each = [&](auto f) {
       if constexpr (Values::kFromMemory) {
 #pragma unroll 1
-        for (int j = 0; j < kRun; ++j) f(j);
+        for (int j = 0; j < kVectors; ++j) f(j);
       } else {
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
+        for (int j = 0; j < kVectors; ++j) {
           f(j);
           here(s, e);
         }
@@ -545,10 +549,10 @@ __device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
   }
   return a;
 }
-// Rows (WAVES = 1: a wave a row) and slices (4) of one run a lane: the logits stay in registers, so
-// candidates are taken from there.  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
+// Rows (WAVES = 1: a wave a row) and slices (4) of one run of R vectors a lane: the logits stay in
+// registers, so candidates are taken from there.  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
 // in 16 slices each 6.7 us, and 4.0 for their join.
-template <typename T, int WAVES, bool TOP>
+template <typename T, int WAVES, int R, bool TOP>
 __global__ __launch_bounds__(256) void run_kernel(Params p) {
   constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
   constexpr int kKeys = WAVES * kQueue;
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
   };
   const Part<T> at(p, unit);
   const bool whole = p.slices == 1;
-  uint4 raw[kRun];
+  uint4 raw[R];
   fetch<NT>(raw, at.body, at.v0, t, at.v1);
   Given given;
   if (t == 0 && whole) given.load<T>(p, at.row);
@@ -578,7 +582,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
     if (alone) single = Elem<T>::load1(at.x + at.single(p, t));
     add_run<1, true>(a, Single{single}, p.c);
   }
-  const Run<T, NT> values{raw, at.v0, t, at.v1};
+  const Run<T, NT, R> values{raw, at.v0, t, at.v1};
   look<T, NT>(a, raw, at.v0, t, at.v1, p.c);
   best = fmaxf(add_run<VEC, TOP>(a, values, p.c), single);
   a = wave_join(a);
@@ -608,10 +612,10 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
     const float tau_x = tau ? value_of(tau) : -INFINITY;
     // A lane marks its candidates (a bit each, the single element last), then writes them behind those
     // of the lanes before it, each looked up once more by its index.
-    constexpr int kBits = kRun * VEC;
+    constexpr int kBits = R * VEC;
     uint64_t marks = static_cast<uint64_t>(alone && single >= tau_x) << kBits;
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < R; ++j) {
       const bool there = values.there(j);
       float x[VEC];
       values.template get<true>(j, x);
@@ -956,19 +960,31 @@ static int64_t slices_of(int64_t N, int64_t V, int64_t es) {
   return std::max<int64_t>(1, std::min<int64_t>({(V + run - 1) / run, 1024 / std::max<int64_t>(N, 1), kMostSlices}));
 }
 
+template <typename T, int WAVES, int R>
+static void launch_run(const Params& p, int64_t groups, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(groups));
+  if (p.top) hipLaunchKernelGGL((run_kernel<T, WAVES, R, true>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((run_kernel<T, WAVES, R, false>), grid, dim3(256), 0, s, p);
+}
+// As many vectors a lane as the longest row or slice needs: those that it does not have cost their
+// instructions all the same.  (100000 rows of 500 bf16 logits: 126 us with four, 53 with one.)
+template <typename T, int WAVES>
+static void launch_runs(const Params& p, int64_t groups, hipStream_t s) {
+  const int64_t lanes = 64 * WAVES, vectors = p.slices == 1 ? p.V / Elem<T>::kVec : p.per;
+  if (vectors <= lanes) launch_run<T, WAVES, 1>(p, groups, s);
+  else if (vectors <= 2 * lanes) launch_run<T, WAVES, 2>(p, groups, s);
+  else launch_run<T, WAVES, kRun>(p, groups, s);
+}
+
 template <typename T>
 static void launch(const Params& p, hipStream_t s) {
   if (short_rows(p.V, sizeof(T))) {
-    const dim3 grid(static_cast<unsigned>((p.N + 3) / 4));
-    if (p.top) hipLaunchKernelGGL((run_kernel<T, 1, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((run_kernel<T, 1, false>), grid, dim3(256), 0, s, p);
+    launch_runs<T, 1>(p, (p.N + 3) / 4, s);
     return;
   }
   const int64_t parts = p.N * p.slices;
   if (p.per <= 256 * kRun) {
-    const dim3 grid(static_cast<unsigned>(parts));
-    if (p.top) hipLaunchKernelGGL((run_kernel<T, 4, true>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((run_kernel<T, 4, false>), grid, dim3(256), 0, s, p);
+    launch_runs<T, 4>(p, parts, s);
   } else {
     // Workgroups that stay, as many as run at once, with as many parts each as can be alike.
     const int64_t most = kCus * kStay, turns = (parts + most - 1) / most;
