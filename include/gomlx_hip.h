@@ -373,7 +373,8 @@ typedef struct {
  * contiguous, D up to 256; out may be x itself (the same strides), else they overlap nothing.
  * cos and sin are taken in 64 bits and rounded to fp32, products and sums are fp32, rounded
  * once.  16-byte vectors where D and half of rotary_dim are whole ones, shorter ones down to
- * single values elsewhere; pointers and strides need no more than an element's alignment.  No reference op (GoMLX composes it of primitives). */
+ * single values elsewhere; pointers and strides need no more than an element's alignment.  No
+ * reference op (GoMLX composes it of primitives). */
 int ghip_rope(int dtype, const void* x, void* out, int64_t B, int64_t H, int64_t S, int64_t D,
               const int64_t* x_strides, const int64_t* out_strides, const GHipRope* rope, int inverse,
               void* stream, GHipError* err);
