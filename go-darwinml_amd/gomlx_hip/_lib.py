@@ -37,6 +37,7 @@ _int = ctypes.c_int
 _vp = ctypes.c_void_p
 _f32 = ctypes.c_float
 _errp = ctypes.POINTER(GHipError)
+_byref = ctypes.byref
 
 # The arrays of these two are spelled out: a structure of scalars is made in a third of the time.
 class Rope(ctypes.Structure):
@@ -150,10 +151,10 @@ def load():
 
 def call(name: str, *args) -> None:
     """Calls entry point `name` with a fresh GHipError; raises BackendError on failure."""
-    L = load()
-    err = GHipError(0, None)
-    rc = getattr(L, name)(*args, ctypes.byref(err))
+    L = _lib or load()
+    err = GHipError()
+    rc = getattr(L, name)(*args, _byref(err))
     if rc != 0:
         msg = err.message.decode() if err.message else "(no message)"
-        L.ghip_error_clear(ctypes.byref(err))
+        L.ghip_error_clear(_byref(err))
         raise BackendError(rc, msg)

@@ -294,12 +294,13 @@ def scale_mask_softmax_ex(x: torch.Tensor, scale: float, causal: bool, mask=None
 
 def _launch(dev: torch.device, name: str, stream, *args):
     """Calls entry point `name` with `dev` current, on `stream` (None: dev's current one)."""
-    if dev.index != torch.cuda.current_device():
+    n = dev.index
+    if n != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             call(name, *args, _stream(stream))
     else:
         # The current stream's handle alone: a torch.cuda.Stream object costs 3 us.
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else int(stream))
+        call(name, *args, torch._C._cuda_getCurrentRawStream(n) if stream is None else int(stream))
 
 
 def _given(what: str, ws):
@@ -689,9 +690,9 @@ def sdpa_paged_kv4_workspace(q: torch.Tensor, k_cache, block_table: torch.Tensor
     """Workspace for sdpa_paged_kv4 at these sizes (None when the sequences never split), for
     calls on `stream`."""
     B, H, D = q.shape
-    n = _lib.load().ghip_sdpa_paged_kv4_workspace_bytes(B, H, k_cache[0].shape[1], D, k_cache[0].shape[2],
-                                                        block_table.shape[1])
-    return _empty((n,), torch.uint8, q.device, stream) if n > 0 else None
+    _, Hkv, size, _ = k_cache[0].shape
+    n = _lib.load().ghip_sdpa_paged_kv4_workspace_bytes(B, H, Hkv, D, size, block_table.shape[1])
+    return _new(q, (n,), stream, torch.uint8) if n > 0 else None
 
 
 def sdpa_paged_kv4(q: torch.Tensor, k_cache, v_cache, block_table: torch.Tensor, lens: torch.Tensor, scale: float,
@@ -738,7 +739,7 @@ def token_logprobs_workspace(logits: torch.Tensor, top: int = 0, stream=None):
     """Workspace for token_logprobs at these sizes (None where a row is never shared), for calls
     on `stream`."""
     n = _lib.load().ghip_token_logprobs_workspace_bytes(dtype_code(logits.dtype), *logits.shape, int(top))
-    return _empty((n,), torch.uint8, logits.device, stream) if n > 0 else None
+    return _new(logits, (n,), stream, torch.uint8) if n > 0 else None
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0, scale: float = 1.0, outs=None, stream=None,
