@@ -70,8 +70,8 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
 }
 
 // Where the tiles of the sequences lie in the common order (sequence, unit of heads,
-// tile), with AHEAD places without a tile before each unit's.  A lane counts one sequence of 64; a sequence has fewer than 2^26 tiles (the host
-// checks), so 64 of them fit 32 bits.
+// tile), with AHEAD places without a tile before each unit's.  A lane counts one sequence of
+// 64; a sequence has fewer than 2^26 tiles (the host checks), so 64 of them fit 32 bits.
 template <int KT, int AHEAD = 0>
 struct Order {
   int64_t total = 0;  // places of all sequences and units

@@ -318,7 +318,8 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
           const int s = 4 * (e & 3) + g, byte = col * (kVals / 2);
           vw[t][e] = *reinterpret_cast<const typename Word<kVals>::type*>(
               sv + (32 * t + 16 * (e >> 2) + 4 * (e & 3)) * kRow + g * kRow + (((byte >> 4) ^ swz(s)) << 4) + (byte & 15));
-          vscale[t][e] = scale_of(ssv[4 * (32 * t + 16 * (e >> 2) + (e & 3)) + 16 * g + (vgroup >> 2) * 256 + (vgroup & 3)], vgroup);
+          const int at = 4 * (32 * t + 16 * (e >> 2) + (e & 3)) + 16 * g;
+          vscale[t][e] = scale_of(ssv[at + (vgroup >> 2) * 256 + (vgroup & 3)], vgroup);
         }
       const uint64_t rows = next;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -333,7 +334,8 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
       for (int u = 0; u < kWords; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const tile::bf16x8 kf = __builtin_bit_cast(tile::bf16x8, kv4::decode8(kw[i][u], kscale[i][u * kQuarterGroups / kWords]));
+          const uint4 values = kv4::decode8(kw[i][u], kscale[i][u * kQuarterGroups / kWords]);
+          const tile::bf16x8 kf = __builtin_bit_cast(tile::bf16x8, values);
 #pragma unroll
           for (int q = 0; q < kQ; ++q) x[i] = mma(kf, qf[u][q], x[i]);
         }
@@ -499,11 +501,12 @@ extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int
                                                        int64_t max_pages) {
   if (B <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 256 || page_size <= 0 || max_pages <= 0) return 0;
   const int64_t heads = H / Hkv;
-  const double units = static_cast<double>(B) * static_cast<double>(Hkv) * static_cast<double>((heads + paged::kHeads - 1) / paged::kHeads);
+  const int64_t blocks = (heads + paged::kHeads - 1) / paged::kHeads;
+  const double units = static_cast<double>(B) * static_cast<double>(Hkv) * static_cast<double>(blocks);
   const double tokens = static_cast<double>(page_size) * static_cast<double>(max_pages);
   if (tokens <= paged4::kTile * (units >= 1024 ? 24. : units >= 512 ? 12. : 6.)) return 0;
   return 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4 +
-         8 * B * Hkv * ((heads + paged::kHeads - 1) / paged::kHeads);
+         8 * B * Hkv * blocks;
 }
 
 extern "C" int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_cache, const GHipKv4* v_cache, void* o,

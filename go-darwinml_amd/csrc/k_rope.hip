@@ -354,7 +354,9 @@ static void plan(Params& p, bool four) {
   const int64_t all = p.tokens * (rows * p.units + rows4 * (four ? p.units4 : 0));
   const int64_t filled = all / (kThreads * 1024), each = filled < 1 ? 1 : filled < 8 ? 2 : 3;
   p.block_tokens = 1;
-  auto parts = [&](int64_t r, int64_t s) { return static_cast<int>(r ? std::max<int64_t>(1, (r + s * each - 1) / (s * each)) : 0); };
+  auto parts = [&](int64_t r, int64_t s) {
+    return static_cast<int>(r ? std::max<int64_t>(1, (r + s * each - 1) / (s * each)) : 0);
+  };
   p.splits = parts(rows, slots);
   p.splits4 = parts(rows4, slots4);
   if (p.splits <= 1 && p.splits4 <= 1 && each > 1) {

@@ -467,8 +467,9 @@ int ghip_token_logprobs(int dtype, const void* logits, int64_t row_stride, const
  *   d_logits_v = scale (d_logp ([v = id] - p_v) - d_entropy p_v (log p_v + entropy))
  * A row whose id is outside [0, V) has no logp (d_logp is not used there); rows of lse -infinity
  * get zeros.  (p is taken beside the lse that is given: from 2^24 on, as in rows of nothing but
- * a large mask, it has no bits of log V, and p is 1.)  d_logits [N, V] in the logits' type with a row stride of its own; it may be the
- * logits themselves (the same stride), else they overlap nothing. */
+ * a large mask, it has no bits of log V, and p is 1.)  d_logits [N, V] in the logits' type with
+ * a row stride of its own; it may be the logits themselves (the same stride), else they
+ * overlap nothing. */
 int ghip_token_logprobs_grad(int dtype, const void* logits, int64_t row_stride, const int32_t* ids,
                              const float* lse, const float* entropy, const float* d_logp,
                              const float* d_entropy, int64_t N, int64_t V, float scale, void* d_logits,
