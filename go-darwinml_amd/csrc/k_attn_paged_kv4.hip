@@ -503,6 +503,7 @@ extern "C" int64_t ghip_sdpa_paged_kv4_workspace_bytes(int64_t B, int64_t H, int
   const int64_t heads = H / Hkv;
   const int64_t blocks = (heads + paged::kHeads - 1) / paged::kHeads;
   const double units = static_cast<double>(B) * static_cast<double>(Hkv) * static_cast<double>(blocks);
+  if (units > tile::kMostGroups) return 0;  // (more than the entry point takes)
   const double tokens = static_cast<double>(page_size) * static_cast<double>(max_pages);
   if (tokens <= paged4::kTile * (units >= 1024 ? 24. : units >= 512 ? 12. : 6.)) return 0;
   return 2 * static_cast<int64_t>(paged4::workers(D <= 128 ? 128 : 256)) * std::min<int64_t>(paged::kHeads, heads) * (D + 1) * 4 +
