@@ -30,8 +30,8 @@ __device__ __forceinline__ double position(const Angles& a, int b, int s, int i)
 
 // (cos, sin) of pos * freq.  The angle is a product in 64 bits, reduced by whole quarter turns in two
 // steps (pi / 2 as the sum of two doubles) to |r| <= pi / 4, so positions of any size keep 2^-52
-// of the angle; there the Taylor sums to r^11 and r^12 are off by less than 2^-36, and each of the
-// two is rounded to fp32 once.  (An fp32 angle of 10^5 is off by 2^-8.  The library's sincos,
+// of the angle; there the Taylor sums to r^13 and r^12 are off by less than 2^-45 and 2^-41, and each of
+// the two is rounded to fp32 once.  (An fp32 angle of 10^5 is off by 2^-8.  The library's sincos,
 // good to 2^-52, takes four times the instructions: a batch of prompts into 4 bits was bound by it.)
 __device__ __forceinline__ float2 turn(double pos, float freq, int inverse) {
   const double a = pos * static_cast<double>(freq);
@@ -39,7 +39,8 @@ __device__ __forceinline__ float2 turn(double pos, float freq, int inverse) {
   double r = fma(-k, 1.5707963267948966, a);
   r = fma(-k, 6.123233995736766e-17, r);
   const double z = r * r;
-  double s = fma(z, -1. / 39916800., 1. / 362880.);
+  double s = fma(z, 1. / 6227020800., -1. / 39916800.);
+  s = fma(z, s, 1. / 362880.);
   s = fma(z, s, -1. / 5040.);
   s = fma(z, s, 1. / 120.);
   s = fma(z, s, -1. / 6.);

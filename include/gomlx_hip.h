@@ -371,7 +371,7 @@ typedef struct {
 /* out[b, h, s] = x[b, h, s] turned; inverse != 0: by -a, which is the gradient of x from the
  * gradient of out.  [B, H, S, D] by ELEMENT strides (batch, head, sequence) with the head dim
  * contiguous, D up to 256; out may be x itself (the same strides), else they overlap nothing.
- * cos and sin are taken in 64 bits and rounded to fp32, products and sums are fp32, rounded
+ * cos and sin are taken in 64 bits, to 2^-40, and rounded to fp32, products and sums are fp32, rounded
  * once.  16-byte vectors where D and half of rotary_dim are whole ones, shorter ones down to
  * single values elsewhere; pointers and strides need no more than an element's alignment.  No
  * reference op (GoMLX composes it of primitives). */
