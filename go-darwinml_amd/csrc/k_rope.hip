@@ -4,16 +4,13 @@
 //   pair i of a row at token (b, s):  a = position * freqs[i],  (x, y) -> (x cos a - y sin a, x sin a + y cos a)
 //
 // No reference op (GoMLX composes it of primitives).  Bound by the bytes of the rows.
-#include <algorithm>
-
 #include "kv4_dev.h"
 #include "rope_dev.h"
+#include "rope_rules.h"
 
 namespace ghip {
 namespace rope {
 
-constexpr int kThreads = 256;
-constexpr int kMostTokens = 16;  // of a workgroup
 constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;  // workgroups of a launch (HIP: fewer than 2^32 threads)
 
 struct Rows {  // [B, heads, S, D]
@@ -35,9 +32,8 @@ struct Params {
   int64_t table_stride;
   int64_t tokens;  // B S
   int S, H, Hkv, D, R, num_pages, page_size, max_pages;
-  int block_tokens, splits, splits4;  // tokens of a workgroup; workgroups that share their rows
-  int both;                           // 4 bits: the one workgroup of a token takes its rows of both kinds
-  int units, units4;                  // threads of a row
+  int units, units4;  // threads of a row
+  Deal deal;
 };
 
 // What the workgroup's tokens need: the angles of their pairs, and where their rows go.
@@ -241,14 +237,14 @@ struct Slots {
 template <typename T, int N, bool FOUR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
   __shared__ Shared sh;
-  const int splits = p.splits + (FOUR ? p.splits4 : 0);
+  const int splits = p.deal.splits + (FOUR ? p.deal.splits4 : 0);
   const int64_t block = blockIdx.x / splits;
   const int split = blockIdx.x - static_cast<int>(block) * splits;
-  const int64_t first = block * p.block_tokens;
-  const int n = static_cast<int>(min(static_cast<int64_t>(p.block_tokens), p.tokens - first));
+  const int64_t first = block * p.deal.block_tokens;
+  const int n = static_cast<int>(min(static_cast<int64_t>(p.deal.block_tokens), p.tokens - first));
   prepare(p, sh, first, n, p.R > 0);
-  if (split < p.splits) {
-    const int heads = FOUR ? p.H : p.H + 2 * p.Hkv, per = (heads + p.splits - 1) / p.splits, h0 = split * per;
+  if (split < p.deal.splits) {
+    const int heads = FOUR ? p.H : p.H + 2 * p.Hkv, per = (heads + p.deal.splits - 1) / p.deal.splits, h0 = split * per;
     Slots at(p.units, min(per, heads - h0));
     for (; at.any && at.t < n; at.next()) {
       const int b = sh.b[at.t], s = sh.s[at.t], head = h0 + at.h;
@@ -267,9 +263,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
     }
   }
   if constexpr (FOUR) {
-    const int part = split - (p.both ? 0 : p.splits);  // (both: this workgroup takes all rows)
+    const int part = split - (p.deal.both ? 0 : p.deal.splits);  // (both: this workgroup takes all rows)
     if (part < 0) return;
-    const int parts = p.both ? 1 : p.splits4, heads = 2 * p.Hkv, per = (heads + parts - 1) / parts, h0 = part * per;
+    const int parts = p.deal.both ? 1 : p.deal.splits4, heads = 2 * p.Hkv, per = (heads + parts - 1) / parts, h0 = part * per;
     Slots at(p.units4, min(per, heads - h0));
     for (; at.any && at.t < n; at.next()) {
       const int b = sh.b[at.t], s = sh.s[at.t], head = h0 + at.h, page = sh.page[at.t];
@@ -340,54 +336,15 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(Read p) {
   }
 }
 
-// How the rows are dealt out: a row in each slot until 1024 workgroups (four a CU) run, then two,
-// beyond eight times as many three, so that a token's angles serve many rows and workgroups still follow each other.
-// us with 1, 2, 3, 4, 6, 12 rows a slot (one: a token a workgroup, whose slots its rows may not fill):
-//   rope, 16 heads of 128, bf16, 2048 tokens       7.5   6.1   7.2   7.0   8.4  10.8
-//   the same, 4 x 2048                            20.2  13.5  15.0  13.9  15.2  15.8
-//   the same, 8 x 8192                             151  94.0  98.5  98.8   104   111
-//   into 16 bits, 32 heads and 8, f16, 8 x 1024   54.2  37.7  35.2  35.2  35.4  36.3
-//   into 4 bits, the same in bf16                 52.0  36.4  36.4  37.8  40.8  51.6
-static void plan(Params& p, bool four) {
-  const int64_t rows = p.H + (four ? 0 : 2 * p.Hkv), rows4 = four ? 2 * p.Hkv : 0;
-  const int64_t slots = kThreads / p.units, slots4 = four ? kThreads / p.units4 : 1;
-  const int64_t all = p.tokens * (rows * p.units + rows4 * (four ? p.units4 : 0));
-  const int64_t filled = all / (kThreads * 1024), each = filled < 1 ? 1 : filled < 8 ? 2 : 3;
-  p.block_tokens = 1;
-  auto parts = [&](int64_t r, int64_t s) {
-    return static_cast<int>(r ? std::max<int64_t>(1, (r + s * each - 1) / (s * each)) : 0);
-  };
-  p.splits = parts(rows, slots);
-  p.splits4 = parts(rows4, slots4);
-  if (p.splits <= 1 && p.splits4 <= 1 && each > 1) {
-    const int64_t by = rows ? std::max<int64_t>(1, slots * each / rows) : kMostTokens;
-    const int64_t by4 = rows4 ? std::max<int64_t>(1, slots4 * each / rows4) : kMostTokens;
-    p.block_tokens = static_cast<int>(std::min<int64_t>({by, by4, kMostTokens}));
-    // Enough tokens for every slot of either kind: the angles are computed once for both.
-    if (four && p.H > 0) {
-      p.both = 1;
-      p.splits4 = 0;
-    }
-  }
-}
-
-// Elements that a thread takes at a time: 16 bytes, or the most that divide the row and half of what
-// turns of it.  (bf16, 4 x 16 heads of 80, 40 of them turned: 33 us one by one, 14 four by four.)
-static int width(const Params& p, int most) {
-  int n = most;
-  while (n > 1 && (p.D % n || p.a.half % n)) n /= 2;
-  return n;
-}
-
 template <typename T, bool FOUR>
 static int launch(Params& p, bool wide4, hipStream_t s, GHipError* err, const char* what) {
   constexpr int V = Elem<T>::kVec;
-  int n = width(p, V);
+  int n = width(p.D, p.a.half, V);
   if (FOUR && n < V) n = 1;
   p.units = (p.D + 2 * n - 1) / (2 * n);  // (half a row's pairs are a multiple of n)
   p.units4 = p.D / 8;
-  plan(p, FOUR);
-  const int64_t blocks = (p.tokens + p.block_tokens - 1) / p.block_tokens * (p.splits + (FOUR ? p.splits4 : 0));
+  p.deal = deal(p.tokens, p.H, p.Hkv, p.units, p.units4, FOUR);
+  const int64_t blocks = (p.tokens + p.deal.block_tokens - 1) / p.deal.block_tokens * (p.deal.splits + p.deal.splits4);
   if (blocks > kMostGroups) return set_error(err, GHIP_ERR_UNSUPPORTED, "%s: problem too large", what);
   const dim3 grid(static_cast<unsigned>(blocks));
   if constexpr (FOUR) {
@@ -411,8 +368,6 @@ static int launch(Params& p, bool wide4, hipStream_t s, GHipError* err, const ch
 using namespace ghip;
 
 namespace {
-
-bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
 
 int64_t elem(int dtype) { return dtype == GHIP_DTYPE_FLOAT32 ? 4 : 2; }
 
