@@ -22,9 +22,12 @@ constexpr int kMostSlices = 64;
 constexpr int kRun = 4;      // vectors a lane takes at a time
 constexpr int kSlots = 16;   // runs of a lane whose maxima are kept apart
 constexpr int kQueue = 256;  // candidates a wave holds
+constexpr int kAhead = 4;    // vectors under way where a long row is read once more
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 constexpr float kFar = -200.f;  // 2^kFar is 0: what stands for log 0 in a product with a weight of 0
 constexpr int64_t kMostGroups = (int64_t{1} << 24) - 1;
+constexpr int kCus = 256, kStay = 5;  // of an MI355X; workgroups of stream_kernel on each
+constexpr int kMostTurns = ((1 << 24) / (kCus * kStay) + 32) / 32 * 32;  // parts that one of them takes, at most
 
 struct Params {
   const char* x;
@@ -222,38 +225,117 @@ struct Given {
 struct Sums : Stats {
   float x0 = 0.f;
   bool none = false;  // nothing but -infinity
+  Sums() = default;
+  __device__ __forceinline__ explicit Sums(const Stats& a) : Stats(a) {}
   __device__ __forceinline__ float exponent(float x, float c) const { return __builtin_fmaf(x - x0, c, -m); }
   __device__ __forceinline__ bool usual() const { return fabsf(m) < kLarge && s > 0.f && s < INFINITY; }
 };
+// A row's logits to f(x, first index, there), thread t of NT: one by one, or (AHEAD > 0) AHEAD vectors at a
+// time and the logits around the row's vectors one by one.  The lanes of a wave are in every call
+// together; -infinity where a lane has none.
+template <typename T, int NT, int AHEAD, typename F>
+__device__ __forceinline__ void each_logit(const Params& p, int64_t row, int t, const F& f) {
+  const char* base = p.x + row * p.stride;
+  const T* x = reinterpret_cast<const T*>(base);
+  auto one = [&](int i, bool there) {
+    float v[1] = {-INFINITY};
+    if (there) v[0] = Elem<T>::load1(x + i);
+    f(v, i, there);
+  };
+  if constexpr (AHEAD == 0) {
+    for (int i = t; i - t < p.V; i += NT) one(i, i < p.V);
+  } else {
+    constexpr int VEC = Elem<T>::kVec;
+    const int head = min(static_cast<int>((-reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T)), p.V);
+    const int nv = (p.V - head) / VEC, rest = p.V - nv * VEC;
+    one(t < head ? t : p.V - rest + t, t < rest);
+    const uint4* body = reinterpret_cast<const uint4*>(x + head);
+#pragma unroll 1
+    for (int v0 = 0; v0 < nv; v0 += NT * AHEAD) {
+      uint4 raw[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (v0 + NT * j + t < nv) raw[j] = body[v0 + NT * j + t];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int v = v0 + NT * j + t;
+        float many[VEC];
+        __builtin_amdgcn_sched_barrier(0);  // (one vector widened at a time)
+        load_vec(reinterpret_cast<const T*>(&raw[j]), many);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) many[e] = v < nv ? many[e] : -INFINITY;
+        f(many, head + v * VEC, v < nv);
+      }
+    }
+  }
+}
+// The largest, the sum (wave after wave) of NT threads' values; `lds` of the workgroup's waves.
+template <int NT>
+__device__ __forceinline__ float group_max(float x, float* lds) {
+  x = wave_max(x);
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w) x = fmaxf(x, lds[w]);
+  }
+  return x;
+}
+template <int NT>
+__device__ __forceinline__ float group_sum(float x, float* lds) {
+  x = wave_sum(x);
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = 0.f;
+    for (int w = 0; w < NT / 64; ++w) x += lds[w];
+  }
+  return x;
+}
 // Rows of one mask, -infinity, 1e10 or a type's lowest number, and rows with a NaN or infinity: the
-// largest logit itself, then u = (x - x0) c.  Every lane of a wave calls it.
-template <typename T>
-__device__ __forceinline__ Sums exact_sums(const Params& p, int64_t row) {
-  const int lane = threadIdx.x & 63;
+// largest logit itself, then u = (x - x0) c.  Every thread of NT calls it, and gets the same.
+// (Padding is such a row.  16 rows of 131072 bf16 logits, one of them nothing but -infinity: 24 us as without it;
+// 439 by one wave that reads its logits one by one.  One with a NaN, and a top of 20: 84 us for 22.)
+template <typename T, int NT, int AHEAD>
+__device__ __forceinline__ Sums exact_sums(const Params& p, int64_t row, int t, float* lds) {
   Sums a;
   float most = -INFINITY;
-  for (int i = lane; i < p.V; i += 64) most = fmaxf(most, logit<T>(p, row, i));
-  a.x0 = wave_max(most);
+  bool nan = false;
+  each_logit<T, NT, AHEAD>(p, row, t, [&](const auto& x, int, bool) {
+#pragma unroll
+    for (const float v : x) {
+      most = fmaxf(most, v);
+      nan |= v != v;
+    }
+  });
   a.m = 0.f;
-  a.none = a.x0 == -INFINITY;
-  if (a.none) a.x0 = 0.f;
-  for (int i = lane; i < p.V; i += 64) {
-    const float u = a.exponent(logit<T>(p, row, i), p.c), w = __builtin_amdgcn_exp2f(u);
-    a.s += w;
-    a.e = __builtin_fmaf(w, fmaxf(u, kFar), a.e);
+  a.x0 = group_max<NT>(nan ? INFINITY : most, lds);
+  if (a.x0 == -INFINITY) {
+    a.x0 = 0.f;
+    a.none = true;
+    return a;
   }
-  a.s = wave_sum(a.s);
-  a.e = wave_sum(a.e);
-  if (a.s != a.s) a.none = false;  // nothing but -infinity and NaN
+  if (a.x0 == INFINITY) {
+    a.s = a.e = NAN;
+    return a;
+  }
+  each_logit<T, NT, AHEAD>(p, row, t, [&](const auto& x, int, bool) {
+#pragma unroll
+    for (const float v : x) {
+      const float u = a.exponent(v, p.c), w = __builtin_amdgcn_exp2f(u);
+      a.s += w;
+      a.e = __builtin_fmaf(w, fmaxf(u, kFar), a.e);
+    }
+  });
+  a.s = group_sum<NT>(a.s, lds);
+  a.e = group_sum<NT>(a.e, lds);
   return a;
 }
-template <typename T>
-__device__ __forceinline__ Sums sums_of(const Params& p, int64_t row, const Stats& a) {
-  Sums r;
-  r.m = a.m;
-  r.s = a.s;
-  r.e = a.e;
-  return r.usual() ? r : exact_sums<T>(p, row);
+template <typename T, int NT, int AHEAD>
+__device__ __forceinline__ Sums sums_of(const Params& p, int64_t row, const Stats& a, int t, float* lds) {
+  const Sums r(a);
+  return r.usual() ? r : exact_sums<T, NT, AHEAD>(p, row, t, lds);
 }
 
 // What a row's sums give; one thread.
@@ -271,31 +353,47 @@ __device__ __forceinline__ void finish_top(const Params& p, int64_t row, const S
   p.top_logps[row * p.top + rank] = a.none ? -INFINITY : kLn2 * (a.exponent(x, p.c) - __builtin_amdgcn_logf(a.s));
 }
 
-// Rows that hold a NaN or +infinity (their sum is NaN, which the bounds above do not see): the
-// largest keys one after the other, a pass over the row for each.  Every thread of NT calls it.
-template <typename T, int NT>
-__device__ __forceinline__ void top_of_nan_row(const Params& p, int64_t row, const Sums& a, uint64_t* lds) {
-  const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  uint64_t last = ~0ull;
-  for (int r = 0; r < p.top; ++r) {
-    uint64_t best = 0;
-    for (int i = t; i < p.V; i += NT) {
-      const uint64_t key = key_of(logit<T>(p, row, i), i);
-      if (key > best && (r == 0 || key < last)) best = key;
-    }
+// The largest logits of a row by comparisons of orders, in one pass: rows that hold a NaN or +infinity,
+// which the bounds by floating-point maxima do not see (their sum is NaN), and others of no usual sum.
+// Every thread of NT calls it; `queues`: [NT / 64][kQueue], `list`: [NT / 64][kMostTop] (one wave: none).
+template <typename T, int NT, int AHEAD>
+__device__ __forceinline__ void top_by_order(const Params& p, int64_t row, const Sums& a, int t, uint64_t* queues,
+                                             uint64_t* list) {
+  const int lane = t & 63, wave = t >> 6;
+  Queue q(queues + wave * kQueue, p.top);
+  uint32_t best = 0;
+  each_logit<T, NT, AHEAD>(p, row, t, [&](const auto& x, int i, bool there) {
+    constexpr int kN = sizeof(x) / sizeof(float);
+    uint32_t order[kN], most = 0;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint64_t o = __shfl_xor(best, d, 64);
-      best = o > best ? o : best;
+    for (int e = 0; e < kN; ++e) {
+      order[e] = there ? order_of(x[e]) : 0u;
+      most = max(most, order[e]);
     }
-    if constexpr (NT > 64) {
-      __syncthreads();
-      if ((t & 63) == 0) lds[t >> 6] = best;
-      __syncthreads();
-      for (int w = 0; w < NT / 64; ++w) best = lds[w] > best ? lds[w] : best;
+    best = max(best, most);
+    // (No key of these is above that of their largest at the first's place.)
+    const uint64_t top = static_cast<uint64_t>(most) << 32 | static_cast<uint32_t>(~i);
+    if (__builtin_amdgcn_ballot_w64(there && top > q.tau) == 0) return;
+    const uint32_t bests[1] = {best};
+    q.bound(kth_bound<uint32_t, 16>(bests, p.top));
+    uint32_t marks = 0;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) marks |= there && order[e] >= static_cast<uint32_t>(q.tau >> 32) ? 1u << e : 0u;
+    while (__builtin_amdgcn_ballot_w64(marks != 0)) {  // (looked up once more: one place that pushes, not kN)
+      const int at = i + __builtin_ctz(marks | 1u << 31);
+      q.push(marks ? key_of(logit<T>(p, row, at), at) : 0);
+      marks &= marks - 1;
     }
-    last = best;
-    if (t == 0) finish_top(p, row, a, r, best);
+  });
+  wave_sync();
+  q.compact();
+  if constexpr (NT == 64) {
+    if (lane < q.n) finish_top(p, row, a, lane, q.q[lane]);
+    wave_sync();
+  } else {
+    if (lane < kMostTop) list[wave * kMostTop + lane] = lane < q.n ? q.q[lane] : 0;
+    __syncthreads();
+    select<NT>(list, NT / 64 * kMostTop, p.top, [&](int rank, uint64_t key) { finish_top(p, row, a, rank, key); });
   }
 }
 
@@ -550,7 +648,7 @@ __device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
   return a;
 }
 // Rows (WAVES = 1: a wave a row) and slices (4) of one run of R vectors a lane: the logits stay in
-// registers, so candidates are taken from there.  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
+// registers, so candidates are taken from there (and weighed twice where a lane has no vector).  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
 // in 16 slices each 6.7 us, and 4.0 for their join.
 template <typename T, int WAVES, int R, bool TOP>
 __global__ __launch_bounds__(256) void run_kernel(Params p) {
@@ -598,7 +696,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
     tau = bound_of(best, p.top);
   }
   Sums row;
-  if (whole) row = sums_of<T>(p, at.row, a);
+  if (whole) row = sums_of<T, NT, 0>(p, at.row, a, t, parts[0]);
   if (t == 0) {
     if (whole) finish(p, at.row, row, given);
     else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
@@ -606,7 +704,7 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
   if constexpr (TOP) {
     uint64_t* list = lists + own * kQueue;
     if (whole && row.s != row.s) {
-      top_of_nan_row<T, NT>(p, at.row, row, lists);
+      top_by_order<T, NT, 0>(p, at.row, row, t, queues + own * kQueue, lists);
       return;
     }
     const float tau_x = tau ? value_of(tau) : -INFINITY;
@@ -673,7 +771,8 @@ __global__ __launch_bounds__(256) void run_kernel(Params p) {
 // of 5.  That the fifth wave picks is what hides it: candidates queued by the waves that stream
 // 287 us, a part's end in these waves 260.  Five workgroups a CU, in the registers of seven waves
 // a SIMD; four, without that bound, 209 us, six in the registers of eight 243.
-// Rows of which most is masked with -infinity take 340: their runs are weighed twice.
+// No register spills.  A run in which a lane has no vector (a part's last one) or a logit of -infinity is weighed
+// twice and read again, so a row of 32000 a quarter of it, and one of which most is masked all: 340 us for 191.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Params p, int64_t parts_n) {
   constexpr int VEC = Elem<T>::kVec, NT = 256, kStep = NT * kRun;
@@ -684,11 +783,11 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
   __shared__ uint16_t picks[TOP ? kPicks : 1];
   __shared__ __attribute__((aligned(16))) uint16_t bests[2][256];
   __shared__ float parts[2][3][4];
+  __shared__ uint32_t unusual[TOP ? kMostTurns / 32 : 1];  // rows without usual sums, a bit each
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = threadIdx.x;
   int parity = 0;
   if (!TOP || wave < 4) {
     int64_t unit = blockIdx.x;
-    if (unit >= parts_n) return;
     uint4 raw[kRun];
     {
       const Part<T> at(p, unit);
@@ -725,10 +824,10 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       if (lane == 0) parts[parity][0][wave] = a.m, parts[parity][1][wave] = a.s, parts[parity][2][wave] = a.e;
       if constexpr (TOP) bests[parity][t] = static_cast<uint16_t>(order_of_best(best) >> 16);
       __syncthreads();
-      if (!TOP && wave == 0) {
+      if constexpr (!TOP) {  // (the workgroup's one part)
         a = waves_join(parts[parity]);
         if (p.slices == 1) {
-          const Sums row = sums_of<T>(p, at.row, a);
+          const Sums row = sums_of<T, NT, kAhead>(p, at.row, a, t, parts[parity ^ 1][0]);
           Given given;
           if (t == 0) given.load<T>(p, at.row), finish(p, at.row, row, given);
         } else if (t == 0) {
@@ -737,7 +836,10 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       }
     }
   } else if constexpr (TOP) {
-    for (int64_t unit = blockIdx.x; unit < parts_n; unit += gridDim.x, parity ^= 1) {
+    for (int i = lane; i < kMostTurns / 32; i += 64) unusual[i] = 0;
+    wave_sync();
+    int turn = 0;
+    for (int64_t unit = blockIdx.x; unit < parts_n; unit += gridDim.x, parity ^= 1, ++turn) {
       const Part<T> at(p, unit);
       const bool whole = p.slices == 1;
       Given given;
@@ -746,15 +848,14 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       const float single = alone ? Elem<T>::load1(at.x + at.single(p, lane)) : -INFINITY;
       __syncthreads();  // the part has been streamed
       const Stats a = waves_join(parts[parity]);
-      Sums row;
-      if (whole) row = sums_of<T>(p, at.row, a);
+      const Sums row(a);
+      if (whole && !row.usual()) {
+        if (lane == 0) unusual[turn >> 5] |= 1u << (turn & 31);
+        continue;
+      }
       if (lane == 0) {
         if (whole) finish(p, at.row, row, given);
         else p.stats[unit] = make_float4(a.m, a.s, a.e, 0.f);
-      }
-      if (whole && row.s != row.s) {
-        top_of_nan_row<T, 64>(p, at.row, row, nullptr);
-        continue;
       }
       const uint32_t tau = bound_of(bests[parity], lane, p.top);
       const float tau_x = tau ? value_of(tau) : -INFINITY;
@@ -823,37 +924,70 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
       wave_sync();
     }
   }
+  if constexpr (TOP) {
+    // Rows without usual sums, by all waves, behind the others (in the fifth wave's turn they held up
+    // the stream, and their registers spilled in it).
+    constexpr int kAll = NT + 64;
+    static_assert(sizeof(slots) >= kAll / 64 * kQueue * sizeof(uint64_t) && kKeys >= kAll / 64 * kMostTop, "queues of all waves");
+    if (p.slices > 1) return;
+    __syncthreads();
+    int64_t unit = blockIdx.x;
+    for (int turn = 0; unit < parts_n; unit += gridDim.x, ++turn) {
+      if (!(unusual[turn >> 5] >> (turn & 31) & 1)) continue;
+      const Sums row = exact_sums<T, kAll, kAhead>(p, unit, t, parts[0][0]);
+      if (t == 0) {
+        Given given;
+        given.load<T>(p, unit);
+        finish(p, unit, row, given);
+      }
+      top_by_order<T, kAll, kAhead>(p, unit, row, t, reinterpret_cast<uint64_t*>(slots), list);
+      __syncthreads();
+    }
+  }
 }
 
-// Joins a row's slices; a wave a row.  Bound by the chain of its loads: 4 us for 16 rows.
+// Joins a row's slices; a wave a row, and three more for rows outside the usual sums.  Bound by the
+// chain of its loads: 4 us for 16 rows.
 template <typename T>
-__global__ __launch_bounds__(64) void join_kernel(Params p) {
+__global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int kHeld = 8;  // keys of a lane in registers
   __shared__ uint64_t list[kMostSlices * kMostTop];
-  const int lane = threadIdx.x;
+  __shared__ uint64_t best_of_waves[4 * kMostTop];
+  __shared__ float parts[4];
+  __shared__ int unusual;
+  static_assert(kMostSlices * kMostTop >= 4 * kQueue, "queues of four waves");
+  const int lane = threadIdx.x & 63, t = threadIdx.x;
   const int64_t row = blockIdx.x;
-  Stats a;
-  Given given;
-  if (lane == 0) given.load<T>(p, row);
-  if (lane < p.slices) {
-    const float4 s = p.stats[row * p.slices + lane];
-    a.m = s.x;
-    a.s = s.y;
-    a.e = s.z;
-  }
   const int n = p.slices * p.top;
   const uint64_t* keys = p.keys + row * n;
-  uint64_t best = 0, held[kHeld];
+  Given given;
+  Sums sums;
+  uint64_t best = 0, held[kHeld] = {};
+  if (t < 64) {
+    Stats a;
+    if (lane == 0) given.load<T>(p, row);
+    if (lane < p.slices) {
+      const float4 s = p.stats[row * p.slices + lane];
+      a.m = s.x;
+      a.s = s.y;
+      a.e = s.z;
+    }
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) held[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
-  a.move(wave_max(a.m));
-  const Sums sums = sums_of<T>(p, row, wave_join(a));
-  if (lane == 0) finish(p, row, sums, given);
+    for (int i = 0; i < kHeld; ++i) held[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
+    a.move(wave_max(a.m));
+    sums = Sums(wave_join(a));
+    if (lane == 0) unusual = !sums.usual();
+  }
+  __syncthreads();
+  const bool exact = unusual != 0;
+  if (exact) sums = exact_sums<T, 256, kAhead>(p, row, t, parts);
+  if (t == 0) finish(p, row, sums, given);
   if (p.top == 0) return;
-  if (sums.s != sums.s) {
-    top_of_nan_row<T, 64>(p, row, sums, nullptr);
+  if (exact && sums.s != sums.s) {
+    top_by_order<T, 256, kAhead>(p, row, sums, t, list, best_of_waves);
     return;
   }
+  if (t >= 64) return;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) best = held[i] > best ? held[i] : best;
   for (int i = lane + 64 * kHeld; i < n; i += 64) best = keys[i] > best ? keys[i] : best;
@@ -946,7 +1080,6 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   }
 }
 
-constexpr int kCus = 256, kStay = 5;  // of an MI355X; workgroups of stream_kernel on each
 
 // Logits of a run of `waves` waves.
 constexpr int64_t run_of(int64_t es, int waves) { return waves * 64 * kRun * 16 / es; }
@@ -982,7 +1115,7 @@ static void launch(const Params& p, hipStream_t s) {
     launch_runs<T, 1>(p, (p.N + 3) / 4, s);
     return;
   }
-  const int64_t parts = p.N * p.slices;
+  const int64_t parts = p.N * p.slices;  // (below 2^24: one row each, or 1024 of them)
   if (p.per <= 256 * kRun) {
     launch_runs<T, 4>(p, parts, s);
   } else {
@@ -992,7 +1125,7 @@ static void launch(const Params& p, hipStream_t s) {
     if (p.top) hipLaunchKernelGGL((stream_kernel<T, true>), grid, dim3(320), 0, s, p, parts);
     else hipLaunchKernelGGL((stream_kernel<T, false>), grid, dim3(256), 0, s, p, parts);
   }
-  if (p.slices > 1) hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>(p.N)), dim3(64), 0, s, p);
+  if (p.slices > 1) hipLaunchKernelGGL((join_kernel<T>), dim3(static_cast<unsigned>(p.N)), dim3(256), 0, s, p);
 }
 
 template <typename T>

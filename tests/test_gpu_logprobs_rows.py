@@ -114,3 +114,42 @@ def test_rows_in_slices(cuda, N, V, dt):
     for top in (0, 5, 32):
         check(x, ids, bad, top, 0.7)
         check(x, ids, bad, top, 0.7, split=False)
+
+
+def least_time(call):
+    """The shortest of some replays of a captured call, after one."""
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    times = []
+    for _ in range(6):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times[1:])
+
+
+@pytest.mark.parametrize("fill", [-INF, torch.finfo(BF16).min, float("nan")])
+@pytest.mark.parametrize("N,every", [(16, 16), (2600, 8)])
+def test_padding_costs_no_multiple(cuda, fill, N, every):
+    """A finished sequence in a step, padded rows in a batch, a row gone wrong: such a row is read twice
+    more at most, by as many waves as an ordinary one, so the call takes 1.5 to 4 times the ordinary
+    rows' time (with one wave a row that read its logits one by one, once more for each of the
+    largest beside a NaN, 12 to 200 times)."""
+    V = 131072
+    x = (torch.randn((N, V), generator=torch.Generator(device=cuda).manual_seed(0), device=cuda) * 2.5).to(BF16)
+    ids = torch.zeros(N, dtype=torch.int32, device=cuda)
+    ws = ops.token_logprobs_workspace(x, 20)
+    plain = least_time(lambda: ops.token_logprobs(x, ids, top=20, workspace=ws, split=ws is not None))
+    if fill != fill:
+        x[3::every, V // 2] = fill
+    else:
+        x[3::every] = fill
+    padded = least_time(lambda: ops.token_logprobs(x, ids, top=20, workspace=ws, split=ws is not None))
+    print(f"{plain * 1e3:.1f} us, padded {padded * 1e3:.1f} us", flush=True)
+    assert padded < 8 * plain
