@@ -52,8 +52,10 @@ template <> struct Parts<bf16_t> { static constexpr int kQ = 1, kP = 2; };
 template <> struct Parts<f16_t> { static constexpr int kQ = 2, kP = 2; };
 template <> struct Parts<float> { static constexpr int kQ = 3, kP = 3; };
 
-// x as the sum of N bf16 values (the last one rounds: 2^-9, 2^-17 or 2^-25 of x).
-template <int N>
+// x as the sum of N bf16 values (the last one rounds: 2^-9, 2^-17 or 2^-25 of x).  CUT: those before the
+// last are cut off, not rounded (three hold an fp32 value's 24 bits either way), so neither they
+// nor their sums pass x: near fp32's largest values a rounded part, or it and the next one, is infinite.
+template <int N, bool CUT = false>
 __device__ __forceinline__ void split8(const float (&x)[8], tile::bf16x8 (&out)[N]) {
   float r[8];
 #pragma unroll
@@ -63,7 +65,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], tile::bf16x8 (&out)[
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      if (CUT && n + 1 < N) w[i] = (__float_as_uint(r[2 * i]) >> 16) | (__float_as_uint(r[2 * i + 1]) & 0xffff0000u);
+      else w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
       if (n + 1 < N) {
         r[2 * i] -= __uint_as_float(w[i] << 16);
         r[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(64, DP == 256 ? 1 : 2) void attend4_kernel(Params p
         const bool in = (col < heads) & (g * (DP / 4) + 8 * s < p.D);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[s][e] = in ? x[s][e] : 0.f;
-        split8<kQ>(x[s], qf[s]);
+        split8<kQ, __is_same(T, float)>(x[s], qf[s]);
       }
 #pragma unroll
       for (int s = 0; s < kVals / 2; ++s) tile::settle(qf[s]);
