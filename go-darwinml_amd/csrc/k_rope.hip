@@ -387,7 +387,7 @@ int read_rope(const GHipRope* r, int64_t D, int64_t S, const int32_t* starts, ro
   for (int i = 0; i < rope::kMostAxes; ++i) {
     if (i < r->axes) {
       if (r->sections[i] < 0) return set_error(err, GHIP_ERR_INVALID_ARG, "%s: negative section", what);
-      end += r->sections[i];
+      end += std::min<int64_t>(r->sections[i], int64_t{1} << 60);  // (so that the sum cannot wrap around)
     }
     p.a.ends[i] = static_cast<int>(std::min<int64_t>(end, rope::kMostHalf));
   }
