@@ -50,21 +50,6 @@ struct Seen {
   __device__ __forceinline__ int tiles(int kt) const { return sink_tiles(kt) + (len - (lo & ~15) + kt - 1) / kt; }
 };
 
-// Sum of x over this lane and the lower ones: shifts within the rows of 16 lanes, then the
-// rows' totals broadcast to the rows after them (one VALU instruction a step).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
-  return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, true));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
-  x = dpp_add<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
-  return x;
-}
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
 }

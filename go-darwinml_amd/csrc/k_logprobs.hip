@@ -88,21 +88,6 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
   return static_cast<uint64_t>(order_of(x)) << 32 | static_cast<uint32_t>(~i);
 }
 
-// Sum of x over this lane and the lower ones: shifts within the rows of 16 lanes, then the rows'
-// totals broadcast to the rows after them.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
-  return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, true));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x = dpp_add<0x111, 0xf>(x);
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);
-  x = dpp_add<0x143, 0xc>(x);
-  return x;
-}
 __device__ __forceinline__ int rank_in(uint64_t mask) {  // set bits below this lane's
   return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
@@ -648,8 +633,10 @@ __device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
   return a;
 }
 // Rows (WAVES = 1: a wave a row) and slices (4) of one run of R vectors a lane: the logits stay in
-// registers, so candidates are taken from there (and weighed twice where a lane has no vector).  Bound by the chain of its steps: 16 rows of 131072 bf16 logits
-// in 16 slices each 6.7 us, and 4.0 for their join.
+// registers, so candidates are taken from there.  A run in which a lane has no vector is weighed twice (0
+// times -infinity), and a wave ends with its row: 65536 rows of 2000 bf16 logits 80 us where their bytes take 47.
+// Bound by the chain of its steps: 16 rows of 131072 bf16 logits in 16 slices each 6.7 us, and 4.0
+// for their join.
 template <typename T, int WAVES, int R, bool TOP>
 __global__ __launch_bounds__(256) void run_kernel(Params p) {
   constexpr int VEC = Elem<T>::kVec, NT = 64 * WAVES;
