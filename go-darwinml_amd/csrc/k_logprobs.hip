@@ -635,7 +635,7 @@ __device__ __forceinline__ Stats waves_join(const float (&parts)[3][4]) {
 // Rows (WAVES = 1: a wave a row) and slices (4) of one run of R vectors a lane: the logits stay in
 // registers, so candidates are taken from there.  A run in which a lane has no vector is weighed twice (0
 // times -infinity), and a wave ends with its row: 65536 rows of 2000 bf16 logits 80 us where their bytes take 47.
-// Bound by the chain of its steps: 16 rows of 131072 bf16 logits in 16 slices each 6.7 us, and 4.0
+// Bound by the chain of its steps: 16 rows of 131072 bf16 logits in 16 slices each 6.6 us, and 4.3
 // for their join.
 template <typename T, int WAVES, int R, bool TOP>
 __global__ __launch_bounds__(256) void run_kernel(Params p) {
@@ -934,7 +934,7 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
 }
 
 // Joins a row's slices; a wave a row, and three more for rows outside the usual sums.  Bound by the
-// chain of its loads: 4 us for 16 rows.
+// chain of its loads: 4.3 us for 16 rows.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
   constexpr int kHeld = 8;  // keys of a lane in registers

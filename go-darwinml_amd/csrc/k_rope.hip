@@ -232,7 +232,7 @@ struct Slots {
 // keys and values go into 4 bits, by threads of their own share of a row.
 // Bound by the bytes of the rows, then, for a few tokens, by the chain position - angle - row:
 // 8192 tokens of 16 heads of 128 in bf16 (67 MB) 12.8 us, 8 prompts of 1024 tokens, 32 heads and
-// 8, into 16 bits (172 MB) 35.7 us, into 4 bits 38; 16 tokens 4.3 and 5.9.  Two rows of a thread
+// 8, into 16 bits (172 MB) 36 us, into 4 bits 38; 16 tokens 4.3 and 5.8.  Two rows of a thread
 // under way at once: 59 us for 35.7 (88 registers).
 template <typename T, int N, bool FOUR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rope_kernel(Params p) {
@@ -340,6 +340,8 @@ template <typename T, bool FOUR>
 static int launch(Params& p, bool wide4, hipStream_t s, GHipError* err, const char* what) {
   constexpr int V = Elem<T>::kVec;
   int n = width(p.D, p.a.half, V);
+  // (Beside rows into 4 bits there are no kernels of the widths between: bf16, 8 x 1024 tokens, 32 heads and
+  // 8 of 96, 24 of them turned, 134 us; q alone four at a time 28, and the call without q 33.)
   if (FOUR && n < V) n = 1;
   p.units = (p.D + 2 * n - 1) / (2 * n);  // (half a row's pairs are a multiple of n)
   p.units4 = p.D / 8;

@@ -448,8 +448,9 @@ int ghip_sdpa_paged_kv4(int dtype, const void* q, const GHipKv4* k_cache, const 
  *   lse = log sum_v exp x_v,  logp = x_id - lse,  entropy = -sum_v p_v log p_v,  p = exp(x - lse)
  * and the `top` (0 .. 32, at most V) largest logits: top_ids by value, then by index (a NaN
  * is above all numbers, -0 equals 0), top_logps their log probabilities.  ids: int32 [N]; logp of
- * an id outside [0, V) is 0.  Outputs [N] and [N, top], dense, float32 and int32; entropy, lse,
- * top_logps and top_ids may be NULL (top = 0: the last two are not used).
+ * an id outside [0, V) is 0.  Outputs [N] and [N, top], dense, float32 and int32; entropy and lse
+ * may be NULL, top_logps and top_ids where top is 0 (they are not used).  Fewer than 2^24 rows of at most
+ * 2^30 logits.
  * Logits of -infinity are tokens that cannot be (p = 0, log p = -infinity); a row of nothing
  * else has lse -infinity, entropy 0, log probabilities -infinity.  A row that holds a NaN or
  * +infinity gets NaN (its top_ids stay as defined).  Sums are fp32, in a fixed order.
