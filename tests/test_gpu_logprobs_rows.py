@@ -90,6 +90,15 @@ def test_rows_one_after_the_other(cuda, N, V, dt):
         check(x, ids, bad, top, 0.7)
 
 
+def test_many_turns(cuda):
+    """More than 32 rows a workgroup, so those without usual sums are noted in several words."""
+    N, V = 90001, 8201
+    g = torch.Generator(device=cuda).manual_seed(N)
+    x = torch.randn((N, V), generator=g, device=cuda, dtype=BF16)
+    ids = torch.randint(0, V, (N,), generator=g, device=cuda, dtype=torch.int32)
+    check(x, ids, rows_of_every_kind(x, ids, 4), 5, 0.7)
+
+
 @pytest.mark.parametrize("dt", [BF16, F32])
 @pytest.mark.parametrize("N,V", [(700, 333), (500, 2001), (300, 5003)])
 def test_rows_of_one_run(cuda, N, V, dt):
