@@ -915,13 +915,15 @@ __global__ __launch_bounds__(TOP ? 320 : 256, TOP ? 7 : 1) void stream_kernel(Pa
     // Rows without usual sums, by all waves, behind the others (in the fifth wave's turn they held up
     // the stream, and their registers spilled in it).
     constexpr int kAll = NT + 64;
-    static_assert(sizeof(slots) >= kAll / 64 * kQueue * sizeof(uint64_t) && kKeys >= kAll / 64 * kMostTop, "queues of all waves");
+    static_assert(sizeof(slots) >= kAll / 64 * kQueue * sizeof(uint64_t) && kKeys >= kAll / 64 * kMostTop,
+                  "queues of all waves");
+    __shared__ float of_waves[kAll / 64];
     if (p.slices > 1) return;
     __syncthreads();
     int64_t unit = blockIdx.x;
     for (int turn = 0; unit < parts_n; unit += gridDim.x, ++turn) {
       if (!(unusual[turn >> 5] >> (turn & 31) & 1)) continue;
-      const Sums row = exact_sums<T, kAll, kAhead>(p, unit, t, parts[0][0]);
+      const Sums row = exact_sums<T, kAll, kAhead>(p, unit, t, of_waves);
       if (t == 0) {
         Given given;
         given.load<T>(p, unit);
